@@ -161,7 +161,7 @@ def prepare(case, seed):
         x = _activations(g, T, H)
         state["x"] = x
         state["q"], state["s"] = _quant_rows(x.float())
-        state["router"] = (0.02 * torch.randn(E, H, generator=g, device="cuda")).to(torch.bfloat16)
+        state["router"] = (0.004 * torch.randn(E, H, generator=g, device="cuda")).to(torch.bfloat16)
 
         def weight(rows, cols):
             codes = torch.empty(E, rows, cols, dtype=F8, device="cuda")
@@ -214,8 +214,9 @@ def _plain_moe(s, dtype=torch.float32):
         p = p / p.sum(1, keepdim=True)
     else:
         p = 1.0 / (1.0 + torch.exp(-logits))
-    top, ids = torch.sort(p, dim=1, descending=True, stable=True)
-    top, ids = top[:, :k], ids[:, :k]
+    # the scores grow with the logits: chosen by the logits, which do not saturate; ties to the lowest index
+    ids = torch.sort(logits, dim=1, descending=True, stable=True).indices[:, :k]
+    top = p.gather(1, ids)
     weight = torch.zeros(T, E, dtype=dtype, device=p.device).scatter(1, ids, top / top.sum(1, keepdim=True))
 
     def spread(w, sw):
@@ -348,11 +349,12 @@ def exact(case, seed):
     T, E, k, H, I = (case[n] for n in ("T", "E", "k", "H", "I"))
     logits = s["x"].double() @ s["router"].double().t()
     p = torch.softmax(logits, 1) if case["scoring"] == "softmax" else torch.sigmoid(logits)
-    top = p.topk(k, dim=1)
-    weight = top.values / top.values.sum(1, keepdim=True)
+    top = logits.topk(k, dim=1).indices
+    weight = p.gather(1, top)
+    weight = weight / weight.sum(1, keepdim=True)
     y = torch.zeros(T, H, dtype=torch.float64, device=logits.device)
     for e in range(E):  # only the tokens that take expert e
-        t, slot = (top.indices == e).nonzero(as_tuple=True)
+        t, slot = (top == e).nonzero(as_tuple=True)
         if not len(t):
             continue
         gu = _exact_product(s["q"][t], s["s"][t], s["w13"][e], s["s13"][e])
