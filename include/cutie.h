@@ -273,6 +273,57 @@ CUTIE_API int cutie_rms_norm_mxfp8_gemm(const void* x, int64_t ldx, const void* 
                                         void* q_scale, void* stream);
 
 /*
+ * Cast of a bf16 matrix x [M, H] (ldx elements between rows) to e4m3 in both
+ * orientations, reading x once:
+ *   s = max(amax / 448, 1e-4), rounded up to a power of two for
+ *   CUTIE_SCALE_FP32_POW2; q = e4m3(x / s)
+ * the rule of cutie_per_token_cast_to_fp8 (src/cutie/vendor/prime_rl/
+ * fp8_utils.py:50-57), over
+ *   CUTIE_TILE_BLOCK: 128 x 128 blocks (weights). s: fp32 [ceil(M/128),
+ *     ceil(H/128)], lds elements between rows. qt / st (both NULL, or both
+ *     given): the codes [H, M] of x's transpose and its scales
+ *     [ceil(H/128), ceil(M/128)].
+ *   CUTIE_TILE_TWO_WAY: 1 x 128 groups of the rows for q, 128 x 1 groups of
+ *     the columns for qt (activations and gradients; qt and st are required).
+ *     Scales are group-major: s element (row, g) at g * lds + row, st element
+ *     (column, g) at g * ldst + column.
+ * Ragged last blocks and groups are reduced over their valid elements. H is a
+ * multiple of 8, M >= 0 any; x rows 16-byte, q and qt rows 8-byte aligned
+ * (16-byte for cutie_fp8_block_gemm). A group with an infinity gets an
+ * infinite scale and NaN codes; a NaN gives a NaN code and does not count for
+ * its group's scale. Asynchronous on `stream`; nothing is allocated.
+ */
+enum {
+  CUTIE_TILE_BLOCK = 0,
+  CUTIE_TILE_TWO_WAY = 1,
+};
+CUTIE_API int cutie_cast_fp8_tiles(const void* x, int64_t ldx, int64_t M, int64_t H,
+                                   int tile_kind, int scale_fmt, void* q, int64_t ldq, void* s,
+                                   int64_t lds, void* qt, int64_t ldqt, void* st, int64_t ldst,
+                                   void* stream);
+
+/*
+ * FP8 product with a scale for each block of 128:
+ *   D[m, n] = sum_kb sA[m, kb] sB[n, kb] sum_{k in block kb} a[m, k] b[n, k]
+ * a: e4m3 [M, K] (lda bytes between rows), a_scale: fp32, element (m, kb) at
+ * m * sa_row + kb * sa_kb (row- or group-major, as the quantizers write it).
+ * b: e4m3 [N, K] (ldb), b_scale: element (n, kb) at (n / 128) * sb_row +
+ * kb * sb_kb for 128 x 128 blocks (b_rows = 0), at n * sb_row + kb * sb_kb
+ * for 1 x 128 groups (b_rows = 1). d: [M, N], ldd elements between rows, bf16
+ * or fp32 (d_dtype: CUTIE_DTYPE_*); accumulate (fp32 only): D += the product.
+ * The sum of a 128-wide block is made on the tensor cores in fp32, the sum
+ * over blocks in fp32 registers, one rounding to bf16 at the end. M, N and K
+ * may be any size >= 0 (K = 0: zeros, or D unchanged); a and b rows 16-byte
+ * aligned (lda and ldb multiples of 16). Asynchronous on `stream`; nothing is
+ * allocated.
+ */
+CUTIE_API int cutie_fp8_block_gemm(const void* a, int64_t lda, const void* a_scale,
+                                   int64_t sa_row, int64_t sa_kb, const void* b, int64_t ldb,
+                                   const void* b_scale, int64_t sb_row, int64_t sb_kb,
+                                   int b_rows, void* d, int64_t ldd, int d_dtype, int accumulate,
+                                   int64_t M, int64_t N, int64_t K, void* stream);
+
+/*
  * Device-side status of this library's kernels on the current device: 0 when
  * no kernel has hit a failure since the last clear; otherwise the first error
  * code recorded (1 = a bulk-copy wait ran out: a row never arrived in shared

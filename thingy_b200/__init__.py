@@ -13,24 +13,37 @@ Drop-in host API for the reference's hot path (S1ro1/thingy, package
                                             backward (no counterpart in the reference):
                                                the gradients autograd gives its forward
 
+    per_block_cast_to_fp8, two_way_cast_to_fp8, fp8_block_gemm, fp8_linear
+                                            what follows the quantizer (no counterpart):
+                                               weight and two-way casts, the product with a
+                                               scale a block of 128, a linear layer with its
+                                               gradients
+
 Every op runs hand-written CUDA from ``lib/libcutie_b200.so`` through the C
 ABI in ``include/cutie.h``; there is no CPU or PyTorch fallback.
 """
 
 from .backward import ResidualRMSNormFP8, rms_norm_fp8_backward
-from .fp8_utils import per_token_cast_to_fp8, per_token_cast_to_fp8_triton
+from .fp8_utils import (per_block_cast_to_fp8, per_token_cast_to_fp8, per_token_cast_to_fp8_triton,
+                        two_way_cast_to_fp8)
 from .fused import empty_scale, residual_rms_norm_fp8, rms_norm_fp8
+from .gemm import fp8_block_gemm
 from .layouts import mx_swizzle, mx_swizzle_offset, mx_swizzled_size, mx_unswizzle
+from .linear import FP8Linear, fp8_linear
 from .rms_norm import RMSNorm, rms_norm, rms_norm_on_stream
 
 __all__ = [
+    "FP8Linear",
     "RMSNorm",
     "ResidualRMSNormFP8",
     "empty_scale",
+    "fp8_block_gemm",
+    "fp8_linear",
     "mx_swizzle",
     "mx_swizzle_offset",
     "mx_swizzled_size",
     "mx_unswizzle",
+    "per_block_cast_to_fp8",
     "per_token_cast_to_fp8",
     "per_token_cast_to_fp8_triton",
     "residual_rms_norm_fp8",
@@ -38,4 +51,5 @@ __all__ = [
     "rms_norm_fp8",
     "rms_norm_fp8_backward",
     "rms_norm_on_stream",
+    "two_way_cast_to_fp8",
 ]

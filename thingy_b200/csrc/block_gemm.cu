@@ -1,0 +1,390 @@
+// FP8 product with a scale for each block of 128 (sm_100a):
+//
+//   D[m, n] = sum_kb sA[m, kb] sB[n, kb] * sum_{k in block kb} a[m, k] b[n, k]
+//
+// a: e4m3 [M, K] with fp32 scales of 1 x 128 groups; b: e4m3 [N, K] with fp32
+// scales of 128 x 128 blocks (a weight) or of 1 x 128 groups (the other
+// operand of a weight gradient). fp32 scales are not powers of two, so the
+// tensor cores' own block scaling cannot apply them: the inner sum of every
+// 128-wide K block is made by tcgen05.mma (kind::f8f6f4, fp32 accumulators in
+// tensor memory, overwritten by each block) and the outer sum by the epilogue
+// warps in fp32 registers, one FMA an element and block.
+#include "cutie.h"
+#include "launch.cuh"
+#include "tcgen05.cuh"
+
+namespace cutie {
+
+static __device__ int g_block_gemm_device_error = 0;
+
+namespace {
+
+constexpr int kBM = 128, kBK = 128;
+constexpr uint32_t kBoxBytes = kBM * kBK;  // one 128-row operand box: 16 KB
+
+using tc::kLayoutSw128;
+using tc::smem_desc;
+
+// Gives up after kWaitLimitCycles, or at once when the CTA's abort flag is
+// set; giving up sets the flag.
+__device__ __forceinline__ bool wait_or_abort(uint32_t bar, uint32_t parity,
+                                              volatile uint32_t* abort_flag) {
+  if (mbar_test(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (!*abort_flag && clock64() - t0 <= kWaitLimitCycles)
+    if (mbar_try_wait(bar, parity)) return true;
+  *abort_flag = 1u;
+  return false;
+}
+
+// ------------------------------------------------------------------ tiled
+//
+// Persistent CTAs of 10 warps, one an SM, each walking tiles of 128 x BN:
+//  * warp 8, one thread: TMA of the A box and the BN / 128 B boxes of a K
+//    block into a ring of stages (128-byte swizzled rows; rows and columns
+//    past the matrices are zero-filled, so M, N and K may be any).
+//  * warp 9, one thread: four MMAs of 128 x BN x 32 a K block into one of two
+//    accumulator buffers in tensor memory; a commit frees the stage, a second
+//    hands the buffer to the epilogue.
+//  * warps 0-7: the outer sum. Warp group g = warp / 4 keeps columns
+//    g BN/2 .. of the tile for its 128 rows, a row a thread, in BN / 2 fp32
+//    registers, and adds scale * buffer to them while the MMAs of the next K
+//    block fill the other buffer. The row's scale and the weight block's are
+//    loaded two K blocks ahead.
+// Tiles are walked in bands of kBand rows of tiles, so that the CTAs of a
+// wave share their operands in L2.
+constexpr int kThreads = 320, kEpiWarps = 8, kBand = 16;
+
+template <int BN>
+struct TilePlan {
+  static constexpr int kNB = BN / 128;
+  static constexpr uint32_t kStageBytes = (1 + kNB) * kBoxBytes;
+  static constexpr int kStages = BN == 256 ? 4 : 6;
+  static constexpr size_t kSmemBytes = kStages * kStageBytes + 1024;
+  static constexpr uint32_t kTmemCols = 2 * BN;
+  static constexpr int kCols = BN / 2;  // columns of a warp group
+  static_assert(kSmemBytes <= 225 * 1024, "shared memory");
+};
+
+struct TileArgs {
+  const float* sa;
+  int64_t sa_row, sa_kb;
+  const float* sb;
+  int64_t sb_row, sb_kb;
+  void* d;
+  int64_t ldd;
+  int M, N, KB, tiles_m, tiles_n;
+  bool d_f32, accumulate, vec;  // vec: rows of D start on 32-byte boundaries
+};
+
+// Tile t of the banded walk.
+__device__ __forceinline__ void tile_at(int t, int tiles_m, int tiles_n, int* tm, int* tn) {
+  const int band = t / (kBand * tiles_n), first = band * kBand;
+  const int rows = tiles_m - first < kBand ? tiles_m - first : kBand;
+  const int in = t - band * kBand * tiles_n;
+  *tm = first + in % rows;
+  *tn = in / rows;
+}
+
+template <int NC>
+__device__ __forceinline__ void store_row(const TileArgs& g, const float2 (&acc)[NC / 2], int row,
+                                          int col) {
+  if (row >= g.M || col >= g.N) return;
+  const int left = g.N - col < NC ? g.N - col : NC;
+  const int64_t at = (int64_t)row * g.ldd + col;
+  if (!g.d_f32) {
+    uint16_t* p = static_cast<uint16_t*>(g.d) + at;
+#pragma unroll
+    for (int c = 0; c < NC; c += 16) {
+      uint32_t w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = f2_to_bf2(acc[c / 2 + i]);
+      if (g.vec && c + 16 <= left) {
+        st_stream8(p + c, w);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (c + i < left) p[c + i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+      }
+    }
+  } else {
+    float* p = static_cast<float*>(g.d) + at;
+#pragma unroll
+    for (int c = 0; c < NC; c += 8) {
+      if (g.vec && c + 8 <= left) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[2 * i] = acc[c / 2 + i].x, v[2 * i + 1] = acc[c / 2 + i].y;
+        if (g.accumulate) {
+          const float4 o0 = *reinterpret_cast<const float4*>(p + c);
+          const float4 o1 = *reinterpret_cast<const float4*>(p + c + 4);
+          v[0] += o0.x, v[1] += o0.y, v[2] += o0.z, v[3] += o0.w;
+          v[4] += o1.x, v[5] += o1.y, v[6] += o1.z, v[7] += o1.w;
+        }
+        st_stream8(p + c, reinterpret_cast<const uint32_t*>(v));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float f = i & 1 ? acc[c / 2 + i / 2].y : acc[c / 2 + i / 2].x;
+          if (c + i < left) p[c + i] = g.accumulate ? p[c + i] + f : f;
+        }
+      }
+    }
+  }
+}
+
+template <int BN, bool SB_ROWS>
+__global__ void __launch_bounds__(kThreads, 1)
+    block_gemm_kernel(const __grid_constant__ CUtensorMap map_a,
+                      const __grid_constant__ CUtensorMap map_b, const TileArgs g) {
+  using P = TilePlan<BN>;
+  constexpr int NC = P::kCols;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t full_bar[P::kStages];
+  __shared__ __align__(8) uint64_t empty_bar[P::kStages];
+  __shared__ __align__(8) uint64_t acc_full[2];
+  __shared__ __align__(8) uint64_t acc_empty[2];
+  __shared__ __align__(16) float sb_rows[SB_ROWS ? 2 : 1][SB_ROWS ? BN : 1];
+  __shared__ uint32_t tmem_base_slot;
+  __shared__ uint32_t abort_flag;
+  __shared__ uint32_t issued;     // K blocks whose copies were issued
+  __shared__ uint32_t committed;  // K blocks whose MMAs were committed
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
+  const int tiles = g.tiles_m * g.tiles_n;
+  volatile uint32_t* abortp = &abort_flag;
+
+  if (threadIdx.x == 0) {
+    tc::prefetch_map(&map_a);
+    tc::prefetch_map(&map_b);
+    for (int s = 0; s < P::kStages; ++s) {
+      mbar_init(smem_addr(&full_bar[s]), 1);
+      mbar_init(smem_addr(&empty_bar[s]), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(smem_addr(&acc_full[b]), 1);
+      mbar_init(smem_addr(&acc_empty[b]), kEpiWarps);
+    }
+    abort_flag = 0;
+    issued = committed = 0;
+    mbar_init_fence();
+  }
+  if (warp == kEpiWarps) tc::tmem_alloc(smem_addr(&tmem_base_slot), P::kTmemCols);
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const uint32_t tmem = tmem_base_slot;
+  griddep_wait();
+  griddep_launch_dependents();
+
+  if (warp == kEpiWarps) {
+    if (lane == 0) {
+      uint32_t it = 0;
+      for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
+        int tm, tn;
+        tile_at(t, g.tiles_m, g.tiles_n, &tm, &tn);
+        for (int kb = 0; kb < g.KB; ++kb, ++it) {
+          const uint32_t s = it % P::kStages, use = it / P::kStages;
+          if (use > 0 && !wait_or_abort(smem_addr(&empty_bar[s]), (use - 1u) & 1u, abortp))
+            goto producer_done;
+          const uint32_t st = base + s * P::kStageBytes, bar = smem_addr(&full_bar[s]);
+          mbar_arrive_expect_tx(bar, P::kStageBytes);
+          tc::tma_load_2d(st, &map_a, kb * kBK, tm * kBM, bar);
+#pragma unroll
+          for (int h = 0; h < P::kNB; ++h)
+            tc::tma_load_2d(st + (1 + h) * kBoxBytes, &map_b, kb * kBK, tn * BN + 128 * h, bar);
+          issued = it + 1;
+        }
+      }
+    producer_done:;
+    }
+  } else if (warp == kEpiWarps + 1) {
+    if (lane == 0) {
+      uint32_t it = 0;
+      constexpr uint32_t idesc = tc::f8_idesc(kBM, BN);
+      for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
+        for (int kb = 0; kb < g.KB; ++kb, ++it) {
+          const uint32_t s = it % P::kStages, use = it / P::kStages, buf = it & 1u;
+          if (!wait_or_abort(smem_addr(&full_bar[s]), use & 1u, abortp)) goto mma_done;
+          if (it >= 2 && !wait_or_abort(smem_addr(&acc_empty[buf]), ((it >> 1) - 1u) & 1u, abortp))
+            goto mma_done;
+          tc::fence_after();
+          const uint32_t st = base + s * P::kStageBytes;
+#pragma unroll
+          for (int kk = 0; kk < kBK / 32; ++kk)
+            tc::mma_f8(tmem + buf * BN, smem_desc(st + 32u * kk, 16, 1024, kLayoutSw128),
+                       smem_desc(st + kBoxBytes + 32u * kk, 16, 1024, kLayoutSw128), idesc, kk != 0);
+          tc::commit(smem_addr(&empty_bar[s]));
+          tc::commit(smem_addr(&acc_full[buf]));
+          committed = it + 1;
+        }
+      }
+    mma_done:;
+    }
+  } else {
+    // ---- the outer sum
+    const int wg = warp >> 2, r = (warp & 3) * 32 + lane;
+    const uint32_t tm_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(wg * NC);
+    uint32_t it = 0;
+    // a cursor two K blocks ahead of the sum, over this CTA's tiles
+    int pf_t = blockIdx.x, pf_kb = 0;
+    const float *pf_a = nullptr, *pf_b = nullptr;
+    bool pf_row = false, pf_b_ok = false;
+    auto pf_tile = [&] {
+      int tm, tn;
+      tile_at(pf_t, g.tiles_m, g.tiles_n, &tm, &tn);
+      const int row = tm * kBM + r, col = tn * BN + wg * NC;
+      pf_row = row < g.M;
+      pf_a = g.sa + (int64_t)row * g.sa_row;
+      if (SB_ROWS) {
+        // thread r of the group loads the scale of its r-th column
+        pf_b_ok = r < NC && col + r < g.N;
+        pf_b = g.sb + (int64_t)(col + r) * g.sb_row;
+      } else {
+        pf_b_ok = col < g.N;
+        pf_b = g.sb + (int64_t)(col / 128) * g.sb_row;
+      }
+    };
+    auto pf_next = [&]() -> float2 {
+      if (pf_t >= tiles) return make_float2(0.f, 0.f);
+      if (pf_kb == 0) pf_tile();
+      const float2 v = make_float2(pf_row ? __ldg(pf_a + pf_kb * g.sa_kb) : 0.f,
+                                   pf_b_ok ? __ldg(pf_b + pf_kb * g.sb_kb) : 0.f);
+      if (++pf_kb == g.KB) pf_kb = 0, pf_t += gridDim.x;
+      return v;
+    };
+    float2 s0 = pf_next(), s1 = pf_next();
+    bool ok = true;
+    // after an abort the SB_ROWS form still walks to the end (its waits return
+    // at once): every warp of a group passes the same number of barriers
+    for (int t = blockIdx.x; t < tiles && (SB_ROWS || ok); t += gridDim.x) {
+      float2 acc[NC / 2];
+#pragma unroll
+      for (int i = 0; i < NC / 2; ++i) acc[i] = make_float2(0.f, 0.f);
+      for (int kb = 0; kb < g.KB; ++kb, ++it) {
+        const uint32_t buf = it & 1u;
+        const float2 s2 = pf_next();
+        float sc = SB_ROWS ? s0.x : s0.x * s0.y;
+        if (SB_ROWS) {
+          // the group's column scales of this K block; two slots: the slot is
+          // rewritten two blocks later, behind the next block's barrier
+          if (r < NC) sb_rows[buf][wg * NC + r] = s0.y;
+          asm volatile("barrier.cta.sync %0, 128;" ::"r"(1 + wg) : "memory");
+        }
+        ok = ok && __all_sync(0xffffffffu, wait_or_abort(smem_addr(&acc_full[buf]),
+                                                         (it >> 1) & 1u, abortp));
+        if (!SB_ROWS && !ok) break;
+        tc::fence_after();
+        const float2 sc2 = make_float2(sc, sc);
+        if (ok) {
+#pragma unroll
+          for (int c = 0; c < NC; c += 16) {
+            uint32_t v[16];
+            tc::tmem_ld16_async(tm_lane + buf * BN + (uint32_t)c, v);
+            tc::tmem_ld_wait(v);
+            if (c + 16 == NC) {
+              tc::fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(smem_addr(&acc_empty[buf]));
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              float2 d = make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+              if (SB_ROWS)
+                d = __fmul2_rn(d, *reinterpret_cast<const float2*>(&sb_rows[buf][wg * NC + c + 2 * i]));
+              acc[c / 2 + i] = __ffma2_rn(d, sc2, acc[c / 2 + i]);
+            }
+          }
+        }
+        s0 = s1;
+        s1 = s2;
+      }
+      if (ok) {
+        int tm, tn;
+        tile_at(t, g.tiles_m, g.tiles_n, &tm, &tn);
+        store_row<NC>(g, acc, tm * kBM + r, tn * BN + wg * NC);
+      }
+    }
+  }
+  __syncwarp();
+  tc::fence_before();
+  __syncthreads();
+  if (*abortp) {
+    // let copies and MMAs in flight finish before their memory goes away
+    if (threadIdx.x == 0) {
+      atomicCAS(&g_block_gemm_device_error, kDevErrNone, kDevErrBulkWaitTimeout);
+      const uint32_t n = issued, m = committed;
+      for (uint32_t k = n > P::kStages ? n - P::kStages : 0; k < n; ++k)
+        mbar_wait_bounded(smem_addr(&full_bar[k % P::kStages]), (k / P::kStages) & 1u,
+                          kDrainLimitCycles);
+      if (m > 0)
+        mbar_wait_bounded(smem_addr(&acc_full[(m - 1) & 1u]), ((m - 1) >> 1) & 1u,
+                          kDrainLimitCycles);
+    }
+    __syncthreads();
+  }
+  if (warp == kEpiWarps) tc::tmem_dealloc(tmem, P::kTmemCols);
+}
+
+template <int BN, bool SB_ROWS>
+cudaError_t launch_tiled(const CUtensorMap& map_a, const CUtensorMap& map_b, TileArgs g,
+                         cudaStream_t stream) {
+  using P = TilePlan<BN>;
+  auto kernel = block_gemm_kernel<BN, SB_ROWS>;
+  const cudaError_t e =
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)P::kSmemBytes);
+  if (e != cudaSuccess) return e;
+  g.tiles_m = (g.M + kBM - 1) / kBM;
+  g.tiles_n = (g.N + BN - 1) / BN;
+  const int64_t tiles = (int64_t)g.tiles_m * g.tiles_n;
+  const int sms = device_sm_count();
+  return launch_pdl(kernel, (unsigned)(tiles < sms ? tiles : sms), kThreads, P::kSmemBytes, stream,
+                    map_a, map_b, g);
+}
+
+}  // namespace
+
+cudaError_t device_error_block_gemm(int* out, bool clear) {
+  int v = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(&v, g_block_gemm_device_error, sizeof(int));
+  if (e != cudaSuccess) return e;
+  if (clear && v != 0) {
+    const int zero = 0;
+    e = cudaMemcpyToSymbol(g_block_gemm_device_error, &zero, sizeof(int));
+  }
+  *out = v;
+  return e;
+}
+
+int block_gemm(const BlockGemmArgs& p, cudaStream_t stream, const char** why) {
+  CUtensorMap map_a, map_b;
+  if (!tc::encode_e4m3_operand(&map_a, p.a, p.M, p.K, p.lda, kBM) ||
+      !tc::encode_e4m3_operand(&map_b, p.b, p.N, p.K, p.ldb, kBM)) {
+    *why = "cuTensorMapEncodeTiled failed for an operand";
+    return CUTIE_ERR_CUDA;
+  }
+  TileArgs g{};
+  g.sa = p.sa, g.sa_row = p.sa_row, g.sa_kb = p.sa_kb;
+  g.sb = p.sb, g.sb_row = p.sb_row, g.sb_kb = p.sb_kb;
+  g.d = p.d, g.ldd = p.ldd;
+  g.M = (int)p.M, g.N = (int)p.N, g.KB = (int)((p.K + kBK - 1) / kBK);
+  g.d_f32 = p.d_f32, g.accumulate = p.accumulate;
+  const int64_t row_bytes = p.ldd * (p.d_f32 ? 4 : 2);
+  g.vec = aligned_rows_host(p.d, row_bytes, 32);
+  // 256-wide tiles while every SM still gets one, else 128-wide ones
+  const int64_t tm = (p.M + kBM - 1) / kBM;
+  const bool wide = tm * ((p.N + 255) / 256) >= device_sm_count();
+  const cudaError_t e =
+      wide ? (p.b_rows ? launch_tiled<256, true>(map_a, map_b, g, stream)
+                       : launch_tiled<256, false>(map_a, map_b, g, stream))
+           : (p.b_rows ? launch_tiled<128, true>(map_a, map_b, g, stream)
+                       : launch_tiled<128, false>(map_a, map_b, g, stream));
+  if (e != cudaSuccess) {
+    *why = cudaGetErrorString(e);
+    return CUTIE_ERR_CUDA;
+  }
+  return CUTIE_OK;
+}
+
+}  // namespace cutie

@@ -796,13 +796,108 @@ extern "C" int cutie_rms_norm_mxfp8_gemm(const void* x, int64_t ldx, const void*
   return CUTIE_OK;
 }
 
+extern "C" int cutie_cast_fp8_tiles(const void* x, int64_t ldx, int64_t M, int64_t H,
+                                    int tile_kind, int scale_fmt, void* q, int64_t ldq, void* s,
+                                    int64_t lds, void* qt, int64_t ldqt, void* st, int64_t ldst,
+                                    void* stream) {
+  g_err[0] = '\0';
+  if (M < 0 || H <= 0)
+    return fail(CUTIE_ERR_INVALID_ARGUMENT, "need M >= 0 and H > 0 (got M=%lld, H=%lld)",
+                (long long)M, (long long)H);
+  if (H % 8 != 0)
+    return fail(CUTIE_ERR_UNSUPPORTED, "H=%lld must be a multiple of 8 (16-byte rows)",
+                (long long)H);
+  if (H > INT32_MAX - 128)
+    return fail(CUTIE_ERR_UNSUPPORTED, "H must be below 2^31 - 128");
+  if (tile_kind != CUTIE_TILE_BLOCK && tile_kind != CUTIE_TILE_TWO_WAY)
+    return fail(CUTIE_ERR_INVALID_ARGUMENT, "unknown tile_kind %d", tile_kind);
+  if (scale_fmt != CUTIE_SCALE_FP32 && scale_fmt != CUTIE_SCALE_FP32_POW2)
+    return fail(CUTIE_ERR_UNSUPPORTED, "tile casts write fp32 scales (scale_fmt %d)", scale_fmt);
+  if ((qt == nullptr) != (st == nullptr))
+    return fail(CUTIE_ERR_INVALID_ARGUMENT, "qt and st must be given together");
+  const bool block = tile_kind == CUTIE_TILE_BLOCK;
+  if (M == 0) return CUTIE_OK;
+  if (!block && qt == nullptr)
+    return fail(CUTIE_ERR_INVALID_ARGUMENT, "the two-way cast needs qt and st");
+  const int64_t GM = (M + 127) / 128, GH = (H + 127) / 128;
+  if (GM > INT32_MAX / GH)
+    return fail(CUTIE_ERR_UNSUPPORTED, "M x H has more than 2^31 tiles");
+  int rc;
+  if ((rc = check_matrix("x", x, ldx, H, 16, 8)) != CUTIE_OK) return rc;
+  if ((rc = check_matrix("q", q, ldq, H, 8, 8)) != CUTIE_OK) return rc;
+  if ((rc = check_matrix("s", s, lds, block ? GH : M, 4, 1)) != CUTIE_OK) return rc;
+  if (qt != nullptr) {
+    if ((rc = check_matrix("qt", qt, ldqt, M, 8, 8)) != CUTIE_OK) return rc;
+    if ((rc = check_matrix("st", st, ldst, block ? GM : H, 4, 1)) != CUTIE_OK) return rc;
+  }
+  CastArgs a{};
+  a.x = static_cast<const uint16_t*>(x), a.ldx = ldx;
+  a.M = M, a.H = (int)H;
+  a.pow2 = scale_fmt == CUTIE_SCALE_FP32_POW2;
+  a.q = static_cast<uint8_t*>(q), a.ldq = ldq;
+  a.s = static_cast<float*>(s), a.lds = lds;
+  a.qt = static_cast<uint8_t*>(qt), a.ldqt = ldqt;
+  a.st = static_cast<float*>(st), a.ldst = ldst;
+  const cudaError_t e = launch_cast_tiles(a, block, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "tile cast launch");
+  return CUTIE_OK;
+}
+
+extern "C" int cutie_fp8_block_gemm(const void* a, int64_t lda, const void* a_scale,
+                                    int64_t sa_row, int64_t sa_kb, const void* b, int64_t ldb,
+                                    const void* b_scale, int64_t sb_row, int64_t sb_kb,
+                                    int b_rows, void* d, int64_t ldd, int d_dtype,
+                                    int accumulate, int64_t M, int64_t N, int64_t K,
+                                    void* stream) {
+  g_err[0] = '\0';
+  if (M < 0 || N < 0 || K < 0)
+    return fail(CUTIE_ERR_INVALID_ARGUMENT, "need M, N and K >= 0 (got %lld, %lld, %lld)",
+                (long long)M, (long long)N, (long long)K);
+  if (M > INT32_MAX - 256 || N > INT32_MAX - 256 || K > INT32_MAX - 256)
+    return fail(CUTIE_ERR_UNSUPPORTED, "M, N and K must be below 2^31 - 256");
+  if (d_dtype != CUTIE_DTYPE_BF16 && d_dtype != CUTIE_DTYPE_F32)
+    return fail(CUTIE_ERR_INVALID_ARGUMENT, "unknown d_dtype %d", d_dtype);
+  if (accumulate && d_dtype != CUTIE_DTYPE_F32)
+    return fail(CUTIE_ERR_UNSUPPORTED, "accumulation needs an fp32 output");
+  if (M == 0 || N == 0) return CUTIE_OK;
+  const int esize = d_dtype == CUTIE_DTYPE_F32 ? 4 : 2;
+  int rc;
+  if ((rc = check_matrix("d", d, ldd, N, esize, 1)) != CUTIE_OK) return rc;
+  if (K == 0) {
+    if (accumulate) return CUTIE_OK;
+    const cudaError_t e = cudaMemset2DAsync(d, (size_t)ldd * esize, 0, (size_t)N * esize, (size_t)M,
+                                            static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? CUTIE_OK : cuda_fail(e, "fp8 block gemm (K = 0)");
+  }
+  if ((rc = check_matrix("a", a, lda, K, 16, 16)) != CUTIE_OK) return rc;
+  if ((rc = check_matrix("b", b, ldb, K, 16, 16)) != CUTIE_OK) return rc;
+  if (a_scale == nullptr || b_scale == nullptr)
+    return fail(CUTIE_ERR_INVALID_ARGUMENT, "a_scale and b_scale must not be NULL");
+  if (!aligned(a_scale, 4) || !aligned(b_scale, 4))
+    return fail(CUTIE_ERR_ALIGNMENT, "fp32 scales must be 4-byte aligned");
+  if (sa_row < 0 || sa_kb < 0 || sb_row < 0 || sb_kb < 0)
+    return fail(CUTIE_ERR_INVALID_ARGUMENT, "scale strides must not be negative");
+  BlockGemmArgs g{};
+  g.a = a, g.lda = lda, g.sa = static_cast<const float*>(a_scale);
+  g.sa_row = sa_row, g.sa_kb = sa_kb;
+  g.b = b, g.ldb = ldb, g.sb = static_cast<const float*>(b_scale);
+  g.sb_row = sb_row, g.sb_kb = sb_kb;
+  g.b_rows = b_rows != 0;
+  g.d = d, g.ldd = ldd, g.d_f32 = esize == 4, g.accumulate = accumulate != 0;
+  g.M = M, g.N = N, g.K = K;
+  const char* why = "";
+  rc = block_gemm(g, static_cast<cudaStream_t>(stream), &why);
+  if (rc != CUTIE_OK) return fail(rc, "fp8 block gemm: %s", why);
+  return CUTIE_OK;
+}
+
 extern "C" int cutie_device_error(int clear) {
   g_err[0] = '\0';
   int any = 0;
   cudaError_t (*readers[])(int*, bool) = {device_error_none, device_error_token, device_error_g32,
                                           device_error_g64, device_error_g128,
                                           device_error_bwd,  device_error_gemm,
-                                          device_error_prologue};
+                                          device_error_prologue, device_error_block_gemm};
   for (auto read : readers) {
     int v = 0;
     const cudaError_t e = read(&v, clear != 0);

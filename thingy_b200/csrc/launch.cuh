@@ -311,6 +311,48 @@ cudaError_t device_error_prologue(int* out, bool clear);
 cudaError_t launch_backward(const BwdArgs& a, float eps, bool dw_wanted, uint16_t* dw,
                             int max_grid, cudaStream_t st);
 
+// Casts to e4m3 in both orientations (cast_tiles.cu).
+struct CastArgs {
+  const uint16_t* x;  // bf16 [M, H]
+  int64_t ldx;
+  int64_t M;
+  int H;
+  bool pow2;
+  uint8_t* q;   // [M, H] codes
+  int64_t ldq;
+  float* s;     // block: [M/128, H/128], else group-major [H/128, M]
+  int64_t lds;
+  uint8_t* qt;  // [H, M] codes of the transpose, or null (block only)
+  int64_t ldqt;
+  float* st;    // block: [H/128, M/128], else group-major [M/128, H]
+  int64_t ldst;
+};
+cudaError_t launch_cast_tiles(const CastArgs& a, bool block, cudaStream_t stream);
+
+// Block-scaled product (block_gemm.cu): D[M, N] = dequant(A) dequant(B)^T.
+struct BlockGemmArgs {
+  const void* a;  // e4m3 [M, K], 1 x 128 scales sa (element strides sa_row, sa_kb)
+  int64_t lda;
+  const float* sa;
+  int64_t sa_row, sa_kb;
+  const void* b;  // e4m3 [N, K], scales sb a 128 x 128 block or a row and 128 columns
+  int64_t ldb;
+  const float* sb;
+  int64_t sb_row, sb_kb;
+  bool b_rows;    // sb has a scale a row, not a block of 128 rows
+  void* d;        // bf16 or fp32 [M, N]
+  int64_t ldd;
+  bool d_f32;
+  bool accumulate;  // fp32 only: D += instead of D =
+  int64_t M, N, K;
+};
+// Rows of `p`, ld_bytes apart, all start on n-byte boundaries.
+inline bool aligned_rows_host(const void* p, int64_t ld_bytes, unsigned n) {
+  return ((reinterpret_cast<uint64_t>(p) | (uint64_t)ld_bytes) & (n - 1u)) == 0;
+}
+int block_gemm(const BlockGemmArgs& g, cudaStream_t stream, const char** why);
+cudaError_t device_error_block_gemm(int* out, bool clear);
+
 struct F32Args {
   const float* x;
   int64_t ldx;

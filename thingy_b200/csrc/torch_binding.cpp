@@ -164,6 +164,113 @@ void rms_norm(const at::Tensor& x, const at::Tensor& weight, double eps, const a
                               out.data_ptr(), ldo, (int)threads_per_row, stream));
 }
 
+// Leading dimension of a matrix whose rows are contiguous and do not overlap.
+int64_t matrix_ld(const at::Tensor& t, const char* name, const at::Device& dev) {
+  if (t.dim() != 2) bad(std::string(name) + " must be 2-D");
+  if (t.device() != dev) bad(std::string(name) + " is on the wrong device");
+  const int64_t R = t.size(0), C = t.size(1);
+  if (C > 1 && t.stride(1) != 1) bad(std::string(name) + " must be contiguous along its last dimension");
+  if (R <= 1) return std::max<int64_t>(C, (C + 15) / 16 * 16);
+  if (t.stride(0) < C) bad(std::string(name) + " must not have overlapping rows");
+  return t.stride(0);
+}
+
+void check_codes(const at::Tensor& t, const char* name) {
+  if (t.scalar_type() != at::kFloat8_e4m3fn && t.scalar_type() != at::kByte)
+    bad(std::string(name) + " must be float8_e4m3fn");
+}
+
+int64_t ceil_to(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
+
+// e4m3 [R, C] with rows on 16-byte boundaries (what the block-scaled GEMM takes).
+at::Tensor empty_codes(int64_t R, int64_t C, const at::Device& dev) {
+  const auto opt = at::TensorOptions().device(dev).dtype(at::kFloat8_e4m3fn);
+  const int64_t ld = ceil_to(C, 16);
+  at::Tensor t = at::empty({R, ld}, opt);
+  return ld == C ? t : t.narrow(1, 0, C);
+}
+
+// Casts to e4m3 in both orientations (cutie_cast_fp8_tiles); qt and st are
+// undefined tensors unless `transposed`.
+std::tuple<at::Tensor, at::Tensor, c10::optional<at::Tensor>, c10::optional<at::Tensor>>
+cast_fp8_tiles(const at::Tensor& x, bool block, bool use_ue8m0, bool transposed) {
+  if (x.dim() != 2) bad("x must be 2-D [M, H]");
+  if (!x.is_cuda()) bad("x must be a CUDA tensor (this library has no CPU path)");
+  if (x.scalar_type() != at::kBFloat16) bad("x must be bfloat16");
+  const int64_t M = x.size(0), H = x.size(1);
+  const at::Device dev = x.device();
+  const int64_t ldx = M <= 1 ? ceil_to(H, 8) : matrix_ld(x, "x", dev);
+  if (H > 1 && x.stride(1) != 1) bad("x must be contiguous along its last dimension");
+  const int64_t GM = (M + 127) / 128, GH = (H + 127) / 128;
+  const auto f32 = at::TensorOptions().device(dev).dtype(at::kFloat);
+  at::Tensor q = empty_codes(M, H, dev);
+  at::Tensor s = block ? at::empty({GM, GH}, f32) : at::empty({GH, M}, f32);
+  at::Tensor qt, st;
+  if (transposed) {
+    qt = empty_codes(H, M, dev);
+    st = block ? at::empty({GH, GM}, f32) : at::empty({GM, H}, f32);
+  }
+  const c10::cuda::CUDAGuard guard(dev);
+  void* stream = at::cuda::getCurrentCUDAStream(dev.index()).stream();
+  check_status(cutie_cast_fp8_tiles(
+      x.data_ptr(), ldx, M, H, block ? CUTIE_TILE_BLOCK : CUTIE_TILE_TWO_WAY,
+      use_ue8m0 ? CUTIE_SCALE_FP32_POW2 : CUTIE_SCALE_FP32, q.data_ptr(), ceil_to(H, 16),
+      s.data_ptr(), block ? GH : M, transposed ? qt.data_ptr() : nullptr,
+      transposed ? ceil_to(M, 16) : 0, transposed ? st.data_ptr() : nullptr,
+      transposed ? (block ? GM : H) : 0, stream));
+  c10::optional<at::Tensor> oqt, ost;
+  if (transposed) oqt = qt, ost = block ? st : st.t();
+  return {q, block ? s : s.t(), oqt, ost};
+}
+
+// D = dequant(a) dequant(b)^T (cutie_fp8_block_gemm) into `out`, or a new tensor.
+at::Tensor fp8_block_gemm(const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor& b,
+                          const at::Tensor& b_scale, const c10::optional<at::Tensor>& out,
+                          bool out_f32, bool accumulate) {
+  if (!a.is_cuda()) bad("a must be a CUDA tensor (this library has no CPU path)");
+  const at::Device dev = a.device();
+  check_codes(a, "a");
+  check_codes(b, "b");
+  const int64_t lda = matrix_ld(a, "a", dev), ldb = matrix_ld(b, "b", dev);
+  const int64_t M = a.size(0), K = a.size(1), N = b.size(0), KB = (K + 127) / 128;
+  if (b.size(1) != K) bad("a and b must have the same number of columns");
+  for (const auto* s : {&a_scale, &b_scale}) {
+    if (s->dim() != 2 || s->scalar_type() != at::kFloat) bad("scales must be 2-D float32 tensors");
+    if (s->device() != dev) bad("scales must be on a's device");
+  }
+  if (a_scale.size(0) != M || a_scale.size(1) != KB)
+    bad("a_scale must have shape [M, ceil(K/128)] = (" + std::to_string(M) + ", " +
+        std::to_string(KB) + ")");
+  const int64_t sb_rows = b_scale.size(0);
+  if ((sb_rows != (N + 127) / 128 && sb_rows != N) || b_scale.size(1) != KB)
+    bad("b_scale must have shape [ceil(N/128), ceil(K/128)] (128 x 128 blocks) or [N, ceil(K/128)]"
+        " (1 x 128 groups)");
+  if (out.has_value()) {
+    if (out->dim() != 2 || out->size(0) != M || out->size(1) != N)
+      bad("out must have shape (" + std::to_string(M) + ", " + std::to_string(N) + ")");
+    if (out->scalar_type() != at::kBFloat16 && out->scalar_type() != at::kFloat)
+      bad("out must be bfloat16 or float32");
+    out_f32 = out->scalar_type() == at::kFloat;
+  } else if (accumulate) {
+    bad("accumulate needs out");
+  }
+  const c10::cuda::CUDAGuard guard(dev);
+  at::Tensor d = out.has_value()
+                     ? *out
+                     : at::empty({M, N}, at::TensorOptions().device(dev).dtype(
+                                             out_f32 ? at::kFloat : at::kBFloat16));
+  const int64_t ldd = M <= 1 ? N : matrix_ld(d, "out", dev);
+  if (N > 1 && d.stride(1) != 1) bad("out must be contiguous along its last dimension");
+  if (d.device() != dev) bad("out is on the wrong device");
+  void* stream = at::cuda::getCurrentCUDAStream(dev.index()).stream();
+  check_status(cutie_fp8_block_gemm(
+      a.data_ptr(), lda, a_scale.data_ptr(), a_scale.stride(0), a_scale.stride(1), b.data_ptr(),
+      ldb, b_scale.data_ptr(), b_scale.stride(0), b_scale.stride(1),
+      sb_rows == N && sb_rows != (N + 127) / 128 ? 1 : 0, d.data_ptr(), ldd,
+      out_f32 ? CUTIE_DTYPE_F32 : CUTIE_DTYPE_BF16, accumulate ? 1 : 0, M, N, K, stream));
+  return d;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -174,5 +281,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("scale_layout"), py::arg("threads_per_row"), py::arg("normalize"));
   m.def("rms_norm", &rms_norm, py::arg("x"), py::arg("weight"), py::arg("eps"), py::arg("out"),
         py::arg("threads_per_row"));
+  m.def("cast_fp8_tiles", &cast_fp8_tiles, py::arg("x"), py::arg("block"), py::arg("use_ue8m0"),
+        py::arg("transposed"));
+  m.def("fp8_block_gemm", &fp8_block_gemm, py::arg("a"), py::arg("a_scale"), py::arg("b"),
+        py::arg("b_scale"), py::arg("out"), py::arg("out_f32"), py::arg("accumulate"));
   m.def("abi_version", []() { return cutie_abi_version(); });
 }

@@ -9,6 +9,10 @@ hand-written tcgen05 kernel), fp32 accumulation, bf16 out:
 ``D = dequant(a) @ dequant(b).T``. The reference has no GEMM on this path
 (src/cutie/rms_norm/bench.py stops before it); this is the consumer its
 quantizer feeds.
+
+``fp8_block_gemm(a, a_scale, b, b_scale)`` is the product for the path's
+headline form, 1 x 128 groups with fp32 scales, against a weight in 128 x 128
+blocks (or, for weight gradients, another operand in 1 x 128 groups).
 """
 
 from __future__ import annotations
@@ -17,7 +21,7 @@ import torch
 
 from . import _lib
 from .layouts import mx_swizzled_size
-from .ops import E8M0_DTYPES, FP8_DTYPE
+from .ops import E8M0_DTYPES, FP8_DTYPE, require_binding
 
 
 def _operand(name: str, t: torch.Tensor, K: int) -> int:
@@ -150,3 +154,22 @@ def rms_norm_mxfp8_gemm(x: torch.Tensor, weight: torch.Tensor, eps: float, b: to
             torch.cuda.current_stream(x.device).cuda_stream)
     _lib.check(status)
     return out
+
+
+def fp8_block_gemm(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor,
+                   out: torch.Tensor | None = None, out_dtype: torch.dtype = torch.bfloat16,
+                   accumulate: bool = False) -> torch.Tensor:
+    """[M, N] = (a * a_scale) @ (b * b_scale).T with a scale for each 128 columns, on the current stream.
+
+    a: e4m3 [M, K], a_scale: fp32 [M, ceil(K/128)] in any layout (what
+    ``rms_norm_fp8(..., group_size=128)`` and the casts of ``fp8_utils``
+    return); b: e4m3 [N, K], b_scale: fp32 [ceil(N/128), ceil(K/128)]
+    (``per_block_cast_to_fp8``) or [N, ceil(K/128)] (1 x 128 groups). M, N and
+    K are any sizes; the rows of a and b start on 16-byte boundaries. out (or
+    out_dtype) is bfloat16 or float32; ``accumulate`` adds the product to an
+    fp32 ``out`` (gradient accumulation). Sums are held in fp32, rounded once.
+    """
+    if out_dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"out_dtype must be bfloat16 or float32, got {out_dtype}")
+    return require_binding().fp8_block_gemm(a, a_scale, b, b_scale, out,
+                                            out_dtype == torch.float32, bool(accumulate))

@@ -35,6 +35,16 @@ def _binding():
             mod = None
         _binding_mod = mod
     return _binding_mod
+
+
+def require_binding():
+    """The torch binding; raises if it was not built (ops that have no ctypes path)."""
+    mod = _binding()
+    if mod is None:
+        raise RuntimeError("thingy_b200 torch binding not built (run `python -m thingy_b200.build`)")
+    return mod
+
+
 from .layouts import SCALE_FORMATS, SCALE_LAYOUTS, mx_swizzled_size, n_groups
 
 _FMT_CODE = {"fp32": _lib.SCALE_FP32, "ue8m0": _lib.SCALE_FP32_POW2, "e8m0": _lib.SCALE_E8M0}
