@@ -324,6 +324,48 @@ CUTIE_API int cutie_fp8_block_gemm(const void* a, int64_t lda, const void* a_sca
                                    int64_t M, int64_t N, int64_t K, void* stream);
 
 /*
+ * A whole mixture-of-experts layer for few tokens in one kernel:
+ *   logits = x router^T (fp32 sums of bf16 products); scores = softmax or
+ *   sigmoid of the logits; each token takes the top_k experts of the largest
+ *   logits (with a bias: of the largest score + bias), ties to the lowest
+ *   index; weights w = the chosen scores, divided by their sum if
+ *   renormalize, times routed_scale
+ *   g, u = dequant(q) dequant(w13[e])^T; h = silu(g) u (fp32);
+ *   (qh, sh) = the 1 x 128 cast of h: s = max(amax / 448, 1e-4), e4m3(h / s)
+ *   out[t] = bf16( sum_j w[t, j] dequant(qh) dequant(w2[e_j])^T )
+ * x: bf16 [T, H] (ldx), the router's input; q: e4m3 [T, H] (ldq bytes) with
+ * fp32 scales of 1 x 128 groups, element (t, g) at t * sq_row + g * sq_kb: x
+ * quantized, as cutie_rms_norm_fp8 writes both (normalized_out, q and scale).
+ * router: bf16 [E, H]; bias: fp32 [E] or NULL. w13: e4m3 [E, 2 I, H], rows
+ * 0..I-1 of an expert its gate, I..2I-1 its up projection, w2: e4m3
+ * [E, H, I]; w13_scale [E, 2 I / 128, H / 128] and w2_scale [E, H / 128,
+ * I / 128]: fp32, 128 x 128 blocks, all contiguous (cutie_cast_fp8_tiles).
+ * out: bf16 [T, H] (ldo). topk_ids (int32) and topk_weights (fp32), [T,
+ * top_k], receive the choices; either may be NULL.
+ * 0 <= T <= 64, 1 <= E <= 512, 1 <= top_k <= min(E, 16), H and I multiples
+ * of 128; rows of x, out 16-byte, of q 16-byte aligned.
+ * workspace: cutie_moe_fp8_workspace(T, E, top_k, H, I) bytes of device
+ * memory, 256-byte aligned, whose first 8 bytes are zero before its first
+ * use; the kernel leaves them ready for the next call, of any sizes, on the
+ * same device. Calls that may overlap on the GPU need workspaces of their
+ * own. The kernel is a cooperative launch over the whole device. Asynchronous
+ * on `stream`; nothing is allocated.
+ */
+enum cutie_moe_scoring {
+  CUTIE_SCORE_SOFTMAX = 0,
+  CUTIE_SCORE_SIGMOID = 1,
+};
+CUTIE_API size_t cutie_moe_fp8_workspace(int64_t T, int64_t E, int64_t top_k, int64_t H, int64_t I);
+CUTIE_API int cutie_moe_fp8(const void* x, int64_t ldx, const void* q, int64_t ldq,
+                            const void* q_scale, int64_t sq_row, int64_t sq_kb,
+                            const void* router, const void* bias, const void* w13,
+                            const void* w13_scale, const void* w2, const void* w2_scale,
+                            int64_t T, int64_t E, int64_t top_k, int64_t H, int64_t I,
+                            int scoring, int renormalize, float routed_scale, void* out,
+                            int64_t ldo, void* topk_ids, void* topk_weights, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
+/*
  * Device-side status of this library's kernels on the current device: 0 when
  * no kernel has hit a failure since the last clear; otherwise the first error
  * code recorded (1 = a bulk-copy wait ran out: a row never arrived in shared

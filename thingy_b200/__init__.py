@@ -18,6 +18,8 @@ Drop-in host API for the reference's hot path (S1ro1/thingy, package
                                                weight and two-way casts, the product with a
                                                scale a block of 128, a linear layer with its
                                                gradients
+    moe_fp8, quantize_experts               a mixture-of-experts layer for few tokens in one
+                                               kernel (no counterpart)
 
 Every op runs hand-written CUDA from ``lib/libcutie_b200.so`` through the C
 ABI in ``include/cutie.h``; there is no CPU or PyTorch fallback.
@@ -30,6 +32,7 @@ from .fused import empty_scale, residual_rms_norm_fp8, rms_norm_fp8
 from .gemm import fp8_block_gemm
 from .layouts import mx_swizzle, mx_swizzle_offset, mx_swizzled_size, mx_unswizzle
 from .linear import FP8Linear, fp8_linear
+from .moe import moe_fp8, moe_workspace, quantize_experts
 from .rms_norm import RMSNorm, rms_norm, rms_norm_on_stream
 
 __all__ = [
@@ -39,6 +42,8 @@ __all__ = [
     "empty_scale",
     "fp8_block_gemm",
     "fp8_linear",
+    "moe_fp8",
+    "moe_workspace",
     "mx_swizzle",
     "mx_swizzle_offset",
     "mx_swizzled_size",
@@ -46,6 +51,7 @@ __all__ = [
     "per_block_cast_to_fp8",
     "per_token_cast_to_fp8",
     "per_token_cast_to_fp8_triton",
+    "quantize_experts",
     "residual_rms_norm_fp8",
     "rms_norm",
     "rms_norm_fp8",

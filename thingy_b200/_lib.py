@@ -26,6 +26,7 @@ SCALE_FP32, SCALE_FP32_POW2, SCALE_E8M0 = 0, 1, 2
 LAYOUT_ROW_MAJOR, LAYOUT_COL_MAJOR, LAYOUT_MX_SWIZZLED, LAYOUT_COL_MAJOR_PACKED = 0, 1, 2, 3
 DTYPE_BF16, DTYPE_F32 = 0, 1
 TILE_BLOCK, TILE_TWO_WAY = 0, 1
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 
 ABI_VERSION = 1
 
@@ -40,6 +41,8 @@ EXPORTED_SYMBOLS = (
     "cutie_rms_norm_mxfp8_gemm",
     "cutie_cast_fp8_tiles",
     "cutie_fp8_block_gemm",
+    "cutie_moe_fp8",
+    "cutie_moe_fp8_workspace",
     "cutie_device_error",
     "cutie_set_wait_limit",
     "cutie_last_error",
@@ -92,6 +95,13 @@ _SIGNATURES = {
         _int,
         [_ptr, _i64, _ptr, _i64, _i64, _ptr, _i64, _ptr, _i64, _i64, _int, _ptr, _i64, _int, _int,
          _i64, _i64, _i64, _ptr],
+    ),
+    "cutie_moe_fp8_workspace": (ctypes.c_size_t, [_i64, _i64, _i64, _i64, _i64]),
+    "cutie_moe_fp8": (
+        _int,
+        [_ptr, _i64, _ptr, _i64, _ptr, _i64, _i64, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr,
+         _i64, _i64, _i64, _i64, _i64, _int, _int, _f32, _ptr, _i64, _ptr, _ptr, _ptr,
+         ctypes.c_size_t, _ptr],
     ),
     "cutie_device_error": (_int, [_int]),
     "cutie_set_wait_limit": (_i64, [_i64]),

@@ -891,13 +891,103 @@ extern "C" int cutie_fp8_block_gemm(const void* a, int64_t lda, const void* a_sc
   return CUTIE_OK;
 }
 
+namespace cutie {
+namespace {
+
+int check_moe_sizes(int64_t T, int64_t E, int64_t k, int64_t H, int64_t I) {
+  if (T < 0 || E <= 0 || k <= 0 || H <= 0 || I <= 0)
+    return fail(CUTIE_ERR_INVALID_ARGUMENT,
+                "need T >= 0 and E, top_k, H, I > 0 (got %lld, %lld, %lld, %lld, %lld)",
+                (long long)T, (long long)E, (long long)k, (long long)H, (long long)I);
+  if (T > kMoeMaxTokens)
+    return fail(CUTIE_ERR_UNSUPPORTED, "the few-token layer takes at most %d tokens (got %lld)",
+                kMoeMaxTokens, (long long)T);
+  if (E > kMoeMaxExperts)
+    return fail(CUTIE_ERR_UNSUPPORTED, "at most %d experts (got %lld)", kMoeMaxExperts,
+                (long long)E);
+  if (k > E || k > kMoeMaxTopK)
+    return fail(CUTIE_ERR_UNSUPPORTED, "top_k must be at most E and %d (got %lld of %lld)",
+                kMoeMaxTopK, (long long)k, (long long)E);
+  if (H % 128 != 0 || I % 128 != 0)
+    return fail(CUTIE_ERR_UNSUPPORTED, "H and I must be multiples of 128 (got %lld, %lld)",
+                (long long)H, (long long)I);
+  // rows of the weights and units of work stay below 2^31
+  if (H > (1 << 20) || I > (1 << 20) || E * 2 * I > INT32_MAX / 2 || E * H > INT32_MAX / 2 ||
+      E * (I / 128) * (H / 128) > INT32_MAX / 2)
+    return fail(CUTIE_ERR_UNSUPPORTED, "the experts' weights are too large (E=%lld, H=%lld, I=%lld)",
+                (long long)E, (long long)H, (long long)I);
+  return CUTIE_OK;
+}
+
+}  // namespace
+}  // namespace cutie
+
+extern "C" size_t cutie_moe_fp8_workspace(int64_t T, int64_t E, int64_t top_k, int64_t H,
+                                          int64_t I) {
+  g_err[0] = '\0';
+  if (check_moe_sizes(T, E, top_k, H, I) != CUTIE_OK) return 0;
+  MoeArgs g{};
+  g.T = (int)(T > 0 ? T : 1), g.E = (int)E, g.k = (int)top_k, g.H = (int)H, g.I = (int)I;
+  return moe_workspace(&g, nullptr);
+}
+
+extern "C" int cutie_moe_fp8(const void* x, int64_t ldx, const void* q, int64_t ldq,
+                             const void* q_scale, int64_t sq_row, int64_t sq_kb,
+                             const void* router, const void* bias, const void* w13,
+                             const void* w13_scale, const void* w2, const void* w2_scale,
+                             int64_t T, int64_t E, int64_t top_k, int64_t H, int64_t I,
+                             int scoring, int renormalize, float routed_scale, void* out,
+                             int64_t ldo, void* topk_ids, void* topk_weights, void* workspace,
+                             size_t workspace_bytes, void* stream) {
+  g_err[0] = '\0';
+  int rc;
+  if ((rc = check_moe_sizes(T, E, top_k, H, I)) != CUTIE_OK) return rc;
+  if (scoring != CUTIE_SCORE_SOFTMAX && scoring != CUTIE_SCORE_SIGMOID)
+    return fail(CUTIE_ERR_INVALID_ARGUMENT, "unknown scoring %d", scoring);
+  if (T == 0) return CUTIE_OK;
+  if ((rc = check_matrix("x", x, ldx, H, 16, 8)) != CUTIE_OK) return rc;
+  if ((rc = check_matrix("q", q, ldq, H, 16, 16)) != CUTIE_OK) return rc;
+  if ((rc = check_matrix("out", out, ldo, H, 16, 8)) != CUTIE_OK) return rc;
+  if ((rc = check_matrix("router", router, H, H, 16, 8)) != CUTIE_OK) return rc;
+  if ((rc = check_matrix("w13", w13, H, H, 16, 16)) != CUTIE_OK) return rc;
+  if ((rc = check_matrix("w2", w2, I, I, 16, 16)) != CUTIE_OK) return rc;
+  if (q_scale == nullptr || w13_scale == nullptr || w2_scale == nullptr)
+    return fail(CUTIE_ERR_INVALID_ARGUMENT, "q_scale, w13_scale and w2_scale must not be NULL");
+  if (!aligned(q_scale, 4) || !aligned(w13_scale, 4) || !aligned(w2_scale, 4) ||
+      !aligned(bias, 4) || !aligned(topk_ids, 4) || !aligned(topk_weights, 4))
+    return fail(CUTIE_ERR_ALIGNMENT, "scales, bias and choices must be 4-byte aligned");
+  if (sq_row < 0 || sq_kb < 0)
+    return fail(CUTIE_ERR_INVALID_ARGUMENT, "scale strides must not be negative");
+  MoeArgs g{};
+  g.x = static_cast<const uint16_t*>(x), g.ldx = ldx;
+  g.q_scale = static_cast<const float*>(q_scale), g.sq_row = sq_row, g.sq_kb = sq_kb;
+  g.router = static_cast<const uint16_t*>(router);
+  g.bias = static_cast<const float*>(bias);
+  g.w13_scale = static_cast<const float*>(w13_scale);
+  g.w2_scale = static_cast<const float*>(w2_scale);
+  g.T = (int)T, g.E = (int)E, g.k = (int)top_k, g.H = (int)H, g.I = (int)I;
+  g.scoring = scoring, g.renormalize = renormalize != 0, g.routed_scale = routed_scale;
+  g.out = static_cast<uint16_t*>(out), g.ldo = ldo;
+  g.ids = static_cast<int*>(topk_ids), g.weights = static_cast<float*>(topk_weights);
+  const size_t need = moe_workspace(&g, workspace);
+  if (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 256))
+    return fail(CUTIE_ERR_INVALID_ARGUMENT,
+                "the layer needs a 256-byte aligned workspace of %zu bytes (got %zu at %p)", need,
+                workspace_bytes, workspace);
+  const char* why = "";
+  rc = moe_fp8(g, q, ldq, w13, w2, static_cast<cudaStream_t>(stream), &why);
+  if (rc != CUTIE_OK) return fail(rc, "moe layer: %s", why);
+  return CUTIE_OK;
+}
+
 extern "C" int cutie_device_error(int clear) {
   g_err[0] = '\0';
   int any = 0;
   cudaError_t (*readers[])(int*, bool) = {device_error_none, device_error_token, device_error_g32,
                                           device_error_g64, device_error_g128,
                                           device_error_bwd,  device_error_gemm,
-                                          device_error_prologue, device_error_block_gemm};
+                                          device_error_prologue, device_error_block_gemm,
+                                          device_error_moe};
   for (auto read : readers) {
     int v = 0;
     const cudaError_t e = read(&v, clear != 0);

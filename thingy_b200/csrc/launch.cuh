@@ -353,6 +353,43 @@ inline bool aligned_rows_host(const void* p, int64_t ld_bytes, unsigned n) {
 int block_gemm(const BlockGemmArgs& g, cudaStream_t stream, const char** why);
 cudaError_t device_error_block_gemm(int* out, bool clear);
 
+// Mixture-of-experts layer for few tokens (moe.cu).
+constexpr int kMoeMaxTokens = 64, kMoeMaxExperts = 512, kMoeMaxTopK = 16;
+struct MoeArgs {
+  const uint16_t* x;  // bf16 [T, H]: the router's input
+  int64_t ldx;
+  const float* q_scale;  // scales of x's codes, element strides sq_row, sq_kb
+  int64_t sq_row, sq_kb;
+  const uint16_t* router;  // bf16 [E, H]
+  const float* bias;       // fp32 [E] added to the scores for the choice, or null
+  const float* w13_scale;  // [E, 2 I/128, H/128]
+  const float* w2_scale;   // [E, H/128, I/128]
+  int T, E, k, H, I;
+  int scoring;  // 0 softmax, 1 sigmoid
+  bool renormalize;
+  float routed_scale;
+  uint16_t* out;  // bf16 [T, H]
+  int64_t ldo;
+  int* ids;        // [T, k] chosen experts and their weights: the caller's, or in the workspace
+  float* weights;
+  // workspace
+  uint64_t* barrier;
+  int* counters;  // arrivals at split items: n_counters1 of the first product, then the second's
+  int n_counters, n_counters1;
+  float* logits;  // [splits, T, E]
+  int splits;
+  bool deal_tokens;
+  uint8_t* hidden;  // [T k, I] codes of the hidden rows and their scales
+  float* h_scale;
+  float* down;     // [T k, H] down products
+  float* partial;  // [SMs, 2, columns, 256] sums of split items
+};
+// Bytes of workspace; fills g's workspace fields from `base` (may be null).
+size_t moe_workspace(MoeArgs* g, void* base);
+int moe_fp8(MoeArgs g, const void* q, int64_t ldq, const void* w13, const void* w2,
+            cudaStream_t stream, const char** why);
+cudaError_t device_error_moe(int* out, bool clear);
+
 struct F32Args {
   const float* x;
   int64_t ldx;

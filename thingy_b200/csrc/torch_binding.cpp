@@ -271,6 +271,80 @@ at::Tensor fp8_block_gemm(const at::Tensor& a, const at::Tensor& a_scale, const 
   return d;
 }
 
+// Bytes of workspace of a mixture-of-experts layer; argument errors raise.
+int64_t moe_workspace_bytes(int64_t T, int64_t E, int64_t top_k, int64_t H, int64_t I) {
+  const size_t n = cutie_moe_fp8_workspace(T, E, top_k, H, I);
+  if (n == 0) bad(cutie_last_error());
+  return (int64_t)n;
+}
+
+void weight_3d(const at::Tensor& t, const char* name, int64_t E, int64_t R, int64_t C,
+               const at::Device& dev) {
+  if (t.dim() != 3 || t.size(0) != E || t.size(1) != R || t.size(2) != C)
+    bad(std::string(name) + " must have shape (" + std::to_string(E) + ", " + std::to_string(R) +
+        ", " + std::to_string(C) + ")");
+  if (t.device() != dev) bad(std::string(name) + " is on the wrong device");
+  if (!t.is_contiguous()) bad(std::string(name) + " must be contiguous");
+}
+
+// Mixture-of-experts layer for few tokens (cutie_moe_fp8).
+at::Tensor moe_fp8(const at::Tensor& x, const at::Tensor& q, const at::Tensor& q_scale,
+                   const at::Tensor& router, const c10::optional<at::Tensor>& bias,
+                   const at::Tensor& w13, const at::Tensor& w13_scale, const at::Tensor& w2,
+                   const at::Tensor& w2_scale, int64_t top_k, int64_t scoring, bool renormalize,
+                   double routed_scale, const c10::optional<at::Tensor>& out,
+                   const c10::optional<at::Tensor>& topk_ids,
+                   const c10::optional<at::Tensor>& topk_weights, const at::Tensor& workspace) {
+  if (!x.is_cuda()) bad("x must be a CUDA tensor (this library has no CPU path)");
+  const at::Device dev = x.device();
+  if (x.dim() != 2 || x.scalar_type() != at::kBFloat16) bad("x must be a 2-D bfloat16 tensor");
+  const int64_t T = x.size(0), H = x.size(1);
+  if (router.dim() != 2 || router.size(1) != H || router.scalar_type() != at::kBFloat16 ||
+      router.device() != dev || !router.is_contiguous())
+    bad("router must be a contiguous bfloat16 [E, H] tensor on x's device");
+  const int64_t E = router.size(0);
+  if (w2.dim() != 3) bad("w2 must be 3-D [E, H, I]");
+  const int64_t I = w2.size(2), KB = (H + 127) / 128, IB = (I + 127) / 128;
+  check_codes(q, "q");
+  check_codes(w13, "w13");
+  check_codes(w2, "w2");
+  if (q.dim() != 2 || q.size(0) != T || q.size(1) != H) bad("q must have x's shape");
+  weight_3d(w13, "w13", E, 2 * I, H, dev);
+  weight_3d(w2, "w2", E, H, I, dev);
+  weight_3d(w13_scale, "w13_scale", E, 2 * IB, KB, dev);
+  weight_3d(w2_scale, "w2_scale", E, KB, IB, dev);
+  if (q_scale.dim() != 2 || q_scale.size(0) != T || q_scale.size(1) != KB || q_scale.device() != dev)
+    bad("scale must be a [T, H/128] tensor on x's device");
+  for (const auto* s : {&q_scale, &w13_scale, &w2_scale})
+    if (s->scalar_type() != at::kFloat) bad("scales must be float32");
+  if (bias.has_value() && (bias->dim() != 1 || bias->size(0) != E || bias->device() != dev ||
+                           bias->scalar_type() != at::kFloat || !bias->is_contiguous()))
+    bad("bias must be a contiguous float32 [E] tensor on x's device");
+  auto choice = [&](const c10::optional<at::Tensor>& t, const char* name, at::ScalarType dtype) {
+    if (t.has_value() && (t->dim() != 2 || t->size(0) != T || t->size(1) != top_k ||
+                          t->scalar_type() != dtype || t->device() != dev || !t->is_contiguous()))
+      bad(std::string(name) + " must be a contiguous [T, top_k] tensor on x's device");
+  };
+  choice(topk_ids, "topk_ids", at::kInt);
+  choice(topk_weights, "topk_weights", at::kFloat);
+  if (workspace.device() != dev || !workspace.is_contiguous())
+    bad("workspace must be a contiguous tensor on x's device");
+  const c10::cuda::CUDAGuard guard(dev);
+  at::Tensor y = out.has_value() ? *out : at::empty({T, H}, x.options());
+  if (y.dim() != 2 || y.size(0) != T || y.size(1) != H || y.scalar_type() != at::kBFloat16)
+    bad("out must be a bfloat16 tensor of x's shape");
+  void* stream = at::cuda::getCurrentCUDAStream(dev.index()).stream();
+  check_status(cutie_moe_fp8(
+      x.data_ptr(), matrix_ld(x, "x", dev), q.data_ptr(), matrix_ld(q, "q", dev),
+      q_scale.data_ptr(), q_scale.stride(0), q_scale.stride(1), router.data_ptr(),
+      ptr_or_null(bias), w13.data_ptr(), w13_scale.data_ptr(), w2.data_ptr(), w2_scale.data_ptr(),
+      T, E, top_k, H, I, (int)scoring, renormalize ? 1 : 0, (float)routed_scale, y.data_ptr(),
+      matrix_ld(y, "out", dev), const_cast<void*>(ptr_or_null(topk_ids)),
+      const_cast<void*>(ptr_or_null(topk_weights)), workspace.data_ptr(),
+      (size_t)(workspace.numel() * workspace.element_size()), stream));
+  return y;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -285,5 +359,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("transposed"));
   m.def("fp8_block_gemm", &fp8_block_gemm, py::arg("a"), py::arg("a_scale"), py::arg("b"),
         py::arg("b_scale"), py::arg("out"), py::arg("out_f32"), py::arg("accumulate"));
+  m.def("moe_workspace_bytes", &moe_workspace_bytes, py::arg("T"), py::arg("E"), py::arg("top_k"),
+        py::arg("H"), py::arg("I"));
+  m.def("moe_fp8", &moe_fp8, py::arg("x"), py::arg("q"), py::arg("scale"), py::arg("router"),
+        py::arg("bias"), py::arg("w13"), py::arg("w13_scale"), py::arg("w2"), py::arg("w2_scale"),
+        py::arg("top_k"), py::arg("scoring"), py::arg("renormalize"), py::arg("routed_scale"),
+        py::arg("out"), py::arg("topk_ids"), py::arg("topk_weights"), py::arg("workspace"));
   m.def("abi_version", []() { return cutie_abi_version(); });
 }
