@@ -48,26 +48,47 @@ constexpr uint32_t kBox = 128 * 128;  // a 128-row weight tile of one K block
 constexpr int kBufs = 4;              // accumulator buffers in tensor memory
 constexpr int kXStride = 132;         // floats between columns of the exchange
 constexpr int kMaxE = kMoeMaxExperts, kMaxK = kMoeMaxTopK;
+constexpr int kChooseTokens = 8;  // tokens up to which every CTA makes all choices
 
 template <int NMAX>
 struct MoePlan {
   static constexpr uint32_t kStageBytes = 2 * kBox + NMAX * 128;
   static constexpr int kStages = NMAX == 16 ? 6 : NMAX == 32 ? 5 : 4;
-  static constexpr uint32_t kXBytes = NMAX * kXStride * 4;
+  static constexpr int kXCols = NMAX == 16 ? 8 : NMAX == 32 ? 16 : 32;  // columns an exchange pass
+  static constexpr uint32_t kXBytes = 2 * kXCols * kXStride * 4;
   static constexpr size_t kSmemBytes = kStages * kStageBytes + kXBytes + 1024;
   static constexpr uint32_t kTmemCols = kBufs * 2 * NMAX;
   static constexpr int kPairs = NMAX * kMaxK;
   static_assert(kStageBytes % 1024 == 0, "swizzled tiles start on 1 KB");
+  static_assert(2 * kChooseTokens * kMaxE * 4 <= kStages * kStageBytes, "logits and keys fit the idle ring");
 };
 
-// Units of a phase dealt in runs of `per`; KB units an item.
+// Units of a phase dealt in runs of `per`; KB units an item, `groups` items an expert.
 struct Deal {
-  int per, units, KB;
-  __device__ Deal(int items, int kb) : units(items * kb), KB(kb) {
+  int per, units, KB, groups;
+  __device__ __forceinline__ void set(int experts, int groups_, int kb) {
+    KB = kb, groups = groups_, units = experts * groups_ * kb;
     per = (units + (int)gridDim.x - 1) / (int)gridDim.x;
   }
-  __device__ int begin() const { return min(per * (int)blockIdx.x, units); }
-  __device__ int end() const { return min(per * ((int)blockIdx.x + 1), units); }
+};
+
+// A walk over this CTA's run: unit u is K block kb of item grp of the a-th active expert.
+struct Walk {
+  int u, end, kb, KB, grp, groups, a;
+  __device__ __forceinline__ void set(const Deal& d) {
+    u = min(d.per * (int)blockIdx.x, d.units), end = min(u + d.per, d.units);
+    const int item = u / d.KB;
+    KB = d.KB, groups = d.groups;
+    kb = u - item * KB, a = item / groups, grp = item - a * groups;
+  }
+  __device__ __forceinline__ bool more() const { return u < end; }
+  __device__ __forceinline__ void next() {
+    ++u;
+    if (++kb == KB) {
+      kb = 0;
+      if (++grp == groups) grp = 0, ++a;
+    }
+  }
 };
 
 template <int NMAX>
@@ -81,7 +102,8 @@ struct MoeShared {
   uint8_t token_at[MoePlan<NMAX>::kPairs]; // token of a hidden row
   uint16_t first_row[kMaxE];
   uint16_t active[kMaxE < MoePlan<NMAX>::kPairs ? kMaxE : MoePlan<NMAX>::kPairs];
-  int n_active;
+  Deal deal[2];
+  Walk walk[2];
   uint32_t tmem_base, abort_flag, last, issued_w, issued_a, committed;
   uint64_t target;  // the grid barrier's count at the next barrier
 };
@@ -103,8 +125,7 @@ __device__ __forceinline__ bool wait_or_abort(uint32_t bar, uint32_t parity,
 // count is a multiple of the grid's size between launches and needs no reset.
 
 __device__ __forceinline__ uint64_t barrier_arrive(uint64_t* count) {
-  __threadfence();
-  asm volatile("fence.proxy.async;" ::: "memory");  // hidden rows are read by TMA
+  __threadfence();  // the CTA's writes, which a barrier of its threads ordered before
   return atomicAdd(reinterpret_cast<unsigned long long*>(count), 1ull);
 }
 
@@ -131,6 +152,17 @@ __device__ __forceinline__ float ld_l2(const float* p) {
   asm volatile("ld.global.cg.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
   return v;
 }
+// Zero where `ok` is false; no branch, so that nothing waits for the load.
+__device__ __forceinline__ float ld_l2_if(bool ok, const float* p) {
+  float v;
+  asm volatile(
+      "{\n .reg .pred q;\n setp.ne.u32 q, %2, 0;\n mov.f32 %0, 0f00000000;\n"
+      " @q ld.global.cg.f32 %0, [%1];\n}"
+      : "=&f"(v)
+      : "l"(p), "r"((uint32_t)ok)
+      : "memory");
+  return v;
+}
 __device__ __forceinline__ int ld_l2(const int* p) {
   int v;
   asm volatile("ld.global.cg.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
@@ -147,37 +179,40 @@ __device__ __forceinline__ float4 ld_l2(const float4* p) {
 
 // ------------------------------------------------------------------ router
 
-// Partial logits of 4 experts x 8 tokens over one share of the columns, a warp
-// a job; the lanes split the columns, so a job ends with 32 sums over 32
-// lanes, folded so that lane l keeps sum l.
-__device__ __forceinline__ void router_job(const MoeArgs& g, int job, int lane) {
+// Logits of 4 experts x 8 tokens over one of `splits` shares of the columns, a
+// CTA a job: the warps take chunks of 256 columns, the lanes 8 columns each, so
+// a warp ends with 32 sums over 32 lanes, folded so that lane l keeps sum l;
+// the warps' are added through shared memory.
+__device__ __forceinline__ void router_job(const MoeArgs& g, int job, int warp, int lane,
+                                           float (*red)[32]) {
   const int eg = (g.E + 3) / 4, tg = (g.T + 7) / 8, chunks = (g.H + 255) / 256;
   const int e0 = 4 * (job % eg), t0 = 8 * ((job / eg) % tg), s = job / (eg * tg);
   const int ne = min(4, g.E - e0), nt = min(8, g.T - t0);
-  const int c0 = chunks * s / g.splits, c1 = chunks * (s + 1) / g.splits;
+  const int c1 = chunks * (s + 1) / g.splits;
   float v[32];
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = 0.f;
-  for (int c = c0; c < c1; ++c) {
+  for (int c = chunks * s / g.splits + warp; c < c1; c += kMoeWarps) {
     const int col = c * 256 + lane * 8;
     if (col >= g.H) continue;
-    float2 w[4][4];
+    uint4 w[4], x[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint4 u = i < ne ? ld_keep(g.router + (int64_t)(e0 + i) * g.H + col) : make_uint4(0, 0, 0, 0);
-      w[i][0] = bf2_to_f2(u.x), w[i][1] = bf2_to_f2(u.y), w[i][2] = bf2_to_f2(u.z), w[i][3] = bf2_to_f2(u.w);
-    }
+    for (int i = 0; i < 4; ++i)
+      w[i] = i < ne ? ld_keep(g.router + (int64_t)(e0 + i) * g.H + col) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (j >= nt) break;
-      const uint4 u = ld_keep(g.x + (int64_t)(t0 + j) * g.ldx + col);
-      const float2 x[4] = {bf2_to_f2(u.x), bf2_to_f2(u.y), bf2_to_f2(u.z), bf2_to_f2(u.w)};
+    for (int j = 0; j < 8; ++j)
+      x[j] = j < nt ? ld_keep(g.x + (int64_t)(t0 + j) * g.ldx + col) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float a = v[i * 8 + j];
+    for (int q = 0; q < 4; ++q) {
+      float2 wf[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) a = __fmaf_rn(w[i][q].x, x[q].x, a), a = __fmaf_rn(w[i][q].y, x[q].y, a);
-        v[i * 8 + j] = a;
+      for (int i = 0; i < 4; ++i) wf[i] = bf2_to_f2(q == 0 ? w[i].x : q == 1 ? w[i].y : q == 2 ? w[i].z : w[i].w);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float2 xf = bf2_to_f2(q == 0 ? x[j].x : q == 1 ? x[j].y : q == 2 ? x[j].z : x[j].w);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          v[i * 8 + j] = __fmaf_rn(wf[i].y, xf.y, __fmaf_rn(wf[i].x, xf.x, v[i * 8 + j]));
       }
     }
   }
@@ -190,8 +225,16 @@ __device__ __forceinline__ void router_job(const MoeArgs& g, int job, int lane) 
       v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
     }
   }
-  const int i = lane >> 3, j = lane & 7;
-  if (i < ne && j < nt) g.logits[((int64_t)s * g.T + t0 + j) * g.E + e0 + i] = v[0];
+  red[warp][lane] = v[0];
+  __syncthreads();
+  if (warp == 0) {
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < kMoeWarps; ++i) sum += red[i][lane];
+    const int i = lane >> 3, j = lane & 7;
+    if (i < ne && j < nt) g.logits[((int64_t)s * g.T + t0 + j) * g.E + e0 + i] = sum;
+  }
+  __syncthreads();
 }
 
 // Order of floats as unsigned; NaN lowest but one, 0 is "none".
@@ -200,65 +243,65 @@ __device__ __forceinline__ uint32_t ordered(float f) {
   return f != f ? 1u : u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
 }
 
-// One token's choice by one warp: k rounds of a warp maximum, ties to the
-// lowest expert. Lane j < k returns with (*id, *w) of slot j.
-__device__ __forceinline__ void choose(const MoeArgs& g, int t, int lane, int* id, float* w) {
-  constexpr int NQ = kMaxE / 32;
-  float l[NQ];
-  uint32_t key[NQ];
-  float m = -INFINITY;
+// Logits of `n` tokens from t0 on, [n][E] into shared memory: the sums of the
+// router's shares, a thread a logit, eight loads in flight.
+__device__ __forceinline__ void sum_logits(const MoeArgs& g, int t0, int n, float* to) {
+  for (int i = threadIdx.x; i < n * g.E; i += kMoeThreads) {
+    const float* p = g.logits + (int64_t)t0 * g.E + i;
+    float sum = 0.f;
+    for (int s = 0; s < g.splits; s += 8) {
+      float v[8];
 #pragma unroll
-  for (int q = 0; q < NQ; ++q) {
-    const int e = q * 32 + lane;
-    l[q] = 0.f;
-    if (e < g.E) {
-      for (int s = 0; s < g.splits; ++s) l[q] += ld_l2(g.logits + ((int64_t)s * g.T + t) * g.E + e);
-      m = fmaxf(m, l[q]);
+      for (int j = 0; j < 8; ++j) v[j] = ld_l2_if(s + j < g.splits, p + (int64_t)(s + j) * g.T * g.E);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum += v[j];
     }
+    to[i] = sum;
   }
-  float z = 1.f;
+}
+
+// One token's choice by one warp from its logits in shared memory: k rounds of
+// a warp maximum, ties to the lowest expert; `key` is E words of scratch. Lane
+// j < k returns with (*id, *w) of slot j. The loops stay rolled: every launch
+// runs this once, and instructions fetched for the first time cost more than
+// they compute (unrolled over 16 registers a lane this took 4 us, not 1.5).
+__device__ __forceinline__ void choose(const MoeArgs& g, const float* logits, uint32_t* key, int lane,
+                                       int* id, float* w) {
   const bool softmax = g.scoring == 0;
+  float m = -INFINITY, z = 1.f;
   if (softmax) {
+#pragma unroll 1
+    for (int e = lane; e < g.E; e += 32) m = fmaxf(m, logits[e]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     z = 0.f;
-#pragma unroll
-    for (int q = 0; q < NQ; ++q)
-      if (q * 32 + lane < g.E) z += expf(l[q] - m);
+#pragma unroll 1
+    for (int e = lane; e < g.E; e += 32) z += expf(logits[e] - m);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
   }
-#pragma unroll
-  for (int q = 0; q < NQ; ++q) {
-    const int e = q * 32 + lane;
-    key[q] = 0;
-    if (e < g.E) {
-      // without a bias the choice goes by the logits, which the scores grow
-      // with (and saturate against); with one by the biased scores
-      float sel = l[q];
-      if (g.bias != nullptr)
-        sel = (softmax ? expf(l[q] - m) / z : 1.f / (1.f + expf(-l[q]))) + g.bias[e];
-      key[q] = ordered(sel);
-    }
+#pragma unroll 1
+  for (int e = lane; e < g.E; e += 32) {
+    // without a bias the choice goes by the logits, which the scores grow with
+    // (and saturate against); with one by the biased scores
+    float sel = logits[e];
+    if (g.bias != nullptr) sel = (softmax ? expf(sel - m) / z : 1.f / (1.f + expf(-sel))) + g.bias[e];
+    key[e] = ordered(sel);
   }
   int my_id = 0;
-  float my_l = 0.f;
+#pragma unroll 1
   for (int j = 0; j < g.k; ++j) {
     uint32_t best = 0, at = 0xffffffffu;
-    float bl = 0.f;
-#pragma unroll
-    for (int q = 0; q < NQ; ++q)
-      if (key[q] > best) best = key[q], at = (uint32_t)(q * 32 + lane), bl = l[q];
+#pragma unroll 1
+    for (int e = lane; e < g.E; e += 32)
+      if (key[e] > best) best = key[e], at = (uint32_t)e;
     const uint32_t top = __reduce_max_sync(0xffffffffu, best);
     const uint32_t e = __reduce_min_sync(0xffffffffu, best == top ? at : 0xffffffffu);
-    const float le = __shfl_sync(0xffffffffu, bl, (int)(e & 31u));
-#pragma unroll
-    for (int q = 0; q < NQ; ++q)
-      if ((uint32_t)(q * 32 + lane) == e) key[q] = 0;
-    if (lane == j) my_id = (int)e, my_l = le;
+    if ((e & 31u) == (uint32_t)lane) key[e] = 0;  // this lane's own entry: no other reads it
+    if (lane == j) my_id = (int)e;
   }
   float p = 0.f;
-  if (lane < g.k) p = softmax ? expf(my_l - m) : 1.f / (1.f + expf(-my_l));
+  if (lane < g.k) p = softmax ? expf(logits[my_id] - m) : 1.f / (1.f + expf(-logits[my_id]));
   float den = softmax ? z : 1.f;
   if (g.renormalize) {
     den = p;
@@ -277,7 +320,7 @@ __device__ __forceinline__ void epi_sync() { asm volatile("barrier.cta.sync 1, 2
 // that arrives last, with the whole sums in acc. n columns, thread = row.
 template <int NMAX>
 __device__ __forceinline__ bool join(const MoeArgs& g, MoeShared<NMAX>& sh, const Deal& deal, int item,
-                                     int* counters, int n, float (&acc)[NMAX]) {
+                                     int* counter, int n, float (&acc)[NMAX]) {
   const int tid = threadIdx.x;
   const int first = item * deal.KB, c0 = first / deal.per, c1 = (first + deal.KB - 1) / deal.per;
   // a run that begins inside the item keeps its part in slot 0, one that ends in it in slot 1
@@ -286,10 +329,10 @@ __device__ __forceinline__ bool join(const MoeArgs& g, MoeShared<NMAX>& sh, cons
 #pragma unroll
   for (int c = 0; c < NMAX; ++c)
     if (c < n) __stcg(p + c * 256, acc[c]);
-  __threadfence();
   epi_sync();
   if (tid == 0) {
-    const int old = atomicAdd(counters + item, 1);
+    __threadfence();
+    const int old = atomicAdd(counter, 1);
     __threadfence();
     sh.last = old == c1 - c0;
   }
@@ -306,57 +349,24 @@ __device__ __forceinline__ bool join(const MoeArgs& g, MoeShared<NMAX>& sh, cons
   return true;
 }
 
-// The outer sums of this CTA's run of one phase; finish(item, n, row0, acc) at
-// each item that is complete here.
-template <int NMAX, class F>
-__device__ __forceinline__ void sum_phase(const MoeArgs& g, MoeShared<NMAX>& sh, const Deal& deal,
-                                          int groups, int* counters, uint32_t tmem, uint32_t& it,
-                                          volatile uint32_t* abortp, F finish) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = warp >> 2;
-  const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(half * NMAX);
-  float acc[NMAX];
-  int item = -1, n = 0, row0 = 0, begun = 0;
-  const int u1 = deal.end();
-  for (int u = deal.begin(); u < u1; ++u, ++it) {
-    const int kb = u % deal.KB;
-    if (item < 0) {
-      item = u / deal.KB, begun = kb;
-      const int e = sh.active[item / groups];
-      n = __popcll(sh.mask[e]), row0 = sh.first_row[e];
+// One group of 128 of a hidden row by one warp: silu(gate) * up, its scale and codes.
+__device__ __noinline__ void hidden_group(const float* gate, const float* up, int lane, uint8_t* codes,
+                                          float* scale) {
+  float h[4], m = 0.f;
 #pragma unroll
-      for (int c = 0; c < NMAX; ++c) acc[c] = 0.f;
-    }
-    const uint32_t buf = it % kBufs, use = it / kBufs;
-    const bool ok = wait_or_abort(smem_addr(&sh.acc_full[buf]), use & 1u, abortp) &&
-                    wait_or_abort(smem_addr(&sh.scale_full[buf]), use & 1u, abortp);
-    if (__all_sync(0xffffffffu, ok)) {
-      tc::fence_after();
-#pragma unroll
-      for (int c = 0; c < NMAX; c += 16) {
-        if (c >= n) break;
-        uint32_t v[16];
-        tc::tmem_ld16_async(lane_base + buf * 2 * NMAX + (uint32_t)c, v);
-        const float4* sc = reinterpret_cast<const float4*>(&sh.scales[buf][half][c]);
-        const float4 f[4] = {sc[0], sc[1], sc[2], sc[3]};
-        tc::tmem_ld_wait(v);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          acc[c + 4 * i] = __fmaf_rn(__uint_as_float(v[4 * i]), f[i].x, acc[c + 4 * i]);
-          acc[c + 4 * i + 1] = __fmaf_rn(__uint_as_float(v[4 * i + 1]), f[i].y, acc[c + 4 * i + 1]);
-          acc[c + 4 * i + 2] = __fmaf_rn(__uint_as_float(v[4 * i + 2]), f[i].z, acc[c + 4 * i + 2]);
-          acc[c + 4 * i + 3] = __fmaf_rn(__uint_as_float(v[4 * i + 3]), f[i].w, acc[c + 4 * i + 3]);
-        }
-      }
-      tc::fence_before();
-    }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(smem_addr(&sh.acc_empty[buf]));
-    if (kb == deal.KB - 1 || u == u1 - 1) {
-      const bool whole = begun == 0 && kb == deal.KB - 1;
-      if (whole || join<NMAX>(g, sh, deal, item, counters, n, acc)) finish(item, n, row0, acc);
-      item = -1;
-    }
+  for (int i = 0; i < 4; ++i) {
+    const float a = gate[lane * 4 + i];
+    h[i] = a / (1.f + expf(-a)) * up[lane * 4 + i];
+    m = fmaxf(m, fabsf(h[i]));
   }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  // h is not bf16: the quantizer's short reciprocal does not apply
+  const float s = fmaxf(__fdiv_rn(m, kE4m3Max), kMinScale);
+  const uint32_t code = f4_to_e4m3x4(make_float2(__fdiv_rn(h[0], s), __fdiv_rn(h[1], s)),
+                                     make_float2(__fdiv_rn(h[2], s), __fdiv_rn(h[3], s)));
+  *reinterpret_cast<uint32_t*>(codes + 4 * lane) = code;
+  if (lane == 0) *scale = s;
 }
 
 // ------------------------------------------------------------------ kernel
@@ -401,8 +411,8 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
   for (int i = blockIdx.x * kMoeThreads + tid; i < g.n_counters; i += gridDim.x * kMoeThreads)
     g.counters[i] = 0;
   const int jobs = ((g.E + 3) / 4) * ((g.T + 7) / 8) * g.splits;
-  for (int j = warp * gridDim.x + blockIdx.x; j < jobs; j += gridDim.x * kMoeWarps)
-    router_job(g, j, lane);
+  for (int j = blockIdx.x; j < jobs; j += gridDim.x)
+    router_job(g, j, warp, lane, reinterpret_cast<float(*)[32]>(smem_raw));  // the ring is idle
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
@@ -418,17 +428,24 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
   // token's is made once and read by all after another barrier
   const int pairs = g.T * g.k;
   const bool deal_tokens = g.deal_tokens;
-  for (int t = deal_tokens ? warp * gridDim.x + blockIdx.x : warp; t < g.T;
-       t += deal_tokens ? kMoeWarps * gridDim.x : kMoeWarps) {
-    int id;
-    float w;
-    choose(g, t, lane, &id, &w);
-    if (lane < g.k) {
-      const int p = t * g.k + lane;
-      if (deal_tokens || blockIdx.x == 0) g.ids[p] = id, g.weights[p] = w;
-      if (!deal_tokens) sh.ids[p] = (uint16_t)id, sh.weight[p] = w;
+  float* logits = reinterpret_cast<float*>(smem_raw);  // the ring is idle: kChooseTokens x E at most
+  for (int t0 = deal_tokens ? blockIdx.x : 0; t0 < g.T; t0 += deal_tokens ? gridDim.x : g.T) {
+    const int n = deal_tokens ? 1 : g.T;
+    sum_logits(g, t0, n, logits);
+    __syncthreads();
+    for (int t = warp; t < n; t += kMoeWarps) {
+      int id;
+      float w;
+      choose(g, logits + t * g.E, reinterpret_cast<uint32_t*>(logits + (n + t) * g.E), lane, &id, &w);
+      if (lane < g.k) {
+        const int p = (t0 + t) * g.k + lane;
+        if (deal_tokens || blockIdx.x == 0) g.ids[p] = id, g.weights[p] = w;
+        if (!deal_tokens) sh.ids[p] = (uint16_t)id, sh.weight[p] = w;
+      }
     }
+    __syncthreads();
   }
+  tc::fence_async_smem();  // the ring's TMA writes come after these accesses
   if (deal_tokens) {
     __syncthreads();
     target += gridDim.x;
@@ -463,7 +480,10 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
       rows += __shfl_sync(0xffffffffu, at, 31);
       n += __popc(some);
     }
-    if (lane == 0) sh.n_active = n;
+    if (lane < 2) {
+      sh.deal[lane].set(n, lane == 0 ? IG : HB, lane == 0 ? KB1 : KB2);
+      sh.walk[lane].set(sh.deal[lane]);
+    }
   }
   __syncthreads();
   for (int p = tid; p < pairs; p += kMoeThreads) {
@@ -475,32 +495,27 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
   __syncthreads();
 
   const uint32_t tmem = sh.tmem_base;
-  const Deal d1(sh.n_active * IG, KB1), d2(sh.n_active * HB, KB2);
   const uint64_t hidden_target = target + gridDim.x, down_target = target + 2 * (uint64_t)gridDim.x;
 
   if (warp == 8) {
     // ---- weight tiles of both phases, without a stop between them
     if (lane == 0) {
+      const uint64_t once = tc::evict_first_policy();
       uint32_t it = 0;
+#pragma unroll 1
       for (int phase = 0; phase < 2 && !*abortp; ++phase) {
-        const Deal& d = phase == 0 ? d1 : d2;
-        const int groups = phase == 0 ? IG : HB;
-        for (int u = d.begin(); u < d.end(); ++u, ++it) {
-          const int item = u / d.KB, kb = u - item * d.KB;
-          const int e = sh.active[item / groups], grp = item % groups;
+        const CUtensorMap* map = phase == 0 ? &map_w13 : &map_w2;
+        const int rows = phase == 0 ? 2 * g.I : g.H, step = phase == 0 ? 128 : 256;
+        const int second = phase == 0 ? g.I : 128;
+#pragma unroll 1
+        for (Walk w = sh.walk[phase]; w.more(); w.next(), ++it) {
           const uint32_t s = it % P::kStages, use = it / P::kStages;
           if (use > 0 && !wait_or_abort(smem_addr(&sh.empty[s]), (use - 1u) & 1u, abortp)) break;
           const uint32_t st = base + s * P::kStageBytes, bar = smem_addr(&sh.full[s]);
+          const int r = sh.active[w.a] * rows + w.grp * step;
           mbar_arrive_expect_tx(bar, 2 * kBox);
-          if (phase == 0) {
-            const int r = e * 2 * g.I + grp * 128;
-            tc::tma_load_2d(st, &map_w13, kb * 128, r, bar);
-            tc::tma_load_2d(st + kBox, &map_w13, kb * 128, r + g.I, bar);
-          } else {
-            const int r = e * g.H + grp * 256;
-            tc::tma_load_2d(st, &map_w2, kb * 128, r, bar);
-            tc::tma_load_2d(st + kBox, &map_w2, kb * 128, r + 128, bar);
-          }
+          tc::tma_load_2d_hint(st, map, w.kb * 128, r, bar, once);
+          tc::tma_load_2d_hint(st + kBox, map, w.kb * 128, r + second, bar, once);
           sh.issued_w = it + 1;
         }
       }
@@ -509,31 +524,30 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
     // ---- the tokens' rows
     if (lane == 0) {
       uint32_t it = 0;
+#pragma unroll 1
       for (int phase = 0; phase < 2 && !*abortp; ++phase) {
-        const Deal& d = phase == 0 ? d1 : d2;
-        const int groups = phase == 0 ? IG : HB;
-        if (phase == 1 && d.begin() < d.end() && !barrier_wait(g.barrier, hidden_target, abortp)) break;
-        for (int u = d.begin(); u < d.end(); ++u, ++it) {
-          const int item = u / d.KB, kb = u - item * d.KB;
-          const int e = sh.active[item / groups];
-          const int n = __popcll(sh.mask[e]), row0 = sh.first_row[e];
+        Walk w = sh.walk[phase];
+        if (phase == 1 && w.more() && !barrier_wait(g.barrier, hidden_target, abortp)) break;
+#pragma unroll 1
+        for (; w.more(); w.next(), ++it) {
+          const int e = sh.active[w.a], n = __popcll(sh.mask[e]), row0 = sh.first_row[e];
           const uint32_t s = it % P::kStages, use = it / P::kStages;
           if (use > 0 && !wait_or_abort(smem_addr(&sh.empty[s]), (use - 1u) & 1u, abortp)) break;
           const uint32_t st = base + s * P::kStageBytes + 2 * kBox, bar = smem_addr(&sh.full[s]);
-          const int np = (n + 15) & ~15;
+          const int np = (n + 15) & ~15, last = row0 + n - 1;
           mbar_arrive_expect_tx(bar, (uint32_t)np * 128u);
           if (phase == 0) {
-            for (int c = 0; c < np; c += 4) {
-              // columns past the expert's tokens repeat its last one and are not used
-              const int last = row0 + n - 1;
-              tc::tma_gather4(st + (uint32_t)c * 128u, &map_q, kb * 128,
+            // columns past the expert's tokens repeat its last one and are not used
+#pragma unroll 1
+            for (int c = 0; c < np; c += 4)
+              tc::tma_gather4(st + (uint32_t)c * 128u, &map_q, w.kb * 128,
                               sh.token_at[min(row0 + c, last)], sh.token_at[min(row0 + c + 1, last)],
                               sh.token_at[min(row0 + c + 2, last)],
                               sh.token_at[min(row0 + c + 3, last)], bar);
-            }
           } else {
+#pragma unroll 1
             for (int c = 0; c < np; c += 16)
-              tc::tma_load_2d(st + (uint32_t)c * 128u, &map_h, kb * 128, row0 + c, bar);
+              tc::tma_load_2d(st + (uint32_t)c * 128u, &map_h, w.kb * 128, row0 + c, bar);
           }
           sh.issued_a = it + 1;
         }
@@ -544,12 +558,11 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
     if (lane == 0) {
       uint32_t it = 0;
       bool ok = true;
+#pragma unroll 1
       for (int phase = 0; phase < 2 && ok; ++phase) {
-        const Deal& d = phase == 0 ? d1 : d2;
-        const int groups = phase == 0 ? IG : HB;
-        for (int u = d.begin(); u < d.end(); ++u, ++it) {
-          const int e = sh.active[u / d.KB / groups];
-          const int np = (__popcll(sh.mask[e]) + 15) & ~15;
+#pragma unroll 1
+        for (Walk w = sh.walk[phase]; w.more(); w.next(), ++it) {
+          const int np = (__popcll(sh.mask[sh.active[w.a]]) + 15) & ~15;
           const uint32_t s = it % P::kStages, buf = it % kBufs;
           ok = wait_or_abort(smem_addr(&sh.full[s]), (it / P::kStages) & 1u, abortp) &&
                (it < kBufs ||
@@ -572,119 +585,161 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
     }
   } else if (warp == 11) {
     // ---- scale products: a token's (or hidden row's) scale of the K block
-    // times each 128-row tile's, loaded two units ahead
+    // times each 128-row tile's, loaded kAhead units ahead (they come from HBM)
     uint32_t it = 0;
     bool ok = true;
-    constexpr int NL = (NMAX + 31) / 32;
+    constexpr int NL = (NMAX + 31) / 32, kAhead = 8;
     struct Vals {
       float a[NL], w0, w1;
     };
+#pragma unroll 1
     for (int phase = 0; phase < 2 && ok; ++phase) {
-      const Deal& d = phase == 0 ? d1 : d2;
-      const int groups = phase == 0 ? IG : HB, u1 = d.end();
-      if (phase == 1 && d.begin() < u1) {
+      // a cursor kAhead units ahead of the products; addresses change at items only
+      Walk w = sh.walk[phase];
+      int left = w.end - w.u, n = 0;
+      if (phase == 1 && left > 0) {
         int pass = 1;
         if (lane == 0) pass = barrier_wait(g.barrier, hidden_target, abortp);
         if (!__shfl_sync(0xffffffffu, pass, 0)) break;
       }
-      auto fetch = [&](int u) {
+      bool two = true;
+      const float *pa[NL], *pw0 = nullptr, *pw1 = nullptr;
+#pragma unroll
+      for (int i = 0; i < NL; ++i) pa[i] = nullptr;
+      auto fetch = [&]() {
+        const bool some = w.more();
+        if (some && (w.kb == 0 || n == 0)) {
+          const int e = sh.active[w.a], row0 = sh.first_row[e];
+          n = __popcll(sh.mask[e]);
+#pragma unroll
+          for (int i = 0; i < NL; ++i) {
+            const int row = row0 + min(lane + 32 * i, n - 1);
+            pa[i] = phase == 0 ? g.q_scale + sh.token_at[row] * g.sq_row : g.h_scale + (int64_t)row * IG;
+          }
+          pw0 = phase == 0 ? g.w13_scale + ((int64_t)e * 2 * IG + w.grp) * KB1
+                           : g.w2_scale + ((int64_t)e * (g.H / 128) + w.grp * 2) * KB2;
+          pw1 = pw0 + (phase == 0 ? (int64_t)IG * KB1 : KB2);
+          two = phase == 0 || w.grp * 2 + 1 < g.H / 128;
+        }
         Vals v;
+        const int64_t step = phase == 0 ? g.sq_kb : 1;
 #pragma unroll
-        for (int i = 0; i < NL; ++i) v.a[i] = 0.f;
-        v.w0 = v.w1 = 0.f;
-        if (u >= u1) return v;
-        const int item = u / d.KB, kb = u - item * d.KB, grp = item % groups;
-        const int e = sh.active[item / groups];
-        const int n = __popcll(sh.mask[e]), row0 = sh.first_row[e];
-#pragma unroll
-        for (int i = 0; i < NL; ++i) {
-          const int c = lane + 32 * i;
-          if (c < n)
-            v.a[i] = phase == 0 ? __ldg(g.q_scale + sh.token_at[row0 + c] * g.sq_row + kb * g.sq_kb)
-                                : ld_l2(g.h_scale + (int64_t)(row0 + c) * IG + kb);
-        }
-        if (phase == 0) {
-          const float* p = g.w13_scale + ((int64_t)e * 2 * IG + grp) * KB1 + kb;
-          v.w0 = __ldg(p), v.w1 = __ldg(p + (int64_t)IG * KB1);
-        } else {
-          const float* p = g.w2_scale + ((int64_t)e * (g.H / 128) + grp * 2) * KB2 + kb;
-          v.w0 = __ldg(p);
-          v.w1 = grp * 2 + 1 < g.H / 128 ? __ldg(p + KB2) : 0.f;
-        }
+        for (int i = 0; i < NL; ++i) v.a[i] = ld_l2_if(some && lane + 32 * i < n, pa[i] + w.kb * step);
+        v.w0 = ld_l2_if(some, pw0 + w.kb);
+        v.w1 = ld_l2_if(some && two, pw1 + w.kb);
+        w.next();
         return v;
       };
-      Vals v0 = fetch(d.begin()), v1 = fetch(d.begin() + 1);
-      for (int u = d.begin(); u < u1; ++u, ++it) {
-        const Vals v2 = fetch(u + 2);
-        const uint32_t buf = it % kBufs;
-        ok = it < kBufs || __all_sync(0xffffffffu, wait_or_abort(smem_addr(&sh.acc_empty[buf]),
-                                                                 (it / kBufs - 1u) & 1u, abortp));
-        if (!ok) break;
+      Vals v[kAhead];
 #pragma unroll
-        for (int i = 0; i < NL; ++i)
-          if (lane + 32 * i < NMAX) {
-            sh.scales[buf][0][lane + 32 * i] = v0.a[i] * v0.w0;
-            sh.scales[buf][1][lane + 32 * i] = v0.a[i] * v0.w1;
-          }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_addr(&sh.scale_full[buf]));
-        v0 = v1;
-        v1 = v2;
+      for (int i = 0; i < kAhead; ++i) v[i] = fetch();
+#pragma unroll 1
+      for (; left > 0 && ok; left -= kAhead) {
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+          if (j >= left) break;
+          const uint32_t buf = it % kBufs;
+          ok = it < kBufs || __all_sync(0xffffffffu, wait_or_abort(smem_addr(&sh.acc_empty[buf]),
+                                                                   (it / kBufs - 1u) & 1u, abortp));
+          if (!ok) break;
+#pragma unroll
+          for (int i = 0; i < NL; ++i)
+            if (lane + 32 * i < NMAX) {
+              sh.scales[buf][0][lane + 32 * i] = v[j].a[i] * v[j].w0;
+              sh.scales[buf][1][lane + 32 * i] = v[j].a[i] * v[j].w1;
+            }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_addr(&sh.scale_full[buf]));
+          ++it;
+          v[j] = fetch();
+        }
       }
     }
   } else {
     // ---- outer sums and epilogues
     uint32_t it = 0;
     const int half = warp >> 2, r = tid & 127;
-    sum_phase<NMAX>(g, sh, d1, IG, g.counters, tmem, it, abortp,
-                    [&](int item, int n, int row0, float (&acc)[NMAX]) {
-                      const int grp = item % IG;
-                      if (half == 1) {
+    const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(half * NMAX);
+#pragma unroll 1
+    for (int phase = 0; phase < 2; ++phase) {
+      float acc[NMAX];
+      int n = 0, row0 = 0;
+      bool begun = false, from_start = false;
+#pragma unroll 1
+      for (Walk w = sh.walk[phase]; w.more(); w.next(), ++it) {
+        if (!begun) {
+          begun = true, from_start = w.kb == 0;
+          const int e = sh.active[w.a];
+          n = __popcll(sh.mask[e]), row0 = sh.first_row[e];
 #pragma unroll
-                        for (int c = 0; c < NMAX; ++c)
-                          if (c < n) exchange[c * kXStride + r] = acc[c];
-                      }
-                      epi_sync();
-                      if (half == 0) {
+          for (int c = 0; c < NMAX; ++c) acc[c] = 0.f;
+        }
+        const uint32_t buf = it % kBufs, use = it / kBufs;
+        const bool ok = wait_or_abort(smem_addr(&sh.acc_full[buf]), use & 1u, abortp) &&
+                        wait_or_abort(smem_addr(&sh.scale_full[buf]), use & 1u, abortp);
+        if (__all_sync(0xffffffffu, ok)) {
+          tc::fence_after();
 #pragma unroll
-                        for (int c = 0; c < NMAX; ++c)
-                          if (c < n) {
-                            const float gate = acc[c], up = exchange[c * kXStride + r];
-                            exchange[c * kXStride + r] = gate / (1.f + expf(-gate)) * up;
-                          }
-                      }
-                      epi_sync();
-                      for (int c = warp; c < n; c += 8) {  // a row's group of 128, a warp
-                        const float4 h = *reinterpret_cast<const float4*>(exchange + c * kXStride + 4 * lane);
-                        float m = fmaxf(fmaxf(fabsf(h.x), fabsf(h.y)), fmaxf(fabsf(h.z), fabsf(h.w)));
+          for (int c = 0; c < NMAX; c += 16) {
+            if (c >= n) break;
+            uint32_t v[16];
+            tc::tmem_ld16_async(lane_base + buf * 2 * NMAX + (uint32_t)c, v);
+            const float4* sc = reinterpret_cast<const float4*>(&sh.scales[buf][half][c]);
+            const float4 f[4] = {sc[0], sc[1], sc[2], sc[3]};
+            tc::tmem_ld_wait(v);
 #pragma unroll
-                        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-                        // h is not bf16: the quantizer's short reciprocal does not
-                        // apply, the divisions are the compiler's
-                        const float s = fmaxf(__fdiv_rn(m, kE4m3Max), kMinScale);
-                        const uint32_t code = f4_to_e4m3x4(
-                            make_float2(__fdiv_rn(h.x, s), __fdiv_rn(h.y, s)),
-                            make_float2(__fdiv_rn(h.z, s), __fdiv_rn(h.w, s)));
-                        *reinterpret_cast<uint32_t*>(g.hidden + (int64_t)(row0 + c) * g.I + grp * 128 +
-                                                     4 * lane) = code;
-                        if (lane == 0) g.h_scale[(int64_t)(row0 + c) * IG + grp] = s;
-                      }
-                      epi_sync();
-                    });
-    __threadfence();
-    asm volatile("fence.proxy.async;" ::: "memory");
-    epi_sync();
-    if (tid == 0) barrier_arrive(g.barrier);
-    sum_phase<NMAX>(g, sh, d2, HB, g.counters + g.n_counters1, tmem, it, abortp,
-                    [&](int item, int n, int row0, float (&acc)[NMAX]) {
-                      const int col = (item % HB) * 256 + half * 128 + r;
-                      if (col < g.H) {
+            for (int i = 0; i < 4; ++i) {
+              acc[c + 4 * i] = __fmaf_rn(__uint_as_float(v[4 * i]), f[i].x, acc[c + 4 * i]);
+              acc[c + 4 * i + 1] = __fmaf_rn(__uint_as_float(v[4 * i + 1]), f[i].y, acc[c + 4 * i + 1]);
+              acc[c + 4 * i + 2] = __fmaf_rn(__uint_as_float(v[4 * i + 2]), f[i].z, acc[c + 4 * i + 2]);
+              acc[c + 4 * i + 3] = __fmaf_rn(__uint_as_float(v[4 * i + 3]), f[i].w, acc[c + 4 * i + 3]);
+            }
+          }
+          tc::fence_before();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_addr(&sh.acc_empty[buf]));
+        const bool to_end = w.kb == w.KB - 1;
+        if (!to_end && w.u != w.end - 1) continue;
+        // ---- the item, or this CTA's part of it, is complete
+        begun = false;
+        if (!from_start || !to_end) {
+          const int item = w.a * w.groups + w.grp;
+          int* counter = g.counters + (phase == 0 ? 0 : g.n_counters1) + item;
+          if (!join<NMAX>(g, sh, sh.deal[phase], item, counter, n, acc)) continue;
+        }
+        if (phase == 0) {
+          // hidden rows: both halves to shared memory, then a row's group of
+          // 128 columns a warp
 #pragma unroll
-                        for (int c = 0; c < NMAX; ++c)
-                          if (c < n) __stcg(g.down + (int64_t)(row0 + c) * g.H + col, acc[c]);
-                      }
-                    });
-    __threadfence();
+          for (int h0 = 0; h0 < NMAX; h0 += P::kXCols) {
+            if (h0 >= n) break;
+#pragma unroll
+            for (int c = 0; c < P::kXCols; ++c)
+              if (h0 + c < n) exchange[(half * P::kXCols + c) * kXStride + r] = acc[h0 + c];
+            epi_sync();
+#pragma unroll 1
+            for (int c = warp; c < P::kXCols && h0 + c < n; c += 8)
+              hidden_group(exchange + c * kXStride, exchange + (P::kXCols + c) * kXStride, lane,
+                           g.hidden + (int64_t)(row0 + h0 + c) * g.I + w.grp * 128,
+                           g.h_scale + (int64_t)(row0 + h0 + c) * IG + w.grp);
+            epi_sync();
+          }
+        } else {
+          const int col = w.grp * 256 + half * 128 + r;
+          if (col < g.H) {
+#pragma unroll
+            for (int c = 0; c < NMAX; ++c)
+              if (c < n) __stcg(g.down + (int64_t)(row0 + c) * g.H + col, acc[c]);
+          }
+        }
+      }
+      if (phase == 0) {
+        asm volatile("fence.proxy.async;" ::: "memory");  // hidden rows are read by TMA
+        epi_sync();
+        if (tid == 0) barrier_arrive(g.barrier);
+      }
+    }
     epi_sync();
     if (tid == 0) {
       // one count serves all barriers: nobody arrives at one before the last is
@@ -736,12 +791,12 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
 
 // ------------------------------------------------------------------ host
 
-// Shares of the router's columns: enough jobs of 4 experts x 8 tokens for
-// every warp of the grid, at most one chunk of 256 columns a job.
+// Shares of the router's columns: as many jobs of 4 experts x 8 tokens as CTAs,
+// while each of a CTA's warps keeps at least one chunk of 256 columns.
 int router_splits(int64_t T, int64_t E, int64_t H, int sms) {
   const int64_t jobs = ((E + 3) / 4) * ((T + 7) / 8), chunks = (H + 255) / 256;
-  int64_t s = (int64_t)sms * kMoeWarps / jobs;
-  return (int)(s < 1 ? 1 : s > chunks ? chunks : s);
+  const int64_t most = (chunks + kMoeWarps - 1) / kMoeWarps, s = sms / jobs;
+  return (int)(s < 1 ? 1 : s > most ? most : s);
 }
 
 int moe_columns(int64_t T) { return T <= 16 ? 16 : T <= 32 ? 32 : 64; }
@@ -812,7 +867,7 @@ int moe_fp8(MoeArgs g, const void* q, int64_t ldq, const void* w13, const void* 
             cudaStream_t stream, const char** why) {
   const int sms = device_sm_count();
   const int64_t pairs = (int64_t)g.T * g.k;
-  g.deal_tokens = g.T > 8;
+  g.deal_tokens = g.T > kChooseTokens;
   CUtensorMap mq, m13, mh, m2;
   if (!tc::encode_e4m3_operand(&mq, q, g.T, g.H, ldq, 1) ||
       !tc::encode_e4m3_operand(&m13, w13, (int64_t)g.E * 2 * g.I, g.H, g.H) ||
