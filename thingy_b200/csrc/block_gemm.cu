@@ -22,9 +22,6 @@ namespace {
 constexpr int kBM = 128, kBK = 128;
 constexpr uint32_t kBoxBytes = kBM * kBK;  // one 128-row operand box: 16 KB
 
-using tc::kLayoutSw128;
-using tc::smem_desc;
-
 // Gives up after kWaitLimitCycles, or at once when the CTA's abort flag is
 // set; giving up sets the flag.
 __device__ __forceinline__ bool wait_or_abort(uint32_t bar, uint32_t parity,
@@ -179,48 +176,62 @@ __global__ void __launch_bounds__(kThreads, 1)
   griddep_launch_dependents();
 
   if (warp == kEpiWarps) {
-    if (lane == 0) {
-      uint32_t it = 0;
-      for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
-        int tm, tn;
-        tile_at(t, g.tiles_m, g.tiles_n, &tm, &tn);
-        for (int kb = 0; kb < g.KB; ++kb, ++it) {
-          const uint32_t s = it % P::kStages, use = it / P::kStages;
-          if (use > 0 && !wait_or_abort(smem_addr(&empty_bar[s]), (use - 1u) & 1u, abortp))
-            goto producer_done;
+    // ---- operands
+    const bool leader = tc::elect_one();
+    uint32_t s = 0, parity = 1;  // a fresh barrier passes a wait for the phase before its first
+    bool ok = true;
+    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      int tm, tn;
+      tile_at(t, g.tiles_m, g.tiles_n, &tm, &tn);
+      for (int kb = 0; kb < g.KB; ++kb) {
+        ok = wait_or_abort(smem_addr(&empty_bar[s]), parity, abortp);
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
+        }
+        if (leader) {
           const uint32_t st = base + s * P::kStageBytes, bar = smem_addr(&full_bar[s]);
           mbar_arrive_expect_tx(bar, P::kStageBytes);
           tc::tma_load_2d(st, &map_a, kb * kBK, tm * kBM, bar);
 #pragma unroll
           for (int h = 0; h < P::kNB; ++h)
             tc::tma_load_2d(st + (1 + h) * kBoxBytes, &map_b, kb * kBK, tn * BN + 128 * h, bar);
-          issued = it + 1;
+          ++issued;
         }
+        if (++s == P::kStages) s = 0, parity ^= 1;
       }
-    producer_done:;
     }
   } else if (warp == kEpiWarps + 1) {
-    if (lane == 0) {
-      uint32_t it = 0;
-      constexpr uint32_t idesc = tc::f8_idesc(kBM, BN);
-      for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
-        for (int kb = 0; kb < g.KB; ++kb, ++it) {
-          const uint32_t s = it % P::kStages, use = it / P::kStages, buf = it & 1u;
-          if (!wait_or_abort(smem_addr(&full_bar[s]), use & 1u, abortp)) goto mma_done;
-          if (it >= 2 && !wait_or_abort(smem_addr(&acc_empty[buf]), ((it >> 1) - 1u) & 1u, abortp))
-            goto mma_done;
-          tc::fence_after();
-          const uint32_t st = base + s * P::kStageBytes;
+    // ---- MMAs
+    const bool leader = tc::elect_one();
+    constexpr uint32_t idesc = tc::f8_idesc(kBM, BN);
+    const uint32_t lo0 = tc::sw128_lo(base), hi = tc::sw128_hi();
+    uint32_t s = 0, parity = 0, buf = 0, buf_parity = 1;
+    bool ok = true;
+    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      for (int kb = 0; kb < g.KB; ++kb) {
+        ok = wait_or_abort(smem_addr(&full_bar[s]), parity, abortp) &&
+             wait_or_abort(smem_addr(&acc_empty[buf]), buf_parity, abortp);
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
+        }
+        tc::fence_after();
+        if (leader) {
+          const uint32_t lo = lo0 + s * (P::kStageBytes >> 4);
 #pragma unroll
           for (int kk = 0; kk < kBK / 32; ++kk)
-            tc::mma_f8(tmem + buf * BN, smem_desc(st + 32u * kk, 16, 1024, kLayoutSw128),
-                       smem_desc(st + kBoxBytes + 32u * kk, 16, 1024, kLayoutSw128), idesc, kk != 0);
+            tc::mma_f8(tmem + buf * BN, lo + 2 * kk, lo + (kBoxBytes >> 4) + 2 * kk, hi, idesc,
+                       kk != 0);
           tc::commit(smem_addr(&empty_bar[s]));
           tc::commit(smem_addr(&acc_full[buf]));
-          committed = it + 1;
+          ++committed;
         }
+        __syncwarp();
+        if (++s == P::kStages) s = 0, parity ^= 1;
+        buf ^= 1;
+        buf_parity ^= buf == 0;
       }
-    mma_done:;
     }
   } else {
     // ---- the outer sum

@@ -40,9 +40,6 @@ static __device__ int g_moe_device_error = 0;
 
 namespace {
 
-using tc::kLayoutSw128;
-using tc::smem_desc;
-
 constexpr int kMoeThreads = 384, kMoeWarps = 12, kEpiThreads = 256;
 constexpr uint32_t kBox = 128 * 128;  // a 128-row weight tile of one K block
 constexpr int kBufs = 4;              // accumulator buffers in tensor memory
@@ -499,40 +496,48 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
 
   if (warp == 8) {
     // ---- weight tiles of both phases, without a stop between them
-    if (lane == 0) {
-      const uint64_t once = tc::evict_first_policy();
-      uint32_t it = 0;
+    const bool leader = tc::elect_one();
+    const uint64_t once = tc::evict_first_policy();
+    uint32_t s = 0, parity = 1;  // a fresh barrier passes a wait for the phase before its first
+    bool ok = true;
 #pragma unroll 1
-      for (int phase = 0; phase < 2 && !*abortp; ++phase) {
-        const CUtensorMap* map = phase == 0 ? &map_w13 : &map_w2;
-        const int rows = phase == 0 ? 2 * g.I : g.H, step = phase == 0 ? 128 : 256;
-        const int second = phase == 0 ? g.I : 128;
+    for (int phase = 0; phase < 2 && ok; ++phase) {
+      const CUtensorMap* map = phase == 0 ? &map_w13 : &map_w2;
+      const int rows = phase == 0 ? 2 * g.I : g.H, step = phase == 0 ? 128 : 256;
+      const int second = phase == 0 ? g.I : 128;
 #pragma unroll 1
-        for (Walk w = sh.walk[phase]; w.more(); w.next(), ++it) {
-          const uint32_t s = it % P::kStages, use = it / P::kStages;
-          if (use > 0 && !wait_or_abort(smem_addr(&sh.empty[s]), (use - 1u) & 1u, abortp)) break;
+      for (Walk w = sh.walk[phase]; w.more(); w.next()) {
+        ok = __all_sync(0xffffffffu, wait_or_abort(smem_addr(&sh.empty[s]), parity, abortp));
+        if (!ok) break;
+        if (leader) {
           const uint32_t st = base + s * P::kStageBytes, bar = smem_addr(&sh.full[s]);
           const int r = sh.active[w.a] * rows + w.grp * step;
           mbar_arrive_expect_tx(bar, 2 * kBox);
           tc::tma_load_2d_hint(st, map, w.kb * 128, r, bar, once);
           tc::tma_load_2d_hint(st + kBox, map, w.kb * 128, r + second, bar, once);
-          sh.issued_w = it + 1;
+          ++sh.issued_w;
         }
+        if (++s == P::kStages) s = 0, parity ^= 1;
       }
     }
   } else if (warp == 9) {
     // ---- the tokens' rows
-    if (lane == 0) {
-      uint32_t it = 0;
+    const bool leader = tc::elect_one();
+    uint32_t s = 0, parity = 1;
+    bool ok = true;
 #pragma unroll 1
-      for (int phase = 0; phase < 2 && !*abortp; ++phase) {
-        Walk w = sh.walk[phase];
-        if (phase == 1 && w.more() && !barrier_wait(g.barrier, hidden_target, abortp)) break;
+    for (int phase = 0; phase < 2 && ok; ++phase) {
+      Walk w = sh.walk[phase];
+      if (phase == 1 && w.more()) {
+        if (leader) ok = barrier_wait(g.barrier, hidden_target, abortp);
+        if (!__all_sync(0xffffffffu, ok)) break;
+      }
 #pragma unroll 1
-        for (; w.more(); w.next(), ++it) {
+      for (; w.more(); w.next()) {
+        ok = __all_sync(0xffffffffu, wait_or_abort(smem_addr(&sh.empty[s]), parity, abortp));
+        if (!ok) break;
+        if (leader) {
           const int e = sh.active[w.a], n = __popcll(sh.mask[e]), row0 = sh.first_row[e];
-          const uint32_t s = it % P::kStages, use = it / P::kStages;
-          if (use > 0 && !wait_or_abort(smem_addr(&sh.empty[s]), (use - 1u) & 1u, abortp)) break;
           const uint32_t st = base + s * P::kStageBytes + 2 * kBox, bar = smem_addr(&sh.full[s]);
           const int np = (n + 15) & ~15, last = row0 + n - 1;
           mbar_arrive_expect_tx(bar, (uint32_t)np * 128u);
@@ -549,38 +554,43 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
             for (int c = 0; c < np; c += 16)
               tc::tma_load_2d(st + (uint32_t)c * 128u, &map_h, w.kb * 128, row0 + c, bar);
           }
-          sh.issued_a = it + 1;
+          ++sh.issued_a;
         }
+        if (++s == P::kStages) s = 0, parity ^= 1;
       }
     }
   } else if (warp == 10) {
     // ---- MMAs
-    if (lane == 0) {
-      uint32_t it = 0;
-      bool ok = true;
+    const bool leader = tc::elect_one();
+    const uint32_t lo0 = tc::sw128_lo(base), hi = tc::sw128_hi();
+    uint32_t s = 0, parity = 0, buf = 0, buf_parity = 1;
+    bool ok = true;
 #pragma unroll 1
-      for (int phase = 0; phase < 2 && ok; ++phase) {
+    for (int phase = 0; phase < 2 && ok; ++phase) {
+      uint32_t idesc = 0;
 #pragma unroll 1
-        for (Walk w = sh.walk[phase]; w.more(); w.next(), ++it) {
-          const int np = (__popcll(sh.mask[sh.active[w.a]]) + 15) & ~15;
-          const uint32_t s = it % P::kStages, buf = it % kBufs;
-          ok = wait_or_abort(smem_addr(&sh.full[s]), (it / P::kStages) & 1u, abortp) &&
-               (it < kBufs ||
-                wait_or_abort(smem_addr(&sh.acc_empty[buf]), (it / kBufs - 1u) & 1u, abortp));
-          if (!ok) break;
-          tc::fence_after();
-          const uint32_t st = base + s * P::kStageBytes, idesc = tc::f8_idesc(128, np);
+      for (Walk w = sh.walk[phase]; w.more(); w.next()) {
+        if (idesc == 0 || w.kb == 0)
+          idesc = tc::f8_idesc(128, (__popcll(sh.mask[sh.active[w.a]]) + 15) & ~15);
+        ok = __all_sync(0xffffffffu, wait_or_abort(smem_addr(&sh.full[s]), parity, abortp) &&
+                                         wait_or_abort(smem_addr(&sh.acc_empty[buf]), buf_parity, abortp));
+        if (!ok) break;
+        tc::fence_after();
+        if (leader) {
+          const uint32_t lo = lo0 + s * (P::kStageBytes >> 4);
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
-              tc::mma_f8(tmem + buf * 2 * NMAX + h * NMAX,
-                         smem_desc(st + h * kBox + 32u * kk, 16, 1024, kLayoutSw128),
-                         smem_desc(st + 2 * kBox + 32u * kk, 16, 1024, kLayoutSw128), idesc, kk != 0);
+              tc::mma_f8(tmem + buf * 2 * NMAX + h * NMAX, lo + h * (kBox >> 4) + 2 * kk,
+                         lo + 2 * (kBox >> 4) + 2 * kk, hi, idesc, kk != 0);
           tc::commit(smem_addr(&sh.empty[s]));
           tc::commit(smem_addr(&sh.acc_full[buf]));
-          sh.committed = it + 1;
+          ++sh.committed;
         }
+        __syncwarp();
+        if (++s == P::kStages) s = 0, parity ^= 1;
+        if (++buf == kBufs) buf = 0, buf_parity ^= 1;
       }
     }
   } else if (warp == 11) {

@@ -48,12 +48,33 @@ __host__ __device__ constexpr uint32_t f8_idesc(int M, int N) {
          | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 
-__device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
+// One lane of the (converged) warp; the same lane every time. Code that issues
+// MMAs keeps the whole warp in its loop and predicates the issue on this:
+// descriptors then stay in uniform registers, which a loop run by one lane
+// does not give (a 128 x 16 x 32 MMA took 90 cycles to issue there).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(r));
+  return r != 0;
+}
+
+// Operand descriptors as 32-bit halves: `lo` is the address (16-byte units) and
+// the leading offset, so that K steps and stages are additions to it; `hi` is
+// common to every 128-byte swizzled K-major operand (8-row groups 1 KB apart).
+__device__ __forceinline__ uint32_t sw128_lo(uint32_t addr) {
+  return (uint32_t)smem_desc(addr, 16, 1024, kLayoutSw128);
+}
+__device__ __forceinline__ uint32_t sw128_hi() {
+  return (uint32_t)(smem_desc(0, 16, 1024, kLayoutSw128) >> 32);
+}
+
+__device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t hi,
                                        uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}" ::"r"(d_tmem),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "{\n .reg .pred p;\n .reg .b64 a, b;\n mov.b64 a, {%1, %3};\n mov.b64 b, {%2, %3};\n"
+      " setp.ne.b32 p, %5, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %4, p;\n}" ::"r"(d_tmem),
+      "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 
