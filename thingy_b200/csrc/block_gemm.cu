@@ -36,7 +36,7 @@ __device__ __forceinline__ bool wait_or_abort(uint32_t bar, uint32_t parity,
 
 // ------------------------------------------------------------------ tiled
 //
-// Persistent CTAs of 10 warps, one an SM, each walking tiles of 128 x BN:
+// Persistent CTAs of 12 warps (the last one idle), one an SM, each walking tiles of 128 x BN:
 //  * warp 8, one thread: TMA of the A box and the BN / 128 B boxes of a K
 //    block into a ring of stages (128-byte swizzled rows; rows and columns
 //    past the matrices are zero-filled, so M, N and K may be any).
@@ -46,11 +46,16 @@ __device__ __forceinline__ bool wait_or_abort(uint32_t bar, uint32_t parity,
 //  * warps 0-7: the outer sum. Warp group g = warp / 4 keeps columns
 //    g BN/2 .. of the tile for its 128 rows, a row a thread, in BN / 2 fp32
 //    registers, and adds scale * buffer to them while the MMAs of the next K
-//    block fill the other buffer. The row's scale and the weight block's are
-//    loaded two K blocks ahead.
+//    block fill the other buffer.
+//  * warp 10: the scales, copied to a ring in shared memory up to kScaleSlots x
+//    kScaleBlocks K blocks ahead, so that the sums spend hardly an instruction
+//    on them (one wait in kScaleBlocks blocks).
 // Tiles are walked in bands of kBand rows of tiles, so that the CTAs of a
 // wave share their operands in L2.
-constexpr int kThreads = 320, kEpiWarps = 8, kBand = 16;
+constexpr int kThreads = 384, kEpiWarps = 8, kBand = 16;
+// registers a thread: 2 x 128 x 216 + 128 x 64 = 63488 of the 384 x 168 = 64512 at launch
+constexpr int kEpiRegs = 216, kIssueRegs = 64;
+constexpr int kScaleSlots = 3, kScaleBlocks = 4;  // ring slots, K blocks a slot
 
 template <int BN>
 struct TilePlan {
@@ -60,7 +65,9 @@ struct TilePlan {
   static constexpr size_t kSmemBytes = kStages * kStageBytes + 1024;
   static constexpr uint32_t kTmemCols = 2 * BN;
   static constexpr int kCols = BN / 2;  // columns of a warp group
-  static_assert(kSmemBytes <= 225 * 1024, "shared memory");
+  // scales of a K block: 128 rows', then the columns' (a scale each, or a block's)
+  static constexpr int kScales = 128 + BN;
+  static_assert(kSmemBytes + kScaleSlots * kScaleBlocks * kScales * 4 + 512 <= 227 * 1024, "shared memory");
 };
 
 struct TileArgs {
@@ -141,7 +148,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ __align__(8) uint64_t empty_bar[P::kStages];
   __shared__ __align__(8) uint64_t acc_full[2];
   __shared__ __align__(8) uint64_t acc_empty[2];
-  __shared__ __align__(16) float sb_rows[SB_ROWS ? 2 : 1][SB_ROWS ? BN : 1];
+  __shared__ __align__(8) uint64_t scale_full[kScaleSlots];
+  __shared__ __align__(8) uint64_t scale_empty[kScaleSlots];
+  __shared__ __align__(16) float scales[kScaleSlots][kScaleBlocks][P::kScales];
   __shared__ uint32_t tmem_base_slot;
   __shared__ uint32_t abort_flag;
   __shared__ uint32_t issued;     // K blocks whose copies were issued
@@ -163,6 +172,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(smem_addr(&acc_full[b]), 1);
       mbar_init(smem_addr(&acc_empty[b]), kEpiWarps);
     }
+    for (int s = 0; s < kScaleSlots; ++s) {
+      mbar_init(smem_addr(&scale_full[s]), 32);
+      mbar_init(smem_addr(&scale_empty[s]), kEpiWarps);
+    }
     abort_flag = 0;
     issued = committed = 0;
     mbar_init_fence();
@@ -175,6 +188,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   griddep_wait();
   griddep_launch_dependents();
 
+  if (warp >= kEpiWarps) {
+    tc::regs_down<kIssueRegs>();
   if (warp == kEpiWarps) {
     // ---- operands
     const bool leader = tc::elect_one();
@@ -233,89 +248,135 @@ __global__ void __launch_bounds__(kThreads, 1)
         buf_parity ^= buf == 0;
       }
     }
+  } else if (warp == kEpiWarps + 2) {
+    // ---- scales; those of rows and columns past the matrices are left as they are
+    uint32_t s = 0, parity = 1;
+    bool ok = true;
+    constexpr int kNS = SB_ROWS ? BN / 32 : 1;
+    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      int tm, tn;
+      tile_at(t, g.tiles_m, g.tiles_n, &tm, &tn);
+      const float *pa[4], *pb[kNS];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = tm * kBM + lane + 32 * i;
+        pa[i] = row < g.M ? g.sa + (int64_t)row * g.sa_row : nullptr;
+      }
+#pragma unroll
+      for (int i = 0; i < kNS; ++i) {
+        const int col = tn * BN + (SB_ROWS ? lane + 32 * i : 128 * lane);
+        const bool some = col < g.N && (SB_ROWS || lane < P::kNB);
+        pb[i] = some ? g.sb + (int64_t)(SB_ROWS ? col : col / 128) * g.sb_row : nullptr;
+      }
+      for (int kb = 0; kb < g.KB; ++kb) {
+        const int j = kb % kScaleBlocks;
+        if (j == 0) {
+          ok = __all_sync(0xffffffffu, wait_or_abort(smem_addr(&scale_empty[s]), parity, abortp));
+          if (!ok) break;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (pa[i] != nullptr) {
+            tc::cp_async_4(smem_addr(&scales[s][j][lane + 32 * i]), pa[i]);
+            pa[i] += g.sa_kb;
+          }
+#pragma unroll
+        for (int i = 0; i < kNS; ++i)
+          if (pb[i] != nullptr) {
+            tc::cp_async_4(smem_addr(&scales[s][j][128 + lane + 32 * i]), pb[i]);
+            pb[i] += g.sb_kb;
+          }
+        if (j == kScaleBlocks - 1 || kb == g.KB - 1) {
+          tc::cp_async_arrive(smem_addr(&scale_full[s]));
+          if (++s == kScaleSlots) s = 0, parity ^= 1;
+        }
+      }
+    }
+    tc::cp_async_wait_all();
+  }
   } else {
     // ---- the outer sum
+    tc::regs_up<kEpiRegs>();
     const int wg = warp >> 2, r = (warp & 3) * 32 + lane;
     const uint32_t tm_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(wg * NC);
-    uint32_t it = 0;
-    // a cursor two K blocks ahead of the sum, over this CTA's tiles
-    int pf_t = blockIdx.x, pf_kb = 0;
-    const float *pf_a = nullptr, *pf_b = nullptr;
-    bool pf_row = false, pf_b_ok = false;
-    auto pf_tile = [&] {
-      int tm, tn;
-      tile_at(pf_t, g.tiles_m, g.tiles_n, &tm, &tn);
-      const int row = tm * kBM + r, col = tn * BN + wg * NC;
-      pf_row = row < g.M;
-      pf_a = g.sa + (int64_t)row * g.sa_row;
-      if (SB_ROWS) {
-        // thread r of the group loads the scale of its r-th column
-        pf_b_ok = r < NC && col + r < g.N;
-        pf_b = g.sb + (int64_t)(col + r) * g.sb_row;
-      } else {
-        pf_b_ok = col < g.N;
-        pf_b = g.sb + (int64_t)(col / 128) * g.sb_row;
-      }
+    // The buffer is read in pieces of 32 columns, each load issued before the
+    // sums of the piece before it, the first of the next K block before those
+    // of the last of this one: no sum waits for its own load's latency. `lo`
+    // and `hi` take turns. After an abort the waits return at once and the
+    // loads go on (tensor memory is still this CTA's).
+    uint32_t lo[32], hi[32];
+    uint32_t buf = 0, buf_parity = 0, slot = 0, slot_parity = 0;
+    float sc = 0.f;  // the row's scale of the block, times the column block's
+    const float* sb = nullptr;  // the columns' scales of the block
+    const bool first = lane == 0;
+    // K block kb of a tile: its first load, and its scales
+    auto begin_block = [&](int kb) {
+      const int j = kb % kScaleBlocks;
+      if (j == 0) wait_or_abort(smem_addr(&scale_full[slot]), slot_parity, abortp);
+      wait_or_abort(smem_addr(&acc_full[buf]), buf_parity, abortp);
+      __syncwarp();
+      tc::fence_after();
+      tc::tmem_ld32_async(tm_lane + buf * BN, lo);
+      sc = scales[slot][j][r];
+      sb = &scales[slot][j][128 + (SB_ROWS ? wg * NC : wg * NC / 128)];
+      if (!SB_ROWS) sc *= *sb;
     };
-    auto pf_next = [&]() -> float2 {
-      if (pf_t >= tiles) return make_float2(0.f, 0.f);
-      if (pf_kb == 0) pf_tile();
-      const float2 v = make_float2(pf_row ? __ldg(pf_a + pf_kb * g.sa_kb) : 0.f,
-                                   pf_b_ok ? __ldg(pf_b + pf_kb * g.sb_kb) : 0.f);
-      if (++pf_kb == g.KB) pf_kb = 0, pf_t += gridDim.x;
-      return v;
-    };
-    float2 s0 = pf_next(), s1 = pf_next();
-    bool ok = true;
-    // after an abort the SB_ROWS form still walks to the end (its waits return
-    // at once): every warp of a group passes the same number of barriers
-    for (int t = blockIdx.x; t < tiles && (SB_ROWS || ok); t += gridDim.x) {
+    if ((int)blockIdx.x < tiles) begin_block(0);
+    for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
       float2 acc[NC / 2];
 #pragma unroll
       for (int i = 0; i < NC / 2; ++i) acc[i] = make_float2(0.f, 0.f);
-      for (int kb = 0; kb < g.KB; ++kb, ++it) {
-        const uint32_t buf = it & 1u;
-        const float2 s2 = pf_next();
-        float sc = SB_ROWS ? s0.x : s0.x * s0.y;
-        if (SB_ROWS) {
-          // the group's column scales of this K block; two slots: the slot is
-          // rewritten two blocks later, behind the next block's barrier
-          if (r < NC) sb_rows[buf][wg * NC + r] = s0.y;
-          asm volatile("barrier.cta.sync %0, 128;" ::"r"(1 + wg) : "memory");
-        }
-        ok = ok && __all_sync(0xffffffffu, wait_or_abort(smem_addr(&acc_full[buf]),
-                                                         (it >> 1) & 1u, abortp));
-        if (!SB_ROWS && !ok) break;
-        tc::fence_after();
-        const float2 sc2 = make_float2(sc, sc);
-        if (ok) {
+      for (int kb = 0; kb < g.KB; ++kb) {
+        const bool last = kb == g.KB - 1;
+        auto add = [&](int c, const uint32_t(&v)[32], float s, const float* col) {
+          const float2 s2 = make_float2(s, s);
 #pragma unroll
-          for (int c = 0; c < NC; c += 16) {
-            uint32_t v[16];
-            tc::tmem_ld16_async(tm_lane + buf * BN + (uint32_t)c, v);
-            tc::tmem_ld_wait(v);
-            if (c + 16 == NC) {
-              tc::fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(smem_addr(&acc_empty[buf]));
+          for (int i = 0; i < 16; i += 2) {
+            float2 d0 = make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+            float2 d1 = make_float2(__uint_as_float(v[2 * i + 2]), __uint_as_float(v[2 * i + 3]));
+            if (SB_ROWS) {
+              const float4 f = *reinterpret_cast<const float4*>(col + c + 2 * i);
+              d0 = __fmul2_rn(d0, make_float2(f.x, f.y));
+              d1 = __fmul2_rn(d1, make_float2(f.z, f.w));
             }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              float2 d = make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
-              if (SB_ROWS)
-                d = __fmul2_rn(d, *reinterpret_cast<const float2*>(&sb_rows[buf][wg * NC + c + 2 * i]));
-              acc[c / 2 + i] = __ffma2_rn(d, sc2, acc[c / 2 + i]);
-            }
+            acc[c / 2 + i] = __ffma2_rn(d0, s2, acc[c / 2 + i]);
+            acc[c / 2 + i + 1] = __ffma2_rn(d1, s2, acc[c / 2 + i + 1]);
           }
+        };
+#pragma unroll
+        for (int c = 0; c < NC - 64; c += 64) {
+          tc::tmem_ld_wait(lo);
+          tc::tmem_ld32_async(tm_lane + buf * BN + (uint32_t)(c + 32), hi);
+          add(c, lo, sc, sb);
+          tc::tmem_ld_wait(hi);
+          tc::tmem_ld32_async(tm_lane + buf * BN + (uint32_t)(c + 64), lo);
+          add(c + 32, hi, sc, sb);
         }
-        s0 = s1;
-        s1 = s2;
+        tc::tmem_ld_wait(lo);
+        tc::tmem_ld32_async(tm_lane + buf * BN + (uint32_t)(NC - 32), hi);
+        add(NC - 64, lo, sc, sb);
+        tc::tmem_ld_wait(hi);
+        // all of the buffer is in registers
+        tc::fence_before();
+        __syncwarp();
+        tc::arrive_if(first, smem_addr(&acc_empty[buf]));
+        buf ^= 1;
+        buf_parity ^= buf == 0;
+        const bool slot_done = last || kb % kScaleBlocks == kScaleBlocks - 1;
+        const uint32_t done = smem_addr(&scale_empty[slot]);
+        const float s = sc;
+        const float* col = sb;
+        if (slot_done && ++slot == kScaleSlots) slot = 0, slot_parity ^= 1;
+        if (!last || t + (int)gridDim.x < tiles) begin_block(last ? 0 : kb + 1);
+        add(NC - 32, hi, s, col);
+        if (slot_done) {
+          __syncwarp();
+          tc::arrive_if(first, done);
+        }
       }
-      if (ok) {
-        int tm, tn;
-        tile_at(t, g.tiles_m, g.tiles_n, &tm, &tn);
-        store_row<NC>(g, acc, tm * kBM + r, tn * BN + wg * NC);
-      }
+      int tm_i, tn_i;
+      tile_at(t, g.tiles_m, g.tiles_n, &tm_i, &tn_i);
+      if (*abortp == 0u) store_row<NC>(g, acc, tm_i * kBM + r, tn_i * BN + wg * NC);
     }
   }
   __syncwarp();

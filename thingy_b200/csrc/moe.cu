@@ -29,7 +29,7 @@
 // Warps: 0-7 the outer sums (warps 0-3 the first 128 rows of an item, 4-7 the
 // second, a row a thread) and the epilogues; 8 the weight tiles (TMA); 9 the
 // tokens' rows (TMA gather of 4 rows for the first product, boxes of 16 hidden
-// rows for the second); 10 the MMAs; 11 the products of the scales.
+// rows for the second); 10 the MMAs; 11 the scales.
 #include "cutie.h"
 #include "launch.cuh"
 #include "tcgen05.cuh"
@@ -43,6 +43,7 @@ namespace {
 constexpr int kMoeThreads = 384, kMoeWarps = 12, kEpiThreads = 256;
 constexpr uint32_t kBox = 128 * 128;  // a 128-row weight tile of one K block
 constexpr int kBufs = 4;              // accumulator buffers in tensor memory
+constexpr int kScaleSlots = 8;        // units whose scales are on their way or in use
 constexpr int kXStride = 132;         // floats between columns of the exchange
 constexpr int kMaxE = kMoeMaxExperts, kMaxK = kMoeMaxTopK;
 constexpr int kChooseTokens = 8;  // tokens up to which every CTA makes all choices
@@ -90,8 +91,9 @@ struct Walk {
 
 template <int NMAX>
 struct MoeShared {
-  uint64_t full[8], empty[8], acc_full[kBufs], acc_empty[kBufs], scale_full[kBufs];
-  float scales[kBufs][2][NMAX];
+  uint64_t full[8], empty[8], acc_full[kBufs], acc_empty[kBufs];
+  uint64_t scale_full[kScaleSlots], scale_empty[kScaleSlots];
+  float scales[kScaleSlots][NMAX + 4];  // the tokens', then the two weight tiles'
   uint64_t mask[kMaxE];       // tokens of an expert
   float weight[MoePlan<NMAX>::kPairs];
   uint16_t ids[MoePlan<NMAX>::kPairs];     // expert of (token, slot)
@@ -395,7 +397,10 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
     for (int b = 0; b < kBufs; ++b) {
       mbar_init(smem_addr(&sh.acc_full[b]), 1);
       mbar_init(smem_addr(&sh.acc_empty[b]), 8);
-      mbar_init(smem_addr(&sh.scale_full[b]), 1);
+    }
+    for (int s = 0; s < kScaleSlots; ++s) {
+      mbar_init(smem_addr(&sh.scale_full[s]), 32);
+      mbar_init(smem_addr(&sh.scale_empty[s]), 8);
     }
     sh.abort_flag = 0;
     sh.issued_w = sh.issued_a = sh.committed = 0;
@@ -594,31 +599,26 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
       }
     }
   } else if (warp == 11) {
-    // ---- scale products: a token's (or hidden row's) scale of the K block
-    // times each 128-row tile's, loaded kAhead units ahead (they come from HBM)
-    uint32_t it = 0;
+    // ---- scales of a unit: each token's (or hidden row's) of the K block and the
+    // two weight tiles', copied to a ring slot kScaleSlots units ahead of their
+    // use (they come from HBM), a copy a lane
+    constexpr int NL = (NMAX + 31) / 32;
+    uint32_t s = 0, parity = 1;
     bool ok = true;
-    constexpr int NL = (NMAX + 31) / 32, kAhead = 8;
-    struct Vals {
-      float a[NL], w0, w1;
-    };
 #pragma unroll 1
     for (int phase = 0; phase < 2 && ok; ++phase) {
-      // a cursor kAhead units ahead of the products; addresses change at items only
       Walk w = sh.walk[phase];
-      int left = w.end - w.u, n = 0;
-      if (phase == 1 && left > 0) {
-        int pass = 1;
-        if (lane == 0) pass = barrier_wait(g.barrier, hidden_target, abortp);
-        if (!__shfl_sync(0xffffffffu, pass, 0)) break;
+      if (phase == 1 && w.more()) {
+        if (lane == 0) ok = barrier_wait(g.barrier, hidden_target, abortp);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
       }
-      bool two = true;
-      const float *pa[NL], *pw0 = nullptr, *pw1 = nullptr;
-#pragma unroll
-      for (int i = 0; i < NL; ++i) pa[i] = nullptr;
-      auto fetch = [&]() {
-        const bool some = w.more();
-        if (some && (w.kb == 0 || n == 0)) {
+      const int64_t step = phase == 0 ? g.sq_kb : 1;
+      const float *pa[NL], *pw = nullptr;
+      int n = 0;
+#pragma unroll 1
+      for (; w.more(); w.next()) {
+        if (n == 0 || w.kb == 0) {  // addresses change at items only
           const int e = sh.active[w.a], row0 = sh.first_row[e];
           n = __popcll(sh.mask[e]);
 #pragma unroll
@@ -626,45 +626,23 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
             const int row = row0 + min(lane + 32 * i, n - 1);
             pa[i] = phase == 0 ? g.q_scale + sh.token_at[row] * g.sq_row : g.h_scale + (int64_t)row * IG;
           }
-          pw0 = phase == 0 ? g.w13_scale + ((int64_t)e * 2 * IG + w.grp) * KB1
-                           : g.w2_scale + ((int64_t)e * (g.H / 128) + w.grp * 2) * KB2;
-          pw1 = pw0 + (phase == 0 ? (int64_t)IG * KB1 : KB2);
-          two = phase == 0 || w.grp * 2 + 1 < g.H / 128;
+          // lane 0: the first tile's row of blocks, lane 1: the second's
+          pw = phase == 0 ? g.w13_scale + ((int64_t)e * 2 * IG + w.grp + lane * IG) * KB1
+                          : g.w2_scale + ((int64_t)e * (g.H / 128) + w.grp * 2 + lane) * KB2;
+          if (lane >= (phase == 0 || w.grp * 2 + 1 < g.H / 128 ? 2 : 1)) pw = nullptr;
         }
-        Vals v;
-        const int64_t step = phase == 0 ? g.sq_kb : 1;
+        ok = __all_sync(0xffffffffu, wait_or_abort(smem_addr(&sh.scale_empty[s]), parity, abortp));
+        if (!ok) break;
 #pragma unroll
-        for (int i = 0; i < NL; ++i) v.a[i] = ld_l2_if(some && lane + 32 * i < n, pa[i] + w.kb * step);
-        v.w0 = ld_l2_if(some, pw0 + w.kb);
-        v.w1 = ld_l2_if(some && two, pw1 + w.kb);
-        w.next();
-        return v;
-      };
-      Vals v[kAhead];
-#pragma unroll
-      for (int i = 0; i < kAhead; ++i) v[i] = fetch();
-#pragma unroll 1
-      for (; left > 0 && ok; left -= kAhead) {
-#pragma unroll
-        for (int j = 0; j < kAhead; ++j) {
-          if (j >= left) break;
-          const uint32_t buf = it % kBufs;
-          ok = it < kBufs || __all_sync(0xffffffffu, wait_or_abort(smem_addr(&sh.acc_empty[buf]),
-                                                                   (it / kBufs - 1u) & 1u, abortp));
-          if (!ok) break;
-#pragma unroll
-          for (int i = 0; i < NL; ++i)
-            if (lane + 32 * i < NMAX) {
-              sh.scales[buf][0][lane + 32 * i] = v[j].a[i] * v[j].w0;
-              sh.scales[buf][1][lane + 32 * i] = v[j].a[i] * v[j].w1;
-            }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_addr(&sh.scale_full[buf]));
-          ++it;
-          v[j] = fetch();
-        }
+        for (int i = 0; i < NL; ++i)
+          if (lane + 32 * i < n)
+            tc::cp_async_4(smem_addr(&sh.scales[s][lane + 32 * i]), pa[i] + w.kb * step);
+        if (pw != nullptr) tc::cp_async_4(smem_addr(&sh.scales[s][NMAX + lane]), pw + w.kb);
+        tc::cp_async_arrive(smem_addr(&sh.scale_full[s]));
+        if (++s == kScaleSlots) s = 0, parity ^= 1;
       }
     }
+    tc::cp_async_wait_all();
   } else {
     // ---- outer sums and epilogues
     uint32_t it = 0;
@@ -684,21 +662,24 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
 #pragma unroll
           for (int c = 0; c < NMAX; ++c) acc[c] = 0.f;
         }
-        const uint32_t buf = it % kBufs, use = it / kBufs;
-        const bool ok = wait_or_abort(smem_addr(&sh.acc_full[buf]), use & 1u, abortp) &&
-                        wait_or_abort(smem_addr(&sh.scale_full[buf]), use & 1u, abortp);
+        const uint32_t buf = it % kBufs, slot = it % kScaleSlots;
+        const bool ok =
+            wait_or_abort(smem_addr(&sh.scale_full[slot]), (it / kScaleSlots) & 1u, abortp) &&
+            wait_or_abort(smem_addr(&sh.acc_full[buf]), (it / kBufs) & 1u, abortp);
         if (__all_sync(0xffffffffu, ok)) {
           tc::fence_after();
+          const float ws = sh.scales[slot][NMAX + half];
 #pragma unroll
           for (int c = 0; c < NMAX; c += 16) {
             if (c >= n) break;
             uint32_t v[16];
             tc::tmem_ld16_async(lane_base + buf * 2 * NMAX + (uint32_t)c, v);
-            const float4* sc = reinterpret_cast<const float4*>(&sh.scales[buf][half][c]);
-            const float4 f[4] = {sc[0], sc[1], sc[2], sc[3]};
+            const float4* sc = reinterpret_cast<const float4*>(&sh.scales[slot][c]);
+            float4 f[4] = {sc[0], sc[1], sc[2], sc[3]};
             tc::tmem_ld_wait(v);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
+              f[i].x *= ws, f[i].y *= ws, f[i].z *= ws, f[i].w *= ws;
               acc[c + 4 * i] = __fmaf_rn(__uint_as_float(v[4 * i]), f[i].x, acc[c + 4 * i]);
               acc[c + 4 * i + 1] = __fmaf_rn(__uint_as_float(v[4 * i + 1]), f[i].y, acc[c + 4 * i + 1]);
               acc[c + 4 * i + 2] = __fmaf_rn(__uint_as_float(v[4 * i + 2]), f[i].z, acc[c + 4 * i + 2]);
@@ -708,7 +689,10 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
           tc::fence_before();
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_addr(&sh.acc_empty[buf]));
+        if (lane == 0) {
+          mbar_arrive(smem_addr(&sh.acc_empty[buf]));
+          mbar_arrive(smem_addr(&sh.scale_empty[slot]));
+        }
         const bool to_end = w.kb == w.KB - 1;
         if (!to_end && w.u != w.end - 1) continue;
         // ---- the item, or this CTA's part of it, is complete
