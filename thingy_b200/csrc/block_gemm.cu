@@ -9,6 +9,8 @@
 // 128-wide K block is made by tcgen05.mma (kind::f8f6f4, fp32 accumulators in
 // tensor memory, overwritten by each block) and the outer sum by the epilogue
 // warps in fp32 registers, one FMA an element and block.
+#include <atomic>
+
 #include "cutie.h"
 #include "launch.cuh"
 #include "tcgen05.cuh"
@@ -415,6 +417,360 @@ cudaError_t launch_tiled(const CUtensorMap& map_a, const CUtensorMap& map_b, Til
                     map_a, map_b, g);
 }
 
+// ------------------------------------------------------------------ few rows
+//
+// At most 128 rows of A: bound by reading the weight once. The weight is the
+// 128-row side of the MMA and the batch its N side (BR = 16, 32, 64 or 128
+// columns, the smallest that holds the batch; rows past M are zero-filled), so
+// a K block costs 16 KB of weight and a batch box of BR rows. N / 128 tiles do
+// not fill the GPU, so K is split over a cluster of S CTAs, with two CTAs an SM
+// (one for BR > 32): every SM then has its share of the weight on the way at
+// once. Two K blocks share a ring stage and its barriers: the hand-over
+// between the warps, not the bytes, set the time of one-block stages.
+// The ranks' partial tiles are reduce-scattered: each rank owns a share of the
+// batch rows, the others send it theirs (bulk copies between shared memories,
+// no multicast), and it adds all in rank order, so the result does not depend
+// on timing.
+// Warps 0-3 sum (a weight row a thread), 4 issues TMA, 5 MMAs, 6 copies scales.
+constexpr int kFewRows = 128;  // rows up to which this form is taken
+constexpr int kFewThreads = 224, kFewScaleSlots = 3, kFewStep = 2, kMaxRanks = 8;
+
+template <int BR>
+struct FewPlan {
+  static constexpr int kCtas = BR <= 32 ? 2 : 1;  // an SM
+  static constexpr uint32_t kBlockBytes = kBoxBytes + BR * kBK;
+  static constexpr uint32_t kStageBytes = kFewStep * kBlockBytes;
+  static constexpr int kStages = BR == 64 ? 3 : 2;
+  // partial sums: batch row m, weight row r at m * 128 + r; this rank's in the
+  // ring once that is idle, the others' in a place of their own
+  static constexpr uint32_t kRowBytes = kBM * 4;
+  static constexpr uint32_t kOffRecv = kStages * kStageBytes;
+  static constexpr size_t kSmemBytes = kOffRecv + (BR + kMaxRanks) * kRowBytes + 1024;
+  static constexpr int kBufs = 2;  // of kFewStep x BR columns
+  static constexpr uint32_t kTmemCols = kBufs * kFewStep * BR;
+  static constexpr int kScales = BR + 4;  // the batch's, then the weight block's
+  static_assert(kCtas * kTmemCols <= 512, "tensor memory columns");
+  static_assert(kCtas * (kSmemBytes + kFewScaleSlots * kScaleBlocks * kScales * 4 + 1536) <= 227 * 1024,
+                "shared memory");
+  static_assert(BR * kRowBytes <= kOffRecv, "the partial tile fits the ring");
+};
+static_assert(kScaleBlocks % kFewStep == 0, "a stage's scales share a slot");
+
+template <int BR>
+__global__ void __launch_bounds__(kFewThreads, FewPlan<BR>::kCtas)
+    block_gemm_few_kernel(const __grid_constant__ CUtensorMap map_a,
+                          const __grid_constant__ CUtensorMap map_b, const TileArgs g) {
+  using P = FewPlan<BR>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t full_bar[P::kStages];
+  __shared__ __align__(8) uint64_t empty_bar[P::kStages];
+  __shared__ __align__(8) uint64_t acc_full[P::kBufs];
+  __shared__ __align__(8) uint64_t acc_empty[P::kBufs];
+  __shared__ __align__(8) uint64_t scale_full[kFewScaleSlots];
+  __shared__ __align__(8) uint64_t scale_empty[kFewScaleSlots];
+  __shared__ __align__(8) uint64_t recv_bar;
+  __shared__ __align__(16) float scales[kFewScaleSlots][kScaleBlocks][P::kScales];
+  __shared__ uint32_t tmem_base_slot;
+  __shared__ uint32_t abort_flag;
+  __shared__ uint32_t issued, committed;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
+  const int n0 = blockIdx.x * kBM, S = (int)gridDim.z;
+  const int rank = (int)tc::cluster_ctarank();  // = blockIdx.z: the cluster spans z
+  const int kb0 = (int)((int64_t)g.KB * rank / S), kb1 = (int)((int64_t)g.KB * (rank + 1) / S);
+  const int steps = (kb1 - kb0 + kFewStep - 1) / kFewStep;
+  // this rank's share of the batch rows
+  const int share = (g.M + S - 1) / S;
+  const int m_lo = min(rank * share, g.M), m_hi = min(m_lo + share, g.M);
+  volatile uint32_t* abortp = &abort_flag;
+
+  if (threadIdx.x == 0) {
+    tc::prefetch_map(&map_a);
+    tc::prefetch_map(&map_b);
+    for (int s = 0; s < P::kStages; ++s) {
+      mbar_init(smem_addr(&full_bar[s]), 1);
+      mbar_init(smem_addr(&empty_bar[s]), 1);
+    }
+    for (int b = 0; b < P::kBufs; ++b) {
+      mbar_init(smem_addr(&acc_full[b]), 1);
+      mbar_init(smem_addr(&acc_empty[b]), 4);
+    }
+    for (int s = 0; s < kFewScaleSlots; ++s) {
+      mbar_init(smem_addr(&scale_full[s]), 32);
+      mbar_init(smem_addr(&scale_empty[s]), 4);
+    }
+    mbar_init(smem_addr(&recv_bar), 1);
+    abort_flag = 0;
+    issued = committed = 0;
+    mbar_init_fence();
+    mbar_arrive_expect_tx(smem_addr(&recv_bar), (uint32_t)((S - 1) * (m_hi - m_lo)) * P::kRowBytes);
+  }
+  if (warp == 5) tc::tmem_alloc(smem_addr(&tmem_base_slot), P::kTmemCols);
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  if (S > 1) tc::cluster_arrive();  // this CTA's barriers are ready for the others' copies
+  const uint32_t tmem = tmem_base_slot;
+  griddep_wait();
+  griddep_launch_dependents();
+
+  if (warp == 4) {
+    const bool leader = tc::elect_one();
+    uint32_t s = 0, parity = 1;
+    for (int i = 0; i < steps; ++i) {
+      const bool ok = wait_or_abort(smem_addr(&empty_bar[s]), parity, abortp);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      if (leader) {
+        const int kb = kb0 + i * kFewStep, n = min(kFewStep, kb1 - kb);
+        uint32_t st = base + s * P::kStageBytes;
+        const uint32_t bar = smem_addr(&full_bar[s]);
+        mbar_arrive_expect_tx(bar, (uint32_t)n * P::kBlockBytes);
+        for (int j = 0; j < n; ++j, st += P::kBlockBytes) {
+          tc::tma_load_2d(st, &map_b, (kb + j) * kBK, n0, bar);
+          tc::tma_load_2d(st + kBoxBytes, &map_a, (kb + j) * kBK, 0, bar);
+        }
+        ++issued;
+      }
+      if (++s == P::kStages) s = 0, parity ^= 1;
+    }
+  } else if (warp == 5) {
+    const bool leader = tc::elect_one();
+    constexpr uint32_t idesc = tc::f8_idesc(kBM, BR);
+    const uint32_t lo0 = tc::sw128_lo(base), hi = tc::sw128_hi();
+    uint32_t s = 0, parity = 0, buf = 0, buf_parity = 1;
+    for (int i = 0; i < steps; ++i) {
+      const bool ok = wait_or_abort(smem_addr(&full_bar[s]), parity, abortp) &&
+                      wait_or_abort(smem_addr(&acc_empty[buf]), buf_parity, abortp);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      tc::fence_after();
+      if (leader) {
+        uint32_t lo = lo0 + s * (P::kStageBytes >> 4), d = tmem + buf * kFewStep * BR;
+        const int n = min(kFewStep, kb1 - kb0 - i * kFewStep);
+        for (int j = 0; j < n; ++j, lo += P::kBlockBytes >> 4, d += BR) {
+#pragma unroll
+          for (int kk = 0; kk < kBK / 32; ++kk)
+            tc::mma_f8(d, lo + 2 * kk, lo + (kBoxBytes >> 4) + 2 * kk, hi, idesc, kk != 0);
+        }
+        tc::commit(smem_addr(&empty_bar[s]));
+        tc::commit(smem_addr(&acc_full[buf]));
+        ++committed;
+      }
+      __syncwarp();
+      if (++s == P::kStages) s = 0, parity ^= 1;
+      if (++buf == P::kBufs) buf = 0, buf_parity ^= 1;
+    }
+  } else if (warp == 6) {
+    uint32_t s = 0, parity = 1;
+    constexpr int kNA = (BR + 31) / 32;
+    const float *pa[kNA], *pb = nullptr;
+#pragma unroll
+    for (int i = 0; i < kNA; ++i) {
+      const int row = lane + 32 * i;
+      pa[i] = row < g.M && row < BR ? g.sa + (int64_t)row * g.sa_row + kb0 * g.sa_kb : nullptr;
+    }
+    if (lane == 0) pb = g.sb + (int64_t)blockIdx.x * g.sb_row + kb0 * g.sb_kb;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      const int j = (kb - kb0) % kScaleBlocks;
+      if (j == 0) {
+        const bool ok = wait_or_abort(smem_addr(&scale_empty[s]), parity, abortp);
+        if (!__all_sync(0xffffffffu, ok)) break;
+      }
+#pragma unroll
+      for (int i = 0; i < kNA; ++i)
+        if (pa[i] != nullptr) {
+          tc::cp_async_4(smem_addr(&scales[s][j][lane + 32 * i]), pa[i]);
+          pa[i] += g.sa_kb;
+        }
+      if (pb != nullptr) {
+        tc::cp_async_4(smem_addr(&scales[s][j][BR]), pb);
+        pb += g.sb_kb;
+      }
+      if (j == kScaleBlocks - 1 || kb == kb1 - 1) {
+        tc::cp_async_arrive(smem_addr(&scale_full[s]));
+        if (++s == kFewScaleSlots) s = 0, parity ^= 1;
+      }
+    }
+    tc::cp_async_wait_all();
+  } else {
+    const int row = warp * 32 + lane;
+    const uint32_t tm_lane = tmem + ((uint32_t)(warp * 32) << 16);
+    uint32_t buf = 0, buf_parity = 0, slot = 0, slot_parity = 0;
+    float2 acc[BR / 2];
+#pragma unroll
+    for (int c = 0; c < BR / 2; ++c) acc[c] = make_float2(0.f, 0.f);
+    bool ok = true;
+    for (int kb = kb0; kb < kb1; kb += kFewStep) {
+      const int j0 = (kb - kb0) % kScaleBlocks;
+      ok = (j0 != 0 || wait_or_abort(smem_addr(&scale_full[slot]), slot_parity, abortp)) &&
+           wait_or_abort(smem_addr(&acc_full[buf]), buf_parity, abortp);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc::fence_after();
+#pragma unroll
+      for (int j = 0; j < kFewStep; ++j) {
+        if (kb + j >= kb1) break;
+        const float* sc = scales[slot][j0 + j];
+        const float2 sw = make_float2(sc[BR], sc[BR]);
+#pragma unroll
+        for (int c = 0; c < BR; c += 16) {
+          if (c >= g.M) break;
+          uint32_t v[16];
+          tc::tmem_ld16_async(tm_lane + (buf * kFewStep + j) * BR + (uint32_t)c, v);
+          float2 f[8];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float4 q = *reinterpret_cast<const float4*>(sc + c + 4 * i);
+            f[2 * i] = __fmul2_rn(make_float2(q.x, q.y), sw);
+            f[2 * i + 1] = __fmul2_rn(make_float2(q.z, q.w), sw);
+          }
+          tc::tmem_ld_wait(v);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            acc[c / 2 + i] = __ffma2_rn(
+                make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), f[i],
+                acc[c / 2 + i]);
+        }
+      }
+      tc::fence_before();
+      __syncwarp();
+      tc::arrive_if(lane == 0, smem_addr(&acc_empty[buf]));
+      if (++buf == P::kBufs) buf = 0, buf_parity ^= 1;
+      if (j0 + kFewStep == kScaleBlocks) {
+        tc::arrive_if(lane == 0, smem_addr(&scale_empty[slot]));
+        if (++slot == kFewScaleSlots) slot = 0, slot_parity ^= 1;
+      }
+    }
+    auto store = [&](int m, float v) {
+      if (n0 + row >= g.N) return;
+      const int64_t at = (int64_t)m * g.ldd + n0 + row;
+      if (g.d_f32) {
+        float* p = static_cast<float*>(g.d) + at;
+        *p = g.accumulate ? *p + v : v;
+      } else {
+        static_cast<uint16_t*>(g.d)[at] = (uint16_t)(f2_to_bf2(make_float2(v, 0.f)) & 0xffffu);
+      }
+    };
+    if (S == 1) {
+      if (ok) {
+#pragma unroll
+        for (int c = 0; c < BR; ++c)
+          if (c < g.M) store(c, c & 1 ? acc[c / 2].y : acc[c / 2].x);
+      }
+    } else {
+      // the last accumulator was complete, so every copy and MMA of the ring is done
+      float* part = reinterpret_cast<float*>(smem_raw + (base - smem_addr(smem_raw)));
+      asm volatile("barrier.cta.sync 1, 128;" ::: "memory");  // all four warps are past the ring
+#pragma unroll
+      for (int c = 0; c < BR; ++c)
+        if (c < g.M) part[c * kBM + row] = c & 1 ? acc[c / 2].y : acc[c / 2].x;
+      tc::fence_async_smem();
+      asm volatile("barrier.cta.sync 1, 128;" ::: "memory");
+      tc::cluster_wait();  // every CTA's barriers exist
+      const uint32_t recv = base + P::kOffRecv;
+      if (threadIdx.x == 0 && ok) {
+        for (int q = 0; q < S; ++q) {
+          const int lo = min(q * share, g.M), n = min(lo + share, g.M) - lo;
+          if (q == rank || n == 0) continue;
+          tc::bulk_s2c(tc::mapa(recv + (uint32_t)(rank * share) * P::kRowBytes, (uint32_t)q),
+                       smem_addr(part + lo * kBM), (uint32_t)n * P::kRowBytes,
+                       tc::mapa(smem_addr(&recv_bar), (uint32_t)q));
+        }
+      }
+      ok = __all_sync(0xffffffffu, wait_or_abort(smem_addr(&recv_bar), 0u, abortp)) && ok;
+      tc::cluster_arrive();  // what the others sent has arrived
+      if (ok) {
+        const float* in = reinterpret_cast<const float*>(smem_raw + (recv - smem_addr(smem_raw)));
+        for (int m = m_lo; m < m_hi; ++m) {
+          float v = 0.f;
+#pragma unroll
+          for (int q = 0; q < kMaxRanks; ++q)
+            if (q < S)
+              v += q == rank ? part[m * kBM + row] : in[(q * share + m - m_lo) * kBM + row];
+          store(m, v);
+        }
+      }
+    }
+  }
+  __syncwarp();
+  if (S > 1) {
+    if (warp >= 4) {
+      tc::cluster_wait();
+      tc::cluster_arrive();
+    }
+    tc::cluster_wait();  // what this CTA sent has arrived: its memory may go
+  }
+  tc::fence_before();
+  __syncthreads();
+  if (*abortp) {
+    if (threadIdx.x == 0) {
+      atomicCAS(&g_block_gemm_device_error, kDevErrNone, kDevErrBulkWaitTimeout);
+      const uint32_t n = issued, m = committed;  // copies and MMAs in flight finish first
+      for (uint32_t k = n > P::kStages ? n - P::kStages : 0; k < n; ++k)
+        mbar_wait_bounded(smem_addr(&full_bar[k % P::kStages]), (k / P::kStages) & 1u,
+                          kDrainLimitCycles);
+      if (m > 0)
+        mbar_wait_bounded(smem_addr(&acc_full[(m - 1) % P::kBufs]), ((m - 1) / P::kBufs) & 1u,
+                          kDrainLimitCycles);
+    }
+    __syncthreads();
+  }
+  if (warp == 5) tc::tmem_dealloc(tmem, P::kTmemCols);
+}
+
+// Clusters of S CTAs that run at once on the current device.
+template <int BR>
+int few_clusters(int S, const cudaLaunchConfig_t& base) {
+  static std::atomic<int> cache[64][kMaxRanks + 1];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  if (dev < 64 && cache[dev][S].load(std::memory_order_relaxed) > 0) return cache[dev][S].load();
+  cudaLaunchConfig_t cfg = base;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 1;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = (unsigned)S;
+  cfg.gridDim = dim3(1, 1, (unsigned)S);
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, block_gemm_few_kernel<BR>, &cfg) != cudaSuccess) return 0;
+  if (dev < 64) cache[dev][S].store(n);
+  return n;
+}
+
+template <int BR>
+cudaError_t launch_few(const CUtensorMap& map_a, const CUtensorMap& map_b, const TileArgs& g,
+                       cudaStream_t stream) {
+  using P = FewPlan<BR>;
+  auto kernel = block_gemm_few_kernel<BR>;
+  const cudaError_t e =
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)P::kSmemBytes);
+  if (e != cudaSuccess) return e;
+  const int tiles = (g.N + kBM - 1) / kBM;
+  cudaLaunchConfig_t cfg{};
+  cfg.blockDim = dim3(kFewThreads);
+  cfg.dynamicSmemBytes = P::kSmemBytes;
+  cfg.stream = stream;
+  // the most ranks with which all tiles still run at once, a full stage a rank
+  // at least: one cluster more than fit doubles the time (5120 x 5120, 1 row:
+  // 6 ranks 16 us, 7 ranks 20 us)
+  int S = kMaxRanks;
+  while (S > 1 && (S * kFewStep > g.KB || few_clusters<BR>(S, cfg) < tiles)) --S;
+  cfg.gridDim = dim3((unsigned)tiles, 1, (unsigned)S);
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 1;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = (unsigned)S;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, kernel, map_a, map_b, g);
+}
+
 }  // namespace
 
 cudaError_t device_error_block_gemm(int* out, bool clear) {
@@ -430,8 +786,10 @@ cudaError_t device_error_block_gemm(int* out, bool clear) {
 }
 
 int block_gemm(const BlockGemmArgs& p, cudaStream_t stream, const char** why) {
+  const bool few = p.M <= kFewRows && !p.b_rows;
+  const int columns = p.M <= 16 ? 16 : p.M <= 32 ? 32 : p.M <= 64 ? 64 : 128;
   CUtensorMap map_a, map_b;
-  if (!tc::encode_e4m3_operand(&map_a, p.a, p.M, p.K, p.lda, kBM) ||
+  if (!tc::encode_e4m3_operand(&map_a, p.a, p.M, p.K, p.lda, few ? columns : kBM) ||
       !tc::encode_e4m3_operand(&map_b, p.b, p.N, p.K, p.ldb, kBM)) {
     *why = "cuTensorMapEncodeTiled failed for an operand";
     return CUTIE_ERR_CUDA;
@@ -447,11 +805,17 @@ int block_gemm(const BlockGemmArgs& p, cudaStream_t stream, const char** why) {
   // 256-wide tiles while every SM still gets one, else 128-wide ones
   const int64_t tm = (p.M + kBM - 1) / kBM;
   const bool wide = tm * ((p.N + 255) / 256) >= device_sm_count();
-  const cudaError_t e =
-      wide ? (p.b_rows ? launch_tiled<256, true>(map_a, map_b, g, stream)
-                       : launch_tiled<256, false>(map_a, map_b, g, stream))
-           : (p.b_rows ? launch_tiled<128, true>(map_a, map_b, g, stream)
-                       : launch_tiled<128, false>(map_a, map_b, g, stream));
+  cudaError_t e;
+  if (few)
+    e = columns == 16   ? launch_few<16>(map_a, map_b, g, stream)
+        : columns == 32 ? launch_few<32>(map_a, map_b, g, stream)
+        : columns == 64 ? launch_few<64>(map_a, map_b, g, stream)
+                        : launch_few<128>(map_a, map_b, g, stream);
+  else
+    e = wide ? (p.b_rows ? launch_tiled<256, true>(map_a, map_b, g, stream)
+                         : launch_tiled<256, false>(map_a, map_b, g, stream))
+             : (p.b_rows ? launch_tiled<128, true>(map_a, map_b, g, stream)
+                         : launch_tiled<128, false>(map_a, map_b, g, stream));
   if (e != cudaSuccess) {
     *why = cudaGetErrorString(e);
     return CUTIE_ERR_CUDA;
