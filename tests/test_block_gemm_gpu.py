@@ -400,6 +400,10 @@ def test_linear_with_cached_weight_leading_dimensions_and_partial_gradients():
     assert dw.shape == w.shape
     with pytest.raises(ValueError, match="transposed"):
         torch.autograd.grad(tb.fp8_linear(xg, w, (*cached[:2], None, None)), xg, torch.ones_like(y))
+    with torch.no_grad():
+        assert not tb.fp8_linear(xg, wg).requires_grad
+    with pytest.raises(RuntimeError, match="second derivatives"):
+        torch.autograd.grad(tb.fp8_linear(xg, w), xg, torch.ones_like(y), create_graph=True)
 
 
 def test_linear_without_tokens():

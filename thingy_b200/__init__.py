@@ -31,12 +31,11 @@ from .fp8_utils import (per_block_cast_to_fp8, per_token_cast_to_fp8, per_token_
 from .fused import empty_scale, residual_rms_norm_fp8, rms_norm_fp8
 from .gemm import fp8_block_gemm
 from .layouts import mx_swizzle, mx_swizzle_offset, mx_swizzled_size, mx_unswizzle
-from .linear import FP8Linear, fp8_linear
+from .linear import fp8_linear
 from .moe import moe_fp8, moe_workspace, quantize_experts
 from .rms_norm import RMSNorm, rms_norm, rms_norm_on_stream
 
 __all__ = [
-    "FP8Linear",
     "RMSNorm",
     "ResidualRMSNormFP8",
     "empty_scale",

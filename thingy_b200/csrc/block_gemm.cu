@@ -402,13 +402,16 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 template <int BN, bool SB_ROWS>
-cudaError_t launch_tiled(const CUtensorMap& map_a, const CUtensorMap& map_b, TileArgs g,
-                         cudaStream_t stream) {
+cudaError_t launch_tiled(const BlockGemmArgs& p, TileArgs g, cudaStream_t stream) {
   using P = TilePlan<BN>;
   auto kernel = block_gemm_kernel<BN, SB_ROWS>;
   const cudaError_t e =
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)P::kSmemBytes);
   if (e != cudaSuccess) return e;
+  CUtensorMap map_a, map_b;
+  if (!tc::encode_e4m3_operand(&map_a, p.a, p.M, p.K, p.lda, kBM) ||
+      !tc::encode_e4m3_operand(&map_b, p.b, p.N, p.K, p.ldb, kBM))
+    return cudaErrorInvalidValue;
   g.tiles_m = (g.M + kBM - 1) / kBM;
   g.tiles_n = (g.N + BN - 1) / BN;
   const int64_t tiles = (int64_t)g.tiles_m * g.tiles_n;
@@ -419,12 +422,11 @@ cudaError_t launch_tiled(const CUtensorMap& map_a, const CUtensorMap& map_b, Til
 
 // ------------------------------------------------------------------ few rows
 //
-// At most 128 rows of A: bound by reading the weight once. The weight is the
-// 128-row side of the MMA and the batch its N side (BR = 16, 32, 64 or 128
-// columns, the smallest that holds the batch; rows past M are zero-filled), so
+// At most 64 rows of A: bound by reading the weight once. The weight is the
+// 128-row side of the MMA and the batch its N side (BR = 16, 32 or 64 columns, the smallest that holds the batch; rows past M are zero-filled), so
 // a K block costs 16 KB of weight and a batch box of BR rows. N / 128 tiles do
 // not fill the GPU, so K is split over a cluster of S CTAs, with two CTAs an SM
-// (one for BR > 32): every SM then has its share of the weight on the way at
+// (one for BR = 64): every SM then has its share of the weight on the way at
 // once. Two K blocks share a ring stage and its barriers: the hand-over
 // between the warps, not the bytes, set the time of one-block stages.
 // The ranks' partial tiles are reduce-scattered: each rank owns a share of the
@@ -432,7 +434,11 @@ cudaError_t launch_tiled(const CUtensorMap& map_a, const CUtensorMap& map_b, Til
 // no multicast), and it adds all in rank order, so the result does not depend
 // on timing.
 // Warps 0-3 sum (a weight row a thread), 4 issues TMA, 5 MMAs, 6 copies scales.
-constexpr int kFewRows = 128;  // rows up to which this form is taken
+// Rows up to which this form is taken, and rows from which it is only while K is
+// split (N leaves SMs idle). Against the tiled form, cold L2: 33 x 5120 x 5120
+// 18 against 22 us, 64 x 7168 x 7168 27 against 29; 64 x 16384 x 4096 (no split)
+// 28 against 24; a 128-column plan lost from 128 x 5120 x 5120 (27 against 23) on.
+constexpr int kFewRows = 64, kFewSplitRows = 32;
 constexpr int kFewThreads = 224, kFewScaleSlots = 3, kFewStep = 2, kMaxRanks = 8;
 
 template <int BR>
@@ -725,6 +731,9 @@ int few_clusters(int S, const cudaLaunchConfig_t& base) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return 0;
   if (dev < 64 && cache[dev][S].load(std::memory_order_relaxed) > 0) return cache[dev][S].load();
+  if (cudaFuncSetAttribute(block_gemm_few_kernel<BR>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           (int)FewPlan<BR>::kSmemBytes) != cudaSuccess)
+    return 0;
   cudaLaunchConfig_t cfg = base;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -740,25 +749,35 @@ int few_clusters(int S, const cudaLaunchConfig_t& base) {
   return n;
 }
 
+// Ranks of the split: the most with which all tiles still run at once, a full
+// stage a rank at least. One cluster more than fit doubles the time (1 x 5120 x
+// 5120: 6 ranks 16 us, 7 ranks 20 us).
 template <int BR>
-cudaError_t launch_few(const CUtensorMap& map_a, const CUtensorMap& map_b, const TileArgs& g,
-                       cudaStream_t stream) {
-  using P = FewPlan<BR>;
-  auto kernel = block_gemm_few_kernel<BR>;
-  const cudaError_t e =
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)P::kSmemBytes);
-  if (e != cudaSuccess) return e;
-  const int tiles = (g.N + kBM - 1) / kBM;
+int few_ranks(int64_t N, int64_t KB) {
+  const int64_t tiles = (N + kBM - 1) / kBM;
   cudaLaunchConfig_t cfg{};
   cfg.blockDim = dim3(kFewThreads);
-  cfg.dynamicSmemBytes = P::kSmemBytes;
-  cfg.stream = stream;
-  // the most ranks with which all tiles still run at once, a full stage a rank
-  // at least: one cluster more than fit doubles the time (5120 x 5120, 1 row:
-  // 6 ranks 16 us, 7 ranks 20 us)
+  cfg.dynamicSmemBytes = FewPlan<BR>::kSmemBytes;
   int S = kMaxRanks;
-  while (S > 1 && (S * kFewStep > g.KB || few_clusters<BR>(S, cfg) < tiles)) --S;
-  cfg.gridDim = dim3((unsigned)tiles, 1, (unsigned)S);
+  while (S > 1 && (S * kFewStep > KB || few_clusters<BR>(S, cfg) < tiles)) --S;
+  return S;
+}
+
+template <int BR>
+cudaError_t launch_few(const BlockGemmArgs& p, const TileArgs& g, int S, cudaStream_t stream) {
+  const cudaError_t e = cudaFuncSetAttribute(block_gemm_few_kernel<BR>,
+                                             cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             (int)FewPlan<BR>::kSmemBytes);
+  if (e != cudaSuccess) return e;
+  CUtensorMap map_a, map_b;
+  if (!tc::encode_e4m3_operand(&map_a, p.a, p.M, p.K, p.lda, BR) ||
+      !tc::encode_e4m3_operand(&map_b, p.b, p.N, p.K, p.ldb, kBM))
+    return cudaErrorInvalidValue;
+  cudaLaunchConfig_t cfg{};
+  cfg.blockDim = dim3(kFewThreads);
+  cfg.dynamicSmemBytes = FewPlan<BR>::kSmemBytes;
+  cfg.stream = stream;
+  cfg.gridDim = dim3((unsigned)((p.N + kBM - 1) / kBM), 1, (unsigned)S);
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -768,7 +787,7 @@ cudaError_t launch_few(const CUtensorMap& map_a, const CUtensorMap& map_b, const
   attr[1].val.clusterDim.z = (unsigned)S;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, kernel, map_a, map_b, g);
+  return cudaLaunchKernelEx(&cfg, block_gemm_few_kernel<BR>, map_a, map_b, g);
 }
 
 }  // namespace
@@ -786,36 +805,32 @@ cudaError_t device_error_block_gemm(int* out, bool clear) {
 }
 
 int block_gemm(const BlockGemmArgs& p, cudaStream_t stream, const char** why) {
-  const bool few = p.M <= kFewRows && !p.b_rows;
-  const int columns = p.M <= 16 ? 16 : p.M <= 32 ? 32 : p.M <= 64 ? 64 : 128;
-  CUtensorMap map_a, map_b;
-  if (!tc::encode_e4m3_operand(&map_a, p.a, p.M, p.K, p.lda, few ? columns : kBM) ||
-      !tc::encode_e4m3_operand(&map_b, p.b, p.N, p.K, p.ldb, kBM)) {
-    *why = "cuTensorMapEncodeTiled failed for an operand";
-    return CUTIE_ERR_CUDA;
-  }
   TileArgs g{};
   g.sa = p.sa, g.sa_row = p.sa_row, g.sa_kb = p.sa_kb;
   g.sb = p.sb, g.sb_row = p.sb_row, g.sb_kb = p.sb_kb;
   g.d = p.d, g.ldd = p.ldd;
   g.M = (int)p.M, g.N = (int)p.N, g.KB = (int)((p.K + kBK - 1) / kBK);
   g.d_f32 = p.d_f32, g.accumulate = p.accumulate;
-  const int64_t row_bytes = p.ldd * (p.d_f32 ? 4 : 2);
-  g.vec = aligned_rows_host(p.d, row_bytes, 32);
-  // 256-wide tiles while every SM still gets one, else 128-wide ones
-  const int64_t tm = (p.M + kBM - 1) / kBM;
-  const bool wide = tm * ((p.N + 255) / 256) >= device_sm_count();
+  g.vec = aligned_rows_host(p.d, p.ldd * (p.d_f32 ? 4 : 2), 32);
+  const int columns = p.M <= 16 ? 16 : p.M <= 32 ? 32 : 64;
+  const int ranks = p.b_rows || p.M > kFewRows ? 0
+                    : columns == 16            ? few_ranks<16>(p.N, g.KB)
+                    : columns == 32            ? few_ranks<32>(p.N, g.KB)
+                                               : few_ranks<64>(p.N, g.KB);
   cudaError_t e;
-  if (few)
-    e = columns == 16   ? launch_few<16>(map_a, map_b, g, stream)
-        : columns == 32 ? launch_few<32>(map_a, map_b, g, stream)
-        : columns == 64 ? launch_few<64>(map_a, map_b, g, stream)
-                        : launch_few<128>(map_a, map_b, g, stream);
-  else
-    e = wide ? (p.b_rows ? launch_tiled<256, true>(map_a, map_b, g, stream)
-                         : launch_tiled<256, false>(map_a, map_b, g, stream))
-             : (p.b_rows ? launch_tiled<128, true>(map_a, map_b, g, stream)
-                         : launch_tiled<128, false>(map_a, map_b, g, stream));
+  if (ranks > (p.M <= kFewSplitRows ? 0 : 1)) {
+    e = columns == 16   ? launch_few<16>(p, g, ranks, stream)
+        : columns == 32 ? launch_few<32>(p, g, ranks, stream)
+                        : launch_few<64>(p, g, ranks, stream);
+  } else {
+    // 256-wide tiles while every SM still gets one, else 128-wide ones
+    const int64_t tm = (p.M + kBM - 1) / kBM;
+    const bool wide = tm * ((p.N + 255) / 256) >= device_sm_count();
+    e = wide ? (p.b_rows ? launch_tiled<256, true>(p, g, stream)
+                         : launch_tiled<256, false>(p, g, stream))
+             : (p.b_rows ? launch_tiled<128, true>(p, g, stream)
+                         : launch_tiled<128, false>(p, g, stream));
+  }
   if (e != cudaSuccess) {
     *why = cudaGetErrorString(e);
     return CUTIE_ERR_CUDA;

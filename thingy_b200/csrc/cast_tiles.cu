@@ -40,7 +40,7 @@ __device__ __forceinline__ float rcp_of(float s, bool pow2) {
 }
 
 template <bool BLOCK, bool TRANSPOSED>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 4)
     cast_tiles_kernel(CastArgs a) {
   __shared__ __align__(16) uint8_t t_codes[TRANSPOSED ? kTile * kTile : 16];
   __shared__ __align__(16) uint32_t part[8][64];  // a warp's column maxima (bf16 pairs)
