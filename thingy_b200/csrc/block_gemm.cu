@@ -49,17 +49,19 @@ __device__ __forceinline__ bool wait_or_abort(uint32_t bar, uint32_t parity,
 //    g BN/2 .. of the tile for its 128 rows, a row a thread, in BN / 2 fp32
 //    registers, and adds scale * buffer to them while the MMAs of the next K
 //    block fill the other buffer.
-//  * warp 10: the scales, copied to a ring in shared memory up to kScaleSlots x
+//  * warp 10: the scales, copied to a ring in shared memory up to two slots of
 //    kScaleBlocks K blocks ahead, so that the sums spend hardly an instruction
 //    on them (one wait in kScaleBlocks blocks).
 // Tiles are walked in bands of kBand rows of tiles, so that the CTAs of a
 // wave share their operands in L2.
 constexpr int kThreads = 384, kEpiWarps = 8, kBand = 16;
-// registers a thread: 2 x 128 x 216 + 128 x 64 = 63488 of the 384 x 168 = 64512 at launch
+// registers a thread: 256 x 216 + 128 x 64 = 63488 of the 384 x 168 = 64512 at launch
 constexpr int kEpiRegs = 216, kIssueRegs = 64;
-constexpr int kScaleSlots = 3, kScaleBlocks = 4;  // ring slots, K blocks a slot
+constexpr int kScaleBlocks = 4;  // K blocks a slot of the scale ring
 
-template <int BN>
+constexpr int kStageRow = 9;  // see store_rows
+
+template <int BN, bool SB_ROWS, bool VEC>
 struct TilePlan {
   static constexpr int kNB = BN / 128;
   static constexpr uint32_t kStageBytes = (1 + kNB) * kBoxBytes;
@@ -68,8 +70,11 @@ struct TilePlan {
   static constexpr uint32_t kTmemCols = 2 * BN;
   static constexpr int kCols = BN / 2;  // columns of a warp group
   // scales of a K block: 128 rows', then the columns' (a scale each, or a block's)
-  static constexpr int kScales = 128 + BN;
-  static_assert(kSmemBytes + kScaleSlots * kScaleBlocks * kScales * 4 + 512 <= 227 * 1024, "shared memory");
+  static constexpr int kScales = 128 + (SB_ROWS ? BN : 4);
+  static constexpr int kScaleSlots = SB_ROWS ? 2 : 4;
+  static_assert(kSmemBytes + kScaleSlots * kScaleBlocks * kScales * 4 + kEpiWarps * 32 * kStageRow * 4 * (VEC ? 0 : 1) + 512 <=
+                    227 * 1024,
+                "shared memory");
 };
 
 struct TileArgs {
@@ -80,7 +85,7 @@ struct TileArgs {
   void* d;
   int64_t ldd;
   int M, N, KB, tiles_m, tiles_n;
-  bool d_f32, accumulate, vec;  // vec: rows of D start on 32-byte boundaries
+  bool d_f32, accumulate;
 };
 
 // Tile t of the banded walk.
@@ -92,32 +97,34 @@ __device__ __forceinline__ void tile_at(int t, int tiles_m, int tiles_n, int* tm
   *tn = in / rows;
 }
 
-template <int NC>
-__device__ __forceinline__ void store_row(const TileArgs& g, const float2 (&acc)[NC / 2], int row,
-                                          int col) {
-  if (row >= g.M || col >= g.N) return;
-  const int left = g.N - col < NC ? g.N - col : NC;
-  const int64_t at = (int64_t)row * g.ldd + col;
-  if (!g.d_f32) {
-    uint16_t* p = static_cast<uint16_t*>(g.d) + at;
+// A warp's 32 rows of NC columns. VEC: the rows of D start on 32-byte
+// boundaries and hold whole 32-byte sectors, which the threads store that have
+// them. Otherwise 8 columns at a time go through the warp's 32 x 9 floats of
+// shared memory and leave as 8 consecutive elements of four rows an instruction
+// (stored an element a thread they cost 30 us instead of 10 at 1001 x 1544).
+// A template, not a branch: the mere presence of the second form cost the main
+// loop of the first 6%.
+template <int NC, bool VEC>
+__device__ __forceinline__ void store_rows(const TileArgs& g, const float2 (&acc)[NC / 2], int row0,
+                                           int col, int lane, float* stage) {
+  if (VEC) {
+    const int row = row0 + lane;
+    if (row >= g.M) return;
+    const int64_t at = (int64_t)row * g.ldd + col;
+    if (!g.d_f32) {
+      uint16_t* p = static_cast<uint16_t*>(g.d) + at;
 #pragma unroll
-    for (int c = 0; c < NC; c += 16) {
-      uint32_t w[8];
+      for (int c = 0; c < NC; c += 16) {
+        uint32_t w[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = f2_to_bf2(acc[c / 2 + i]);
-      if (g.vec && c + 16 <= left) {
-        st_stream8(p + c, w);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (c + i < left) p[c + i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+        for (int i = 0; i < 8; ++i) w[i] = f2_to_bf2(acc[c / 2 + i]);
+        if (col + c < g.N) st_stream8(p + c, w);
       }
-    }
-  } else {
-    float* p = static_cast<float*>(g.d) + at;
+    } else {
+      float* p = static_cast<float*>(g.d) + at;
 #pragma unroll
-    for (int c = 0; c < NC; c += 8) {
-      if (g.vec && c + 8 <= left) {
+      for (int c = 0; c < NC; c += 8) {
+        if (col + c >= g.N) break;
         float v[8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[2 * i] = acc[c / 2 + i].x, v[2 * i + 1] = acc[c / 2 + i].y;
@@ -128,31 +135,53 @@ __device__ __forceinline__ void store_row(const TileArgs& g, const float2 (&acc)
           v[4] += o1.x, v[5] += o1.y, v[6] += o1.z, v[7] += o1.w;
         }
         st_stream8(p + c, reinterpret_cast<const uint32_t*>(v));
-      } else {
+      }
+    }
+  } else {
+    const int r4 = lane >> 3, c8 = lane & 7;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float f = i & 1 ? acc[c / 2 + i / 2].y : acc[c / 2 + i / 2].x;
-          if (c + i < left) p[c + i] = g.accumulate ? p[c + i] + f : f;
+    for (int c = 0; c < NC; c += 8) {
+      if (col + c >= g.N) break;
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        stage[lane * kStageRow + 2 * i] = acc[c / 2 + i].x;
+        stage[lane * kStageRow + 2 * i + 1] = acc[c / 2 + i].y;
+      }
+      __syncwarp();
+      const int cc = col + c + c8;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = row0 + 4 * i + r4;
+        if (r >= g.M || cc >= g.N) break;
+        const float v = stage[(4 * i + r4) * kStageRow + c8];
+        const int64_t to = (int64_t)r * g.ldd + cc;
+        if (g.d_f32) {
+          float* p = static_cast<float*>(g.d) + to;
+          *p = g.accumulate ? *p + v : v;
+        } else {
+          static_cast<uint16_t*>(g.d)[to] = (uint16_t)(f2_to_bf2(make_float2(v, 0.f)) & 0xffffu);
         }
       }
     }
   }
 }
 
-template <int BN, bool SB_ROWS>
+template <int BN, bool SB_ROWS, bool VEC>
 __global__ void __launch_bounds__(kThreads, 1)
     block_gemm_kernel(const __grid_constant__ CUtensorMap map_a,
                       const __grid_constant__ CUtensorMap map_b, const TileArgs g) {
-  using P = TilePlan<BN>;
+  using P = TilePlan<BN, SB_ROWS, VEC>;
   constexpr int NC = P::kCols;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full_bar[P::kStages];
   __shared__ __align__(8) uint64_t empty_bar[P::kStages];
   __shared__ __align__(8) uint64_t acc_full[2];
   __shared__ __align__(8) uint64_t acc_empty[2];
-  __shared__ __align__(8) uint64_t scale_full[kScaleSlots];
-  __shared__ __align__(8) uint64_t scale_empty[kScaleSlots];
-  __shared__ __align__(16) float scales[kScaleSlots][kScaleBlocks][P::kScales];
+  __shared__ __align__(8) uint64_t scale_full[P::kScaleSlots];
+  __shared__ __align__(8) uint64_t scale_empty[P::kScaleSlots];
+  __shared__ __align__(16) float scales[P::kScaleSlots][kScaleBlocks][P::kScales];
+  __shared__ float stage[VEC ? 1 : kEpiWarps][32 * kStageRow];
   __shared__ uint32_t tmem_base_slot;
   __shared__ uint32_t abort_flag;
   __shared__ uint32_t issued;     // K blocks whose copies were issued
@@ -174,7 +203,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(smem_addr(&acc_full[b]), 1);
       mbar_init(smem_addr(&acc_empty[b]), kEpiWarps);
     }
-    for (int s = 0; s < kScaleSlots; ++s) {
+    for (int s = 0; s < P::kScaleSlots; ++s) {
       mbar_init(smem_addr(&scale_full[s]), 32);
       mbar_init(smem_addr(&scale_empty[s]), kEpiWarps);
     }
@@ -290,7 +319,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         if (j == kScaleBlocks - 1 || kb == g.KB - 1) {
           tc::cp_async_arrive(smem_addr(&scale_full[s]));
-          if (++s == kScaleSlots) s = 0, parity ^= 1;
+          if (++s == P::kScaleSlots) s = 0, parity ^= 1;
         }
       }
     }
@@ -301,12 +330,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc::regs_up<kEpiRegs>();
     const int wg = warp >> 2, r = (warp & 3) * 32 + lane;
     const uint32_t tm_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(wg * NC);
-    // The buffer is read in pieces of 32 columns, each load issued before the
+    // The buffer is read in pieces of CH columns, each load issued before the
     // sums of the piece before it, the first of the next K block before those
     // of the last of this one: no sum waits for its own load's latency. `lo`
-    // and `hi` take turns. After an abort the waits return at once and the
-    // loads go on (tensor memory is still this CTA's).
-    uint32_t lo[32], hi[32];
+    // and `hi` take turns. With a scale a column the pieces are half as wide and
+    // the piece's scales are in registers before its load is waited for. After
+    // an abort the waits return at once and the loads go on (tensor memory is
+    // still this CTA's).
+    constexpr int CH = SB_ROWS ? 16 : 32;
+    uint32_t lo[CH], hi[CH];
     uint32_t buf = 0, buf_parity = 0, slot = 0, slot_parity = 0;
     float sc = 0.f;  // the row's scale of the block, times the column block's
     const float* sb = nullptr;  // the columns' scales of the block
@@ -318,7 +350,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       wait_or_abort(smem_addr(&acc_full[buf]), buf_parity, abortp);
       __syncwarp();
       tc::fence_after();
-      tc::tmem_ld32_async(tm_lane + buf * BN, lo);
+      tc::tmem_ld_async(tm_lane + buf * BN, lo);
       sc = scales[slot][j][r];
       sb = &scales[slot][j][128 + (SB_ROWS ? wg * NC : wg * NC / 128)];
       if (!SB_ROWS) sc *= *sb;
@@ -330,47 +362,53 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int i = 0; i < NC / 2; ++i) acc[i] = make_float2(0.f, 0.f);
       for (int kb = 0; kb < g.KB; ++kb) {
         const bool last = kb == g.KB - 1;
-        auto add = [&](int c, const uint32_t(&v)[32], float s, const float* col) {
-          const float2 s2 = make_float2(s, s);
-#pragma unroll
-          for (int i = 0; i < 16; i += 2) {
-            float2 d0 = make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
-            float2 d1 = make_float2(__uint_as_float(v[2 * i + 2]), __uint_as_float(v[2 * i + 3]));
-            if (SB_ROWS) {
-              const float4 f = *reinterpret_cast<const float4*>(col + c + 2 * i);
-              d0 = __fmul2_rn(d0, make_float2(f.x, f.y));
-              d1 = __fmul2_rn(d1, make_float2(f.z, f.w));
-            }
-            acc[c / 2 + i] = __ffma2_rn(d0, s2, acc[c / 2 + i]);
-            acc[c / 2 + i + 1] = __ffma2_rn(d1, s2, acc[c / 2 + i + 1]);
-          }
-        };
-#pragma unroll
-        for (int c = 0; c < NC - 64; c += 64) {
-          tc::tmem_ld_wait(lo);
-          tc::tmem_ld32_async(tm_lane + buf * BN + (uint32_t)(c + 32), hi);
-          add(c, lo, sc, sb);
-          tc::tmem_ld_wait(hi);
-          tc::tmem_ld32_async(tm_lane + buf * BN + (uint32_t)(c + 64), lo);
-          add(c + 32, hi, sc, sb);
-        }
-        tc::tmem_ld_wait(lo);
-        tc::tmem_ld32_async(tm_lane + buf * BN + (uint32_t)(NC - 32), hi);
-        add(NC - 64, lo, sc, sb);
-        tc::tmem_ld_wait(hi);
-        // all of the buffer is in registers
-        tc::fence_before();
-        __syncwarp();
-        tc::arrive_if(first, smem_addr(&acc_empty[buf]));
-        buf ^= 1;
-        buf_parity ^= buf == 0;
-        const bool slot_done = last || kb % kScaleBlocks == kScaleBlocks - 1;
-        const uint32_t done = smem_addr(&scale_empty[slot]);
         const float s = sc;
         const float* col = sb;
-        if (slot_done && ++slot == kScaleSlots) slot = 0, slot_parity ^= 1;
-        if (!last || t + (int)gridDim.x < tiles) begin_block(last ? 0 : kb + 1);
-        add(NC - 32, hi, s, col);
+        const uint32_t tm = tm_lane + buf * BN;
+        float4 f[SB_ROWS ? CH / 4 : 1];
+        auto column_scales = [&](int c) {  // of piece c, before its load is waited for
+          if (SB_ROWS) {
+#pragma unroll
+            for (int i = 0; i < CH / 4; ++i) f[i] = *reinterpret_cast<const float4*>(col + c + 4 * i);
+          }
+        };
+        auto add = [&](int c, const uint32_t(&v)[CH]) {
+          const float2 s2 = make_float2(s, s);
+#pragma unroll
+          for (int i = 0; i < CH / 4; ++i) {
+            float2 d0 = make_float2(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]));
+            float2 d1 = make_float2(__uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]));
+            if (SB_ROWS) {
+              d0 = __fmul2_rn(d0, make_float2(f[i].x, f[i].y));
+              d1 = __fmul2_rn(d1, make_float2(f[i].z, f[i].w));
+            }
+            acc[c / 2 + 2 * i] = __ffma2_rn(d0, s2, acc[c / 2 + 2 * i]);
+            acc[c / 2 + 2 * i + 1] = __ffma2_rn(d1, s2, acc[c / 2 + 2 * i + 1]);
+          }
+        };
+        const bool slot_done = last || kb % kScaleBlocks == kScaleBlocks - 1;
+        const uint32_t done = smem_addr(&scale_empty[slot]);
+#pragma unroll
+        for (int c = 0; c < NC; c += 2 * CH) {
+          column_scales(c);
+          tc::tmem_ld_wait(lo);
+          tc::tmem_ld_async(tm + (uint32_t)(c + CH), hi);
+          add(c, lo);
+          column_scales(c + CH);
+          tc::tmem_ld_wait(hi);
+          if (c + 2 * CH < NC) {
+            tc::tmem_ld_async(tm + (uint32_t)(c + 2 * CH), lo);
+          } else {  // all of the buffer is in registers
+            tc::fence_before();
+            __syncwarp();
+            tc::arrive_if(first, smem_addr(&acc_empty[buf]));
+            buf ^= 1;
+            buf_parity ^= buf == 0;
+            if (slot_done && ++slot == P::kScaleSlots) slot = 0, slot_parity ^= 1;
+            if (!last || t + (int)gridDim.x < tiles) begin_block(last ? 0 : kb + 1);
+          }
+          add(c + CH, hi);
+        }
         if (slot_done) {
           __syncwarp();
           tc::arrive_if(first, done);
@@ -378,7 +416,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       int tm_i, tn_i;
       tile_at(t, g.tiles_m, g.tiles_n, &tm_i, &tn_i);
-      if (*abortp == 0u) store_row<NC>(g, acc, tm_i * kBM + r, tn_i * BN + wg * NC);
+      if (*abortp == 0u) store_rows<NC, VEC>(g, acc, tm_i * kBM + (warp & 3) * 32, tn_i * BN + wg * NC, lane,
+                            stage[VEC ? 0 : warp]);
     }
   }
   __syncwarp();
@@ -401,10 +440,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == kEpiWarps) tc::tmem_dealloc(tmem, P::kTmemCols);
 }
 
-template <int BN, bool SB_ROWS>
+template <int BN, bool SB_ROWS, bool VEC>
 cudaError_t launch_tiled(const BlockGemmArgs& p, TileArgs g, cudaStream_t stream) {
-  using P = TilePlan<BN>;
-  auto kernel = block_gemm_kernel<BN, SB_ROWS>;
+  using P = TilePlan<BN, SB_ROWS, VEC>;
+  auto kernel = block_gemm_kernel<BN, SB_ROWS, VEC>;
   const cudaError_t e =
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)P::kSmemBytes);
   if (e != cudaSuccess) return e;
@@ -622,7 +661,7 @@ __global__ void __launch_bounds__(kFewThreads, FewPlan<BR>::kCtas)
         for (int c = 0; c < BR; c += 16) {
           if (c >= g.M) break;
           uint32_t v[16];
-          tc::tmem_ld16_async(tm_lane + (buf * kFewStep + j) * BR + (uint32_t)c, v);
+          tc::tmem_ld_async(tm_lane + (buf * kFewStep + j) * BR + (uint32_t)c, v);
           float2 f[8];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -811,7 +850,6 @@ int block_gemm(const BlockGemmArgs& p, cudaStream_t stream, const char** why) {
   g.d = p.d, g.ldd = p.ldd;
   g.M = (int)p.M, g.N = (int)p.N, g.KB = (int)((p.K + kBK - 1) / kBK);
   g.d_f32 = p.d_f32, g.accumulate = p.accumulate;
-  g.vec = aligned_rows_host(p.d, p.ldd * (p.d_f32 ? 4 : 2), 32);
   const int columns = p.M <= 16 ? 16 : p.M <= 32 ? 32 : 64;
   const int ranks = p.b_rows || p.M > kFewRows ? 0
                     : columns == 16            ? few_ranks<16>(p.N, g.KB)
@@ -826,10 +864,15 @@ int block_gemm(const BlockGemmArgs& p, cudaStream_t stream, const char** why) {
     // 256-wide tiles while every SM still gets one, else 128-wide ones
     const int64_t tm = (p.M + kBM - 1) / kBM;
     const bool wide = tm * ((p.N + 255) / 256) >= device_sm_count();
-    e = wide ? (p.b_rows ? launch_tiled<256, true>(p, g, stream)
-                         : launch_tiled<256, false>(p, g, stream))
-             : (p.b_rows ? launch_tiled<128, true>(p, g, stream)
-                         : launch_tiled<128, false>(p, g, stream));
+    const bool vec = aligned_rows_host(p.d, p.ldd * (p.d_f32 ? 4 : 2), 32) && p.N % (p.d_f32 ? 8 : 16) == 0;
+    e = wide ? (p.b_rows ? (vec ? launch_tiled<256, true, true>(p, g, stream)
+                                : launch_tiled<256, true, false>(p, g, stream))
+                         : (vec ? launch_tiled<256, false, true>(p, g, stream)
+                                : launch_tiled<256, false, false>(p, g, stream)))
+             : (p.b_rows ? (vec ? launch_tiled<128, true, true>(p, g, stream)
+                                : launch_tiled<128, true, false>(p, g, stream))
+                         : (vec ? launch_tiled<128, false, true>(p, g, stream)
+                                : launch_tiled<128, false, false>(p, g, stream)));
   }
   if (e != cudaSuccess) {
     *why = cudaGetErrorString(e);

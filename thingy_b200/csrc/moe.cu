@@ -673,7 +673,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
           for (int c = 0; c < NMAX; c += 16) {
             if (c >= n) break;
             uint32_t v[16];
-            tc::tmem_ld16_async(lane_base + buf * 2 * NMAX + (uint32_t)c, v);
+            tc::tmem_ld_async(lane_base + buf * 2 * NMAX + (uint32_t)c, v);
             const float4* sc = reinterpret_cast<const float4*>(&sh.scales[slot][c]);
             float4 f[4] = {sc[0], sc[1], sc[2], sc[3]};
             tc::tmem_ld_wait(v);
