@@ -374,15 +374,16 @@ struct MoeArgs {
   float* weights;
   // workspace
   uint64_t* barrier;
-  int* counters;  // arrivals at split items: n_counters1 of the first product, then the second's
-  int n_counters, n_counters1;
+  int* part_flag;  // [2, SMs] parts of split items sent, then
+  int* ready;      // [experts] hidden row groups complete; n_counts in all, zeroed by each launch
+  int n_counts;
   float* logits;  // [splits, T, E]
   int splits;
   bool deal_tokens;
   uint8_t* hidden;  // [T k, I] codes of the hidden rows and their scales
   float* h_scale;
   float* down;     // [T k, H] down products
-  float* partial;  // [SMs, 2, columns, 256] sums of split items
+  float* partial;  // [2, SMs, columns, 256] parts of split items
 };
 // Bytes of workspace; fills g's workspace fields from `base` (may be null).
 size_t moe_workspace(MoeArgs* g, void* base);

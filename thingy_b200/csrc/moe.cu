@@ -17,14 +17,16 @@
 // (item, K block) of 32 KB of weights. An item is 128 gate rows with their
 // 128 up rows, or 256 rows of the down weight, of one expert; units are dealt
 // to the CTAs in contiguous runs, so an item may be split over K between
-// neighbours. A split item's partial sums go to the workspace, and the CTA
-// that arrives last adds them in the order of K (the result does not depend
-// on who that is) and finishes the item.
+// neighbours: the CTA whose run begins it owns it, the others send their part
+// (the first thing in their run) through the workspace, and the owner (whose
+// run ends with it) adds them in the order of K. The result does not depend on
+// timing.
 //
-// Three grid barriers: logits complete (and, for many tokens, the choices),
-// hidden rows complete, down products complete. The weight stream does not
-// stop at the second: its TMA thread needs only the choices, and fills the
-// ring with down tiles while the last hidden rows are finished.
+// Between CTAs: a grid barrier when the logits are complete (for many tokens
+// another when the choices are), a count a hidden row group of each expert that
+// its down products wait for, and a grid barrier before the weighted sum. The
+// weight stream does not stop for the hidden rows: its TMA thread needs only
+// the choices, and fills the ring with down tiles in the meantime.
 //
 // Warps: 0-7 the outer sums (warps 0-3 the first 128 rows of an item, 4-7 the
 // second, a row a thread) and the epilogues; 8 the weight tiles (TMA); 9 the
@@ -103,7 +105,7 @@ struct MoeShared {
   uint16_t active[kMaxE < MoePlan<NMAX>::kPairs ? kMaxE : MoePlan<NMAX>::kPairs];
   Deal deal[2];
   Walk walk[2];
-  uint32_t tmem_base, abort_flag, last, issued_w, issued_a, committed;
+  uint32_t tmem_base, abort_flag, issued_w, issued_a, committed;
   uint64_t target;  // the grid barrier's count at the next barrier
 };
 
@@ -174,6 +176,31 @@ __device__ __forceinline__ float4 ld_l2(const float4* p) {
                : "l"(p)
                : "memory");
   return v;
+}
+
+// Counts between CTAs of one launch: add one, ordered after the CTA's writes
+// that a barrier of its threads ordered before; wait for a number of them.
+__device__ __forceinline__ void release_add(int* count) {
+  __threadfence();
+  asm volatile("red.release.gpu.global.add.s32 [%0], 1;" ::"l"(count) : "memory");
+}
+__device__ __forceinline__ bool wait_count(const int* count, int target, volatile uint32_t* abort_flag) {
+  const long long t0 = clock64();
+  for (;;) {
+    int v;
+    asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(count) : "memory");
+    if (v >= target) return true;
+    if (*abort_flag || clock64() - t0 > kWaitLimitCycles) {
+      *abort_flag = 1u;
+      return false;
+    }
+  }
+}
+// The same before TMA reads what was waited for.
+__device__ __forceinline__ bool wait_count_tma(const int* count, int target, volatile uint32_t* abort_flag) {
+  const bool ok = wait_count(count, target, abort_flag);
+  asm volatile("fence.proxy.async;" ::: "memory");
+  return ok;
 }
 
 // ------------------------------------------------------------------ router
@@ -268,16 +295,18 @@ __device__ __forceinline__ void choose(const MoeArgs& g, const float* logits, ui
                                        int* id, float* w) {
   const bool softmax = g.scoring == 0;
   float m = -INFINITY, z = 1.f;
-  if (softmax) {
+  if (softmax) {  // the sum over all experts only where the weights need it
 #pragma unroll 1
     for (int e = lane; e < g.E; e += 32) m = fmaxf(m, logits[e]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    z = 0.f;
+    if (!g.renormalize || g.bias != nullptr) {
+      z = 0.f;
 #pragma unroll 1
-    for (int e = lane; e < g.E; e += 32) z += expf(logits[e] - m);
+      for (int e = lane; e < g.E; e += 32) z += expf(logits[e] - m);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+      for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+    }
   }
 #pragma unroll 1
   for (int e = lane; e < g.E; e += 32) {
@@ -315,37 +344,39 @@ __device__ __forceinline__ void choose(const MoeArgs& g, const float* logits, ui
 
 __device__ __forceinline__ void epi_sync() { asm volatile("barrier.cta.sync 1, 256;" ::: "memory"); }
 
-// Sums of a split item: this CTA's partial to the workspace; true in the CTA
-// that arrives last, with the whole sums in acc. n columns, thread = row.
+// A split item belongs to the CTA whose run begins it (and ends in it); the
+// others' runs begin inside it, so their part is the first thing they finish.
+// send_part: such a part to the workspace, and its flag. n columns, thread = row.
 template <int NMAX>
-__device__ __forceinline__ bool join(const MoeArgs& g, MoeShared<NMAX>& sh, const Deal& deal, int item,
-                                     int* counter, int n, float (&acc)[NMAX]) {
-  const int tid = threadIdx.x;
-  const int first = item * deal.KB, c0 = first / deal.per, c1 = (first + deal.KB - 1) / deal.per;
-  // a run that begins inside the item keeps its part in slot 0, one that ends in it in slot 1
-  const int mine = first < deal.per * (int)blockIdx.x ? 0 : 1;
-  float* p = g.partial + (int64_t)(blockIdx.x * 2 + mine) * NMAX * 256 + tid;
+__device__ __forceinline__ void send_part(const MoeArgs& g, int phase, int n, const float (&acc)[NMAX]) {
+  float* p = g.partial + (int64_t)(phase * (int)gridDim.x + (int)blockIdx.x) * NMAX * 256 + threadIdx.x;
 #pragma unroll
   for (int c = 0; c < NMAX; ++c)
     if (c < n) __stcg(p + c * 256, acc[c]);
   epi_sync();
-  if (tid == 0) {
-    __threadfence();
-    const int old = atomicAdd(counter, 1);
-    __threadfence();
-    sh.last = old == c1 - c0;
-  }
-  epi_sync();
-  if (!sh.last) return false;
+  if (threadIdx.x == 0) release_add(g.part_flag + phase * gridDim.x + blockIdx.x);
+}
+
+// add_parts: the owner's sums plus the others' in the order of K.
+template <int NMAX>
+__device__ __forceinline__ void add_parts(const MoeArgs& g, const Deal& deal, int phase, int item, int n,
+                                          float (&acc)[NMAX], volatile uint32_t* abortp) {
+  const int last = ((item + 1) * deal.KB - 1) / deal.per;
+#pragma unroll 1
+  for (int b = (int)blockIdx.x + 1; b <= last; ++b) {
+    if ((threadIdx.x & 31) == 0) wait_count(g.part_flag + phase * gridDim.x + b, 1, abortp);
+    __syncwarp();
+    const float* o = g.partial + (int64_t)(phase * (int)gridDim.x + b) * NMAX * 256 + threadIdx.x;
 #pragma unroll
-  for (int c = 0; c < NMAX; ++c) acc[c] = 0.f;
-  for (int b = c0; b <= c1; ++b) {
-    const float* o = g.partial + (int64_t)(b * 2 + (first < deal.per * b ? 0 : 1)) * NMAX * 256 + tid;
+    for (int c0 = 0; c0 < NMAX; c0 += 16) {
+      if (c0 >= n) break;
+      float v[16];
 #pragma unroll
-    for (int c = 0; c < NMAX; ++c)
-      if (c < n) acc[c] += ld_l2(o + c * 256);
+      for (int c = 0; c < 16; ++c) v[c] = ld_l2_if(c0 + c < n, o + (c0 + c) * 256);
+#pragma unroll
+      for (int c = 0; c < 16; ++c) acc[c0 + c] += v[c];
+    }
   }
-  return true;
 }
 
 // One group of 128 of a hidden row by one warp: silu(gate) * up, its scale and codes.
@@ -409,9 +440,9 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
   if (warp == 10) tc::tmem_alloc(smem_addr(&sh.tmem_base), P::kTmemCols);
   for (int e = tid; e < g.E; e += kMoeThreads) sh.mask[e] = 0;
 
-  // ---- router: partial logits, and the counters of split items to zero
-  for (int i = blockIdx.x * kMoeThreads + tid; i < g.n_counters; i += gridDim.x * kMoeThreads)
-    g.counters[i] = 0;
+  // ---- router: partial logits, and this launch's counts to zero
+  for (int i = blockIdx.x * kMoeThreads + tid; i < g.n_counts; i += gridDim.x * kMoeThreads)
+    g.part_flag[i] = 0;
   const int jobs = ((g.E + 3) / 4) * ((g.T + 7) / 8) * g.splits;
   for (int j = blockIdx.x; j < jobs; j += gridDim.x)
     router_job(g, j, warp, lane, reinterpret_cast<float(*)[32]>(smem_raw));  // the ring is idle
@@ -488,16 +519,19 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
     }
   }
   __syncthreads();
-  for (int p = tid; p < pairs; p += kMoeThreads) {
-    const int t = p / g.k, e = sh.ids[p] < g.E ? sh.ids[p] : 0;
-    const int row = sh.first_row[e] + __popcll(sh.mask[e] & ((1ull << t) - 1ull));
-    sh.row_of[p] = (uint16_t)row;
-    sh.token_at[row] = (uint8_t)t;
+  // the weight stream needs no more than this; the others, the rows' tables
+  if (warp != 8) {
+    for (int p = tid < 256 ? tid : tid - 32; p < pairs; p += kMoeThreads - 32) {
+      const int t = p / g.k, e = sh.ids[p] < g.E ? sh.ids[p] : 0;
+      const int row = sh.first_row[e] + __popcll(sh.mask[e] & ((1ull << t) - 1ull));
+      sh.row_of[p] = (uint16_t)row;
+      sh.token_at[row] = (uint8_t)t;
+    }
+    asm volatile("barrier.cta.sync 2, 352;" ::: "memory");
   }
-  __syncthreads();
 
   const uint32_t tmem = sh.tmem_base;
-  const uint64_t hidden_target = target + gridDim.x, down_target = target + 2 * (uint64_t)gridDim.x;
+  const uint64_t down_target = target + gridDim.x;
 
   if (warp == 8) {
     // ---- weight tiles of both phases, without a stop between them
@@ -532,13 +566,15 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
     bool ok = true;
 #pragma unroll 1
     for (int phase = 0; phase < 2 && ok; ++phase) {
-      Walk w = sh.walk[phase];
-      if (phase == 1 && w.more()) {
-        if (leader) ok = barrier_wait(g.barrier, hidden_target, abortp);
-        if (!__all_sync(0xffffffffu, ok)) break;
-      }
+      int hidden_of = -1;  // the expert whose hidden rows are known to be complete
 #pragma unroll 1
-      for (; w.more(); w.next()) {
+      for (Walk w = sh.walk[phase]; w.more(); w.next()) {
+        if (phase == 1 && w.a != hidden_of) {
+          hidden_of = w.a;
+          if (leader) ok = wait_count_tma(g.ready + w.a, IG, abortp);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+        }
         ok = __all_sync(0xffffffffu, wait_or_abort(smem_addr(&sh.empty[s]), parity, abortp));
         if (!ok) break;
         if (leader) {
@@ -607,17 +643,18 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
     bool ok = true;
 #pragma unroll 1
     for (int phase = 0; phase < 2 && ok; ++phase) {
-      Walk w = sh.walk[phase];
-      if (phase == 1 && w.more()) {
-        if (lane == 0) ok = barrier_wait(g.barrier, hidden_target, abortp);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-      }
+      int hidden_of = -1;
       const int64_t step = phase == 0 ? g.sq_kb : 1;
       const float *pa[NL], *pw = nullptr;
       int n = 0;
 #pragma unroll 1
-      for (; w.more(); w.next()) {
+      for (Walk w = sh.walk[phase]; w.more(); w.next()) {
+        if (phase == 1 && w.a != hidden_of) {
+          hidden_of = w.a;
+          if (lane == 0) ok = wait_count(g.ready + w.a, IG, abortp);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+        }
         if (n == 0 || w.kb == 0) {  // addresses change at items only
           const int e = sh.active[w.a], row0 = sh.first_row[e];
           n = __popcll(sh.mask[e]);
@@ -697,11 +734,11 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
         if (!to_end && w.u != w.end - 1) continue;
         // ---- the item, or this CTA's part of it, is complete
         begun = false;
-        if (!from_start || !to_end) {
-          const int item = w.a * w.groups + w.grp;
-          int* counter = g.counters + (phase == 0 ? 0 : g.n_counters1) + item;
-          if (!join<NMAX>(g, sh, sh.deal[phase], item, counter, n, acc)) continue;
+        if (!from_start) {
+          send_part<NMAX>(g, phase, n, acc);
+          continue;
         }
+        if (!to_end) add_parts<NMAX>(g, sh.deal[phase], phase, w.a * w.groups + w.grp, n, acc, abortp);
         if (phase == 0) {
           // hidden rows: both halves to shared memory, then a row's group of
           // 128 columns a warp
@@ -717,8 +754,10 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
               hidden_group(exchange + c * kXStride, exchange + (P::kXCols + c) * kXStride, lane,
                            g.hidden + (int64_t)(row0 + h0 + c) * g.I + w.grp * 128,
                            g.h_scale + (int64_t)(row0 + h0 + c) * IG + w.grp);
+            asm volatile("fence.proxy.async;" ::: "memory");  // hidden rows are read by TMA
             epi_sync();
           }
+          if (tid == 0) release_add(g.ready + w.a);
         } else {
           const int col = w.grp * 256 + half * 128 + r;
           if (col < g.H) {
@@ -728,17 +767,9 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
           }
         }
       }
-      if (phase == 0) {
-        asm volatile("fence.proxy.async;" ::: "memory");  // hidden rows are read by TMA
-        epi_sync();
-        if (tid == 0) barrier_arrive(g.barrier);
-      }
     }
     epi_sync();
     if (tid == 0) {
-      // one count serves all barriers: nobody arrives at one before the last is
-      // complete (a CTA without a run in the second phase has not waited for it)
-      barrier_wait(g.barrier, hidden_target, abortp);
       barrier_arrive(g.barrier);
       barrier_wait(g.barrier, down_target, abortp);
     }
@@ -834,8 +865,7 @@ size_t moe_workspace(MoeArgs* g, void* base) {
   const int sms = device_sm_count();
   const int64_t pairs = (int64_t)g->T * g->k, experts = pairs < g->E ? pairs : g->E;
   g->splits = router_splits(g->T, g->E, g->H, sms);
-  g->n_counters1 = (int)(experts * (g->I / 128));
-  g->n_counters = g->n_counters1 + (int)(experts * ((g->H + 255) / 256));
+  g->n_counts = 2 * sms + (int)experts;
   size_t at = 0;
   uint8_t* p = static_cast<uint8_t*>(base);
   auto take = [&](size_t bytes) {
@@ -844,7 +874,8 @@ size_t moe_workspace(MoeArgs* g, void* base) {
     return r;
   };
   g->barrier = reinterpret_cast<uint64_t*>(take(8));
-  g->counters = reinterpret_cast<int*>(take((size_t)g->n_counters * 4));
+  g->part_flag = reinterpret_cast<int*>(take((size_t)g->n_counts * 4));
+  g->ready = g->part_flag + 2 * sms;
   g->logits = reinterpret_cast<float*>(take((size_t)g->splits * g->T * g->E * 4));
   int* ids = reinterpret_cast<int*>(take((size_t)pairs * 4));
   float* weights = reinterpret_cast<float*>(take((size_t)pairs * 4));
