@@ -7,18 +7,19 @@
 // 128 x 1 groups of the columns (activations and gradients: the products of a
 // training step contract over either axis).
 //
-// One CTA casts one 128 x 128 tile, 256 threads: thread (rg, v) holds rows
-// 8 rg .. 8 rg + 7, columns 8 v .. 8 v + 7, eight 16-byte loads, a warp two
-// whole 256-byte row pieces a load. The tile stays in registers: a row's
-// maximum is a butterfly over the 16 lanes that share it, a column's a step
-// over the warp's two row groups and one over the 8 warps through shared
-// memory. The codes of the transpose go through a 16 KB shared tile, its
-// 8-byte pieces permuted by the column's piece number (a warp's stores then
-// cover every bank once instead of one), so that they too leave as whole
-// 128-byte row pieces.
+// One CTA casts one 128 x 128 tile, 256 threads, four CTAs an SM: thread (rg, v)
+// holds rows 8 rg .. 8 rg + 7, columns 8 v .. 8 v + 7, eight 16-byte loads, a
+// warp two whole 256-byte row pieces a load. The tile stays in registers. The
+// codes of the transpose go through a 16 KB shared tile, its 8-byte pieces
+// permuted by the column's piece number (a warp's stores then cover every bank
+// once instead of one), so that they too leave as whole 128-byte row pieces.
 //
 // Bound: memory, 2 bytes read and 2 written an element (1 without the
-// transpose).
+// transpose); next to it the instruction issue, so the block kind converts an
+// element once and transposes the bytes, and the two-way kind makes a row's
+// scale in two of the 16 lanes that share it. (A persistent form that read the
+// tiles by TMA two ahead, two CTAs an SM, was slower: 113 against 105 us at
+// 16384 x 7168.)
 #include "cutie.h"
 #include "launch.cuh"
 
@@ -39,12 +40,29 @@ __device__ __forceinline__ float rcp_of(float s, bool pow2) {
   return s <= 3.4e38f ? r : __uint_as_float(0x7fffffffu);
 }
 
+// Codes of 8 bf16 values (four pairs) over one scale; rc = RN(1 / s).
+__device__ __forceinline__ uint2 codes_of(uint32_t a, uint32_t b, uint32_t c, uint32_t d, float s,
+                                          float rc) {
+  const float2 ns = make_float2(-s, -s), r2 = make_float2(rc, rc);
+  return make_uint2(f4_to_e4m3x4(div2_rn(bf2_to_f2(a), ns, r2), div2_rn(bf2_to_f2(b), ns, r2)),
+                    f4_to_e4m3x4(div2_rn(bf2_to_f2(c), ns, r2), div2_rn(bf2_to_f2(d), ns, r2)));
+}
+
+// Four rows of four bytes -> four columns.
+__device__ __forceinline__ void transpose4(uint32_t a, uint32_t b, uint32_t c, uint32_t d,
+                                           uint32_t (&t)[4]) {
+  const uint32_t ab0 = __byte_perm(a, b, 0x5140), ab1 = __byte_perm(a, b, 0x7362);
+  const uint32_t cd0 = __byte_perm(c, d, 0x5140), cd1 = __byte_perm(c, d, 0x7362);
+  t[0] = __byte_perm(ab0, cd0, 0x5410), t[1] = __byte_perm(ab0, cd0, 0x7632);
+  t[2] = __byte_perm(ab1, cd1, 0x5410), t[3] = __byte_perm(ab1, cd1, 0x7632);
+}
+
 template <bool BLOCK, bool TRANSPOSED>
 __global__ void __launch_bounds__(kThreads, 4)
     cast_tiles_kernel(CastArgs a) {
   __shared__ __align__(16) uint8_t t_codes[TRANSPOSED ? kTile * kTile : 16];
   __shared__ __align__(16) uint32_t part[8][64];  // a warp's column maxima (bf16 pairs)
-  __shared__ float2 col_scale[kTile];             // (scale, reciprocal) of a column
+  __shared__ float2 col_scale[8][16];             // (scale, reciprocal) of column 8 v + j at [j][v]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rg = tid >> 4, v = tid & 15;
   const int tiles_c = (a.H + kTile - 1) / kTile;
@@ -63,23 +81,16 @@ __global__ void __launch_bounds__(kThreads, 4)
     if (col_ok && r0 + i < a.M) w = ld_stream(a.x + (r0 + i) * a.ldx + c0);
     x[i][0] = w.x, x[i][1] = w.y, x[i][2] = w.z, x[i][3] = w.w;
   }
-  // magnitudes: a row's over 8 columns, a column pair's over 8 rows
-  uint32_t rmax[8], cmax[4];
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    rmax[i] = absmax_bf2(absmax_bf2(x[i][0], x[i][1]), absmax_bf2(x[i][2], x[i][3])) & 0x7fff7fffu;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    uint32_t m = x[0][j];
-#pragma unroll
-    for (int i = 1; i < 8; ++i) m = absmax_bf2(m, x[i][j]);
-    cmax[j] = m & 0x7fff7fffu;
-  }
-  float row_s[8];
+  const uint32_t all = 0xffffffffu;
+  uint2 codes[BLOCK ? 8 : 1];  // block kind: the rows' codes, which its transpose shares
   if (BLOCK) {
-    uint32_t m = max_bf2(max_bf2(cmax[0], cmax[1]), max_bf2(cmax[2], cmax[3]));
+    uint32_t m = 0;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = max_bf2(m, __shfl_xor_sync(0xffffffffu, m, o));
+    for (int i = 0; i < 8; ++i)
+      m = absmax_bf2(m, absmax_bf2(absmax_bf2(x[i][0], x[i][1]), absmax_bf2(x[i][2], x[i][3])));
+    m &= 0x7fff7fffu;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = max_bf2(m, __shfl_xor_sync(all, m, o));
     if (lane == 0) part[warp][0] = m;
     __syncthreads();
     m = part[0][0];
@@ -87,73 +98,99 @@ __global__ void __launch_bounds__(kThreads, 4)
     for (int w = 1; w < 8; ++w) m = max_bf2(m, part[w][0]);
     const float2 f = bf2_to_f2(m);
     const float s = tile_scale(fmaxf(f.x, f.y), a.pow2);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) row_s[i] = s;
     if (tid == 0) {
       a.s[tr * a.lds + tc] = s;
       if (TRANSPOSED) a.st[(int64_t)tc * a.ldst + tr] = s;
     }
+    const float rc = rcp_of(s, a.pow2);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) codes[i] = codes_of(x[i][0], x[i][1], x[i][2], x[i][3], s, rc);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (col_ok && r0 + i < a.M) st_stream2(a.q + (r0 + i) * a.ldq + c0, codes[i].x, codes[i].y);
   } else {
+    // column maxima over the thread's 8 rows, the warp's two row groups, the warps
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t m = x[0][j];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) m = absmax_bf2(m, x[i][j]);
+      m &= 0x7fff7fffu;
+      m = max_bf2(m, __shfl_xor_sync(all, m, 16));
+      if (lane < 16) part[warp][v * 4 + j] = m;
+    }
+    // row maxima over the 16 lanes of a row group, folded so that lanes 2 i and
+    // 2 i + 1 end with row i's: each lane then makes one scale, not eight
+    uint32_t m[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      m[i] = absmax_bf2(absmax_bf2(x[i][0], x[i][1]), absmax_bf2(x[i][2], x[i][3])) & 0x7fff7fffu;
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) {
+      const bool up = (v & (2 * o)) != 0;
+#pragma unroll
+      for (int i = 0; i < o; ++i) {
+        const uint32_t keep = up ? m[i + o] : m[i], send = up ? m[i] : m[i + o];
+        m[i] = max_bf2(keep, __shfl_xor_sync(all, send, 2 * o));
+      }
+    }
+    const float2 f = bf2_to_f2(max_bf2(m[0], __shfl_xor_sync(all, m[0], 1)));
+    const float my_s = tile_scale(fmaxf(f.x, f.y), a.pow2), my_rc = rcp_of(my_s, a.pow2);
+    if ((v & 1) == 0 && r0 + (v >> 1) < a.M) a.s[(int64_t)tc * a.lds + r0 + (v >> 1)] = my_s;
+    __syncthreads();
+    if (tid < 64) {  // columns 2 tid and 2 tid + 1, kept so that a warp's 16 reads below are in a row
+      uint32_t c = part[0][tid];
+#pragma unroll
+      for (int w = 1; w < 8; ++w) c = max_bf2(c, part[w][tid]);
+      const float2 g = bf2_to_f2(c);
+      const float s0 = tile_scale(g.x, a.pow2), s1 = tile_scale(g.y, a.pow2);
+      col_scale[2 * (tid & 3)][tid >> 2] = make_float2(s0, rcp_of(s0, a.pow2));
+      col_scale[2 * (tid & 3) + 1][tid >> 2] = make_float2(s1, rcp_of(s1, a.pow2));
+      const int at = tc * kTile + 2 * tid;
+      if (at < a.H) {  // H is even
+        a.st[tr * a.ldst + at] = s0;
+        a.st[tr * a.ldst + at + 1] = s1;
+      }
+    }
+    // codes along the rows: 8 a thread, 128 contiguous bytes a row of the tile
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      uint32_t m = rmax[i];
-#pragma unroll
-      for (int o = 8; o > 0; o >>= 1) m = max_bf2(m, __shfl_xor_sync(0xffffffffu, m, o));
-      const float2 f = bf2_to_f2(m);
-      row_s[i] = tile_scale(fmaxf(f.x, f.y), a.pow2);
-      if (v == i && r0 + i < a.M) a.s[(int64_t)tc * a.lds + r0 + i] = row_s[i];
+      const float s = __shfl_sync(all, my_s, 2 * i, 16), rc = __shfl_sync(all, my_rc, 2 * i, 16);
+      const uint2 w = codes_of(x[i][0], x[i][1], x[i][2], x[i][3], s, rc);
+      if (col_ok && r0 + i < a.M) st_stream2(a.q + (r0 + i) * a.ldq + c0, w.x, w.y);
     }
-    if (TRANSPOSED) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        cmax[j] = max_bf2(cmax[j], __shfl_xor_sync(0xffffffffu, cmax[j], 16));
-        if (lane < 16) part[warp][v * 4 + j] = cmax[j];
-      }
-      __syncthreads();
-      if (tid < 64) {
-        uint32_t m = part[0][tid];
-#pragma unroll
-        for (int w = 1; w < 8; ++w) m = max_bf2(m, part[w][tid]);
-        const float2 f = bf2_to_f2(m);
-        const float s0 = tile_scale(f.x, a.pow2), s1 = tile_scale(f.y, a.pow2);
-        col_scale[2 * tid] = make_float2(s0, rcp_of(s0, a.pow2));
-        col_scale[2 * tid + 1] = make_float2(s1, rcp_of(s1, a.pow2));
-        const int c = tc * kTile + 2 * tid;
-        if (c < a.H) a.st[tr * a.ldst + c] = s0;
-        if (c + 1 < a.H) a.st[tr * a.ldst + c + 1] = s1;
-      }
-    }
-  }
-  // codes along the rows: 8 a thread, 128 contiguous bytes a row of the tile
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float s = row_s[i], rc = rcp_of(s, a.pow2);
-    const float2 ns = make_float2(-s, -s), r2 = make_float2(rc, rc);
-    float2 y[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) y[j] = div2_rn(bf2_to_f2(x[i][j]), ns, r2);
-    const uint32_t lo = f4_to_e4m3x4(y[0], y[1]), hi = f4_to_e4m3x4(y[2], y[3]);
-    if (col_ok && r0 + i < a.M) st_stream2(a.q + (r0 + i) * a.ldq + c0, lo, hi);
   }
   if (!TRANSPOSED) return;
-  // codes along the columns: a column's 8 rows of this thread are 8 bytes
-  if (!BLOCK) __syncthreads();
+  // codes along the columns: a column's 8 rows of this thread are 8 bytes, piece
+  // rg of its column, permuted by c / 8 = v
+  if (BLOCK) {
+    // the 8 x 8 bytes transposed in registers: 4 x 4 blocks
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
+    for (int q = 0; q < 2; ++q) {
+      uint32_t top[4], low[4];
+      transpose4(q ? codes[0].y : codes[0].x, q ? codes[1].y : codes[1].x, q ? codes[2].y : codes[2].x,
+                 q ? codes[3].y : codes[3].x, top);
+      transpose4(q ? codes[4].y : codes[4].x, q ? codes[5].y : codes[5].x, q ? codes[6].y : codes[6].x,
+                 q ? codes[7].y : codes[7].x, low);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int c = v * 8 + 2 * j + h;
-      const float2 sc = BLOCK ? make_float2(row_s[0], rcp_of(row_s[0], a.pow2)) : col_scale[c];
-      const float2 ns = make_float2(-sc.x, -sc.x), r2 = make_float2(sc.y, sc.y);
-      float2 y[4];
+      for (int c = 0; c < 4; ++c)
+        *reinterpret_cast<uint2*>(t_codes + (v * 8 + 4 * q + c) * kTile + ((rg ^ v) << 3)) =
+            make_uint2(top[c], low[c]);
+    }
+  } else {
+    __syncthreads();
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 p = bf2_to_f2(x[2 * i][j]), q = bf2_to_f2(x[2 * i + 1][j]);
-        y[i] = div2_rn(h ? make_float2(p.y, q.y) : make_float2(p.x, q.x), ns, r2);
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float2 sc = col_scale[2 * j + h][v];
+        // rows 2 i and 2 i + 1 of the column as a pair
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = __byte_perm(x[2 * i][j], x[2 * i + 1][j], h ? 0x7632 : 0x5410);
+        *reinterpret_cast<uint2*>(t_codes + (v * 8 + 2 * j + h) * kTile + ((rg ^ v) << 3)) =
+            codes_of(w[0], w[1], w[2], w[3], sc.x, sc.y);
       }
-      // piece rg of column c, permuted by c / 8 = v
-      *reinterpret_cast<uint2*>(t_codes + c * kTile + ((rg ^ v) << 3)) =
-          make_uint2(f4_to_e4m3x4(y[0], y[1]), f4_to_e4m3x4(y[2], y[3]));
     }
   }
   __syncthreads();

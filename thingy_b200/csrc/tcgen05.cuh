@@ -341,6 +341,19 @@ inline PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return fn;
 }
 
+// The encoder needs a current context, which a thread that has made no runtime
+// call yet (autograd's) lacks: bind the device's and try once more.
+template <class F>
+inline bool encode_with_context(F encode) {
+  CUresult r = encode();
+  if (r != CUDA_SUCCESS) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return false;
+    r = encode();
+  }
+  return r == CUDA_SUCCESS;
+}
+
 // A [rows, K] e4m3 operand, K contiguous, `ld` bytes between rows: boxes of
 // 128 K bytes x box_rows rows, 128-byte swizzle, zero fill past the last row.
 inline bool encode_e4m3_operand(CUtensorMap* map, const void* ptr, int64_t rows, int64_t K,
@@ -351,9 +364,11 @@ inline bool encode_e4m3_operand(CUtensorMap* map, const void* ptr, int64_t rows,
   const cuuint64_t strides[1] = {(cuuint64_t)ld};
   const cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
   const cuuint32_t estr[2] = {1, 1};
-  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box,
-            estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return encode_with_context([&] {
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box,
+              estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  });
 }
 
 }  // namespace tc

@@ -184,10 +184,8 @@ int64_t ceil_to(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
 
 // e4m3 [R, C] with rows on 16-byte boundaries (what the block-scaled GEMM takes).
 at::Tensor empty_codes(int64_t R, int64_t C, const at::Device& dev) {
-  const auto opt = at::TensorOptions().device(dev).dtype(at::kFloat8_e4m3fn);
-  const int64_t ld = ceil_to(C, 16);
-  at::Tensor t = at::empty({R, ld}, opt);
-  return ld == C ? t : t.narrow(1, 0, C);
+  return at::empty_strided({R, C}, {ceil_to(C, 16), 1},
+                           at::TensorOptions().device(dev).dtype(at::kFloat8_e4m3fn));
 }
 
 // Casts to e4m3 in both orientations (cutie_cast_fp8_tiles); qt and st are
@@ -204,11 +202,11 @@ cast_fp8_tiles(const at::Tensor& x, bool block, bool use_ue8m0, bool transposed)
   const int64_t GM = (M + 127) / 128, GH = (H + 127) / 128;
   const auto f32 = at::TensorOptions().device(dev).dtype(at::kFloat);
   at::Tensor q = empty_codes(M, H, dev);
-  at::Tensor s = block ? at::empty({GM, GH}, f32) : at::empty({GH, M}, f32);
+  at::Tensor s = block ? at::empty({GM, GH}, f32) : at::empty_strided({M, GH}, {1, M}, f32);
   at::Tensor qt, st;
   if (transposed) {
     qt = empty_codes(H, M, dev);
-    st = block ? at::empty({GH, GM}, f32) : at::empty({GM, H}, f32);
+    st = block ? at::empty({GH, GM}, f32) : at::empty_strided({H, GM}, {1, H}, f32);
   }
   const c10::cuda::CUDAGuard guard(dev);
   void* stream = at::cuda::getCurrentCUDAStream(dev.index()).stream();
@@ -219,8 +217,8 @@ cast_fp8_tiles(const at::Tensor& x, bool block, bool use_ue8m0, bool transposed)
       transposed ? ceil_to(M, 16) : 0, transposed ? st.data_ptr() : nullptr,
       transposed ? (block ? GM : H) : 0, stream));
   c10::optional<at::Tensor> oqt, ost;
-  if (transposed) oqt = qt, ost = block ? st : st.t();
-  return {q, block ? s : s.t(), oqt, ost};
+  if (transposed) oqt = qt, ost = st;
+  return {q, s, oqt, ost};
 }
 
 // D = dequant(a) dequant(b)^T (cutie_fp8_block_gemm) into `out`, or a new tensor.
@@ -271,81 +269,147 @@ at::Tensor fp8_block_gemm(const at::Tensor& a, const at::Tensor& a_scale, const 
   return d;
 }
 
-// A linear layer in 8 bits under autograd: y = q(x) q(w)^T, dx = q(dy) q(w),
+// ---- A linear layer in 8 bits under autograd: y = q(x) q(w)^T, dx = q(dy) q(w),
 // dw = q(dy)^T q(x), x and dy in 1 x 128 groups along both axes, w in 128 x 128
-// blocks. In C++: the Python form of the same calls spent 150 us of host time a
-// step, twice what the kernels of a 1001 x 1544 x 2048 step take.
+// blocks. In C++, and with a cast's four results in one buffer: as Python calls
+// of the functions above a step took 150 us of host time, twice what the
+// kernels of a 1001 x 1544 x 2048 step take.
+
+// An operand of the block-scaled product.
+struct Operand {
+  const void* q = nullptr;
+  int64_t ld = 0;
+  const void* s = nullptr;
+  int64_t s_row = 0, s_kb = 0;
+};
+
+// A matrix's codes and its transpose's, in one buffer.
+struct CastBuffer {
+  int64_t R, C;
+  bool block;
+  at::Tensor hold;
+  int64_t off_s, off_qt, off_st, bytes;
+
+  CastBuffer(int64_t rows, int64_t cols, bool blocks) : R(rows), C(cols), block(blocks) {
+    const int64_t GR = (R + 127) / 128, GC = (C + 127) / 128;
+    off_s = ceil_to(R * ceil_to(C, 16), 256);
+    off_qt = off_s + ceil_to(4 * (block ? GR * GC : GC * R), 256);
+    off_st = off_qt + ceil_to(C * ceil_to(R, 16), 256);
+    bytes = off_st + 4 * (block ? GR * GC : GR * C);
+  }
+  uint8_t* base() const { return static_cast<uint8_t*>(hold.data_ptr()); }
+  Operand rows() const {
+    return {base(), ceil_to(C, 16), base() + off_s, block ? (C + 127) / 128 : 1, block ? 1 : R};
+  }
+  Operand columns() const {
+    return {base() + off_qt, ceil_to(R, 16), base() + off_st, block ? (R + 127) / 128 : 1, block ? 1 : C};
+  }
+  void cast(const at::Tensor& x, bool transposed, void* stream) {
+    if (R > 1 && (x.stride(1) != 1 || x.stride(0) < C)) bad("x must be contiguous along its last dimension");
+    hold = at::empty({transposed ? bytes : off_qt}, x.options().dtype(at::kByte));
+    check_status(cutie_cast_fp8_tiles(
+        x.data_ptr(), R <= 1 ? ceil_to(C, 8) : x.stride(0), R, C,
+        block ? CUTIE_TILE_BLOCK : CUTIE_TILE_TWO_WAY, CUTIE_SCALE_FP32, base(), ceil_to(C, 16),
+        base() + off_s, block ? (C + 127) / 128 : R, transposed ? base() + off_qt : nullptr,
+        transposed ? ceil_to(R, 16) : 0, transposed ? base() + off_st : nullptr,
+        transposed ? (block ? (R + 127) / 128 : C) : 0, stream));
+  }
+};
+
+at::Tensor product(const Operand& a, const Operand& b, bool b_rows, int64_t M, int64_t N, int64_t K,
+                   const at::Tensor& like, bool f32, void* stream) {
+  at::Tensor d = at::empty({M, N}, like.options().dtype(f32 ? at::kFloat : at::kBFloat16));
+  check_status(cutie_fp8_block_gemm(a.q, a.ld, a.s, a.s_row, a.s_kb, b.q, b.ld, b.s, b.s_row, b.s_kb,
+                                    b_rows ? 1 : 0, d.data_ptr(), N,
+                                    f32 ? CUTIE_DTYPE_F32 : CUTIE_DTYPE_BF16, 0, M, N, K, stream));
+  return d;
+}
+
+Operand given(const at::Tensor& q, const at::Tensor& s, int64_t rows, int64_t cols, const at::Device& dev) {
+  check_codes(q, "weight_fp8");
+  if (q.dim() != 2 || q.size(0) != rows || q.size(1) != cols)
+    bad("weight_fp8's codes must have the weight's shape, transposed for qt");
+  if (s.dim() != 2 || s.size(0) != (rows + 127) / 128 || s.size(1) != (cols + 127) / 128 ||
+      s.scalar_type() != at::kFloat || s.device() != dev)
+    bad("weight_fp8's scales must be float32, one a 128 x 128 block");
+  return {q.data_ptr(), matrix_ld(q, "weight_fp8", dev), s.data_ptr(), s.stride(0), s.stride(1)};
+}
+
 struct FP8Linear : public torch::autograd::Function<FP8Linear> {
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x,
-                            const at::Tensor& weight, const at::Tensor& wq, const at::Tensor& ws,
+                            const at::Tensor& weight, const c10::optional<at::Tensor>& wq,
+                            const c10::optional<at::Tensor>& ws,
                             const c10::optional<at::Tensor>& wqt,
                             const c10::optional<at::Tensor>& wst, bool need_dx, bool need_dw) {
-    at::Tensor q, s, qt, st;
-    // without a weight gradient the rows alone would do; the transposed codes
-    // come from the same read
-    auto c = cast_fp8_tiles(x, false, false, true);
-    q = std::get<0>(c), s = std::get<1>(c);
-    if (need_dw) qt = *std::get<2>(c), st = *std::get<3>(c);
-    ctx->save_for_backward({qt, st, need_dx ? *wqt : at::Tensor(), need_dx ? *wst : at::Tensor()});
-    ctx->saved_data["need_dx"] = need_dx;
-    ctx->saved_data["need_dw"] = need_dw;
-    ctx->saved_data["dw_f32"] = weight.scalar_type() == at::kFloat;
-    return fp8_block_gemm(q, s, wq, ws, c10::nullopt, false, false);
+    const at::Device dev = x.device();
+    const int64_t M = x.size(0), K = x.size(1), N = weight.size(0);
+    const c10::cuda::CUDAGuard guard(dev);
+    void* stream = at::cuda::getCurrentCUDAStream(dev.index()).stream();
+    CastBuffer w(N, K, true), xs(M, K, false);
+    if (!wq.has_value())
+      w.cast(weight.scalar_type() == at::kBFloat16 ? weight : weight.to(at::kBFloat16), need_dx, stream);
+    xs.cast(x, true, stream);
+    at::Tensor y = product(xs.rows(), wq.has_value() ? given(*wq, *ws, N, K, dev) : w.rows(), false, M,
+                           N, K, x, false, stream);
+    ctx->save_for_backward({need_dw ? xs.hold : at::Tensor(),
+                            !need_dx ? at::Tensor() : wq.has_value() ? *wqt : w.hold,
+                            need_dx && wq.has_value() ? *wst : at::Tensor()});
+    ctx->saved_data["sizes"] = std::vector<int64_t>{N, K, need_dx, need_dw, wq.has_value(),
+                                                    weight.scalar_type() == at::kFloat};
+    return y;
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grads) {
     if (at::GradMode::is_enabled())
       throw std::runtime_error("fp8_linear has no second derivatives (create_graph)");
+    torch::autograd::variable_list out(8);
+    if (!grads[0].defined()) return out;
     const auto saved = ctx->get_saved_variables();
-    const bool need_dx = ctx->saved_data["need_dx"].toBool();
-    const bool need_dw = ctx->saved_data["need_dw"].toBool();
-    at::Tensor dx, dw;
-    if (grads[0].defined()) {
-      auto c = cast_fp8_tiles(grads[0].contiguous(), false, false, true);
-      if (need_dx)
-        dx = fp8_block_gemm(std::get<0>(c), std::get<1>(c), saved[2], saved[3], c10::nullopt, false,
-                            false);
-      if (need_dw)
-        dw = fp8_block_gemm(*std::get<2>(c), *std::get<3>(c), saved[0], saved[1], c10::nullopt,
-                            ctx->saved_data["dw_f32"].toBool(), false);
+    const auto sizes = ctx->saved_data["sizes"].toIntVector();
+    const int64_t N = sizes[0], K = sizes[1];
+    const at::Tensor dy = grads[0].contiguous();
+    const int64_t M = dy.size(0);
+    const at::Device dev = dy.device();
+    const c10::cuda::CUDAGuard guard(dev);
+    void* stream = at::cuda::getCurrentCUDAStream(dev.index()).stream();
+    CastBuffer d(M, N, false), w(N, K, true), xs(M, K, false);
+    d.cast(dy, true, stream);
+    if (sizes[2]) {
+      Operand wt;
+      if (sizes[4]) {
+        wt = given(saved[1], saved[2], K, N, dev);
+      } else {
+        w.hold = saved[1];
+        wt = w.columns();
+      }
+      out[0] = product(d.rows(), wt, false, M, K, N, dy, false, stream);
     }
-    return {dx, dw, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(),
-            at::Tensor()};
+    if (sizes[3]) {
+      xs.hold = saved[0];
+      out[1] = product(d.columns(), xs.columns(), true, N, K, M, dy, sizes[5] != 0, stream);
+    }
+    return out;
   }
 };
 
 at::Tensor fp8_linear(const at::Tensor& x, const at::Tensor& weight,
-                      const c10::optional<at::Tensor>& wq_, const c10::optional<at::Tensor>& ws_,
-                      const c10::optional<at::Tensor>& wqt_,
-                      const c10::optional<at::Tensor>& wst_) {
+                      const c10::optional<at::Tensor>& wq, const c10::optional<at::Tensor>& ws,
+                      const c10::optional<at::Tensor>& wqt,
+                      const c10::optional<at::Tensor>& wst) {
   if (x.dim() < 1 || weight.dim() != 2 || x.size(-1) != weight.size(1))
     bad("x and weight must be [..., K] and [N, K]");
+  if (!x.is_cuda()) bad("x must be a CUDA tensor (this library has no CPU path)");
+  if (weight.device() != x.device()) bad("weight is on the wrong device");
   if (x.scalar_type() != at::kBFloat16) bad("x must be bfloat16");
   if (weight.scalar_type() != at::kBFloat16 && weight.scalar_type() != at::kFloat)
     bad("weight must be bfloat16 or float32");
   if (weight.size(0) % 8 != 0 || weight.size(1) % 8 != 0) bad("weight's sizes must be multiples of 8");
   const bool grad = at::GradMode::is_enabled();
   const bool need_dx = grad && x.requires_grad(), need_dw = grad && weight.requires_grad();
-  at::Tensor wq, ws;
-  c10::optional<at::Tensor> wqt, wst;
-  if (wq_.has_value()) {
-    if (!ws_.has_value()) bad("weight_fp8 must be (q, s, qt, st)");
-    if (wq_->dim() != 2 || wq_->sizes() != weight.sizes()) bad("weight_fp8's codes must have the weight's shape");
-    wq = *wq_, ws = *ws_;
-    if (need_dx) {
-      if (!wqt_.has_value() || !wst_.has_value())
-        bad("weight_fp8 has no transposed codes: make it with "
-            "per_block_cast_to_fp8(weight, transposed=True)");
-      if (wqt_->dim() != 2 || wqt_->size(0) != weight.size(1) || wqt_->size(1) != weight.size(0))
-        bad("weight_fp8's transposed codes must have the transposed weight's shape");
-      wqt = wqt_, wst = wst_;
-    }
-  } else {
-    at::NoGradGuard no_grad;
-    auto c = cast_fp8_tiles(weight.to(at::kBFloat16), true, false, need_dx);
-    wq = std::get<0>(c), ws = std::get<1>(c);
-    if (need_dx) wqt = std::get<2>(c), wst = std::get<3>(c);
-  }
+  if (wq.has_value() != ws.has_value()) bad("weight_fp8 must be (q, s, qt, st)");
+  if (wq.has_value() && need_dx && (!wqt.has_value() || !wst.has_value()))
+    bad("weight_fp8 has no transposed codes: make it with "
+        "per_block_cast_to_fp8(weight, transposed=True)");
   const at::Tensor x2 = x.dim() == 2 ? x : x.reshape({-1, x.size(-1)});
   at::Tensor y = FP8Linear::apply(x2, weight, wq, ws, wqt, wst, need_dx, need_dw);
   if (x.dim() == 2) return y;
