@@ -757,6 +757,9 @@ __global__ void __launch_bounds__(kFewThreads, FewPlan<BR>::kCtas)
       if (m > 0)
         mbar_wait_bounded(smem_addr(&acc_full[(m - 1) % P::kBufs]), ((m - 1) / P::kBufs) & 1u,
                           kDrainLimitCycles);
+      // and what other ranks may have sent here: nothing counts it now
+      for (const long long t0 = clock64(); clock64() - t0 < kDrainLimitCycles / 100;) {
+      }
     }
     __syncthreads();
   }

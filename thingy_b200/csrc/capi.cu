@@ -820,8 +820,6 @@ extern "C" int cutie_cast_fp8_tiles(const void* x, int64_t ldx, int64_t M, int64
   if (!block && qt == nullptr)
     return fail(CUTIE_ERR_INVALID_ARGUMENT, "the two-way cast needs qt and st");
   const int64_t GM = (M + 127) / 128, GH = (H + 127) / 128;
-  if (M > INT32_MAX - 128)
-    return fail(CUTIE_ERR_UNSUPPORTED, "M must be below 2^31 - 128");
   if (GM > INT32_MAX / GH)
     return fail(CUTIE_ERR_UNSUPPORTED, "M x H has more than 2^31 tiles");
   int rc;

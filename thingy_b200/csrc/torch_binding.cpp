@@ -419,7 +419,8 @@ at::Tensor fp8_linear(const at::Tensor& x, const at::Tensor& weight,
 }
 
 // Bytes of workspace of a mixture-of-experts layer; argument errors raise.
-int64_t moe_workspace_bytes(int64_t T, int64_t E, int64_t top_k, int64_t H, int64_t I) {
+int64_t moe_workspace_bytes(int64_t T, int64_t E, int64_t top_k, int64_t H, int64_t I, int64_t device) {
+  const c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
   const size_t n = cutie_moe_fp8_workspace(T, E, top_k, H, I);
   if (n == 0) bad(cutie_last_error());
   return (int64_t)n;
@@ -509,7 +510,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("fp8_linear", &fp8_linear, py::arg("x"), py::arg("weight"), py::arg("wq"), py::arg("ws"),
         py::arg("wqt"), py::arg("wst"));
   m.def("moe_workspace_bytes", &moe_workspace_bytes, py::arg("T"), py::arg("E"), py::arg("top_k"),
-        py::arg("H"), py::arg("I"));
+        py::arg("H"), py::arg("I"), py::arg("device"));
   m.def("moe_fp8", &moe_fp8, py::arg("x"), py::arg("q"), py::arg("scale"), py::arg("router"),
         py::arg("bias"), py::arg("w13"), py::arg("w13_scale"), py::arg("w2"), py::arg("w2_scale"),
         py::arg("top_k"), py::arg("scoring"), py::arg("renormalize"), py::arg("routed_scale"),

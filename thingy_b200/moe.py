@@ -23,23 +23,26 @@ def moe_workspace(T: int, E: int, top_k: int, H: int, I: int, device=None) -> to
     """A workspace for ``moe_fp8`` calls of at most these sizes, on the current stream.
 
     Calls that share one must not overlap on the GPU."""
-    device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
-    with torch.cuda.device(device):
-        n = require_binding().moe_workspace_bytes(int(T), int(E), int(top_k), int(H), int(I))
-        w = torch.empty(n, dtype=torch.uint8, device=device)
-        w[:256].zero_()  # the barrier's count; every call leaves it ready for the next
+    device = torch.device("cuda" if device is None else device)
+    if device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
+    n = require_binding().moe_workspace_bytes(int(T), int(E), int(top_k), int(H), int(I), device.index)
+    w = torch.empty(n, dtype=torch.uint8, device=device)
+    w[:256].zero_()  # the barrier's count; every call leaves it ready for the next
     return w
 
 
 def _own_workspace(x, E, top_k, H, I):
     """The current stream's workspace: calls of one stream do not overlap. A captured
     graph gets one of its own, which lives in the graph's memory."""
-    if torch.cuda.is_current_stream_capturing():
-        return moe_workspace(x.shape[0], E, top_k, H, I, x.device)
+    sizes = (x.shape[0], E, top_k, H, I)
+    with torch.cuda.device(x.device):
+        if torch.cuda.is_current_stream_capturing():
+            return moe_workspace(*sizes, x.device)
     key = (x.device.index, torch.cuda.current_stream(x.device).cuda_stream)
     w = _workspaces.get(key)
-    if w is None or w.numel() < require_binding().moe_workspace_bytes(x.shape[0], E, top_k, H, I):
-        w = _workspaces[key] = moe_workspace(x.shape[0], E, top_k, H, I, x.device)
+    if w is None or w.numel() < require_binding().moe_workspace_bytes(*sizes, x.device.index):
+        w = _workspaces[key] = moe_workspace(*sizes, x.device)
     return w
 
 
