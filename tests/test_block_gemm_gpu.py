@@ -198,7 +198,9 @@ PRODUCTS = [
     (1, 128, 128), (1, 5120, 5120), (3, 8, 16), (5, 1000, 384), (8, 136, 2048), (16, 256, 7168),
     (17, 257, 1040), (24, 640, 640), (32, 384, 129), (33, 129, 1000), (48, 2048, 4096),
     (64, 5120, 5120), (65, 130, 160), (100, 1024, 2048), (128, 128, 7168), (129, 100, 48),
-    (200, 1000, 1000), (1000, 384, 7168), (2049, 2100, 272), (4800, 8192, 512), (4097, 9000, 400),
+    (200, 1000, 1000), (1000, 384, 7168),
+    # few tiles and a long K: K split over a cluster, ragged tiles, uneven K ranges
+    (128, 2048, 7168), (150, 333, 2900), (513, 130, 2561), (300, 1000, 4096), (257, 385, 16400), (2049, 2100, 272), (4800, 8192, 512), (4097, 9000, 400),
 ]
 
 
@@ -211,14 +213,16 @@ def test_block_product(M, N, K, dtype):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("M,N,K", [(2, 3, 5), (128, 128, 128), (129, 100, 48), (130, 515, 1001),
-                                   (640, 300, 2056), (2049, 2100, 272), (4097, 9000, 400)])
+                                   (640, 300, 2056), (2049, 2100, 272), (4097, 9000, 400),
+                                   (512, 512, 8200), (131, 77, 5001), (640, 515, 2600)])
 def test_group_product(M, N, K, dtype):
     ops = _operands(M, N, K, "rows", seed=M * 3 + N + K, layout="col" if N % 2 else "row")
     _check(tb.fp8_block_gemm(*ops, out_dtype=dtype), *ops)
 
 
 @pytest.mark.parametrize("M,N,K,kind", [(9, 300, 640, "blocks"), (700, 515, 1000, "rows"),
-                                        (300, 264, 512, "blocks")])
+                                        (300, 264, 512, "blocks"), (200, 264, 4096, "blocks"),
+                                        (200, 263, 4100, "rows")])
 def test_accumulation(M, N, K, kind):
     ops = _operands(M, N, K, kind, seed=K)
     base = torch.randn(M, N, device="cuda")
@@ -228,10 +232,10 @@ def test_accumulation(M, N, K, kind):
     _check(out, *ops, base=base)
 
 
-@pytest.mark.parametrize("M", [3, 200])
+@pytest.mark.parametrize("M,K", [(3, 256), (200, 256), (200, 4096)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-def test_strided_output_is_written_between_its_columns_only(M, dtype):
-    ops = _operands(M, 200, 256, "blocks", seed=7)
+def test_strided_output_is_written_between_its_columns_only(M, K, dtype):
+    ops = _operands(M, 200, K, "blocks", seed=7)
     wide = torch.full((M, 209), -7.0, dtype=dtype, device="cuda")
     tb.fp8_block_gemm(*ops, out=wide[:, 3:203])
     _check(wide[:, 3:203], *ops)
@@ -288,7 +292,7 @@ def test_another_stream_and_graph():
 
 
 def test_product_is_the_same_every_time():
-    for M, N, K in [(20, 1000, 7168), (900, 700, 4096)]:
+    for M, N, K in [(20, 1000, 7168), (900, 700, 4096), (200, 300, 7168)]:
         ops = _operands(M, N, K, "blocks", seed=6)
         first = tb.fp8_block_gemm(*ops)
         for _ in range(5):

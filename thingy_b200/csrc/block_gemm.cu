@@ -23,6 +23,7 @@ namespace {
 
 constexpr int kBM = 128, kBK = 128;
 constexpr uint32_t kBoxBytes = kBM * kBK;  // one 128-row operand box: 16 KB
+constexpr int kMaxRanks = 8;               // of a K split: a portable cluster
 
 // Gives up after kWaitLimitCycles, or at once when the CTA's abort flag is
 // set; giving up sets the flag.
@@ -34,6 +35,52 @@ __device__ __forceinline__ bool wait_or_abort(uint32_t bar, uint32_t parity,
     if (mbar_try_wait(bar, parity)) return true;
   *abort_flag = 1u;
   return false;
+}
+
+// Clusters of S CTAs along z that run at once on the current device, remembered.
+int max_clusters(const void* kernel, int threads, size_t smem, int S,
+                 std::atomic<int> (&cache)[64][kMaxRanks + 1]) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  if (dev < 64 && cache[dev][S].load(std::memory_order_relaxed) > 0) return cache[dev][S].load();
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    return 0;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(1, 1, (unsigned)S);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 1;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = (unsigned)S;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) return 0;
+  if (dev < 64) cache[dev][S].store(n);
+  return n;
+}
+
+// Launch with clusters along z (grid.z CTAs each) and programmatic stream serialization.
+template <class K, class... A>
+cudaError_t launch_cluster(K kernel, dim3 grid, int threads, size_t smem, cudaStream_t stream,
+                           const A&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 1;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = grid.z;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 // ------------------------------------------------------------------ tiled
@@ -58,6 +105,7 @@ constexpr int kThreads = 384, kEpiWarps = 8, kBand = 16;
 // registers a thread: 256 x 216 + 128 x 64 = 63488 of the 384 x 168 = 64512 at launch
 constexpr int kEpiRegs = 216, kIssueRegs = 64;
 constexpr int kScaleBlocks = 4;  // K blocks a slot of the scale ring
+constexpr int kSplitBlocks = 16;  // see split_ranks
 
 constexpr int kStageRow = 9;  // see store_rows
 
@@ -76,6 +124,12 @@ struct TilePlan {
                     227 * 1024,
                 "shared memory");
 };
+
+// Split form: a partial tile of 128 x 128 in shared memory, rows 4 floats apart
+// from 128 (16-byte stores of 32 rows then fall into different banks).
+constexpr int kPartRow = 132;
+constexpr uint32_t kPartRowBytes = kPartRow * 4, kPartBytes = kBM * kPartRowBytes;
+static_assert(kPartBytes + (kBM + kMaxRanks) * kPartRowBytes <= 6 * 2 * kBoxBytes, "parts fit the ring");
 
 struct TileArgs {
   const float* sa;
@@ -167,7 +221,38 @@ __device__ __forceinline__ void store_rows(const TileArgs& g, const float2 (&acc
   }
 }
 
-template <int BN, bool SB_ROWS, bool VEC>
+// Four columns of a row. VEC: they are aligned in D and all or none in it.
+template <bool VEC>
+__device__ __forceinline__ void store_four(const TileArgs& g, int row, int col, float4 v) {
+  const int64_t at = (int64_t)row * g.ldd + col;
+  const float f[4] = {v.x, v.y, v.z, v.w};
+  if (g.d_f32) {
+    float* p = static_cast<float*>(g.d) + at;
+    if (VEC) {
+      if (g.accumulate) {
+        const float4 o = *reinterpret_cast<const float4*>(p);
+        v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+      }
+      *reinterpret_cast<float4*>(p) = v;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (col + i < g.N) p[i] = g.accumulate ? p[i] + f[i] : f[i];
+    }
+  } else {
+    uint16_t* p = static_cast<uint16_t*>(g.d) + at;
+    const uint32_t lo = f2_to_bf2(make_float2(v.x, v.y)), hi = f2_to_bf2(make_float2(v.z, v.w));
+    if (VEC) {
+      *reinterpret_cast<uint2*>(p) = make_uint2(lo, hi);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (col + i < g.N) p[i] = (uint16_t)((i < 2 ? lo : hi) >> (16 * (i & 1)));
+    }
+  }
+}
+
+template <int BN, bool SB_ROWS, bool VEC, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
     block_gemm_kernel(const __grid_constant__ CUtensorMap map_a,
                       const __grid_constant__ CUtensorMap map_b, const TileArgs g) {
@@ -181,7 +266,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ __align__(8) uint64_t scale_full[P::kScaleSlots];
   __shared__ __align__(8) uint64_t scale_empty[P::kScaleSlots];
   __shared__ __align__(16) float scales[P::kScaleSlots][kScaleBlocks][P::kScales];
-  __shared__ float stage[VEC ? 1 : kEpiWarps][32 * kStageRow];
+  __shared__ float stage[VEC || SPLIT ? 1 : kEpiWarps][32 * kStageRow];
+  __shared__ __align__(8) uint64_t recv_bar;
   __shared__ uint32_t tmem_base_slot;
   __shared__ uint32_t abort_flag;
   __shared__ uint32_t issued;     // K blocks whose copies were issued
@@ -190,6 +276,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
   const int tiles = g.tiles_m * g.tiles_n;
+  // K blocks of this CTA: all, or the rank's of its cluster
+  const int S = SPLIT ? (int)gridDim.z : 1, rank = SPLIT ? (int)tc::cluster_ctarank() : 0;
+  const int kb0 = SPLIT ? (int)((int64_t)g.KB * rank / S) : 0;
+  const int nkb = SPLIT ? (int)((int64_t)g.KB * (rank + 1) / S) - kb0 : g.KB;
+  // and the tile's rows that it adds up
+  const int share = (kBM + S - 1) / S, own_lo = min(rank * share, kBM), own_n = min(share, kBM - own_lo);
   volatile uint32_t* abortp = &abort_flag;
 
   if (threadIdx.x == 0) {
@@ -207,9 +299,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(smem_addr(&scale_full[s]), 32);
       mbar_init(smem_addr(&scale_empty[s]), kEpiWarps);
     }
+    if (SPLIT) mbar_init(smem_addr(&recv_bar), 1);
     abort_flag = 0;
     issued = committed = 0;
     mbar_init_fence();
+    if (SPLIT) mbar_arrive_expect_tx(smem_addr(&recv_bar), (uint32_t)((S - 1) * own_n) * kPartRowBytes);
   }
   if (warp == kEpiWarps) tc::tmem_alloc(smem_addr(&tmem_base_slot), P::kTmemCols);
   tc::fence_before();
@@ -229,7 +323,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
       int tm, tn;
       tile_at(t, g.tiles_m, g.tiles_n, &tm, &tn);
-      for (int kb = 0; kb < g.KB; ++kb) {
+      for (int kb = 0; kb < nkb; ++kb) {
         ok = wait_or_abort(smem_addr(&empty_bar[s]), parity, abortp);
         if (!__all_sync(0xffffffffu, ok)) {
           ok = false;
@@ -238,10 +332,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (leader) {
           const uint32_t st = base + s * P::kStageBytes, bar = smem_addr(&full_bar[s]);
           mbar_arrive_expect_tx(bar, P::kStageBytes);
-          tc::tma_load_2d(st, &map_a, kb * kBK, tm * kBM, bar);
+          tc::tma_load_2d(st, &map_a, (kb0 + kb) * kBK, tm * kBM, bar);
 #pragma unroll
           for (int h = 0; h < P::kNB; ++h)
-            tc::tma_load_2d(st + (1 + h) * kBoxBytes, &map_b, kb * kBK, tn * BN + 128 * h, bar);
+            tc::tma_load_2d(st + (1 + h) * kBoxBytes, &map_b, (kb0 + kb) * kBK, tn * BN + 128 * h, bar);
           ++issued;
         }
         if (++s == P::kStages) s = 0, parity ^= 1;
@@ -255,7 +349,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t s = 0, parity = 0, buf = 0, buf_parity = 1;
     bool ok = true;
     for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-      for (int kb = 0; kb < g.KB; ++kb) {
+      for (int kb = 0; kb < nkb; ++kb) {
         ok = wait_or_abort(smem_addr(&full_bar[s]), parity, abortp) &&
              wait_or_abort(smem_addr(&acc_empty[buf]), buf_parity, abortp);
         if (!__all_sync(0xffffffffu, ok)) {
@@ -291,15 +385,15 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int row = tm * kBM + lane + 32 * i;
-        pa[i] = row < g.M ? g.sa + (int64_t)row * g.sa_row : nullptr;
+        pa[i] = row < g.M ? g.sa + (int64_t)row * g.sa_row + kb0 * g.sa_kb : nullptr;
       }
 #pragma unroll
       for (int i = 0; i < kNS; ++i) {
         const int col = tn * BN + (SB_ROWS ? lane + 32 * i : 128 * lane);
         const bool some = col < g.N && (SB_ROWS || lane < P::kNB);
-        pb[i] = some ? g.sb + (int64_t)(SB_ROWS ? col : col / 128) * g.sb_row : nullptr;
+        pb[i] = some ? g.sb + (int64_t)(SB_ROWS ? col : col / 128) * g.sb_row + kb0 * g.sb_kb : nullptr;
       }
-      for (int kb = 0; kb < g.KB; ++kb) {
+      for (int kb = 0; kb < nkb; ++kb) {
         const int j = kb % kScaleBlocks;
         if (j == 0) {
           ok = __all_sync(0xffffffffu, wait_or_abort(smem_addr(&scale_empty[s]), parity, abortp));
@@ -317,7 +411,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc::cp_async_4(smem_addr(&scales[s][j][128 + lane + 32 * i]), pb[i]);
             pb[i] += g.sb_kb;
           }
-        if (j == kScaleBlocks - 1 || kb == g.KB - 1) {
+        if (j == kScaleBlocks - 1 || kb == nkb - 1) {
           tc::cp_async_arrive(smem_addr(&scale_full[s]));
           if (++s == P::kScaleSlots) s = 0, parity ^= 1;
         }
@@ -360,8 +454,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       float2 acc[NC / 2];
 #pragma unroll
       for (int i = 0; i < NC / 2; ++i) acc[i] = make_float2(0.f, 0.f);
-      for (int kb = 0; kb < g.KB; ++kb) {
-        const bool last = kb == g.KB - 1;
+      for (int kb = 0; kb < nkb; ++kb) {
+        const bool last = kb == nkb - 1;
         const float s = sc;
         const float* col = sb;
         const uint32_t tm = tm_lane + buf * BN;
@@ -416,11 +510,65 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       int tm_i, tn_i;
       tile_at(t, g.tiles_m, g.tiles_n, &tm_i, &tn_i);
-      if (*abortp == 0u) store_rows<NC, VEC>(g, acc, tm_i * kBM + (warp & 3) * 32, tn_i * BN + wg * NC, lane,
-                            stage[VEC ? 0 : warp]);
+      if constexpr (!SPLIT) {
+        if (*abortp == 0u)
+          store_rows<NC, VEC>(g, acc, tm_i * kBM + (warp & 3) * 32, tn_i * BN + wg * NC, lane,
+                              stage[VEC ? 0 : warp]);
+      } else {
+        // the last accumulator was complete, so this CTA's ring is idle, and so
+        // are the others' once they have arrived too: the partial tile to the
+        // ring, every rank's share of its rows to that rank, and what came from
+        // the others added in rank order
+        float* part = reinterpret_cast<float*>(smem_raw + (base - smem_addr(smem_raw)));
+        asm volatile("barrier.cta.sync 1, 256;" ::: "memory");  // all warps are past the ring
+#pragma unroll
+        for (int c = 0; c < NC; c += 4)
+          *reinterpret_cast<float4*>(part + r * kPartRow + wg * NC + c) =
+              make_float4(acc[c / 2].x, acc[c / 2].y, acc[c / 2 + 1].x, acc[c / 2 + 1].y);
+        tc::fence_async_smem();
+        asm volatile("barrier.cta.sync 1, 256;" ::: "memory");
+        tc::cluster_arrive();
+        tc::cluster_wait();
+        if (threadIdx.x == 0 && *abortp == 0u) {
+          for (int q = 0; q < S; ++q) {
+            const int lo_q = min(q * share, kBM), n = min(share, kBM - lo_q);
+            if (q == rank || n == 0) continue;
+            tc::bulk_s2c(tc::mapa(base + kPartBytes + (uint32_t)(rank * share) * kPartRowBytes, (uint32_t)q),
+                         smem_addr(part + lo_q * kPartRow), (uint32_t)n * kPartRowBytes,
+                         tc::mapa(smem_addr(&recv_bar), (uint32_t)q));
+          }
+        }
+        const bool got = __all_sync(0xffffffffu, wait_or_abort(smem_addr(&recv_bar), 0u, abortp));
+        tc::cluster_arrive();  // what the others sent has arrived
+        if (got) {
+          const float* in = part + kPartBytes / 4;
+          const int col = tn_i * BN + lane * 4;
+          for (int i = warp; i < own_n; i += kEpiWarps) {
+            const int row = tm_i * kBM + own_lo + i;
+            if (row >= g.M || col >= g.N) continue;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int q = 0; q < kMaxRanks; ++q)
+              if (q < S) {
+                const float4 o = *reinterpret_cast<const float4*>(
+                    (q == rank ? part + (own_lo + i) * kPartRow : in + (q * share + i) * kPartRow) + lane * 4);
+                v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+              }
+            store_four<VEC>(g, row, col, v);
+          }
+        }
+      }
     }
   }
   __syncwarp();
+  if (SPLIT) {
+    if (warp >= kEpiWarps) {
+      tc::cluster_arrive();
+      tc::cluster_wait();
+      tc::cluster_arrive();
+    }
+    tc::cluster_wait();  // what this CTA sent has arrived: its memory may go
+  }
   tc::fence_before();
   __syncthreads();
   if (*abortp) {
@@ -434,6 +582,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (m > 0)
         mbar_wait_bounded(smem_addr(&acc_full[(m - 1) & 1u]), ((m - 1) >> 1) & 1u,
                           kDrainLimitCycles);
+      // and what other ranks may have sent here: nothing counts it now
+      for (const long long t0 = clock64(); SPLIT && clock64() - t0 < kDrainLimitCycles / 100;) {
+      }
     }
     __syncthreads();
   }
@@ -443,7 +594,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 template <int BN, bool SB_ROWS, bool VEC>
 cudaError_t launch_tiled(const BlockGemmArgs& p, TileArgs g, cudaStream_t stream) {
   using P = TilePlan<BN, SB_ROWS, VEC>;
-  auto kernel = block_gemm_kernel<BN, SB_ROWS, VEC>;
+  auto kernel = block_gemm_kernel<BN, SB_ROWS, VEC, false>;
   const cudaError_t e =
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)P::kSmemBytes);
   if (e != cudaSuccess) return e;
@@ -457,6 +608,44 @@ cudaError_t launch_tiled(const BlockGemmArgs& p, TileArgs g, cudaStream_t stream
   const int sms = device_sm_count();
   return launch_pdl(kernel, (unsigned)(tiles < sms ? tiles : sms), kThreads, P::kSmemBytes, stream,
                     map_a, map_b, g);
+}
+
+// The split form: tiles of 128 x 128 that leave SMs idle, K split over a cluster.
+template <bool SB_ROWS, bool VEC>
+int split_clusters(int S) {
+  static std::atomic<int> cache[64][kMaxRanks + 1];
+  return max_clusters(reinterpret_cast<const void*>(block_gemm_kernel<128, SB_ROWS, VEC, true>), kThreads,
+                      TilePlan<128, SB_ROWS, true>::kSmemBytes, S, cache);
+}
+
+// Ranks: the most with which all tiles still run at once; 1, not split, where that
+// leaves out fewer than kSplitBlocks K blocks of a CTA's time: adding the parts
+// costs 2 to 3 us (cold L2, unsplit against split: 512 x 2048 x 2048, 8 blocks
+// left out, 14 against 16 us; 512 x 2048 x 4096, 16 left out, 22 against 20;
+// 128 x 2048 x 7168, 28 to 49 left out, 27 against 22 to 18).
+template <bool SB_ROWS, bool VEC>
+int split_ranks(const TileArgs& g) {
+  const int64_t tiles = (int64_t)((g.M + kBM - 1) / kBM) * ((g.N + 127) / 128);
+  int S = kMaxRanks;
+  while (S > 1 && (S > g.KB || split_clusters<SB_ROWS, VEC>(S) < tiles)) --S;
+  return g.KB - (g.KB + S - 1) / S >= kSplitBlocks ? S : 1;
+}
+
+template <bool SB_ROWS, bool VEC>
+cudaError_t launch_split(const BlockGemmArgs& p, TileArgs g, int S, cudaStream_t stream) {
+  using P = TilePlan<128, SB_ROWS, true>;
+  auto kernel = block_gemm_kernel<128, SB_ROWS, VEC, true>;
+  const cudaError_t e =
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)P::kSmemBytes);
+  if (e != cudaSuccess) return e;
+  CUtensorMap map_a, map_b;
+  if (!tc::encode_e4m3_operand(&map_a, p.a, p.M, p.K, p.lda, kBM) ||
+      !tc::encode_e4m3_operand(&map_b, p.b, p.N, p.K, p.ldb, kBM))
+    return cudaErrorInvalidValue;
+  g.tiles_m = (g.M + kBM - 1) / kBM;
+  g.tiles_n = (g.N + 127) / 128;
+  return launch_cluster(kernel, dim3((unsigned)(g.tiles_m * g.tiles_n), 1, (unsigned)S), kThreads,
+                        P::kSmemBytes, stream, map_a, map_b, g);
 }
 
 // ------------------------------------------------------------------ few rows
@@ -478,7 +667,7 @@ cudaError_t launch_tiled(const BlockGemmArgs& p, TileArgs g, cudaStream_t stream
 // 18 against 22 us, 64 x 7168 x 7168 27 against 29; 64 x 16384 x 4096 (no split)
 // 28 against 24; a 128-column plan lost from 128 x 5120 x 5120 (27 against 23) on.
 constexpr int kFewRows = 64, kFewSplitRows = 32;
-constexpr int kFewThreads = 224, kFewScaleSlots = 3, kFewStep = 2, kMaxRanks = 8;
+constexpr int kFewThreads = 224, kFewScaleSlots = 3, kFewStep = 2;
 
 template <int BR>
 struct FewPlan {
@@ -766,42 +955,19 @@ __global__ void __launch_bounds__(kFewThreads, FewPlan<BR>::kCtas)
   if (warp == 5) tc::tmem_dealloc(tmem, P::kTmemCols);
 }
 
-// Clusters of S CTAs that run at once on the current device.
-template <int BR>
-int few_clusters(int S, const cudaLaunchConfig_t& base) {
-  static std::atomic<int> cache[64][kMaxRanks + 1];
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-  if (dev < 64 && cache[dev][S].load(std::memory_order_relaxed) > 0) return cache[dev][S].load();
-  if (cudaFuncSetAttribute(block_gemm_few_kernel<BR>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           (int)FewPlan<BR>::kSmemBytes) != cudaSuccess)
-    return 0;
-  cudaLaunchConfig_t cfg = base;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 1;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = (unsigned)S;
-  cfg.gridDim = dim3(1, 1, (unsigned)S);
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  int n = 0;
-  if (cudaOccupancyMaxActiveClusters(&n, block_gemm_few_kernel<BR>, &cfg) != cudaSuccess) return 0;
-  if (dev < 64) cache[dev][S].store(n);
-  return n;
-}
-
 // Ranks of the split: the most with which all tiles still run at once, a full
 // stage a rank at least. One cluster more than fit doubles the time (1 x 5120 x
 // 5120: 6 ranks 16 us, 7 ranks 20 us).
 template <int BR>
 int few_ranks(int64_t N, int64_t KB) {
+  static std::atomic<int> cache[64][kMaxRanks + 1];
   const int64_t tiles = (N + kBM - 1) / kBM;
-  cudaLaunchConfig_t cfg{};
-  cfg.blockDim = dim3(kFewThreads);
-  cfg.dynamicSmemBytes = FewPlan<BR>::kSmemBytes;
+  auto fit = [&](int S) {
+    return max_clusters(reinterpret_cast<const void*>(block_gemm_few_kernel<BR>), kFewThreads,
+                        FewPlan<BR>::kSmemBytes, S, cache);
+  };
   int S = kMaxRanks;
-  while (S > 1 && (S * kFewStep > KB || few_clusters<BR>(S, cfg) < tiles)) --S;
+  while (S > 1 && (S * kFewStep > KB || fit(S) < tiles)) --S;
   return S;
 }
 
@@ -815,21 +981,19 @@ cudaError_t launch_few(const BlockGemmArgs& p, const TileArgs& g, int S, cudaStr
   if (!tc::encode_e4m3_operand(&map_a, p.a, p.M, p.K, p.lda, BR) ||
       !tc::encode_e4m3_operand(&map_b, p.b, p.N, p.K, p.ldb, kBM))
     return cudaErrorInvalidValue;
-  cudaLaunchConfig_t cfg{};
-  cfg.blockDim = dim3(kFewThreads);
-  cfg.dynamicSmemBytes = FewPlan<BR>::kSmemBytes;
-  cfg.stream = stream;
-  cfg.gridDim = dim3((unsigned)((p.N + kBM - 1) / kBM), 1, (unsigned)S);
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = 1;
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = (unsigned)S;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, block_gemm_few_kernel<BR>, map_a, map_b, g);
+  return launch_cluster(block_gemm_few_kernel<BR>,
+                        dim3((unsigned)((p.N + kBM - 1) / kBM), 1, (unsigned)S), kFewThreads,
+                        FewPlan<BR>::kSmemBytes, stream, map_a, map_b, g);
+}
+
+// 256-wide tiles while every SM still gets one, else 128-wide ones, with K split
+// where they leave SMs idle.
+template <bool SB_ROWS, bool VEC>
+cudaError_t launch_large(const BlockGemmArgs& p, const TileArgs& g, cudaStream_t stream) {
+  const int64_t tm = (p.M + kBM - 1) / kBM;
+  if (tm * ((p.N + 255) / 256) >= device_sm_count()) return launch_tiled<256, SB_ROWS, VEC>(p, g, stream);
+  const int S = split_ranks<SB_ROWS, VEC>(g);
+  return S > 1 ? launch_split<SB_ROWS, VEC>(p, g, S, stream) : launch_tiled<128, SB_ROWS, VEC>(p, g, stream);
 }
 
 }  // namespace
@@ -864,18 +1028,9 @@ int block_gemm(const BlockGemmArgs& p, cudaStream_t stream, const char** why) {
         : columns == 32 ? launch_few<32>(p, g, ranks, stream)
                         : launch_few<64>(p, g, ranks, stream);
   } else {
-    // 256-wide tiles while every SM still gets one, else 128-wide ones
-    const int64_t tm = (p.M + kBM - 1) / kBM;
-    const bool wide = tm * ((p.N + 255) / 256) >= device_sm_count();
     const bool vec = aligned_rows_host(p.d, p.ldd * (p.d_f32 ? 4 : 2), 32) && p.N % (p.d_f32 ? 8 : 16) == 0;
-    e = wide ? (p.b_rows ? (vec ? launch_tiled<256, true, true>(p, g, stream)
-                                : launch_tiled<256, true, false>(p, g, stream))
-                         : (vec ? launch_tiled<256, false, true>(p, g, stream)
-                                : launch_tiled<256, false, false>(p, g, stream)))
-             : (p.b_rows ? (vec ? launch_tiled<128, true, true>(p, g, stream)
-                                : launch_tiled<128, true, false>(p, g, stream))
-                         : (vec ? launch_tiled<128, false, true>(p, g, stream)
-                                : launch_tiled<128, false, false>(p, g, stream)));
+    e = p.b_rows ? (vec ? launch_large<true, true>(p, g, stream) : launch_large<true, false>(p, g, stream))
+                 : (vec ? launch_large<false, true>(p, g, stream) : launch_large<false, false>(p, g, stream));
   }
   if (e != cudaSuccess) {
     *why = cudaGetErrorString(e);
