@@ -200,7 +200,7 @@ PRODUCTS = [
     (64, 5120, 5120), (65, 130, 160), (100, 1024, 2048), (128, 128, 7168), (129, 100, 48),
     (200, 1000, 1000), (1000, 384, 7168),
     # few tiles and a long K: K split over a cluster, ragged tiles, uneven K ranges
-    (128, 2048, 7168), (150, 333, 2900), (513, 130, 2561), (300, 1000, 4096), (257, 385, 16400), (2049, 2100, 272), (4800, 8192, 512), (4097, 9000, 400),
+    (128, 2048, 7168), (2500, 2304, 4100), (6500, 800, 4112), (150, 333, 2900), (513, 130, 2561), (300, 1000, 4096), (257, 385, 16400), (2049, 2100, 272), (4800, 8192, 512), (4097, 9000, 400),
 ]
 
 
@@ -214,7 +214,8 @@ def test_block_product(M, N, K, dtype):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("M,N,K", [(2, 3, 5), (128, 128, 128), (129, 100, 48), (130, 515, 1001),
                                    (640, 300, 2056), (2049, 2100, 272), (4097, 9000, 400),
-                                   (512, 512, 8200), (131, 77, 5001), (640, 515, 2600)])
+                                   (512, 512, 8200), (131, 77, 5001), (640, 515, 2600),
+                                   (2500, 2303, 4100)])
 def test_group_product(M, N, K, dtype):
     ops = _operands(M, N, K, "rows", seed=M * 3 + N + K, layout="col" if N % 2 else "row")
     _check(tb.fp8_block_gemm(*ops, out_dtype=dtype), *ops)

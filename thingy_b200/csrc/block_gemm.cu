@@ -105,7 +105,7 @@ constexpr int kThreads = 384, kEpiWarps = 8, kBand = 16;
 // registers a thread: 256 x 216 + 128 x 64 = 63488 of the 384 x 168 = 64512 at launch
 constexpr int kEpiRegs = 216, kIssueRegs = 64;
 constexpr int kScaleBlocks = 4;  // K blocks a slot of the scale ring
-constexpr int kSplitBlocks = 16;  // see split_ranks
+constexpr int kSplitBlocks = 16, kCutBlocks = 32;  // see split_ranks, launch_large
 
 constexpr int kStageRow = 9;  // see store_rows
 
@@ -139,6 +139,8 @@ struct TileArgs {
   void* d;
   int64_t ldd;
   int M, N, KB, tiles_m, tiles_n;
+  int tiles;  // to walk
+  int tail;   // 128-wide form: >= 0: the halves of the 256-wide tiles from this one on
   bool d_f32, accumulate;
 };
 
@@ -149,6 +151,16 @@ __device__ __forceinline__ void tile_at(int t, int tiles_m, int tiles_n, int* tm
   const int in = t - band * kBand * tiles_n;
   *tm = first + in % rows;
   *tn = in / rows;
+}
+
+template <int BN>
+__device__ __forceinline__ void tile_of(const TileArgs& g, int t, int* tm, int* tn) {
+  if (BN == 128 && g.tail >= 0) {
+    tile_at(g.tail + t / 2, g.tiles_m, g.tiles_n, tm, tn);
+    *tn = 2 * *tn + (t & 1);
+  } else {
+    tile_at(t, g.tiles_m, g.tiles_n, tm, tn);
+  }
 }
 
 // A warp's 32 rows of NC columns. VEC: the rows of D start on 32-byte
@@ -275,7 +287,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
-  const int tiles = g.tiles_m * g.tiles_n;
+  const int tiles = g.tiles;
   // K blocks of this CTA: all, or the rank's of its cluster
   const int S = SPLIT ? (int)gridDim.z : 1, rank = SPLIT ? (int)tc::cluster_ctarank() : 0;
   const int kb0 = SPLIT ? (int)((int64_t)g.KB * rank / S) : 0;
@@ -322,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
       int tm, tn;
-      tile_at(t, g.tiles_m, g.tiles_n, &tm, &tn);
+      tile_of<BN>(g, t, &tm, &tn);
       for (int kb = 0; kb < nkb; ++kb) {
         ok = wait_or_abort(smem_addr(&empty_bar[s]), parity, abortp);
         if (!__all_sync(0xffffffffu, ok)) {
@@ -380,7 +392,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr int kNS = SB_ROWS ? BN / 32 : 1;
     for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
       int tm, tn;
-      tile_at(t, g.tiles_m, g.tiles_n, &tm, &tn);
+      tile_of<BN>(g, t, &tm, &tn);
       const float *pa[4], *pb[kNS];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -509,7 +521,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       int tm_i, tn_i;
-      tile_at(t, g.tiles_m, g.tiles_n, &tm_i, &tn_i);
+      tile_of<BN>(g, t, &tm_i, &tn_i);
       if constexpr (!SPLIT) {
         if (*abortp == 0u)
           store_rows<NC, VEC>(g, acc, tm_i * kBM + (warp & 3) * 32, tn_i * BN + wg * NC, lane,
@@ -602,11 +614,8 @@ cudaError_t launch_tiled(const BlockGemmArgs& p, TileArgs g, cudaStream_t stream
   if (!tc::encode_e4m3_operand(&map_a, p.a, p.M, p.K, p.lda, kBM) ||
       !tc::encode_e4m3_operand(&map_b, p.b, p.N, p.K, p.ldb, kBM))
     return cudaErrorInvalidValue;
-  g.tiles_m = (g.M + kBM - 1) / kBM;
-  g.tiles_n = (g.N + BN - 1) / BN;
-  const int64_t tiles = (int64_t)g.tiles_m * g.tiles_n;
   const int sms = device_sm_count();
-  return launch_pdl(kernel, (unsigned)(tiles < sms ? tiles : sms), kThreads, P::kSmemBytes, stream,
+  return launch_pdl(kernel, (unsigned)(g.tiles < sms ? g.tiles : sms), kThreads, P::kSmemBytes, stream,
                     map_a, map_b, g);
 }
 
@@ -625,7 +634,7 @@ int split_clusters(int S) {
 // 128 x 2048 x 7168, 28 to 49 left out, 27 against 22 to 18).
 template <bool SB_ROWS, bool VEC>
 int split_ranks(const TileArgs& g) {
-  const int64_t tiles = (int64_t)((g.M + kBM - 1) / kBM) * ((g.N + 127) / 128);
+  const int tiles = g.tiles;
   int S = kMaxRanks;
   while (S > 1 && (S > g.KB || split_clusters<SB_ROWS, VEC>(S) < tiles)) --S;
   return g.KB - (g.KB + S - 1) / S >= kSplitBlocks ? S : 1;
@@ -642,9 +651,7 @@ cudaError_t launch_split(const BlockGemmArgs& p, TileArgs g, int S, cudaStream_t
   if (!tc::encode_e4m3_operand(&map_a, p.a, p.M, p.K, p.lda, kBM) ||
       !tc::encode_e4m3_operand(&map_b, p.b, p.N, p.K, p.ldb, kBM))
     return cudaErrorInvalidValue;
-  g.tiles_m = (g.M + kBM - 1) / kBM;
-  g.tiles_n = (g.N + 127) / 128;
-  return launch_cluster(kernel, dim3((unsigned)(g.tiles_m * g.tiles_n), 1, (unsigned)S), kThreads,
+  return launch_cluster(kernel, dim3((unsigned)g.tiles, 1, (unsigned)S), kThreads,
                         P::kSmemBytes, stream, map_a, map_b, g);
 }
 
@@ -986,14 +993,36 @@ cudaError_t launch_few(const BlockGemmArgs& p, const TileArgs& g, int S, cudaStr
                         FewPlan<BR>::kSmemBytes, stream, map_a, map_b, g);
 }
 
-// 256-wide tiles while every SM still gets one, else 128-wide ones, with K split
-// where they leave SMs idle.
+// The 128-wide tiles of `g`, with K split where they leave SMs idle.
 template <bool SB_ROWS, bool VEC>
-cudaError_t launch_large(const BlockGemmArgs& p, const TileArgs& g, cudaStream_t stream) {
-  const int64_t tm = (p.M + kBM - 1) / kBM;
-  if (tm * ((p.N + 255) / 256) >= device_sm_count()) return launch_tiled<256, SB_ROWS, VEC>(p, g, stream);
+cudaError_t launch_narrow(const BlockGemmArgs& p, const TileArgs& g, cudaStream_t stream) {
   const int S = split_ranks<SB_ROWS, VEC>(g);
   return S > 1 ? launch_split<SB_ROWS, VEC>(p, g, S, stream) : launch_tiled<128, SB_ROWS, VEC>(p, g, stream);
+}
+
+// 256-wide tiles while every SM still gets one, else 128-wide ones. Where the last
+// round of 256-wide tiles would use at most half of the SMs, it is a launch of
+// its own of 128-wide tiles, which takes half as long or (split) less, from
+// kCutBlocks K blocks on: 5120 x 4096 x 8192 with a scale a row (4.3 rounds) 309 ->
+// 292 us, 5000 x 1024 x 4096 (1.1 rounds) 47 -> 42; 2048 x 2816 x 2048 28.6 -> 29.6.
+template <bool SB_ROWS, bool VEC>
+cudaError_t launch_large(const BlockGemmArgs& p, TileArgs g, cudaStream_t stream) {
+  const int sms = device_sm_count();
+  g.tiles_m = (g.M + kBM - 1) / kBM;
+  g.tiles_n = (g.N + 255) / 256;
+  const int tiles = g.tiles_m * g.tiles_n, last = tiles % sms;
+  g.tail = -1;
+  if (tiles < sms) {
+    g.tiles_n = (g.N + 127) / 128;
+    g.tiles = g.tiles_m * g.tiles_n;
+    return launch_narrow<SB_ROWS, VEC>(p, g, stream);
+  }
+  const bool cut = last > 0 && 2 * last <= sms && g.KB >= kCutBlocks;
+  g.tiles = cut ? tiles - last : tiles;
+  const cudaError_t e = launch_tiled<256, SB_ROWS, VEC>(p, g, stream);
+  if (e != cudaSuccess || !cut) return e;
+  g.tail = g.tiles, g.tiles = 2 * last;
+  return launch_narrow<SB_ROWS, VEC>(p, g, stream);
 }
 
 }  // namespace
