@@ -969,8 +969,11 @@ template <int BR>
 int few_ranks(int64_t N, int64_t KB) {
   static std::atomic<int> cache[64][kMaxRanks + 1];
   const int64_t tiles = (N + kBM - 1) / kBM;
+  // the occupancy query counts one CTA an SM for a kernel that allocates tensor
+  // memory; kCtas of them do run together
   auto fit = [&](int S) {
-    return max_clusters(reinterpret_cast<const void*>(block_gemm_few_kernel<BR>), kFewThreads,
+    return FewPlan<BR>::kCtas *
+           max_clusters(reinterpret_cast<const void*>(block_gemm_few_kernel<BR>), kFewThreads,
                         FewPlan<BR>::kSmemBytes, S, cache);
   };
   int S = kMaxRanks;
