@@ -430,3 +430,23 @@ def test_linear_refusals():
         tb.fp8_linear(x, w[:60])
     with pytest.raises(ValueError, match="float32"):
         tb.fp8_linear(x, w.half())
+
+
+# Enough 256 x 256 tiles for pairs of CTAs: one round and a rest, the rest cut into
+# 128 x 128 tiles (from 32 K blocks on), a last row tile with one CTA's rows only, a
+# last column tile with half of its columns, odd columns and a short last K block.
+PAIRS = [(2300, 2100, 300), (2300, 2304, 4200), (4737, 1025, 520), (2560, 2048, 128), (19000, 250, 1000)]
+
+
+@pytest.mark.parametrize("kind", ["blocks", "rows"])
+@pytest.mark.parametrize("M,N,K", PAIRS)
+def test_product_of_many_tiles(M, N, K, kind):
+    a, sa, b, sb = _operands(M, N, K, kind, seed=M + N + K)
+    _check(tb.fp8_block_gemm(a, sa, b, sb), a, sa, b, sb)
+    base = torch.randn(M, N, generator=torch.Generator().manual_seed(K)).cuda()
+    d = base.clone()
+    tb.fp8_block_gemm(a, sa, b, sb, out=d, accumulate=True)
+    _check(d, a, sa, b, sb, base)
+    again = base.clone()
+    tb.fp8_block_gemm(a, sa, b, sb, out=again, accumulate=True)
+    assert torch.equal(d, again)

@@ -37,23 +37,24 @@ __device__ __forceinline__ bool wait_or_abort(uint32_t bar, uint32_t parity,
   return false;
 }
 
-// Clusters of S CTAs along z that run at once on the current device, remembered.
-int max_clusters(const void* kernel, int threads, size_t smem, int S,
+// Clusters of S CTAs (along z; pairs along x) that run at once on the current device, remembered.
+int max_clusters(const void* kernel, int threads, size_t smem, dim3 cluster,
                  std::atomic<int> (&cache)[64][kMaxRanks + 1]) {
   int dev = 0;
+  const unsigned S = cluster.x * cluster.z;
   if (cudaGetDevice(&dev) != cudaSuccess) return 0;
   if (dev < 64 && cache[dev][S].load(std::memory_order_relaxed) > 0) return cache[dev][S].load();
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
     return 0;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(1, 1, (unsigned)S);
+  cfg.gridDim = cluster;
   cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = smem;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 1;
+  attr[0].val.clusterDim.x = cluster.x;
   attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = (unsigned)S;
+  attr[0].val.clusterDim.z = cluster.z;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   int n = 0;
@@ -62,9 +63,9 @@ int max_clusters(const void* kernel, int threads, size_t smem, int S,
   return n;
 }
 
-// Launch with clusters along z (grid.z CTAs each) and programmatic stream serialization.
+// Launch with clusters of `pair` CTAs along x, grid.z along z, and programmatic stream serialization.
 template <class K, class... A>
-cudaError_t launch_cluster(K kernel, dim3 grid, int threads, size_t smem, cudaStream_t stream,
+cudaError_t launch_cluster(K kernel, dim3 grid, unsigned pair, int threads, size_t smem, cudaStream_t stream,
                            const A&... args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
@@ -75,7 +76,7 @@ cudaError_t launch_cluster(K kernel, dim3 grid, int threads, size_t smem, cudaSt
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = 1;
+  attr[1].val.clusterDim.x = pair;
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = grid.z;
   cfg.attrs = attr;
@@ -90,8 +91,8 @@ cudaError_t launch_cluster(K kernel, dim3 grid, int threads, size_t smem, cudaSt
 //    block into a ring of stages (128-byte swizzled rows; rows and columns
 //    past the matrices are zero-filled, so M, N and K may be any).
 //  * warp 9, one thread: four MMAs of 128 x BN x 32 a K block into one of two
-//    accumulator buffers in tensor memory; a commit frees the stage, a second
-//    hands the buffer to the epilogue.
+//    accumulator buffers in tensor memory; a commit hands the buffer to the
+//    epilogue, a second frees the stage.
 //  * warps 0-7: the outer sum. Warp group g = warp / 4 keeps columns
 //    g BN/2 .. of the tile for its 128 rows, a row a thread, in BN / 2 fp32
 //    registers, and adds scale * buffer to them while the MMAs of the next K
@@ -101,6 +102,20 @@ cudaError_t launch_cluster(K kernel, dim3 grid, int threads, size_t smem, cudaSt
 //    on them (one wait in kScaleBlocks blocks).
 // Tiles are walked in bands of kBand rows of tiles, so that the CTAs of a
 // wave share their operands in L2.
+//
+// Pairs (cta_group::2): two CTAs of a cluster make a tile of 256 x 256, 128 rows
+// each. Each loads its rows of A and half of the rows of B; rank 0's MMAs (256 x
+// 256 x 32) read both, so a K block brings 32 KB instead of 48 KB into an SM's
+// shared memory and the ring holds six. Rank 0 waits for the loads and the
+// buffers of both, its commits go to both, and every CTA sums its own 128 rows.
+//
+// Bound: the tensor cores' 512 cycles a K block of 256 columns, the sums' about
+// 700 and the hand-overs between them (a buffer is free once its last piece is in
+// registers, then a signal, the next MMAs and a signal back) make 870 cycles;
+// over seconds it is power, at 1.5 GHz. Tried without gain: accumulators handed
+// over in halves (MMAs of 128 columns read A twice), 16 summing warps, spinning
+// waits, deeper scale rings. A release at cluster scope on the arrival that frees
+// a buffer cost 1000 cycles; it orders tensor memory only, which the fences do.
 constexpr int kThreads = 384, kEpiWarps = 8, kBand = 16;
 // registers a thread: 256 x 216 + 128 x 64 = 63488 of the 384 x 168 = 64512 at launch
 constexpr int kEpiRegs = 216, kIssueRegs = 64;
@@ -109,11 +124,11 @@ constexpr int kSplitBlocks = 16, kCutBlocks = 32;  // see split_ranks, launch_la
 
 constexpr int kStageRow = 9;  // see store_rows
 
-template <int BN, bool SB_ROWS, bool VEC>
+template <int BN, bool SB_ROWS, bool VEC, bool PAIR = false>
 struct TilePlan {
-  static constexpr int kNB = BN / 128;
+  static constexpr int kNB = PAIR ? 1 : BN / 128;  // boxes of B that a CTA loads
   static constexpr uint32_t kStageBytes = (1 + kNB) * kBoxBytes;
-  static constexpr int kStages = BN == 256 ? 4 : 6;
+  static constexpr int kStages = kNB == 2 ? 4 : 6;
   static constexpr size_t kSmemBytes = kStages * kStageBytes + 1024;
   static constexpr uint32_t kTmemCols = 2 * BN;
   static constexpr int kCols = BN / 2;  // columns of a warp group
@@ -140,15 +155,17 @@ struct TileArgs {
   int64_t ldd;
   int M, N, KB, tiles_m, tiles_n;
   int tiles;  // to walk
-  int tail;   // 128-wide form: >= 0: the halves of the 256-wide tiles from this one on
+  int band;   // rows of tiles that are walked together
+  int tail;   // 128-wide form: >= 0: the parts of the larger tiles from this one on,
+  int parts;  // 2 (columns) or 4 (columns and rows) each
   bool d_f32, accumulate;
 };
 
 // Tile t of the banded walk.
-__device__ __forceinline__ void tile_at(int t, int tiles_m, int tiles_n, int* tm, int* tn) {
-  const int band = t / (kBand * tiles_n), first = band * kBand;
-  const int rows = tiles_m - first < kBand ? tiles_m - first : kBand;
-  const int in = t - band * kBand * tiles_n;
+__device__ __forceinline__ void tile_at(const TileArgs& g, int t, int* tm, int* tn) {
+  const int band = t / (g.band * g.tiles_n), first = band * g.band;
+  const int rows = g.tiles_m - first < g.band ? g.tiles_m - first : g.band;
+  const int in = t - band * g.band * g.tiles_n;
   *tm = first + in % rows;
   *tn = in / rows;
 }
@@ -156,10 +173,11 @@ __device__ __forceinline__ void tile_at(int t, int tiles_m, int tiles_n, int* tm
 template <int BN>
 __device__ __forceinline__ void tile_of(const TileArgs& g, int t, int* tm, int* tn) {
   if (BN == 128 && g.tail >= 0) {
-    tile_at(g.tail + t / 2, g.tiles_m, g.tiles_n, tm, tn);
+    tile_at(g, g.tail + t / g.parts, tm, tn);
     *tn = 2 * *tn + (t & 1);
+    if (g.parts == 4) *tm = 2 * *tm + ((t >> 1) & 1);
   } else {
-    tile_at(t, g.tiles_m, g.tiles_n, tm, tn);
+    tile_at(g, t, tm, tn);
   }
 }
 
@@ -264,11 +282,12 @@ __device__ __forceinline__ void store_four(const TileArgs& g, int row, int col, 
   }
 }
 
-template <int BN, bool SB_ROWS, bool VEC, bool SPLIT>
+template <int BN, bool SB_ROWS, bool VEC, bool SPLIT, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
     block_gemm_kernel(const __grid_constant__ CUtensorMap map_a,
                       const __grid_constant__ CUtensorMap map_b, const TileArgs g) {
-  using P = TilePlan<BN, SB_ROWS, VEC>;
+  using P = TilePlan<BN, SB_ROWS, VEC, PAIR>;
+  static_assert(!PAIR || (BN == 256 && !SPLIT), "pairs make 256 x 256 tiles");
   constexpr int NC = P::kCols;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full_bar[P::kStages];
@@ -287,9 +306,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
-  const int tiles = g.tiles;
+  // tiles begin, begin + step, ... are this CTA's, or its pair's
+  const int tiles = g.tiles, begin = PAIR ? blockIdx.x / 2 : blockIdx.x, step = PAIR ? gridDim.x / 2 : gridDim.x;
   // K blocks of this CTA: all, or the rank's of its cluster
-  const int S = SPLIT ? (int)gridDim.z : 1, rank = SPLIT ? (int)tc::cluster_ctarank() : 0;
+  const int S = SPLIT ? (int)gridDim.z : 1, rank = SPLIT || PAIR ? (int)tc::cluster_ctarank() : 0;
   const int kb0 = SPLIT ? (int)((int64_t)g.KB * rank / S) : 0;
   const int nkb = SPLIT ? (int)((int64_t)g.KB * (rank + 1) / S) - kb0 : g.KB;
   // and the tile's rows that it adds up
@@ -305,7 +325,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(smem_addr(&acc_full[b]), 1);
-      mbar_init(smem_addr(&acc_empty[b]), kEpiWarps);
+      mbar_init(smem_addr(&acc_empty[b]), (PAIR ? 2 : 1) * kEpiWarps);
     }
     for (int s = 0; s < P::kScaleSlots; ++s) {
       mbar_init(smem_addr(&scale_full[s]), 32);
@@ -317,9 +337,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init_fence();
     if (SPLIT) mbar_arrive_expect_tx(smem_addr(&recv_bar), (uint32_t)((S - 1) * own_n) * kPartRowBytes);
   }
-  if (warp == kEpiWarps) tc::tmem_alloc(smem_addr(&tmem_base_slot), P::kTmemCols);
+  if (warp == kEpiWarps) {
+    if (PAIR) tc::tmem_alloc_pair(smem_addr(&tmem_base_slot), P::kTmemCols);
+    else tc::tmem_alloc(smem_addr(&tmem_base_slot), P::kTmemCols);
+  }
   tc::fence_before();
   __syncthreads();
+  if (PAIR) tc::cluster_sync();  // both CTAs' barriers and tensor memory are ready
   tc::fence_after();
   const uint32_t tmem = tmem_base_slot;
   griddep_wait();
@@ -332,7 +356,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool leader = tc::elect_one();
     uint32_t s = 0, parity = 1;  // a fresh barrier passes a wait for the phase before its first
     bool ok = true;
-    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+    for (int t = begin; t < tiles && ok; t += step) {
       int tm, tn;
       tile_of<BN>(g, t, &tm, &tn);
       for (int kb = 0; kb < nkb; ++kb) {
@@ -343,24 +367,37 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (leader) {
           const uint32_t st = base + s * P::kStageBytes, bar = smem_addr(&full_bar[s]);
-          mbar_arrive_expect_tx(bar, P::kStageBytes);
-          tc::tma_load_2d(st, &map_a, (kb0 + kb) * kBK, tm * kBM, bar);
+          if constexpr (PAIR) {
+            // both CTAs' loads are counted on rank 0's barrier
+            if (rank == 0) mbar_arrive_expect_tx(bar, 2 * P::kStageBytes);
+            const uint32_t to = tc::mapa(bar, 0);
+            tc::tma_load_2d_pair(st, &map_a, kb * kBK, (2 * tm + rank) * kBM, to);
+            tc::tma_load_2d_pair(st + kBoxBytes, &map_b, kb * kBK, tn * BN + 128 * rank, to);
+          } else {
+            mbar_arrive_expect_tx(bar, P::kStageBytes);
+            tc::tma_load_2d(st, &map_a, (kb0 + kb) * kBK, tm * kBM, bar);
 #pragma unroll
-          for (int h = 0; h < P::kNB; ++h)
-            tc::tma_load_2d(st + (1 + h) * kBoxBytes, &map_b, (kb0 + kb) * kBK, tn * BN + 128 * h, bar);
+            for (int h = 0; h < P::kNB; ++h)
+              tc::tma_load_2d(st + (1 + h) * kBoxBytes, &map_b, (kb0 + kb) * kBK, tn * BN + 128 * h, bar);
+          }
           ++issued;
         }
         if (++s == P::kStages) s = 0, parity ^= 1;
       }
     }
+    if (PAIR)  // rank 0's commits arrive here: all before this CTA's memory goes
+      for (int i = 0; i < P::kStages && ok; ++i) {
+        ok = __all_sync(0xffffffffu, wait_or_abort(smem_addr(&empty_bar[s]), parity, abortp));
+        if (++s == P::kStages) s = 0, parity ^= 1;
+      }
   } else if (warp == kEpiWarps + 1) {
     // ---- MMAs
     const bool leader = tc::elect_one();
-    constexpr uint32_t idesc = tc::f8_idesc(kBM, BN);
+    constexpr uint32_t idesc = tc::f8_idesc(PAIR ? 2 * kBM : kBM, BN);
     const uint32_t lo0 = tc::sw128_lo(base), hi = tc::sw128_hi();
     uint32_t s = 0, parity = 0, buf = 0, buf_parity = 1;
-    bool ok = true;
-    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+    bool ok = !PAIR || rank == 0;  // rank 0 issues for both
+    for (int t = begin; t < tiles && ok; t += step) {
       for (int kb = 0; kb < nkb; ++kb) {
         ok = wait_or_abort(smem_addr(&full_bar[s]), parity, abortp) &&
              wait_or_abort(smem_addr(&acc_empty[buf]), buf_parity, abortp);
@@ -373,10 +410,19 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t lo = lo0 + s * (P::kStageBytes >> 4);
 #pragma unroll
           for (int kk = 0; kk < kBK / 32; ++kk)
-            tc::mma_f8(tmem + buf * BN, lo + 2 * kk, lo + (kBoxBytes >> 4) + 2 * kk, hi, idesc,
-                       kk != 0);
-          tc::commit(smem_addr(&empty_bar[s]));
-          tc::commit(smem_addr(&acc_full[buf]));
+            if (PAIR)
+              tc::mma_f8_pair(tmem + buf * BN, lo + 2 * kk, lo + (kBoxBytes >> 4) + 2 * kk, hi, idesc,
+                              kk != 0);
+            else
+              tc::mma_f8(tmem + buf * BN, lo + 2 * kk, lo + (kBoxBytes >> 4) + 2 * kk, hi, idesc,
+                         kk != 0);
+          if (PAIR) {
+            tc::commit_pair(smem_addr(&acc_full[buf]));
+            tc::commit_pair(smem_addr(&empty_bar[s]));
+          } else {
+            tc::commit(smem_addr(&acc_full[buf]));
+            tc::commit(smem_addr(&empty_bar[s]));
+          }
           ++committed;
         }
         __syncwarp();
@@ -390,19 +436,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t s = 0, parity = 1;
     bool ok = true;
     constexpr int kNS = SB_ROWS ? BN / 32 : 1;
-    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+    for (int t = begin; t < tiles && ok; t += step) {
       int tm, tn;
       tile_of<BN>(g, t, &tm, &tn);
       const float *pa[4], *pb[kNS];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int row = tm * kBM + lane + 32 * i;
+        const int row = (PAIR ? 2 * tm + rank : tm) * kBM + lane + 32 * i;
         pa[i] = row < g.M ? g.sa + (int64_t)row * g.sa_row + kb0 * g.sa_kb : nullptr;
       }
 #pragma unroll
       for (int i = 0; i < kNS; ++i) {
         const int col = tn * BN + (SB_ROWS ? lane + 32 * i : 128 * lane);
-        const bool some = col < g.N && (SB_ROWS || lane < P::kNB);
+        const bool some = col < g.N && (SB_ROWS || lane < BN / 128);
         pb[i] = some ? g.sb + (int64_t)(SB_ROWS ? col : col / 128) * g.sb_row + kb0 * g.sb_kb : nullptr;
       }
       for (int kb = 0; kb < nkb; ++kb) {
@@ -453,16 +499,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto begin_block = [&](int kb) {
       const int j = kb % kScaleBlocks;
       if (j == 0) wait_or_abort(smem_addr(&scale_full[slot]), slot_parity, abortp);
+      sc = scales[slot][j][r];
+      sb = &scales[slot][j][128 + (SB_ROWS ? wg * NC : wg * NC / 128)];
+      if (!SB_ROWS) sc *= *sb;
       wait_or_abort(smem_addr(&acc_full[buf]), buf_parity, abortp);
       __syncwarp();
       tc::fence_after();
       tc::tmem_ld_async(tm_lane + buf * BN, lo);
-      sc = scales[slot][j][r];
-      sb = &scales[slot][j][128 + (SB_ROWS ? wg * NC : wg * NC / 128)];
-      if (!SB_ROWS) sc *= *sb;
     };
-    if ((int)blockIdx.x < tiles) begin_block(0);
-    for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
+    if (begin < tiles) begin_block(0);
+    for (int t = begin; t < tiles; t += step) {
       float2 acc[NC / 2];
 #pragma unroll
       for (int i = 0; i < NC / 2; ++i) acc[i] = make_float2(0.f, 0.f);
@@ -507,11 +553,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           } else {  // all of the buffer is in registers
             tc::fence_before();
             __syncwarp();
-            tc::arrive_if(first, smem_addr(&acc_empty[buf]));
+            if (PAIR) tc::arrive_cluster_if(first, tc::mapa(smem_addr(&acc_empty[buf]), 0));
+            else tc::arrive_if(first, smem_addr(&acc_empty[buf]));
             buf ^= 1;
             buf_parity ^= buf == 0;
             if (slot_done && ++slot == P::kScaleSlots) slot = 0, slot_parity ^= 1;
-            if (!last || t + (int)gridDim.x < tiles) begin_block(last ? 0 : kb + 1);
+            if (!last || t + step < tiles) begin_block(last ? 0 : kb + 1);
           }
           add(c + CH, hi);
         }
@@ -524,7 +571,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tile_of<BN>(g, t, &tm_i, &tn_i);
       if constexpr (!SPLIT) {
         if (*abortp == 0u)
-          store_rows<NC, VEC>(g, acc, tm_i * kBM + (warp & 3) * 32, tn_i * BN + wg * NC, lane,
+          store_rows<NC, VEC>(g, acc, (PAIR ? 2 * tm_i + rank : tm_i) * kBM + (warp & 3) * 32, tn_i * BN + wg * NC, lane,
                               stage[VEC ? 0 : warp]);
       } else {
         // the last accumulator was complete, so this CTA's ring is idle, and so
@@ -588,25 +635,32 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (threadIdx.x == 0) {
       atomicCAS(&g_block_gemm_device_error, kDevErrNone, kDevErrBulkWaitTimeout);
       const uint32_t n = issued, m = committed;
-      for (uint32_t k = n > P::kStages ? n - P::kStages : 0; k < n; ++k)
+      for (uint32_t k = n > P::kStages ? n - P::kStages : 0; k < n && (!PAIR || rank == 0); ++k)
         mbar_wait_bounded(smem_addr(&full_bar[k % P::kStages]), (k / P::kStages) & 1u,
                           kDrainLimitCycles);
       if (m > 0)
         mbar_wait_bounded(smem_addr(&acc_full[(m - 1) & 1u]), ((m - 1) >> 1) & 1u,
                           kDrainLimitCycles);
-      // and what other ranks may have sent here: nothing counts it now
-      for (const long long t0 = clock64(); SPLIT && clock64() - t0 < kDrainLimitCycles / 100;) {
+      // and what other ranks may have sent here, or this one has on its way: nothing counts it now
+      for (const long long t0 = clock64(); (SPLIT || PAIR) && clock64() - t0 < kDrainLimitCycles / 100;) {
       }
     }
     __syncthreads();
   }
-  if (warp == kEpiWarps) tc::tmem_dealloc(tmem, P::kTmemCols);
+  if (PAIR) {
+    tc::cluster_arrive();
+    tc::cluster_wait();
+  }
+  if (warp == kEpiWarps) {
+    if (PAIR) tc::tmem_dealloc_pair(tmem, P::kTmemCols);
+    else tc::tmem_dealloc(tmem, P::kTmemCols);
+  }
 }
 
 template <int BN, bool SB_ROWS, bool VEC>
 cudaError_t launch_tiled(const BlockGemmArgs& p, TileArgs g, cudaStream_t stream) {
   using P = TilePlan<BN, SB_ROWS, VEC>;
-  auto kernel = block_gemm_kernel<BN, SB_ROWS, VEC, false>;
+  auto kernel = block_gemm_kernel<BN, SB_ROWS, VEC, false, false>;
   const cudaError_t e =
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)P::kSmemBytes);
   if (e != cudaSuccess) return e;
@@ -619,12 +673,35 @@ cudaError_t launch_tiled(const BlockGemmArgs& p, TileArgs g, cudaStream_t stream
                     map_a, map_b, g);
 }
 
+// 256 x 256 tiles by pairs of CTAs; how many pairs run at once.
+template <bool SB_ROWS, bool VEC>
+int pair_clusters() {
+  static std::atomic<int> cache[64][kMaxRanks + 1];
+  return max_clusters(reinterpret_cast<const void*>(block_gemm_kernel<256, SB_ROWS, VEC, false, true>),
+                      kThreads, TilePlan<256, SB_ROWS, VEC, true>::kSmemBytes, dim3(2, 1, 1), cache);
+}
+
+template <bool SB_ROWS, bool VEC>
+cudaError_t launch_pairs(const BlockGemmArgs& p, TileArgs g, int pairs, cudaStream_t stream) {
+  using P = TilePlan<256, SB_ROWS, VEC, true>;
+  auto kernel = block_gemm_kernel<256, SB_ROWS, VEC, false, true>;
+  const cudaError_t e =
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)P::kSmemBytes);
+  if (e != cudaSuccess) return e;
+  CUtensorMap map_a, map_b;
+  if (!tc::encode_e4m3_operand(&map_a, p.a, p.M, p.K, p.lda, kBM) ||
+      !tc::encode_e4m3_operand(&map_b, p.b, p.N, p.K, p.ldb, kBM))
+    return cudaErrorInvalidValue;
+  return launch_cluster(kernel, dim3(2u * (unsigned)(g.tiles < pairs ? g.tiles : pairs)), 2, kThreads,
+                        P::kSmemBytes, stream, map_a, map_b, g);
+}
+
 // The split form: tiles of 128 x 128 that leave SMs idle, K split over a cluster.
 template <bool SB_ROWS, bool VEC>
 int split_clusters(int S) {
   static std::atomic<int> cache[64][kMaxRanks + 1];
-  return max_clusters(reinterpret_cast<const void*>(block_gemm_kernel<128, SB_ROWS, VEC, true>), kThreads,
-                      TilePlan<128, SB_ROWS, true>::kSmemBytes, S, cache);
+  return max_clusters(reinterpret_cast<const void*>(block_gemm_kernel<128, SB_ROWS, VEC, true, false>), kThreads,
+                      TilePlan<128, SB_ROWS, true>::kSmemBytes, dim3(1, 1, (unsigned)S), cache);
 }
 
 // Ranks: the most with which all tiles still run at once; 1, not split, where that
@@ -643,7 +720,7 @@ int split_ranks(const TileArgs& g) {
 template <bool SB_ROWS, bool VEC>
 cudaError_t launch_split(const BlockGemmArgs& p, TileArgs g, int S, cudaStream_t stream) {
   using P = TilePlan<128, SB_ROWS, true>;
-  auto kernel = block_gemm_kernel<128, SB_ROWS, VEC, true>;
+  auto kernel = block_gemm_kernel<128, SB_ROWS, VEC, true, false>;
   const cudaError_t e =
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)P::kSmemBytes);
   if (e != cudaSuccess) return e;
@@ -651,7 +728,7 @@ cudaError_t launch_split(const BlockGemmArgs& p, TileArgs g, int S, cudaStream_t
   if (!tc::encode_e4m3_operand(&map_a, p.a, p.M, p.K, p.lda, kBM) ||
       !tc::encode_e4m3_operand(&map_b, p.b, p.N, p.K, p.ldb, kBM))
     return cudaErrorInvalidValue;
-  return launch_cluster(kernel, dim3((unsigned)g.tiles, 1, (unsigned)S), kThreads,
+  return launch_cluster(kernel, dim3((unsigned)g.tiles, 1, (unsigned)S), 1, kThreads,
                         P::kSmemBytes, stream, map_a, map_b, g);
 }
 
@@ -974,7 +1051,7 @@ int few_ranks(int64_t N, int64_t KB) {
   auto fit = [&](int S) {
     return FewPlan<BR>::kCtas *
            max_clusters(reinterpret_cast<const void*>(block_gemm_few_kernel<BR>), kFewThreads,
-                        FewPlan<BR>::kSmemBytes, S, cache);
+                        FewPlan<BR>::kSmemBytes, dim3(1, 1, (unsigned)S), cache);
   };
   int S = kMaxRanks;
   while (S > 1 && (S * kFewStep > KB || fit(S) < tiles)) --S;
@@ -992,7 +1069,7 @@ cudaError_t launch_few(const BlockGemmArgs& p, const TileArgs& g, int S, cudaStr
       !tc::encode_e4m3_operand(&map_b, p.b, p.N, p.K, p.ldb, kBM))
     return cudaErrorInvalidValue;
   return launch_cluster(block_gemm_few_kernel<BR>,
-                        dim3((unsigned)((p.N + kBM - 1) / kBM), 1, (unsigned)S), kFewThreads,
+                        dim3((unsigned)((p.N + kBM - 1) / kBM), 1, (unsigned)S), 1, kFewThreads,
                         FewPlan<BR>::kSmemBytes, stream, map_a, map_b, g);
 }
 
@@ -1003,28 +1080,47 @@ cudaError_t launch_narrow(const BlockGemmArgs& p, const TileArgs& g, cudaStream_
   return S > 1 ? launch_split<SB_ROWS, VEC>(p, g, S, stream) : launch_tiled<128, SB_ROWS, VEC>(p, g, stream);
 }
 
-// 256-wide tiles while every SM still gets one, else 128-wide ones. Where the last
-// round of 256-wide tiles would use at most half of the SMs, it is a launch of
-// its own of 128-wide tiles, which takes half as long or (split) less, from
+// Tiles of rows x 256 columns over `units` CTAs or pairs: `last` of them in a round
+// that is not full. Where those are at most half a round, they become a launch of
+// their own of 128 x 128 tiles, which takes half as long or (split) less, from
 // kCutBlocks K blocks on: 5120 x 4096 x 8192 with a scale a row (4.3 rounds) 309 ->
 // 292 us, 5000 x 1024 x 4096 (1.1 rounds) 47 -> 42; 2048 x 2816 x 2048 28.6 -> 29.6.
+struct Rounds {
+  int tiles_m, tiles, last, halves;  // halves: the time, in half rounds
+  bool cut;
+  Rounds(const TileArgs& g, int rows, int units)
+      : tiles_m((g.M + rows - 1) / rows), tiles(tiles_m * ((g.N + 255) / 256)), last(tiles % units),
+        cut(last > 0 && 2 * last <= units && g.KB >= kCutBlocks) {
+    halves = 2 * (tiles / units) + (last == 0 ? 0 : cut ? 1 : 2);
+  }
+};
+
+// 256-wide tiles while every SM gets one, else 128-wide ones. Pairs unless their
+// taller tiles need more rounds (a round takes either the same). A pair moves two
+// thirds of the bytes through shared memory; the SM's clock under the power cap
+// gains more by it than a short run shows, us of single CTAs against pairs over
+// seconds: 16384 x 7168 x 7168 889 -> 849, 4096 x 4096 x 4096 86 -> 80, 5120 x 4096 x
+// 8208 with a scale a row 316 -> 297; in short runs 5120 x 5120 x 8192 300 -> 292.
 template <bool SB_ROWS, bool VEC>
 cudaError_t launch_large(const BlockGemmArgs& p, TileArgs g, cudaStream_t stream) {
-  const int sms = device_sm_count();
-  g.tiles_m = (g.M + kBM - 1) / kBM;
-  g.tiles_n = (g.N + 255) / 256;
-  const int tiles = g.tiles_m * g.tiles_n, last = tiles % sms;
-  g.tail = -1;
-  if (tiles < sms) {
-    g.tiles_n = (g.N + 127) / 128;
+  const int sms = device_sm_count(), pairs = pair_clusters<SB_ROWS, VEC>();
+  const Rounds one(g, kBM, sms), two(g, 2 * kBM, pairs > 0 ? pairs : 1);
+  g.band = kBand, g.tail = -1;
+  if (one.tiles < sms) {
+    g.tiles_m = one.tiles_m, g.tiles_n = (g.N + 127) / 128;
     g.tiles = g.tiles_m * g.tiles_n;
     return launch_narrow<SB_ROWS, VEC>(p, g, stream);
   }
-  const bool cut = last > 0 && 2 * last <= sms && g.KB >= kCutBlocks;
-  g.tiles = cut ? tiles - last : tiles;
-  const cudaError_t e = launch_tiled<256, SB_ROWS, VEC>(p, g, stream);
-  if (e != cudaSuccess || !cut) return e;
-  g.tail = g.tiles, g.tiles = 2 * last;
+  const bool pair = pairs > 0 && two.halves <= one.halves;
+  const Rounds& r = pair ? two : one;
+  g.tiles_m = r.tiles_m, g.tiles_n = (g.N + 255) / 256;
+  g.tiles = r.cut ? r.tiles - r.last : r.tiles;
+  if (pair) g.band = kBand / 2;
+  const cudaError_t e = pair ? launch_pairs<SB_ROWS, VEC>(p, g, pairs, stream)
+                             : launch_tiled<256, SB_ROWS, VEC>(p, g, stream);
+  if (e != cudaSuccess || !r.cut) return e;
+  g.parts = pair ? 4 : 2;
+  g.tail = g.tiles, g.tiles = g.parts * r.last;
   return launch_narrow<SB_ROWS, VEC>(p, g, stream);
 }
 
