@@ -735,8 +735,9 @@ cudaError_t launch_split(const BlockGemmArgs& p, TileArgs g, int S, cudaStream_t
 // ------------------------------------------------------------------ few rows
 //
 // At most 64 rows of A: bound by reading the weight once. The weight is the
-// 128-row side of the MMA and the batch its N side (BR = 16, 32 or 64 columns, the smallest that holds the batch; rows past M are zero-filled), so
-// a K block costs 16 KB of weight and a batch box of BR rows. N / 128 tiles do
+// 128-row side of the MMA and the batch its N side (BR = 16, 32 or 64 columns,
+// the smallest that holds the batch; rows past M are zero-filled), so a K block
+// costs 16 KB of weight and a batch box of BR rows. N / 128 tiles do
 // not fill the GPU, so K is split over a cluster of S CTAs, with two CTAs an SM
 // (one for BR = 64): every SM then has its share of the weight on the way at
 // once. Two K blocks share a ring stage and its barriers: the hand-over
