@@ -1,0 +1,65 @@
+"""fp8_linear takes any layout of its tensors: each test compares a call whose input or
+incoming gradient is laid out otherwise with the same call on a dense copy, bit for bit."""
+
+import pytest
+import torch
+
+import thingy_b200 as tb
+
+pytestmark = pytest.mark.gpu
+
+
+def _matrix(M, H, seed, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (scale * torch.randn(M, H, generator=g)).to(torch.bfloat16).cuda()
+
+
+def _step(x, w, dy=None):
+    """y, dx and dw of one step; dx in x's own shape."""
+    x, w = x.detach().requires_grad_(), w.detach().requires_grad_()
+    y = tb.fp8_linear(x, w)
+    return (y.detach(), *torch.autograd.grad(y, (x, w), torch.ones_like(y) if dy is None else dy))
+
+
+def _same(got, want):
+    for a, b in zip(got, want):
+        assert a.shape == b.shape and torch.equal(a, b)
+
+
+def _strided(kind):
+    """A row of 256 elements (or a matrix of such rows) whose last dimension is not dense, in a
+    storage large enough that a dense reading of it stays inside."""
+    wide = _matrix(600, 600, seed=11)
+    return {
+        "column": lambda: wide[:256, 8],  # 1-D, stride 600
+        "column as a row": lambda: wide.t()[8:9, :256],
+        "stepped row": lambda: wide[:1, 0:512:2],
+        "stepped row in three dimensions": lambda: wide[None, 8:9, 0:512:2],
+        "rows of a transpose": lambda: wide.t()[8:40, :256],
+        "stepped rows": lambda: wide[:40, 0:512:2],
+        "rows off the 16-byte boundaries": lambda: wide[:40, 3:259],
+    }[kind]()
+
+
+@pytest.mark.parametrize("kind", ["column", "column as a row", "stepped row", "stepped row in three dimensions",
+                                  "rows of a transpose", "stepped rows"])
+def test_input_of_any_strides(kind):
+    x, w = _strided(kind), _matrix(136, 256, seed=2, scale=0.02)
+    assert x.stride(-1) != 1
+    _same(_step(x, w), _step(x.contiguous(), w))
+
+
+@pytest.mark.parametrize("shape", [(256,), (1, 256), (24, 256)])
+def test_expanded_input(shape):
+    """Broadcast inputs: nothing past their storage is read, and the gradient reaches them."""
+    x, w = _matrix(1, 1, seed=3), _matrix(136, 256, seed=2, scale=0.02)
+    wide = x.reshape(()).expand(shape)
+    _same(_step(wide, w), _step(wide.contiguous(), w))
+    row = _matrix(1, 256, seed=4)
+    _same(_step(row.expand(24, 256), w), _step(row.expand(24, 256).contiguous(), w))
+
+
+def test_weight_of_any_strides():
+    x, wide = _matrix(24, 256, seed=3), _matrix(512, 512, seed=2, scale=0.02)
+    for w in (wide.t()[:136, :256], wide[:136, 0:512:2], wide[:8, :256][:1].expand(8, 256)):
+        _same(_step(x, w), _step(x, w.contiguous()))

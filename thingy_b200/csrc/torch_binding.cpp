@@ -304,8 +304,11 @@ struct CastBuffer {
   Operand columns() const {
     return {base() + off_qt, ceil_to(R, 16), base() + off_st, block ? (R + 127) / 128 : 1, block ? 1 : C};
   }
-  void cast(const at::Tensor& x, bool transposed, void* stream) {
-    if (R > 1 && (x.stride(1) != 1 || x.stride(0) < C)) bad("x must be contiguous along its last dimension");
+  // A matrix whose rows are not dense, or overlap, is copied first; that of a
+  // single row too: the kernel reads C neighbouring elements.
+  void cast(const at::Tensor& any, bool transposed, void* stream) {
+    const bool dense = (C <= 1 || any.stride(1) == 1) && (R <= 1 || any.stride(0) >= C);
+    const at::Tensor x = dense ? any : any.contiguous();
     hold = at::empty({transposed ? bytes : off_qt}, x.options().dtype(at::kByte));
     check_status(cutie_cast_fp8_tiles(
         x.data_ptr(), R <= 1 ? ceil_to(C, 8) : x.stride(0), R, C,
