@@ -63,3 +63,31 @@ def test_weight_of_any_strides():
     x, wide = _matrix(24, 256, seed=3), _matrix(512, 512, seed=2, scale=0.02)
     for w in (wide.t()[:136, :256], wide[:136, 0:512:2], wide[:8, :256][:1].expand(8, 256)):
         _same(_step(x, w), _step(x, w.contiguous()))
+
+
+def test_input_and_weight_off_the_16_byte_boundaries():
+    x, w = _strided("rows off the 16-byte boundaries"), _matrix(136, 600, seed=2, scale=0.02)[:, 5:261]
+    _same(_step(x, w), _step(x.contiguous(), w.contiguous()))
+    flat = _matrix(1, 3 + 24 * 256, seed=5).view(-1)
+    x = flat[3:].view(24, 256)
+    assert x.is_contiguous() and x.data_ptr() % 16 != 0
+    _same(_step(x, w), _step(x.clone(), w.contiguous()))
+
+
+@pytest.mark.parametrize("rows", [1, 24])
+def test_gradient_off_the_16_byte_boundaries(rows):
+    """The gradient that autograd hands back for one part of a concatenation is a view into the whole."""
+    x, w = _matrix(rows, 256, seed=3).requires_grad_(), _matrix(136, 256, seed=2, scale=0.02).requires_grad_()
+    weight = _matrix(1, 3 + rows * 136, seed=6).view(-1)
+    y = tb.fp8_linear(x, w)
+    joined = torch.cat([torch.zeros(3, dtype=torch.bfloat16, device="cuda"), y.view(-1)])
+    got = torch.autograd.grad(joined, (x, w), weight)
+    _same(got, _step(x, w, weight[3:].clone().view(rows, 136))[1:])
+
+
+@pytest.mark.parametrize("rows", [1, 24])
+def test_gradient_of_any_strides(rows):
+    x, w = _matrix(rows, 256, seed=3), _matrix(136, 256, seed=2, scale=0.02)
+    wide = _matrix(600, 600, seed=7)
+    for dy in (wide.t()[:rows, :136], wide[:rows, 0:272:2], wide[:1, :1].expand(rows, 136), wide[:1, :136].expand(rows, 136)):
+        _same(_step(x, w, dy), _step(x, w, dy.contiguous()))

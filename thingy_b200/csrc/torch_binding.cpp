@@ -304,11 +304,14 @@ struct CastBuffer {
   Operand columns() const {
     return {base() + off_qt, ceil_to(R, 16), base() + off_st, block ? (R + 127) / 128 : 1, block ? 1 : C};
   }
-  // A matrix whose rows are not dense, or overlap, is copied first; that of a
-  // single row too: the kernel reads C neighbouring elements.
+  // A matrix whose rows are not dense, overlap or start off the 16-byte
+  // boundaries is copied first; that of a single row too: the kernel reads C
+  // neighbouring elements.
   void cast(const at::Tensor& any, bool transposed, void* stream) {
-    const bool dense = (C <= 1 || any.stride(1) == 1) && (R <= 1 || any.stride(0) >= C);
-    const at::Tensor x = dense ? any : any.contiguous();
+    const bool dense = (C <= 1 || any.stride(1) == 1) &&
+                       (R <= 1 || (any.stride(0) >= C && any.stride(0) % 8 == 0)) &&
+                       reinterpret_cast<uintptr_t>(any.data_ptr()) % 16 == 0;
+    const at::Tensor x = dense ? any : any.clone(at::MemoryFormat::Contiguous);
     hold = at::empty({transposed ? bytes : off_qt}, x.options().dtype(at::kByte));
     check_status(cutie_cast_fp8_tiles(
         x.data_ptr(), R <= 1 ? ceil_to(C, 8) : x.stride(0), R, C,
@@ -370,7 +373,7 @@ struct FP8Linear : public torch::autograd::Function<FP8Linear> {
     const auto saved = ctx->get_saved_variables();
     const auto sizes = ctx->saved_data["sizes"].toIntVector();
     const int64_t N = sizes[0], K = sizes[1];
-    const at::Tensor dy = grads[0].contiguous();
+    const at::Tensor& dy = grads[0];  // of any layout: a view into another gradient, an expanded sum's
     const int64_t M = dy.size(0);
     const at::Device dev = dy.device();
     const c10::cuda::CUDAGuard guard(dev);

@@ -19,7 +19,8 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_fp8=None) -> torch.
     """``x @ weight.T`` on e4m3 codes with fp32 sums, bf16 out, differentiable in x and weight.
 
     x: bf16 [..., K]; weight: bf16 or fp32 [N, K]; K and N multiples of 8.
-    Both may have any strides; a matrix whose rows are not dense is copied first.
+    Both, and y's gradient, may have any strides; a matrix whose rows are not
+    dense and on 16-byte boundaries is copied first.
     ``weight_fp8``: (q, s, qt, st) of ``per_block_cast_to_fp8(weight,
     transposed=True)`` where the caller casts the weight once for several
     calls (an optimizer step, inference: there (q, s, None, None) does);
