@@ -91,3 +91,13 @@ def test_gradient_of_any_strides(rows):
     wide = _matrix(600, 600, seed=7)
     for dy in (wide.t()[:rows, :136], wide[:rows, 0:272:2], wide[:1, :1].expand(rows, 136), wide[:1, :136].expand(rows, 136)):
         _same(_step(x, w, dy), _step(x, w, dy.contiguous()))
+
+
+@pytest.mark.parametrize("M,N,K", [(24, 0, 256), (24, 136, 0), (0, 136, 256), (0, 0, 256), (24, 0, 0)])
+def test_sizes_of_zero(M, N, K):
+    """A sum over nothing is zero, and nothing has a gradient of its own shape."""
+    x, w = torch.ones(M, K, dtype=torch.bfloat16, device="cuda"), torch.ones(N, K, dtype=torch.bfloat16, device="cuda")
+    y, dx, dw = _step(x, w)
+    assert y.shape == (M, N) and dx.shape == (M, K) and dw.shape == (N, K)
+    for t in (y, dx, dw):
+        assert bool((t == 0).all())

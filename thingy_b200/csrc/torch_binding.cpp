@@ -313,6 +313,7 @@ struct CastBuffer {
                        reinterpret_cast<uintptr_t>(any.data_ptr()) % 16 == 0;
     const at::Tensor x = dense ? any : any.clone(at::MemoryFormat::Contiguous);
     hold = at::empty({transposed ? bytes : off_qt}, x.options().dtype(at::kByte));
+    if (R == 0 || C == 0) return;  // no codes
     check_status(cutie_cast_fp8_tiles(
         x.data_ptr(), R <= 1 ? ceil_to(C, 8) : x.stride(0), R, C,
         block ? CUTIE_TILE_BLOCK : CUTIE_TILE_TWO_WAY, CUTIE_SCALE_FP32, base(), ceil_to(C, 16),
