@@ -286,7 +286,11 @@ CUTIE_API int cutie_rms_norm_mxfp8_gemm(const void* x, int64_t ldx, const void* 
  *   CUTIE_TILE_TWO_WAY: 1 x 128 groups of the rows for q, 128 x 1 groups of
  *     the columns for qt (activations and gradients; qt and st are required).
  *     Scales are group-major: s element (row, g) at g * lds + row, st element
- *     (column, g) at g * ldst + column.
+ *     (column, g) at g * ldst + column. CUTIE_SCALE_GRADIENT added to
+ *     scale_fmt: a group with amax < 1e-4 has s = max(amax / 448, 2^-92). At
+ *     the scale 1e-4 the codes of |x| < 9.8e-8 are all zero, and gradients are
+ *     often smaller than that (2^-92 is the least scale for which the division
+ *     stays correctly rounded; the codes of |x| < 2^-102 are zero).
  * Ragged last blocks and groups are reduced over their valid elements. H is a
  * multiple of 8, M >= 0 any; x rows 16-byte, q and qt rows 8-byte aligned
  * (16-byte for cutie_fp8_block_gemm). A group with an infinity gets an
@@ -296,6 +300,9 @@ CUTIE_API int cutie_rms_norm_mxfp8_gemm(const void* x, int64_t ldx, const void* 
 enum {
   CUTIE_TILE_BLOCK = 0,
   CUTIE_TILE_TWO_WAY = 1,
+};
+enum {
+  CUTIE_SCALE_GRADIENT = 16, /* added to scale_fmt, CUTIE_TILE_TWO_WAY only  */
 };
 CUTIE_API int cutie_cast_fp8_tiles(const void* x, int64_t ldx, int64_t M, int64_t H,
                                    int tile_kind, int scale_fmt, void* q, int64_t ldq, void* s,

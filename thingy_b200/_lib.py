@@ -26,6 +26,7 @@ SCALE_FP32, SCALE_FP32_POW2, SCALE_E8M0 = 0, 1, 2
 LAYOUT_ROW_MAJOR, LAYOUT_COL_MAJOR, LAYOUT_MX_SWIZZLED, LAYOUT_COL_MAJOR_PACKED = 0, 1, 2, 3
 DTYPE_BF16, DTYPE_F32 = 0, 1
 TILE_BLOCK, TILE_TWO_WAY = 0, 1
+SCALE_GRADIENT = 16
 SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 
 ABI_VERSION = 1

@@ -811,8 +811,13 @@ extern "C" int cutie_cast_fp8_tiles(const void* x, int64_t ldx, int64_t M, int64
     return fail(CUTIE_ERR_UNSUPPORTED, "H must be below 2^31 - 128");
   if (tile_kind != CUTIE_TILE_BLOCK && tile_kind != CUTIE_TILE_TWO_WAY)
     return fail(CUTIE_ERR_INVALID_ARGUMENT, "unknown tile_kind %d", tile_kind);
-  if (scale_fmt != CUTIE_SCALE_FP32 && scale_fmt != CUTIE_SCALE_FP32_POW2)
+  const bool gradient = (scale_fmt & CUTIE_SCALE_GRADIENT) != 0;
+  const int fmt = scale_fmt & ~CUTIE_SCALE_GRADIENT;
+  if (fmt != CUTIE_SCALE_FP32 && fmt != CUTIE_SCALE_FP32_POW2)
     return fail(CUTIE_ERR_UNSUPPORTED, "tile casts write fp32 scales (scale_fmt %d)", scale_fmt);
+  if (gradient && tile_kind != CUTIE_TILE_TWO_WAY)
+    return fail(CUTIE_ERR_UNSUPPORTED, "gradients are cast by the two-way kind (scale_fmt %d)",
+                scale_fmt);
   if ((qt == nullptr) != (st == nullptr))
     return fail(CUTIE_ERR_INVALID_ARGUMENT, "qt and st must be given together");
   const bool block = tile_kind == CUTIE_TILE_BLOCK;
@@ -833,7 +838,8 @@ extern "C" int cutie_cast_fp8_tiles(const void* x, int64_t ldx, int64_t M, int64
   CastArgs a{};
   a.x = static_cast<const uint16_t*>(x), a.ldx = ldx;
   a.M = M, a.H = (int)H;
-  a.pow2 = scale_fmt == CUTIE_SCALE_FP32_POW2;
+  a.pow2 = fmt == CUTIE_SCALE_FP32_POW2;
+  a.gradient = gradient;
   a.q = static_cast<uint8_t*>(q), a.ldq = ldq;
   a.s = static_cast<float*>(s), a.lds = lds;
   a.qt = static_cast<uint8_t*>(qt), a.ldqt = ldqt;

@@ -5,7 +5,8 @@
 // with amax over 128 x 128 blocks (weights: x's codes and its transpose's share
 // the scale) or over 1 x 128 groups of the rows and, for the transposed codes,
 // 128 x 1 groups of the columns (activations and gradients: the products of a
-// training step contract over either axis).
+// training step contract over either axis). Gradients (tile_scale): a group
+// with amax < 1e-4 has s = max(RN(amax / 448), 2^-92).
 //
 // One CTA casts one 128 x 128 tile, 256 threads, four CTAs an SM: thread (rg, v)
 // holds rows 8 rg .. 8 rg + 7, columns 8 v .. 8 v + 7, eight 16-byte loads, a
@@ -30,8 +31,14 @@ constexpr int kTile = 128, kThreads = 256;
 
 // The scale of a group's maximum. An infinite maximum stays infinite (the
 // division's remainder would turn it into a NaN, and that into the floor).
-__device__ __forceinline__ float tile_scale(float amax, bool pow2) {
-  return amax <= 3.4e38f ? make_scale(amax, pow2) : amax;
+// The activation quantizer's floor of 1e-4 loses a group whose maximum is far
+// below it: every |x| < 9.8e-8 has the code zero, and gradients are often that
+// small. While amax >= 1e-4 the floor costs an element at most 2^-10 of amax
+// (half the least code's step), 2^-10 sqrt(128 / 3) = 0.6% of the group's norm
+// in the mean square; below, a gradient's group goes without it.
+__device__ __forceinline__ float tile_scale(float amax, const CastArgs& a) {
+  const float least = a.gradient && amax < kMinScale ? kMinGradientScale : kMinScale;
+  return amax <= 3.4e38f ? make_scale(amax, a.pow2, least) : amax;
 }
 // RN(1 / s): the negated exponent for a power of two, else rcp_scale; NaN for
 // an infinite scale, so that every code of its group is NaN.
@@ -97,7 +104,7 @@ __global__ void __launch_bounds__(kThreads, 4)
 #pragma unroll
     for (int w = 1; w < 8; ++w) m = max_bf2(m, part[w][0]);
     const float2 f = bf2_to_f2(m);
-    const float s = tile_scale(fmaxf(f.x, f.y), a.pow2);
+    const float s = tile_scale(fmaxf(f.x, f.y), a);
     if (tid == 0) {
       a.s[tr * a.lds + tc] = s;
       if (TRANSPOSED) a.st[(int64_t)tc * a.ldst + tr] = s;
@@ -135,7 +142,7 @@ __global__ void __launch_bounds__(kThreads, 4)
       }
     }
     const float2 f = bf2_to_f2(max_bf2(m[0], __shfl_xor_sync(all, m[0], 1)));
-    const float my_s = tile_scale(fmaxf(f.x, f.y), a.pow2), my_rc = rcp_of(my_s, a.pow2);
+    const float my_s = tile_scale(fmaxf(f.x, f.y), a), my_rc = rcp_of(my_s, a.pow2);
     if ((v & 1) == 0 && r0 + (v >> 1) < a.M) a.s[(int64_t)tc * a.lds + r0 + (v >> 1)] = my_s;
     __syncthreads();
     if (tid < 64) {  // columns 2 tid and 2 tid + 1, kept so that a warp's 16 reads below are in a row
@@ -143,7 +150,7 @@ __global__ void __launch_bounds__(kThreads, 4)
 #pragma unroll
       for (int w = 1; w < 8; ++w) c = max_bf2(c, part[w][tid]);
       const float2 g = bf2_to_f2(c);
-      const float s0 = tile_scale(g.x, a.pow2), s1 = tile_scale(g.y, a.pow2);
+      const float s0 = tile_scale(g.x, a), s1 = tile_scale(g.y, a);
       col_scale[2 * (tid & 3)][tid >> 2] = make_float2(s0, rcp_of(s0, a.pow2));
       col_scale[2 * (tid & 3) + 1][tid >> 2] = make_float2(s1, rcp_of(s1, a.pow2));
       const int at = tc * kTile + 2 * tid;

@@ -368,12 +368,17 @@ constexpr float kE4m3Max = 448.0f;
 constexpr float kRcpE4m3Max = 1.0f / 448.0f;  // RN(1/448), folded by the compiler
 constexpr float kMinScale = 1e-4f;            // fp8_utils.py:51 clamp
 
+// The least scale of small gradients, whose codes 1e-4 would make zero: the
+// least one for which no step of the divisions below leaves fp32's range while
+// a code is not zero (tests/test_gradient_scale.py).
+constexpr float kMinGradientScale = 0x1p-92f;
+
 // s = max(RN(amax / 448), 1e-4) [rounded up to a power of two for POW2/E8M0].
-__device__ __forceinline__ float make_scale(float amax, bool pow2) {
-  float s = fmaxf(div_rn(amax, kE4m3Max, kRcpE4m3Max), kMinScale);
+__device__ __forceinline__ float make_scale(float amax, bool pow2, float least = kMinScale) {
+  float s = fmaxf(div_rn(amax, kE4m3Max, kRcpE4m3Max), least);
   if (pow2) {
     // 2^ceil(log2 s), exactly: keep the exponent, bump it if any mantissa bit
-    // is set (s >= 1e-4 is a normal number).
+    // is set (s >= 2^-92 is a normal number).
     uint32_t u = __float_as_uint(s);
     u = (u & 0x007fffffu) ? (u & 0x7f800000u) + 0x00800000u : u;
     s = __uint_as_float(u);
@@ -386,8 +391,9 @@ __device__ __forceinline__ float make_scale(float amax, bool pow2) {
 // Dev. 34(1), 1990): y0 = rcp.approx(s), at most 1 ulp from 1/s (PTX ISA);
 // e = RN(1 - s*y0); y1 = RN(y0 + e*y0). One step is not correctly rounded for
 // every fp32 s, but it is for every scale this path can produce, s =
-// max(RN(a / 448), 1e-4) with a a bf16 magnitude (16969 values), from any
-// start within 2 ulps of 1/s: tests/test_scale_reciprocal.py checks all of
+// max(RN(a / 448), 1e-4) with a a bf16 magnitude (16969 values; for gradients
+// max(RN(a / 448), 2^-92)), from any start within 2 ulps of 1/s:
+// tests/test_scale_reciprocal.py and tests/test_gradient_scale.py check all of
 // them in exact rational arithmetic. Three instructions instead of the
 // general correctly rounded reciprocal.
 __device__ __forceinline__ float rcp_scale(float s) {

@@ -318,6 +318,7 @@ struct CastArgs {
   int64_t M;
   int H;
   bool pow2;
+  bool gradient;  // groups below 1e-4 have scales of their own, see tile_scale
   uint8_t* q;   // [M, H] codes
   int64_t ldq;
   float* s;     // block: [M/128, H/128], else group-major [H/128, M]

@@ -191,7 +191,7 @@ at::Tensor empty_codes(int64_t R, int64_t C, const at::Device& dev) {
 // Casts to e4m3 in both orientations (cutie_cast_fp8_tiles); qt and st are
 // undefined tensors unless `transposed`.
 std::tuple<at::Tensor, at::Tensor, c10::optional<at::Tensor>, c10::optional<at::Tensor>>
-cast_fp8_tiles(const at::Tensor& x, bool block, bool use_ue8m0, bool transposed) {
+cast_fp8_tiles(const at::Tensor& x, bool block, bool use_ue8m0, bool transposed, bool gradient) {
   if (x.dim() != 2) bad("x must be 2-D [M, H]");
   if (!x.is_cuda()) bad("x must be a CUDA tensor (this library has no CPU path)");
   if (x.scalar_type() != at::kBFloat16) bad("x must be bfloat16");
@@ -212,7 +212,8 @@ cast_fp8_tiles(const at::Tensor& x, bool block, bool use_ue8m0, bool transposed)
   void* stream = at::cuda::getCurrentCUDAStream(dev.index()).stream();
   check_status(cutie_cast_fp8_tiles(
       x.data_ptr(), ldx, M, H, block ? CUTIE_TILE_BLOCK : CUTIE_TILE_TWO_WAY,
-      use_ue8m0 ? CUTIE_SCALE_FP32_POW2 : CUTIE_SCALE_FP32, q.data_ptr(), ceil_to(H, 16),
+      (use_ue8m0 ? CUTIE_SCALE_FP32_POW2 : CUTIE_SCALE_FP32) + (gradient ? CUTIE_SCALE_GRADIENT : 0),
+      q.data_ptr(), ceil_to(H, 16),
       s.data_ptr(), block ? GH : M, transposed ? qt.data_ptr() : nullptr,
       transposed ? ceil_to(M, 16) : 0, transposed ? st.data_ptr() : nullptr,
       transposed ? (block ? GM : H) : 0, stream));
@@ -286,11 +287,12 @@ struct Operand {
 // A matrix's codes and its transpose's, in one buffer.
 struct CastBuffer {
   int64_t R, C;
-  bool block;
+  bool block, gradient;
   at::Tensor hold;
   int64_t off_s, off_qt, off_st, bytes;
 
-  CastBuffer(int64_t rows, int64_t cols, bool blocks) : R(rows), C(cols), block(blocks) {
+  CastBuffer(int64_t rows, int64_t cols, bool blocks, bool of_gradient = false)
+      : R(rows), C(cols), block(blocks), gradient(of_gradient) {
     const int64_t GR = (R + 127) / 128, GC = (C + 127) / 128;
     off_s = ceil_to(R * ceil_to(C, 16), 256);
     off_qt = off_s + ceil_to(4 * (block ? GR * GC : GC * R), 256);
@@ -316,8 +318,8 @@ struct CastBuffer {
     if (R == 0 || C == 0) return;  // no codes
     check_status(cutie_cast_fp8_tiles(
         x.data_ptr(), R <= 1 ? ceil_to(C, 8) : x.stride(0), R, C,
-        block ? CUTIE_TILE_BLOCK : CUTIE_TILE_TWO_WAY, CUTIE_SCALE_FP32, base(), ceil_to(C, 16),
-        base() + off_s, block ? (C + 127) / 128 : R, transposed ? base() + off_qt : nullptr,
+        block ? CUTIE_TILE_BLOCK : CUTIE_TILE_TWO_WAY,
+        CUTIE_SCALE_FP32 + (gradient ? CUTIE_SCALE_GRADIENT : 0), base(), ceil_to(C, 16), base() + off_s, block ? (C + 127) / 128 : R, transposed ? base() + off_qt : nullptr,
         transposed ? ceil_to(R, 16) : 0, transposed ? base() + off_st : nullptr,
         transposed ? (block ? (R + 127) / 128 : C) : 0, stream));
   }
@@ -379,7 +381,7 @@ struct FP8Linear : public torch::autograd::Function<FP8Linear> {
     const at::Device dev = dy.device();
     const c10::cuda::CUDAGuard guard(dev);
     void* stream = at::cuda::getCurrentCUDAStream(dev.index()).stream();
-    CastBuffer d(M, N, false), w(N, K, true), xs(M, K, false);
+    CastBuffer d(M, N, false, true), w(N, K, true), xs(M, K, false);
     d.cast(dy, true, stream);
     if (sizes[2]) {
       Operand wt;
@@ -511,7 +513,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rms_norm", &rms_norm, py::arg("x"), py::arg("weight"), py::arg("eps"), py::arg("out"),
         py::arg("threads_per_row"));
   m.def("cast_fp8_tiles", &cast_fp8_tiles, py::arg("x"), py::arg("block"), py::arg("use_ue8m0"),
-        py::arg("transposed"));
+        py::arg("transposed"), py::arg("gradient"));
   m.def("fp8_block_gemm", &fp8_block_gemm, py::arg("a"), py::arg("a_scale"), py::arg("b"),
         py::arg("b_scale"), py::arg("out"), py::arg("out_f32"), py::arg("accumulate"));
   m.def("fp8_linear", &fp8_linear, py::arg("x"), py::arg("weight"), py::arg("wq"), py::arg("ws"),

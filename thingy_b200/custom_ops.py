@@ -80,12 +80,12 @@ def _per_block_cast_fake(w, use_ue8m0):
 
 
 @torch.library.custom_op("thingy_b200::two_way_cast_to_fp8", mutates_args=())
-def two_way_cast_op(x: torch.Tensor, use_ue8m0: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
-    return two_way_cast_to_fp8(x, use_ue8m0)
+def two_way_cast_op(x: torch.Tensor, use_ue8m0: bool, gradient: bool = False) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    return two_way_cast_to_fp8(x, use_ue8m0, gradient)
 
 
 @two_way_cast_op.register_fake
-def _two_way_cast_fake(x, use_ue8m0):
+def _two_way_cast_fake(x, use_ue8m0, gradient=False):
     R, C = x.shape
     GR, GC = -(-R // GROUP_SIZE), -(-C // GROUP_SIZE)
     return (_codes(x, R, C), x.new_empty_strided((R, GC), (1, R), dtype=torch.float32),

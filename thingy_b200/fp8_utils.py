@@ -9,8 +9,9 @@ It runs the hand-written sm_100a kernel; gran_k may also be 32 or 64.
 
 ``per_block_cast_to_fp8`` (weights, 128 x 128 blocks) and ``two_way_cast_to_fp8``
 (activations and gradients, 1 x 128 groups along both axes) make the operands
-of ``thingy_b200.fp8_block_gemm`` by the same rule; they have no counterpart
-in the reference, which quantizes activations along their rows only.
+of ``thingy_b200.fp8_block_gemm`` by the same rule (on request with scales for
+small gradients); they have no counterpart in the reference, which quantizes
+activations along their rows only.
 """
 
 from __future__ import annotations
@@ -55,18 +56,20 @@ def per_block_cast_to_fp8(w: torch.Tensor, use_ue8m0: bool = False, transposed: 
     start on 16-byte boundaries (a view of a wider buffer when the width is
     not a multiple of 16). Runs on the current stream.
     """
-    q, s, qt, st = require_binding().cast_fp8_tiles(w, True, bool(use_ue8m0), bool(transposed))
+    q, s, qt, st = require_binding().cast_fp8_tiles(w, True, bool(use_ue8m0), bool(transposed), False)
     return (q, s, qt, st) if transposed else (q, s)
 
 
-def two_way_cast_to_fp8(x: torch.Tensor, use_ue8m0: bool = False):
+def two_way_cast_to_fp8(x: torch.Tensor, use_ue8m0: bool = False, gradient: bool = False):
     """bf16 [M, H] -> (q, s, qt, st): e4m3 codes in 1 x 128 groups along the rows and along the columns.
 
     q [M, H] with s [M, ceil(H/128)] quantizes rows (the forward product and
     the input gradient contract over H); qt [H, M] with st [H, ceil(M/128)]
     the rows of x's transpose (the weight gradient contracts over M). x is
     read once. Scales are group-major views (strides (1, M) and (1, H)), the
-    codes' rows start on 16-byte boundaries. H must be a multiple of 8. Runs
-    on the current stream.
+    codes' rows start on 16-byte boundaries. H must be a multiple of 8. With
+    ``gradient`` a group whose maximum is below 1e-4 has the scale max(amax/448,
+    2^-92) instead of 1e-4, at which values below 9.8e-8 become zero. Runs on
+    the current stream.
     """
-    return require_binding().cast_fp8_tiles(x, False, bool(use_ue8m0), True)
+    return require_binding().cast_fp8_tiles(x, False, bool(use_ue8m0), True, bool(gradient))

@@ -27,7 +27,10 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_fp8=None) -> torch.
     without it the weight is cast in the call. The gradients are the
     straight-through ones of quantized operands: dx = q(dy) q(w), dw = q(dy)^T
     q(x), with x and dy quantized along the token axis for dw; dw has the
-    weight's dtype. Runs on the current stream.
+    weight's dtype. x and the weight are cast with the quantizers' least scale
+    of 1e-4; a group of dy that is below 1e-4 throughout has a scale of its own
+    (``two_way_cast_to_fp8(..., gradient=True)``), so no gradient is too small.
+    Runs on the current stream.
     """
     wq, ws, wqt, wst = (None, None, None, None) if weight_fp8 is None else weight_fp8
     return require_binding().fp8_linear(x, weight, wq, ws, wqt, wst)
