@@ -271,6 +271,10 @@ __device__ __forceinline__ uint32_t ordered(float f) {
   return f != f ? 1u : u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
 }
 
+__device__ __forceinline__ float unordered(uint32_t key) {
+  return __uint_as_float(key ^ (key >> 31 ? 0x80000000u : 0xffffffffu));
+}
+
 // Logits of `n` tokens from t0 on, [n][E] into shared memory: the sums of the
 // router's shares, a thread a logit, eight loads in flight.
 __device__ __forceinline__ void sum_logits(const MoeArgs& g, int t0, int n, float* to) {
@@ -331,7 +335,17 @@ __device__ __forceinline__ void choose(const MoeArgs& g, const float* logits, ui
     if (lane == j) my_id = (int)e;
   }
   float p = 0.f;
-  if (lane < g.k) p = softmax ? expf(logits[my_id] - m) : 1.f / (1.f + expf(-logits[my_id]));
+  const float l = lane < g.k ? logits[my_id] : -INFINITY;
+  // Renormalized weights are ratios: where the chosen scores are all below e^-64
+  // (a bias chose them, or every sigmoid is that small) and might underflow, they
+  // are taken relative to the largest of them instead.
+  bool rescale = false;
+  if (g.renormalize) {
+    const float top = unordered(__reduce_max_sync(0xffffffffu, ordered(l)));
+    rescale = softmax ? top < m - 64.f && m < INFINITY : top < -64.f;
+    if (rescale) m = top;
+  }
+  if (lane < g.k) p = softmax || rescale ? expf(l - m) : 1.f / (1.f + expf(-l));
   float den = softmax ? z : 1.f;
   if (g.renormalize) {
     den = p;
