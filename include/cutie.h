@@ -335,8 +335,9 @@ CUTIE_API int cutie_fp8_block_gemm(const void* a, int64_t lda, const void* a_sca
  *   logits = x router^T (fp32 sums of bf16 products); scores = softmax or
  *   sigmoid of the logits; each token takes the top_k experts of the largest
  *   logits (with a bias: of the largest score + bias), ties to the lowest
- *   index; weights w = the chosen scores, divided by their sum if
- *   renormalize, times routed_scale
+ *   index, NaN last; weights w = the chosen scores, divided by their sum if
+ *   renormalize, times routed_scale (all NaN under softmax if any of the
+ *   token's logits is)
  *   g, u = dequant(q) dequant(w13[e])^T; h = silu(g) u (fp32);
  *   (qh, sh) = the 1 x 128 cast of h: s = max(amax / 448, 1e-4), e4m3(h / s)
  *   out[t] = bf16( sum_j w[t, j] dequant(qh) dequant(w2[e_j])^T )

@@ -79,3 +79,53 @@ def test_scores_that_are_not_renormalized_may_be_zero(scoring):
     y, ids, weights = _call(ops, 3, scoring=scoring, bias=bias, renormalize=False)
     assert torch.equal(ids, torch.tensor([2, 3, 4], device="cuda").expand(3, 3))
     assert bool((weights == 0).all()) and bool((y == 0).all())
+
+
+@pytest.mark.parametrize("T", [1, 4, 20])
+@pytest.mark.parametrize("renormalize", [True, False])
+@pytest.mark.parametrize("biased", [False, True])
+def test_nan_logit_of_one_expert_under_softmax(T, renormalize, biased):
+    """A softmax over a NaN is a NaN everywhere, whichever experts are chosen."""
+    ops = list(_layer(T, 8, torch.arange(8.0, device="cuda"), seed=4))
+    ops[3][2, 1] = float("nan")  # a NaN in one expert's router row: the least likely choice
+    bias = 0.5 * torch.ones(8, device="cuda") if biased else None
+    y, ids, weights = _call(ops, 3, renormalize=renormalize, bias=bias)
+    assert bool(torch.isnan(weights).all()) and bool(torch.isnan(y).all())
+    assert bool(((ids >= 0) & (ids < 8)).all())
+    assert all(len(set(row)) == 3 for row in ids.tolist())
+
+
+@pytest.mark.parametrize("T", [1, 4, 20])
+def test_nan_logit_of_one_expert_under_sigmoid(T):
+    """Scores of their own: the expert is chosen last, and the others' weights do not know it."""
+    ops = list(_layer(T, 8, torch.arange(8.0, device="cuda") - 4, seed=5))
+    want = _call(ops, 3, scoring="sigmoid")
+    broken = list(ops)
+    broken[3] = ops[3].clone()
+    broken[3][2, 1] = float("nan")
+    for got, ref in zip(_call(broken, 3, scoring="sigmoid"), want):
+        assert torch.equal(got, ref)
+
+
+@pytest.mark.parametrize("T", [1, 4, 20])
+def test_logits_of_minus_infinity(T):
+    """Masked experts: no weight, and no NaN while any other is left."""
+    ops = list(_layer(T, 8, torch.arange(8.0, device="cuda"), seed=6))
+    ops[3][4:, 0] = float("-inf")
+    y, ids, weights = _call(ops, 3)
+    p = torch.softmax(torch.arange(4.0, dtype=torch.float64, device="cuda"), 0).flip(0)[:3]
+    assert torch.equal(ids, torch.tensor([3, 2, 1], device="cuda").expand(T, 3))
+    assert torch.allclose(weights, (p / p.sum()).expand(T, 3), rtol=1e-4, atol=1e-35)
+    assert bool(torch.isfinite(y).all())
+
+
+@pytest.mark.parametrize("T", [1, 20])
+@pytest.mark.parametrize("renormalize", [True, False])
+def test_infinite_logit_that_a_bias_passes_over(T, renormalize):
+    """inf - inf in the softmax's sum: no weight of the token is a number, whoever is chosen."""
+    ops = list(_layer(T, 8, torch.arange(8.0, device="cuda"), seed=7))
+    ops[3][7, 0] = float("inf")
+    bias = torch.zeros(8, device="cuda")
+    bias[:3] = 100.0
+    y, ids, weights = _call(ops, 3, renormalize=renormalize, bias=bias)
+    assert bool(torch.isnan(weights).all()) and bool(torch.isnan(y).all())

@@ -271,6 +271,12 @@ __device__ __forceinline__ uint32_t ordered(float f) {
   return f != f ? 1u : u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
 }
 
+// The larger one, or a NaN if either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 __device__ __forceinline__ float unordered(uint32_t key) {
   return __uint_as_float(key ^ (key >> 31 ? 0x80000000u : 0xffffffffu));
 }
@@ -294,7 +300,9 @@ __device__ __forceinline__ void sum_logits(const MoeArgs& g, int t0, int n, floa
 
 // One token's choice by one warp from its logits in shared memory: k rounds of
 // a warp maximum, ties to the lowest expert; `key` is E words of scratch. Lane
-// j < k returns with (*id, *w) of slot j. The loops stay rolled: every launch
+// j < k returns with (*id, *w) of slot j. A NaN logit is chosen last; under
+// softmax it makes every weight of the token a NaN (m carries it), as the sum
+// over all experts would. The loops stay rolled: every launch
 // runs this once, and instructions fetched for the first time cost more than
 // they compute (unrolled over 16 registers a lane this took 4 us, not 1.5).
 __device__ __forceinline__ void choose(const MoeArgs& g, const float* logits, uint32_t* key, int lane,
@@ -303,9 +311,9 @@ __device__ __forceinline__ void choose(const MoeArgs& g, const float* logits, ui
   float m = -INFINITY, z = 1.f;
   if (softmax) {  // the sum over all experts only where the weights need it
 #pragma unroll 1
-    for (int e = lane; e < g.E; e += 32) m = fmaxf(m, logits[e]);
+    for (int e = lane; e < g.E; e += 32) m = max_nan(m, logits[e]);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (!g.renormalize || g.bias != nullptr) {
       z = 0.f;
 #pragma unroll 1

@@ -78,7 +78,8 @@ def moe_fp8(
     Each token takes the top_k experts of the largest logits, ties to the
     lowest index; ``bias`` (fp32 [E]) is added to the scores for that choice
     only. Its weights are the scores (softmax over all experts, or sigmoid),
-    divided by their sum if ``renormalize``, times ``routed_scale``. The
+    divided by their sum if ``renormalize``, times ``routed_scale``. A NaN
+    logit is chosen last; under softmax all weights of its token are NaN. The
     hidden rows silu(gate) * up are cast to e4m3 in 1 x 128 groups; sums are
     fp32, rounded once to bf16. topk_ids (int32) and topk_weights (float32),
     [T, top_k], receive the choices. workspace: ``moe_workspace(...)``;
