@@ -1,7 +1,8 @@
-"""The experts' weights where their scores leave fp32's range, and where a logit is a NaN.
+"""The experts' weights where their scores leave fp32's range and where a logit is a NaN, and the order of
+what CTAs write for one another.
 
 Reference in 64 bits, where the scores below do not underflow. The router's logits come from
-single products, x[t, 0] router[e, 0] and a second column, so they are the same numbers in both.
+one column, x[t, 0] router[e, 0] with x[t, 0] = 1, so they are the same numbers in both.
 """
 
 import pytest
@@ -129,3 +130,22 @@ def test_infinite_logit_that_a_bias_passes_over(T, renormalize):
     bias[:3] = 100.0
     y, ids, weights = _call(ops, 3, renormalize=renormalize, bias=bias)
     assert bool(torch.isnan(weights).all()) and bool(torch.isnan(y).all())
+
+
+@pytest.mark.parametrize("T,E,k,H,I", [(64, 24, 6, 1024, 128), (40, 60, 4, 512, 128), (16, 8, 4, 2048, 256), (6, 16, 4, 1024, 128)])
+def test_scales_of_hidden_rows_that_other_ctas_write(T, E, k, H, I):
+    """One or two hidden groups a row: the scales of up to eight rows share a 32-byte piece of memory, and
+    each expert's are written by other CTAs just before they are read. Every repeat gives the same bits."""
+    g = torch.Generator(device="cuda").manual_seed(T)
+    x = torch.randn(T, H, generator=g, device="cuda").to(torch.bfloat16)
+    q, s, _, n = tb.rms_norm_fp8(x, torch.ones(H, dtype=torch.bfloat16, device="cuda"), 1e-6, return_normalized=True)
+    router = (0.05 * torch.randn(E, H, generator=g, device="cuda")).to(torch.bfloat16)
+    w13 = quantize_experts((0.05 * torch.randn(E, 2 * I, H, generator=g, device="cuda")).to(torch.bfloat16))
+    w2 = quantize_experts((0.05 * torch.randn(E, H, I, generator=g, device="cuda")).to(torch.bfloat16))
+    workspace = tb.moe_workspace(T, E, k, H, I)
+    workspace[256:] = 0xFF  # NaN codes and scales from before: a read that comes too early shows
+    first = tb.moe_fp8(n, q, s, router, *w13, *w2, top_k=k, workspace=workspace)
+    assert bool(torch.isfinite(first).all())
+    for _ in range(40):
+        workspace[256:] = 0xFF
+        assert torch.equal(tb.moe_fp8(n, q, s, router, *w13, *w2, top_k=k, workspace=workspace), first)

@@ -736,6 +736,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
         if (phase == 1 && w.a != hidden_of) {
           hidden_of = w.a;
           if (lane == 0) ok = wait_count(g.ready + w.a, IG, abortp);
+          __syncwarp();  // orders the other lanes' copies of h_scale after lane 0's acquire; a vote does not
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
         }
