@@ -387,10 +387,11 @@ CUTIE_API int cutie_device_error(int clear);
 
 /*
  * Limit, in SM clock cycles, on every wait that the kernels launched later
- * by the calling thread make for their own bulk copies and row exchanges
- * (the default, about 2 s, bounds a copy that never lands). A wait that runs
- * out stops the kernel early with device error 1 (cutie_device_error); the
- * kernel first lets the copies it issued land, so the GPU stays usable.
+ * by the calling thread make for their own bulk copies and exchanges
+ * (cutie_gemm_mxfp8's keep the default). The default, about 2 s, bounds a copy
+ * that never lands. A wait that runs out stops the kernel early with device
+ * error 1 (cutie_device_error); the kernel first lets the copies it issued
+ * land, so the GPU stays usable.
  * cycles == 0 restores the default; cycles < 0 makes every wait that would
  * have to block give up at once, which exercises that failure path with
  * valid inputs (the outputs of such a launch are incomplete). Affects this

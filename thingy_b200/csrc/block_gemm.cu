@@ -25,18 +25,6 @@ constexpr int kBM = 128, kBK = 128;
 constexpr uint32_t kBoxBytes = kBM * kBK;  // one 128-row operand box: 16 KB
 constexpr int kMaxRanks = 8;               // of a K split: a portable cluster
 
-// Gives up after kWaitLimitCycles, or at once when the CTA's abort flag is
-// set; giving up sets the flag.
-__device__ __forceinline__ bool wait_or_abort(uint32_t bar, uint32_t parity,
-                                              volatile uint32_t* abort_flag) {
-  if (mbar_test(bar, parity)) return true;
-  const long long t0 = clock64();
-  while (!*abort_flag && clock64() - t0 <= kWaitLimitCycles)
-    if (mbar_try_wait(bar, parity)) return true;
-  *abort_flag = 1u;
-  return false;
-}
-
 // Clusters of S CTAs (along z; pairs along x) that run at once on the current device, remembered.
 int max_clusters(const void* kernel, int threads, size_t smem, dim3 cluster,
                  std::atomic<int> (&cache)[64][kMaxRanks + 1]) {
@@ -159,6 +147,7 @@ struct TileArgs {
   int tail;   // 128-wide form: >= 0: the parts of the larger tiles from this one on,
   int parts;  // 2 (columns) or 4 (columns and rows) each
   bool d_f32, accumulate;
+  long long wait_limit;  // SM cycles a wait may block before it gives up (< 0: never blocks)
 };
 
 // Tile t of the banded walk.
@@ -360,7 +349,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int tm, tn;
       tile_of<BN>(g, t, &tm, &tn);
       for (int kb = 0; kb < nkb; ++kb) {
-        ok = wait_or_abort(smem_addr(&empty_bar[s]), parity, abortp);
+        ok = tc::wait_or_abort(smem_addr(&empty_bar[s]), parity, abortp, g.wait_limit);
         if (!__all_sync(0xffffffffu, ok)) {
           ok = false;
           break;
@@ -387,7 +376,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (PAIR)  // rank 0's commits arrive here: all before this CTA's memory goes
       for (int i = 0; i < P::kStages && ok; ++i) {
-        ok = __all_sync(0xffffffffu, wait_or_abort(smem_addr(&empty_bar[s]), parity, abortp));
+        ok = __all_sync(0xffffffffu, tc::wait_or_abort(smem_addr(&empty_bar[s]), parity, abortp, g.wait_limit));
         if (++s == P::kStages) s = 0, parity ^= 1;
       }
   } else if (warp == kEpiWarps + 1) {
@@ -399,8 +388,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = !PAIR || rank == 0;  // rank 0 issues for both
     for (int t = begin; t < tiles && ok; t += step) {
       for (int kb = 0; kb < nkb; ++kb) {
-        ok = wait_or_abort(smem_addr(&full_bar[s]), parity, abortp) &&
-             wait_or_abort(smem_addr(&acc_empty[buf]), buf_parity, abortp);
+        ok = tc::wait_or_abort(smem_addr(&full_bar[s]), parity, abortp, g.wait_limit) &&
+             tc::wait_or_abort(smem_addr(&acc_empty[buf]), buf_parity, abortp, g.wait_limit);
         if (!__all_sync(0xffffffffu, ok)) {
           ok = false;
           break;
@@ -454,7 +443,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int kb = 0; kb < nkb; ++kb) {
         const int j = kb % kScaleBlocks;
         if (j == 0) {
-          ok = __all_sync(0xffffffffu, wait_or_abort(smem_addr(&scale_empty[s]), parity, abortp));
+          ok = __all_sync(0xffffffffu,
+                          tc::wait_or_abort(smem_addr(&scale_empty[s]), parity, abortp, g.wait_limit));
           if (!ok) break;
         }
 #pragma unroll
@@ -498,11 +488,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     // K block kb of a tile: its first load, and its scales
     auto begin_block = [&](int kb) {
       const int j = kb % kScaleBlocks;
-      if (j == 0) wait_or_abort(smem_addr(&scale_full[slot]), slot_parity, abortp);
+      if (j == 0) tc::wait_or_abort(smem_addr(&scale_full[slot]), slot_parity, abortp, g.wait_limit);
       sc = scales[slot][j][r];
       sb = &scales[slot][j][128 + (SB_ROWS ? wg * NC : wg * NC / 128)];
       if (!SB_ROWS) sc *= *sb;
-      wait_or_abort(smem_addr(&acc_full[buf]), buf_parity, abortp);
+      tc::wait_or_abort(smem_addr(&acc_full[buf]), buf_parity, abortp, g.wait_limit);
       __syncwarp();
       tc::fence_after();
       tc::tmem_ld_async(tm_lane + buf * BN, lo);
@@ -588,7 +578,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         asm volatile("barrier.cta.sync 1, 256;" ::: "memory");
         tc::cluster_arrive();
         tc::cluster_wait();
-        if (threadIdx.x == 0 && *abortp == 0u) {
+        // also after an abort, so that every copy between the ranks is counted
+        // and over before one of them ends
+        if (threadIdx.x == 0) {
           for (int q = 0; q < S; ++q) {
             const int lo_q = min(q * share, kBM), n = min(share, kBM - lo_q);
             if (q == rank || n == 0) continue;
@@ -597,9 +589,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                          tc::mapa(smem_addr(&recv_bar), (uint32_t)q));
           }
         }
-        const bool got = __all_sync(0xffffffffu, wait_or_abort(smem_addr(&recv_bar), 0u, abortp));
+        const bool got = __all_sync(
+            0xffffffffu, tc::wait_or_abort(smem_addr(&recv_bar), 0u, abortp, g.wait_limit));
+        if (!got) mbar_wait_bounded(smem_addr(&recv_bar), 0u, kDrainLimitCycles);
+        __syncwarp();
         tc::cluster_arrive();  // what the others sent has arrived
-        if (got) {
+        if (got && *abortp == 0u) {
           const float* in = part + kPartBytes / 4;
           const int col = tn_i * BN + lane * 4;
           for (int i = warp; i < own_n; i += kEpiWarps) {
@@ -641,7 +636,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (m > 0)
         mbar_wait_bounded(smem_addr(&acc_full[(m - 1) & 1u]), ((m - 1) >> 1) & 1u,
                           kDrainLimitCycles);
-      // and what other ranks may have sent here, or this one has on its way: nothing counts it now
+      // and what nothing counts now: a pair's loads on their way here, or parts of
+      // a rank that gave up later than this one
       for (const long long t0 = clock64(); (SPLIT || PAIR) && clock64() - t0 < kDrainLimitCycles / 100;) {
       }
     }
@@ -838,7 +834,7 @@ __global__ void __launch_bounds__(kFewThreads, FewPlan<BR>::kCtas)
     const bool leader = tc::elect_one();
     uint32_t s = 0, parity = 1;
     for (int i = 0; i < steps; ++i) {
-      const bool ok = wait_or_abort(smem_addr(&empty_bar[s]), parity, abortp);
+      const bool ok = tc::wait_or_abort(smem_addr(&empty_bar[s]), parity, abortp, g.wait_limit);
       if (!__all_sync(0xffffffffu, ok)) break;
       if (leader) {
         const int kb = kb0 + i * kFewStep, n = min(kFewStep, kb1 - kb);
@@ -859,8 +855,8 @@ __global__ void __launch_bounds__(kFewThreads, FewPlan<BR>::kCtas)
     const uint32_t lo0 = tc::sw128_lo(base), hi = tc::sw128_hi();
     uint32_t s = 0, parity = 0, buf = 0, buf_parity = 1;
     for (int i = 0; i < steps; ++i) {
-      const bool ok = wait_or_abort(smem_addr(&full_bar[s]), parity, abortp) &&
-                      wait_or_abort(smem_addr(&acc_empty[buf]), buf_parity, abortp);
+      const bool ok = tc::wait_or_abort(smem_addr(&full_bar[s]), parity, abortp, g.wait_limit) &&
+                      tc::wait_or_abort(smem_addr(&acc_empty[buf]), buf_parity, abortp, g.wait_limit);
       if (!__all_sync(0xffffffffu, ok)) break;
       tc::fence_after();
       if (leader) {
@@ -892,7 +888,7 @@ __global__ void __launch_bounds__(kFewThreads, FewPlan<BR>::kCtas)
     for (int kb = kb0; kb < kb1; ++kb) {
       const int j = (kb - kb0) % kScaleBlocks;
       if (j == 0) {
-        const bool ok = wait_or_abort(smem_addr(&scale_empty[s]), parity, abortp);
+        const bool ok = tc::wait_or_abort(smem_addr(&scale_empty[s]), parity, abortp, g.wait_limit);
         if (!__all_sync(0xffffffffu, ok)) break;
       }
 #pragma unroll
@@ -921,8 +917,8 @@ __global__ void __launch_bounds__(kFewThreads, FewPlan<BR>::kCtas)
     bool ok = true;
     for (int kb = kb0; kb < kb1; kb += kFewStep) {
       const int j0 = (kb - kb0) % kScaleBlocks;
-      ok = (j0 != 0 || wait_or_abort(smem_addr(&scale_full[slot]), slot_parity, abortp)) &&
-           wait_or_abort(smem_addr(&acc_full[buf]), buf_parity, abortp);
+      ok = (j0 != 0 || tc::wait_or_abort(smem_addr(&scale_full[slot]), slot_parity, abortp, g.wait_limit)) &&
+           tc::wait_or_abort(smem_addr(&acc_full[buf]), buf_parity, abortp, g.wait_limit);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc::fence_after();
@@ -987,7 +983,9 @@ __global__ void __launch_bounds__(kFewThreads, FewPlan<BR>::kCtas)
       asm volatile("barrier.cta.sync 1, 128;" ::: "memory");
       tc::cluster_wait();  // every CTA's barriers exist
       const uint32_t recv = base + P::kOffRecv;
-      if (threadIdx.x == 0 && ok) {
+      // also after an abort, so that every copy between the ranks is counted and
+      // over before one of them ends
+      if (threadIdx.x == 0) {
         for (int q = 0; q < S; ++q) {
           const int lo = min(q * share, g.M), n = min(lo + share, g.M) - lo;
           if (q == rank || n == 0) continue;
@@ -996,7 +994,9 @@ __global__ void __launch_bounds__(kFewThreads, FewPlan<BR>::kCtas)
                        tc::mapa(smem_addr(&recv_bar), (uint32_t)q));
         }
       }
-      ok = __all_sync(0xffffffffu, wait_or_abort(smem_addr(&recv_bar), 0u, abortp)) && ok;
+      ok = __all_sync(0xffffffffu, tc::wait_or_abort(smem_addr(&recv_bar), 0u, abortp, g.wait_limit)) && ok;
+      if (!ok) mbar_wait_bounded(smem_addr(&recv_bar), 0u, kDrainLimitCycles);
+      __syncwarp();
       tc::cluster_arrive();  // what the others sent has arrived
       if (ok) {
         const float* in = reinterpret_cast<const float*>(smem_raw + (recv - smem_addr(smem_raw)));
@@ -1031,7 +1031,7 @@ __global__ void __launch_bounds__(kFewThreads, FewPlan<BR>::kCtas)
       if (m > 0)
         mbar_wait_bounded(smem_addr(&acc_full[(m - 1) % P::kBufs]), ((m - 1) / P::kBufs) & 1u,
                           kDrainLimitCycles);
-      // and what other ranks may have sent here: nothing counts it now
+      // and parts of a rank that gave up later than this one: nothing counts them now
       for (const long long t0 = clock64(); clock64() - t0 < kDrainLimitCycles / 100;) {
       }
     }
@@ -1146,6 +1146,7 @@ int block_gemm(const BlockGemmArgs& p, cudaStream_t stream, const char** why) {
   g.d = p.d, g.ldd = p.ldd;
   g.M = (int)p.M, g.N = (int)p.N, g.KB = (int)((p.K + kBK - 1) / kBK);
   g.d_f32 = p.d_f32, g.accumulate = p.accumulate;
+  g.wait_limit = p.wait_limit;
   const int columns = p.M <= 16 ? 16 : p.M <= 32 ? 32 : 64;
   const int ranks = p.b_rows || p.M > kFewRows ? 0
                     : columns == 16            ? few_ranks<16>(p.N, g.KB)

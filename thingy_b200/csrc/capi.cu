@@ -891,6 +891,7 @@ extern "C" int cutie_fp8_block_gemm(const void* a, int64_t lda, const void* a_sc
   g.b_rows = b_rows != 0;
   g.d = d, g.ldd = ldd, g.d_f32 = esize == 4, g.accumulate = accumulate != 0;
   g.M = M, g.N = N, g.K = K;
+  g.wait_limit = g_wait_limit;
   const char* why = "";
   rc = block_gemm(g, static_cast<cudaStream_t>(stream), &why);
   if (rc != CUTIE_OK) return fail(rc, "fp8 block gemm: %s", why);
@@ -973,6 +974,7 @@ extern "C" int cutie_moe_fp8(const void* x, int64_t ldx, const void* q, int64_t 
   g.w2_scale = static_cast<const float*>(w2_scale);
   g.T = (int)T, g.E = (int)E, g.k = (int)top_k, g.H = (int)H, g.I = (int)I;
   g.scoring = scoring, g.renormalize = renormalize != 0, g.routed_scale = routed_scale;
+  g.wait_limit = g_wait_limit;
   g.out = static_cast<uint16_t*>(out), g.ldo = ldo;
   g.ids = static_cast<int*>(topk_ids), g.weights = static_cast<float*>(topk_weights);
   const size_t need = moe_workspace(&g, workspace);

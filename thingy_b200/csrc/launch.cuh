@@ -346,6 +346,7 @@ struct BlockGemmArgs {
   bool d_f32;
   bool accumulate;  // fp32 only: D += instead of D =
   int64_t M, N, K;
+  long long wait_limit;
 };
 // Rows of `p`, ld_bytes apart, all start on n-byte boundaries.
 inline bool aligned_rows_host(const void* p, int64_t ld_bytes, unsigned n) {
@@ -369,6 +370,7 @@ struct MoeArgs {
   int scoring;  // 0 softmax, 1 sigmoid
   bool renormalize;
   float routed_scale;
+  long long wait_limit;  // SM cycles a wait may block before it gives up (< 0: never blocks)
   uint16_t* out;  // bf16 [T, H]
   int64_t ldo;
   int* ids;        // [T, k] chosen experts and their weights: the caller's, or in the workspace

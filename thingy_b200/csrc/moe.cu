@@ -111,16 +111,6 @@ struct MoeShared {
   uint64_t target;  // the grid barrier's count at the next barrier
 };
 
-__device__ __forceinline__ bool wait_or_abort(uint32_t bar, uint32_t parity,
-                                              volatile uint32_t* abort_flag) {
-  if (mbar_test(bar, parity)) return true;
-  const long long t0 = clock64();
-  while (!*abort_flag && clock64() - t0 <= kWaitLimitCycles)
-    if (mbar_try_wait(bar, parity)) return true;
-  *abort_flag = 1u;
-  return false;
-}
-
 // ------------------------------------------------------------------ grid barrier
 //
 // A 64-bit count in the workspace, zero before its first use. Every CTA adds
@@ -134,13 +124,13 @@ __device__ __forceinline__ uint64_t barrier_arrive(uint64_t* count) {
 }
 
 __device__ __forceinline__ bool barrier_wait(const uint64_t* count, uint64_t target,
-                                             volatile uint32_t* abort_flag) {
+                                             volatile uint32_t* abort_flag, long long limit) {
   const long long t0 = clock64();
   for (;;) {
     uint64_t v;
     asm volatile("ld.acquire.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(count) : "memory");
     if (v >= target) break;
-    if (clock64() - t0 > kWaitLimitCycles) {
+    if (clock64() - t0 > limit) {
       *abort_flag = 1u;
       return false;
     }
@@ -186,21 +176,23 @@ __device__ __forceinline__ float4 ld_l2(const float4* p) {
 __device__ __forceinline__ void release_add(int* count) {
   asm volatile("red.release.gpu.global.add.s32 [%0], 1;" ::"l"(count) : "memory");
 }
-__device__ __forceinline__ bool wait_count(const int* count, int target, volatile uint32_t* abort_flag) {
+__device__ __forceinline__ bool wait_count(const int* count, int target, volatile uint32_t* abort_flag,
+                                           long long limit) {
   const long long t0 = clock64();
   for (;;) {
     int v;
     asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(count) : "memory");
     if (v >= target) return true;
-    if (*abort_flag || clock64() - t0 > kWaitLimitCycles) {
+    if (*abort_flag || clock64() - t0 > limit) {
       *abort_flag = 1u;
       return false;
     }
   }
 }
 // The same before TMA reads what was waited for.
-__device__ __forceinline__ bool wait_count_tma(const int* count, int target, volatile uint32_t* abort_flag) {
-  const bool ok = wait_count(count, target, abort_flag);
+__device__ __forceinline__ bool wait_count_tma(const int* count, int target, volatile uint32_t* abort_flag,
+                                               long long limit) {
+  const bool ok = wait_count(count, target, abort_flag, limit);
   asm volatile("fence.proxy.async;" ::: "memory");
   return ok;
 }
@@ -431,7 +423,7 @@ __device__ __forceinline__ void add_parts(const MoeArgs& g, const Deal& deal, in
 #pragma unroll
         for (int c = 0; c < kTaggedTokens; ++c) here &= (v[c] >> 32) != 0;
         if (here) break;
-        if (*abortp || clock64() - t0 > kWaitLimitCycles) {
+        if (*abortp || clock64() - t0 > g.wait_limit) {
           *abortp = 1u;
           break;
         }
@@ -443,7 +435,7 @@ __device__ __forceinline__ void add_parts(const MoeArgs& g, const Deal& deal, in
   }
 #pragma unroll 1
   for (int b = (int)blockIdx.x + 1; b <= last; ++b) {
-    if ((threadIdx.x & 31) == 0) wait_count(g.part_flag + phase * gridDim.x + b, 1, abortp);
+    if ((threadIdx.x & 31) == 0) wait_count(g.part_flag + phase * gridDim.x + b, 1, abortp, g.wait_limit);
     __syncwarp();
     const float* o = g.partial + (int64_t)(phase * (int)gridDim.x + b) * NMAX * 256 + threadIdx.x;
 #pragma unroll
@@ -536,7 +528,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
   if (tid == 0) {
     const uint64_t old = barrier_arrive(g.barrier);
     sh.target = (old / gridDim.x + 1) * gridDim.x;
-    barrier_wait(g.barrier, sh.target, abortp);
+    barrier_wait(g.barrier, sh.target, abortp, g.wait_limit);
   }
   __syncthreads();
   uint64_t target = sh.target;
@@ -568,7 +560,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
     target += gridDim.x;
     if (tid == 0) {
       barrier_arrive(g.barrier);
-      barrier_wait(g.barrier, target, abortp);
+      barrier_wait(g.barrier, target, abortp, g.wait_limit);
     }
     __syncthreads();
     for (int p = tid; p < pairs; p += kMoeThreads) {
@@ -630,7 +622,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
       const int second = phase == 0 ? g.I : 128;
 #pragma unroll 1
       for (Walk w = sh.walk[phase]; w.more(); w.next()) {
-        ok = __all_sync(0xffffffffu, wait_or_abort(smem_addr(&sh.empty[s]), parity, abortp));
+        ok = __all_sync(0xffffffffu, tc::wait_or_abort(smem_addr(&sh.empty[s]), parity, abortp, g.wait_limit));
         if (!ok) break;
         if (leader) {
           const uint32_t st = base + s * P::kStageBytes, bar = smem_addr(&sh.full[s]);
@@ -655,11 +647,11 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
       for (Walk w = sh.walk[phase]; w.more(); w.next()) {
         if (phase == 1 && w.a != hidden_of) {
           hidden_of = w.a;
-          if (leader) ok = wait_count_tma(g.ready + w.a, IG, abortp);
+          if (leader) ok = wait_count_tma(g.ready + w.a, IG, abortp, g.wait_limit);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
         }
-        ok = __all_sync(0xffffffffu, wait_or_abort(smem_addr(&sh.empty[s]), parity, abortp));
+        ok = __all_sync(0xffffffffu, tc::wait_or_abort(smem_addr(&sh.empty[s]), parity, abortp, g.wait_limit));
         if (!ok) break;
         if (leader) {
           const int e = sh.active[w.a], n = __popcll(sh.mask[e]), row0 = sh.first_row[e];
@@ -697,8 +689,9 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
       for (Walk w = sh.walk[phase]; w.more(); w.next()) {
         if (idesc == 0 || w.kb == 0)
           idesc = tc::f8_idesc(128, (__popcll(sh.mask[sh.active[w.a]]) + 15) & ~15);
-        ok = __all_sync(0xffffffffu, wait_or_abort(smem_addr(&sh.full[s]), parity, abortp) &&
-                                         wait_or_abort(smem_addr(&sh.acc_empty[buf]), buf_parity, abortp));
+        ok = __all_sync(0xffffffffu,
+                        tc::wait_or_abort(smem_addr(&sh.full[s]), parity, abortp, g.wait_limit) &&
+                            tc::wait_or_abort(smem_addr(&sh.acc_empty[buf]), buf_parity, abortp, g.wait_limit));
         if (!ok) break;
         tc::fence_after();
         if (leader) {
@@ -735,7 +728,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
       for (Walk w = sh.walk[phase]; w.more(); w.next()) {
         if (phase == 1 && w.a != hidden_of) {
           hidden_of = w.a;
-          if (lane == 0) ok = wait_count(g.ready + w.a, IG, abortp);
+          if (lane == 0) ok = wait_count(g.ready + w.a, IG, abortp, g.wait_limit);
           __syncwarp();  // orders the other lanes' copies of h_scale after lane 0's acquire; a vote does not
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
@@ -753,7 +746,8 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
                           : g.w2_scale + ((int64_t)e * (g.H / 128) + w.grp * 2 + lane) * KB2;
           if (lane >= (phase == 0 || w.grp * 2 + 1 < g.H / 128 ? 2 : 1)) pw = nullptr;
         }
-        ok = __all_sync(0xffffffffu, wait_or_abort(smem_addr(&sh.scale_empty[s]), parity, abortp));
+        ok = __all_sync(0xffffffffu,
+                        tc::wait_or_abort(smem_addr(&sh.scale_empty[s]), parity, abortp, g.wait_limit));
         if (!ok) break;
 #pragma unroll
         for (int i = 0; i < NL; ++i)
@@ -786,8 +780,8 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
         }
         const uint32_t buf = it % kBufs, slot = it % kScaleSlots;
         const bool ok =
-            wait_or_abort(smem_addr(&sh.scale_full[slot]), (it / kScaleSlots) & 1u, abortp) &&
-            wait_or_abort(smem_addr(&sh.acc_full[buf]), (it / kBufs) & 1u, abortp);
+            tc::wait_or_abort(smem_addr(&sh.scale_full[slot]), (it / kScaleSlots) & 1u, abortp, g.wait_limit) &&
+            tc::wait_or_abort(smem_addr(&sh.acc_full[buf]), (it / kBufs) & 1u, abortp, g.wait_limit);
         if (__all_sync(0xffffffffu, ok)) {
           tc::fence_after();
           const float ws = sh.scales[slot][NMAX + half];
@@ -856,7 +850,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1)
     epi_sync();
     if (tid == 0) {
       barrier_arrive(g.barrier);
-      barrier_wait(g.barrier, down_target, abortp);
+      barrier_wait(g.barrier, down_target, abortp, g.wait_limit);
     }
     epi_sync();
     // ---- the weighted sum over a token's experts, four columns a thread

@@ -256,6 +256,20 @@ __device__ __forceinline__ void regs_down() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
+// ------------------------------------------------------------------ waits
+
+// Phase `parity` of an mbarrier has completed. Gives up after `limit` cycles (at
+// once for a negative one), or when the CTA's abort flag is set; giving up sets it.
+__device__ __forceinline__ bool wait_or_abort(uint32_t bar, uint32_t parity,
+                                              volatile uint32_t* abort_flag, long long limit) {
+  if (mbar_test(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (!*abort_flag && clock64() - t0 <= limit)
+    if (mbar_try_wait(bar, parity)) return true;
+  *abort_flag = 1u;
+  return false;
+}
+
 // ------------------------------------------------------------------ clusters
 
 // Pairs of CTAs (cta_group::2): the forms of the above for a kernel whose CTAs
