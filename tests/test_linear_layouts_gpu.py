@@ -101,3 +101,19 @@ def test_sizes_of_zero(M, N, K):
     assert y.shape == (M, N) and dx.shape == (M, K) and dw.shape == (N, K)
     for t in (y, dx, dw):
         assert bool((t == 0).all())
+
+
+@pytest.mark.parametrize("wdtype", [torch.bfloat16, torch.float32])
+def test_backward_holds_the_codes_that_it_reads(wdtype):
+    """Between the passes a layer holds x's and the weight's codes along their columns, a byte an
+    element and the scales, and nothing of the codes along the rows."""
+    M, N, K = 2048, 768, 1024
+    x, w = _matrix(M, K, seed=3).requires_grad_(), _matrix(N, K, seed=2, scale=0.02).to(wdtype).requires_grad_()
+    tb.fp8_linear(x, w).sum().backward()  # what the library keeps for itself is there
+    x.grad = w.grad = None
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    y = tb.fp8_linear(x, w)
+    held = torch.cuda.memory_allocated() - before
+    codes = K * M + 4 * K * (M // 128) + K * N + 4 * (K // 128) * (N // 128)
+    assert held <= y.numel() * 2 + codes + 3 * 512  # the allocator's rounding of three blocks

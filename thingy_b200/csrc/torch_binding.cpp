@@ -272,7 +272,7 @@ at::Tensor fp8_block_gemm(const at::Tensor& a, const at::Tensor& a_scale, const 
 
 // ---- A linear layer in 8 bits under autograd: y = q(x) q(w)^T, dx = q(dy) q(w),
 // dw = q(dy)^T q(x), x and dy in 1 x 128 groups along both axes, w in 128 x 128
-// blocks. In C++, and with a cast's four results in one buffer: as Python calls
+// blocks. In C++, and with the casts' results in few buffers: as Python calls
 // of the functions above a step took 150 us of host time, twice what the
 // kernels of a 1001 x 1544 x 2048 step take.
 
@@ -284,46 +284,52 @@ struct Operand {
   int64_t s_row = 0, s_kb = 0;
 };
 
-// A matrix's codes and its transpose's, in one buffer.
-struct CastBuffer {
+// Where a matrix's codes and scales go, and its transpose's: two places, since
+// backward reads the transpose's alone and holds nothing else.
+struct CastPlace {
   int64_t R, C;
   bool block, gradient;
-  at::Tensor hold;
-  int64_t off_s, off_qt, off_st, bytes;
+  int64_t off_s, row_bytes, off_st, column_bytes;
+  uint8_t *row_base = nullptr, *column_base = nullptr;
 
-  CastBuffer(int64_t rows, int64_t cols, bool blocks, bool of_gradient = false)
+  CastPlace(int64_t rows, int64_t cols, bool blocks, bool of_gradient = false)
       : R(rows), C(cols), block(blocks), gradient(of_gradient) {
     const int64_t GR = (R + 127) / 128, GC = (C + 127) / 128;
     off_s = ceil_to(R * ceil_to(C, 16), 256);
-    off_qt = off_s + ceil_to(4 * (block ? GR * GC : GC * R), 256);
-    off_st = off_qt + ceil_to(C * ceil_to(R, 16), 256);
-    bytes = off_st + 4 * (block ? GR * GC : GR * C);
+    row_bytes = off_s + ceil_to(4 * (block ? GR * GC : GC * R), 256);
+    off_st = ceil_to(C * ceil_to(R, 16), 256);
+    column_bytes = off_st + ceil_to(4 * (block ? GR * GC : GR * C), 256);
   }
-  uint8_t* base() const { return static_cast<uint8_t*>(hold.data_ptr()); }
   Operand rows() const {
-    return {base(), ceil_to(C, 16), base() + off_s, block ? (C + 127) / 128 : 1, block ? 1 : R};
+    return {row_base, ceil_to(C, 16), row_base + off_s, block ? (C + 127) / 128 : 1, block ? 1 : R};
   }
   Operand columns() const {
-    return {base() + off_qt, ceil_to(R, 16), base() + off_st, block ? (R + 127) / 128 : 1, block ? 1 : C};
+    return {column_base, ceil_to(R, 16), column_base + off_st, block ? (R + 127) / 128 : 1, block ? 1 : C};
   }
-  // A matrix whose rows are not dense, overlap or start off the 16-byte
-  // boundaries is copied first; that of a single row too: the kernel reads C
-  // neighbouring elements.
-  void cast(const at::Tensor& any, bool transposed, void* stream) {
+  // Without a place for the transpose's the block kind writes none. A matrix
+  // whose rows are not dense, overlap or start off the 16-byte boundaries is
+  // copied first; that of a single row too: the kernel reads C neighbouring
+  // elements.
+  void cast(const at::Tensor& any, void* stream) const {
+    if (R == 0 || C == 0) return;  // no codes
     const bool dense = (C <= 1 || any.stride(1) == 1) &&
                        (R <= 1 || (any.stride(0) >= C && any.stride(0) % 8 == 0)) &&
                        reinterpret_cast<uintptr_t>(any.data_ptr()) % 16 == 0;
     const at::Tensor x = dense ? any : any.clone(at::MemoryFormat::Contiguous);
-    hold = at::empty({transposed ? bytes : off_qt}, x.options().dtype(at::kByte));
-    if (R == 0 || C == 0) return;  // no codes
+    const Operand q = rows(), qt = column_base != nullptr ? columns() : Operand();
     check_status(cutie_cast_fp8_tiles(
         x.data_ptr(), R <= 1 ? ceil_to(C, 8) : x.stride(0), R, C,
         block ? CUTIE_TILE_BLOCK : CUTIE_TILE_TWO_WAY,
-        CUTIE_SCALE_FP32 + (gradient ? CUTIE_SCALE_GRADIENT : 0), base(), ceil_to(C, 16), base() + off_s, block ? (C + 127) / 128 : R, transposed ? base() + off_qt : nullptr,
-        transposed ? ceil_to(R, 16) : 0, transposed ? base() + off_st : nullptr,
-        transposed ? (block ? (R + 127) / 128 : C) : 0, stream));
+        CUTIE_SCALE_FP32 + (gradient ? CUTIE_SCALE_GRADIENT : 0), row_base, q.ld, row_base + off_s,
+        block ? q.s_row : q.s_kb, column_base, qt.ld,
+        column_base != nullptr ? column_base + off_st : nullptr, block ? qt.s_row : qt.s_kb, stream));
   }
 };
+
+at::Tensor bytes(int64_t n, const at::Tensor& like) {
+  return at::empty({n}, like.options().dtype(at::kByte));
+}
+uint8_t* address(const at::Tensor& t) { return static_cast<uint8_t*>(t.data_ptr()); }
 
 at::Tensor product(const Operand& a, const Operand& b, bool b_rows, int64_t M, int64_t N, int64_t K,
                    const at::Tensor& like, bool f32, void* stream) {
@@ -354,16 +360,24 @@ struct FP8Linear : public torch::autograd::Function<FP8Linear> {
     const int64_t M = x.size(0), K = x.size(1), N = weight.size(0);
     const c10::cuda::CUDAGuard guard(dev);
     void* stream = at::cuda::getCurrentCUDAStream(dev.index()).stream();
-    CastBuffer w(N, K, true), xs(M, K, false);
-    if (!wq.has_value())
-      w.cast(weight.scalar_type() == at::kBFloat16 ? weight : weight.to(at::kBFloat16), need_dx, stream);
-    xs.cast(x, true, stream);
-    at::Tensor y = product(xs.rows(), wq.has_value() ? given(*wq, *ws, N, K, dev) : w.rows(), false, M,
+    CastPlace w(N, K, true), xs(M, K, false);
+    const bool own = !wq.has_value();
+    const at::Tensor rows = bytes(xs.row_bytes + (own ? w.row_bytes : 0), x);
+    const at::Tensor x_columns = bytes(xs.column_bytes, x);
+    const at::Tensor w_columns = own && need_dx ? bytes(w.column_bytes, x) : at::Tensor();
+    xs.row_base = address(rows), xs.column_base = address(x_columns);
+    if (own) {
+      w.row_base = address(rows) + xs.row_bytes;
+      if (need_dx) w.column_base = address(w_columns);
+      w.cast(weight.scalar_type() == at::kBFloat16 ? weight : weight.to(at::kBFloat16), stream);
+    }
+    xs.cast(x, stream);
+    at::Tensor y = product(xs.rows(), own ? w.rows() : given(*wq, *ws, N, K, dev), false, M,
                            N, K, x, false, stream);
-    ctx->save_for_backward({need_dw ? xs.hold : at::Tensor(),
-                            !need_dx ? at::Tensor() : wq.has_value() ? *wqt : w.hold,
-                            need_dx && wq.has_value() ? *wst : at::Tensor()});
-    ctx->saved_data["sizes"] = std::vector<int64_t>{N, K, need_dx, need_dw, wq.has_value(),
+    ctx->save_for_backward({need_dw ? x_columns : at::Tensor(),
+                            own ? w_columns : need_dx ? *wqt : at::Tensor(),
+                            !own && need_dx ? *wst : at::Tensor()});
+    ctx->saved_data["sizes"] = std::vector<int64_t>{N, K, need_dx, need_dw, !own,
                                                     weight.scalar_type() == at::kFloat};
     return y;
   }
@@ -381,20 +395,22 @@ struct FP8Linear : public torch::autograd::Function<FP8Linear> {
     const at::Device dev = dy.device();
     const c10::cuda::CUDAGuard guard(dev);
     void* stream = at::cuda::getCurrentCUDAStream(dev.index()).stream();
-    CastBuffer d(M, N, false, true), w(N, K, true), xs(M, K, false);
-    d.cast(dy, true, stream);
+    CastPlace d(M, N, false, true), w(N, K, true), xs(M, K, false);
+    const at::Tensor codes = bytes(d.row_bytes + d.column_bytes, dy);
+    d.row_base = address(codes), d.column_base = address(codes) + d.row_bytes;
+    d.cast(dy, stream);
     if (sizes[2]) {
       Operand wt;
       if (sizes[4]) {
         wt = given(saved[1], saved[2], K, N, dev);
       } else {
-        w.hold = saved[1];
+        w.column_base = address(saved[1]);
         wt = w.columns();
       }
       out[0] = product(d.rows(), wt, false, M, K, N, dy, false, stream);
     }
     if (sizes[3]) {
-      xs.hold = saved[0];
+      xs.column_base = address(saved[0]);
       out[1] = product(d.columns(), xs.columns(), true, N, K, M, dy, sizes[5] != 0, stream);
     }
     return out;
