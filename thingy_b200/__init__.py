@@ -32,12 +32,13 @@ from .fused import empty_scale, residual_rms_norm_fp8, rms_norm_fp8
 from .gemm import fp8_block_gemm
 from .layouts import mx_swizzle, mx_swizzle_offset, mx_swizzled_size, mx_unswizzle
 from .linear import fp8_linear
-from .moe import moe_fp8, moe_workspace, quantize_experts
+from .moe import clear_moe_workspaces, moe_fp8, moe_workspace, quantize_experts
 from .rms_norm import RMSNorm, rms_norm, rms_norm_on_stream
 
 __all__ = [
     "RMSNorm",
     "ResidualRMSNormFP8",
+    "clear_moe_workspaces",
     "empty_scale",
     "fp8_block_gemm",
     "fp8_linear",

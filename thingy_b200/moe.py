@@ -46,6 +46,15 @@ def _own_workspace(x, E, top_k, H, I):
     return w
 
 
+def clear_moe_workspaces() -> None:
+    """Drop the workspaces that ``moe_fp8`` keeps, one a stream, for calls that were given none.
+
+    Each is a block of its stream's, so calls still running on the stream are safe. Also to be
+    called before a stream made outside torch is destroyed: another could get its handle.
+    """
+    _workspaces.clear()
+
+
 def moe_fp8(
     x: torch.Tensor,
     q: torch.Tensor,
@@ -84,7 +93,7 @@ def moe_fp8(
     fp32, rounded once to bf16. topk_ids (int32) and topk_weights (float32),
     [T, top_k], receive the choices. workspace: ``moe_workspace(...)``;
     without it the call uses one kept for the stream (a fresh one under graph
-    capture).
+    capture; ``clear_moe_workspaces`` drops them).
     """
     if scoring not in _SCORING:
         raise ValueError(f"scoring must be one of {tuple(_SCORING)}, got {scoring!r}")
