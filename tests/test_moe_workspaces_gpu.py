@@ -38,3 +38,12 @@ def test_kept_workspaces_can_be_dropped():
     assert torch.equal(tb.moe_fp8(*ops, top_k=2), want) and torch.equal(other, want)
     torch.cuda.synchronize()
     tb.clear_moe_workspaces()
+
+
+def test_result_carries_no_gradient():
+    ops = list(_layer())
+    want = tb.moe_fp8(*ops, top_k=2)
+    ops[0] = ops[0].clone().requires_grad_()
+    ops[3] = ops[3].clone().requires_grad_()
+    y = tb.moe_fp8(*ops, top_k=2)
+    assert not y.requires_grad and torch.equal(y, want)

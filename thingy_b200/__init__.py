@@ -19,7 +19,7 @@ Drop-in host API for the reference's hot path (S1ro1/thingy, package
                                                scale a block of 128, a linear layer with its
                                                gradients
     moe_fp8, quantize_experts               a mixture-of-experts layer for few tokens in one
-                                               kernel (no counterpart)
+                                               kernel, forward only (no counterpart)
 
 Every op runs hand-written CUDA from ``lib/libcutie_b200.so`` through the C
 ABI in ``include/cutie.h``; there is no CPU or PyTorch fallback.

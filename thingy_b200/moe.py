@@ -77,6 +77,9 @@ def moe_fp8(
 ) -> torch.Tensor:
     """bf16 [T, H]: router, top-k, the experts' gated MLPs and their weighted sum, T <= 64, on the current stream.
 
+    Forward only: the result carries no gradient, also of an x or router that
+    requires one.
+
     x: bf16 [T, H], the router's input; q, scale: x in e4m3 with 1 x 128 fp32
     scales, any layout (``rms_norm_fp8(..., return_normalized=True)`` gives all
     three). router: bf16 [E, H]; w13: e4m3 [E, 2 I, H] (an expert's gate rows,
