@@ -103,6 +103,11 @@ def test_sizes_of_zero(M, N, K):
         assert bool((t == 0).all())
 
 
+def _requested():
+    """Bytes asked of the allocator and not given back, without its own rounding to blocks."""
+    return torch.cuda.memory_stats()["requested_bytes.all.current"]
+
+
 @pytest.mark.parametrize("wdtype", [torch.bfloat16, torch.float32])
 def test_backward_holds_the_codes_that_it_reads(wdtype):
     """Between the passes a layer holds x's and the weight's codes along their columns, a byte an
@@ -112,8 +117,29 @@ def test_backward_holds_the_codes_that_it_reads(wdtype):
     tb.fp8_linear(x, w).sum().backward()  # what the library keeps for itself is there
     x.grad = w.grad = None
     torch.cuda.synchronize()
-    before = torch.cuda.memory_allocated()
+    before = _requested()
     y = tb.fp8_linear(x, w)
-    held = torch.cuda.memory_allocated() - before
+    held = _requested() - before
     codes = K * M + 4 * K * (M // 128) + K * N + 4 * (K // 128) * (N // 128)
-    assert held <= y.numel() * 2 + codes + 3 * 512  # the allocator's rounding of three blocks
+    assert held <= y.numel() * 2 + codes + 3 * 512  # the layer's own alignment of its parts
+
+
+@pytest.mark.parametrize("need_dx,need_dw,cached", [(True, False, False), (False, True, False), (True, True, True),
+                                                    (True, False, True), (False, False, False)])
+def test_backward_holds_no_more_than_its_gradients_need(need_dx, need_dw, cached):
+    M, N, K = 2048, 768, 1024
+    x, w = _matrix(M, K, seed=3).requires_grad_(need_dx), _matrix(N, K, seed=2, scale=0.02).requires_grad_(need_dw)
+    codes = tb.per_block_cast_to_fp8(w.detach(), transposed=True) if cached else None
+    dy = _matrix(M, N, seed=4, scale=0.1)
+    want = _step(x, w, dy)
+    torch.cuda.synchronize()
+    before = _requested()
+    y = tb.fp8_linear(x, w, codes)
+    held = _requested() - before
+    need = (K * M + 4 * K * (M // 128) if need_dw else 0) + (K * N + 4 * (K // 128) * (N // 128) if need_dx and not cached else 0)
+    assert held <= y.numel() * 2 + need + 3 * 512
+    wanted = [(t, g) for t, g, need_it in ((x, want[1], need_dx), (w, want[2], need_dw)) if need_it]
+    assert torch.equal(y, want[0])
+    if wanted:
+        for got, (_, ref) in zip(torch.autograd.grad(y, [t for t, _ in wanted], dy), wanted):
+            assert torch.equal(got, ref)

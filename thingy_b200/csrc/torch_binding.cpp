@@ -329,7 +329,9 @@ struct CastPlace {
 at::Tensor bytes(int64_t n, const at::Tensor& like) {
   return at::empty({n}, like.options().dtype(at::kByte));
 }
-uint8_t* address(const at::Tensor& t) { return static_cast<uint8_t*>(t.data_ptr()); }
+uint8_t* address(const at::Tensor& t) {
+  return t.defined() ? static_cast<uint8_t*>(t.data_ptr()) : nullptr;
+}
 
 at::Tensor product(const Operand& a, const Operand& b, bool b_rows, int64_t M, int64_t N, int64_t K,
                    const at::Tensor& like, bool f32, void* stream) {
@@ -362,21 +364,25 @@ struct FP8Linear : public torch::autograd::Function<FP8Linear> {
     void* stream = at::cuda::getCurrentCUDAStream(dev.index()).stream();
     CastPlace w(N, K, true), xs(M, K, false);
     const bool own = !wq.has_value();
-    const at::Tensor rows = bytes(xs.row_bytes + (own ? w.row_bytes : 0), x);
-    const at::Tensor x_columns = bytes(xs.column_bytes, x);
-    const at::Tensor w_columns = own && need_dx ? bytes(w.column_bytes, x) : at::Tensor();
-    xs.row_base = address(rows), xs.column_base = address(x_columns);
+    // what backward reads: the weight's transposed codes, then x's; the rest goes with this call
+    const int64_t held_w = own && need_dx ? w.column_bytes : 0, held_x = need_dw ? xs.column_bytes : 0;
+    const at::Tensor held = held_w + held_x > 0 ? bytes(held_w + held_x, x) : at::Tensor();
+    const at::Tensor scratch =
+        bytes(xs.row_bytes + (own ? w.row_bytes : 0) + (need_dw ? 0 : xs.column_bytes), x);
+    xs.row_base = address(scratch);
     if (own) {
-      w.row_base = address(rows) + xs.row_bytes;
-      if (need_dx) w.column_base = address(w_columns);
+      w.row_base = xs.row_base + xs.row_bytes;
+      if (held_w > 0) w.column_base = address(held);
       w.cast(weight.scalar_type() == at::kBFloat16 ? weight : weight.to(at::kBFloat16), stream);
     }
+    // the two-way cast always writes both
+    if (held_x > 0) xs.column_base = address(held) + held_w;
+    else xs.column_base = xs.row_base + xs.row_bytes + (own ? w.row_bytes : 0);
     xs.cast(x, stream);
     at::Tensor y = product(xs.rows(), own ? w.rows() : given(*wq, *ws, N, K, dev), false, M,
                            N, K, x, false, stream);
-    ctx->save_for_backward({need_dw ? x_columns : at::Tensor(),
-                            own ? w_columns : need_dx ? *wqt : at::Tensor(),
-                            !own && need_dx ? *wst : at::Tensor()});
+    ctx->save_for_backward(
+        {held, !own && need_dx ? *wqt : at::Tensor(), !own && need_dx ? *wst : at::Tensor()});
     ctx->saved_data["sizes"] = std::vector<int64_t>{N, K, need_dx, need_dw, !own,
                                                     weight.scalar_type() == at::kFloat};
     return y;
@@ -404,13 +410,13 @@ struct FP8Linear : public torch::autograd::Function<FP8Linear> {
       if (sizes[4]) {
         wt = given(saved[1], saved[2], K, N, dev);
       } else {
-        w.column_base = address(saved[1]);
+        w.column_base = address(saved[0]);
         wt = w.columns();
       }
       out[0] = product(d.rows(), wt, false, M, K, N, dy, false, stream);
     }
     if (sizes[3]) {
-      xs.column_base = address(saved[0]);
+      xs.column_base = address(saved[0]) + (sizes[2] && !sizes[4] ? w.column_bytes : 0);
       out[1] = product(d.columns(), xs.columns(), true, N, K, M, dy, sizes[5] != 0, stream);
     }
     return out;
