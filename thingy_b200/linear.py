@@ -18,7 +18,8 @@ from .ops import require_binding
 def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_fp8=None) -> torch.Tensor:
     """``x @ weight.T`` on e4m3 codes with fp32 sums, bf16 out, differentiable in x and weight.
 
-    x: bf16 [..., K]; weight: bf16 or fp32 [N, K]; K and N multiples of 8.
+    x: bf16 [..., K]; weight: bf16 or fp32 [N, K] (fp32 is rounded to bf16
+    first, then to e4m3); K and N multiples of 8.
     Both, and y's gradient, may have any strides; a matrix whose rows are not
     dense and on 16-byte boundaries is copied first.
     ``weight_fp8``: (q, s, qt, st) of ``per_block_cast_to_fp8(weight,
