@@ -142,3 +142,14 @@ def test_gradient_cast_of_nonfinite_values():
     assert torch.isnan(q[1, 3]) and torch.isnan(qt[3, 1]) and torch.isinf(s[5, 1]) and torch.isinf(st[200, 0])
     assert torch.isnan(q[5, 128:]).all() and torch.isnan(qt[200, :128]).all()
     assert int(torch.isnan(q).sum()) == 129 and int(torch.isnan(qt).sum()) == 129
+
+
+def test_library_op_of_the_gradient_cast():
+    import thingy_b200.custom_ops  # noqa: F401
+
+    x = (1e-7 * _normal(40, 264, 5)).to(torch.bfloat16).cuda()
+    op = torch.ops.thingy_b200.two_way_cast_to_fp8
+    for gradient, got in ((True, op(x, False, True)), (False, op(x, False))):
+        for a, b in zip(got, tb.two_way_cast_to_fp8(x, gradient=gradient)):
+            assert a.stride() == b.stride() and torch.equal(a.float(), b.float())
+    torch.library.opcheck(op, (x, False, True), test_utils="test_faketensor")
