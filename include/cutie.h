@@ -95,6 +95,7 @@ enum cutie_scale_layout {
 enum cutie_dtype {
   CUTIE_DTYPE_BF16 = 0,
   CUTIE_DTYPE_F32 = 1,
+  CUTIE_DTYPE_F16 = 2, /* moe rows and optimizer only */
 };
 
 /*
@@ -372,6 +373,59 @@ CUTIE_API int cutie_moe_fp8(const void* x, int64_t ldx, const void* q, int64_t l
                             int scoring, int renormalize, float routed_scale, void* out,
                             int64_t ldo, void* topk_ids, void* topk_weights, void* workspace,
                             size_t workspace_bytes, void* stream);
+
+/*
+ * Tokens sorted by expert: the plan by which rows go to experts and back.
+ * ids: int32 or int64 (wide) [T, k], contiguous: the experts that each token
+ * takes; an id outside [0, E) is an absent choice (dropped, or another rank's).
+ * Choices are sorted by expert, those of one expert in the order t k + j;
+ * every expert's rows begin at a multiple of `align` (fp8 products: 128).
+ *   sources[r]      = t k + j of sorted row r, -1 in padding       int32 [R]
+ *   positions[t, j] = its sorted row, -1 where absent              int32 [T, k]
+ *   offsets[e]      = where expert e's rows begin; offsets[E] ends int32 [E + 1]
+ *   counts[e]       = its rows, without padding                    int32 [E]
+ * R >= cutie_moe_plan_rows(T, k, E, align), the most rows that any ids need;
+ * sources behind offsets[E] are -1. 1 <= E <= 512, 1 <= align <= 65536, k >= 1,
+ * T k <= 2^30, R < 2^31. workspace: cutie_moe_sort_workspace(T, k, E) bytes, 4-byte
+ * aligned (0: NULL will do). Asynchronous on `stream`; nothing is allocated.
+ */
+CUTIE_API int64_t cutie_moe_plan_rows(int64_t T, int64_t k, int64_t E, int64_t align);
+CUTIE_API size_t cutie_moe_sort_workspace(int64_t T, int64_t k, int64_t E);
+CUTIE_API int cutie_moe_sort(const void* ids, int wide, int64_t T, int64_t k, int64_t E,
+                             int64_t align, void* sources, int64_t R, void* positions,
+                             void* offsets, void* counts, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
+/*
+ * Rows to their experts: out[r] = x[sources[r] / k], zeros where sources[r]
+ * is -1. x: [T, H], out: [R, H] of elements of element_bytes (1, 2, 4; codes
+ * and scales too), leading dimensions in elements. The gradient of it is
+ * cutie_moe_combine without weights.
+ */
+CUTIE_API int cutie_moe_permute(const void* x, int64_t ldx, int element_bytes, int64_t T,
+                                int64_t H, int64_t k, const void* positions, const void* sources,
+                                int64_t R, void* out, int64_t ldo, void* stream);
+
+/*
+ * Rows back to their tokens: out[t] = sum_j weights[t, j] rows[positions[t, j]],
+ * absent choices left out; weights: fp32 [T, k] or NULL (all one). rows: [R, H],
+ * out: [T, H], dtype CUTIE_DTYPE_*; sums in fp32 in the order of j, rounded once.
+ */
+CUTIE_API int cutie_moe_combine(const void* rows, int64_t ldr, int dtype, const void* weights,
+                                const void* positions, int64_t T, int64_t k, int64_t H,
+                                int64_t R, void* out, int64_t ldo, void* stream);
+
+/*
+ * Its gradients: d_rows[positions[t, j]] = weights[t, j] d_out[t], zeros where
+ * sources[r] is -1; d_weights[t, j] = <d_out[t], rows[positions[t, j]]> in fp32,
+ * 0 for absent choices. Either of d_rows and d_weights may be NULL; rows may be
+ * NULL without d_weights.
+ */
+CUTIE_API int cutie_moe_combine_backward(const void* d_out, int64_t ldd, const void* rows,
+                                         int64_t ldr, int dtype, const void* weights,
+                                         const void* positions, const void* sources, int64_t T,
+                                         int64_t k, int64_t H, int64_t R, void* d_rows,
+                                         int64_t lddr, void* d_weights, void* stream);
 
 /*
  * Device-side status of this library's kernels on the current device: 0 when

@@ -20,12 +20,15 @@ Drop-in host API for the reference's hot path (S1ro1/thingy, package
                                                gradients
     moe_fp8, quantize_experts               a mixture-of-experts layer for few tokens in one
                                                kernel, forward only (no counterpart)
+    moe_sort, moe_permute, moe_combine      tokens sorted by expert and back, with weights
+                                               applied, and the gradients (no counterpart)
 
 Every op runs hand-written CUDA from ``lib/libcutie_b200.so`` through the C
 ABI in ``include/cutie.h``; there is no CPU or PyTorch fallback.
 """
 
 from .backward import ResidualRMSNormFP8, rms_norm_fp8_backward
+from .dispatch import MoePlan, moe_combine, moe_permute, moe_plan_rows, moe_sort
 from .fp8_utils import (per_block_cast_to_fp8, per_token_cast_to_fp8, per_token_cast_to_fp8_triton,
                         two_way_cast_to_fp8)
 from .fused import empty_scale, residual_rms_norm_fp8, rms_norm_fp8
@@ -36,13 +39,18 @@ from .moe import clear_moe_workspaces, moe_fp8, moe_workspace, quantize_experts
 from .rms_norm import RMSNorm, rms_norm, rms_norm_on_stream
 
 __all__ = [
+    "MoePlan",
     "RMSNorm",
     "ResidualRMSNormFP8",
     "clear_moe_workspaces",
     "empty_scale",
     "fp8_block_gemm",
     "fp8_linear",
+    "moe_combine",
     "moe_fp8",
+    "moe_permute",
+    "moe_plan_rows",
+    "moe_sort",
     "moe_workspace",
     "mx_swizzle",
     "mx_swizzle_offset",

@@ -24,7 +24,7 @@ ERR_CUDA = -4
 QUANT_NONE, QUANT_TOKEN, QUANT_GROUP = 0, 1, 2
 SCALE_FP32, SCALE_FP32_POW2, SCALE_E8M0 = 0, 1, 2
 LAYOUT_ROW_MAJOR, LAYOUT_COL_MAJOR, LAYOUT_MX_SWIZZLED, LAYOUT_COL_MAJOR_PACKED = 0, 1, 2, 3
-DTYPE_BF16, DTYPE_F32 = 0, 1
+DTYPE_BF16, DTYPE_F32, DTYPE_F16 = 0, 1, 2
 TILE_BLOCK, TILE_TWO_WAY = 0, 1
 SCALE_GRADIENT = 16
 SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
@@ -44,6 +44,12 @@ EXPORTED_SYMBOLS = (
     "cutie_fp8_block_gemm",
     "cutie_moe_fp8",
     "cutie_moe_fp8_workspace",
+    "cutie_moe_plan_rows",
+    "cutie_moe_sort_workspace",
+    "cutie_moe_sort",
+    "cutie_moe_permute",
+    "cutie_moe_combine",
+    "cutie_moe_combine_backward",
     "cutie_device_error",
     "cutie_set_wait_limit",
     "cutie_last_error",
@@ -103,6 +109,22 @@ _SIGNATURES = {
         [_ptr, _i64, _ptr, _i64, _ptr, _i64, _i64, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr,
          _i64, _i64, _i64, _i64, _i64, _int, _int, _f32, _ptr, _i64, _ptr, _ptr, _ptr,
          ctypes.c_size_t, _ptr],
+    ),
+    "cutie_moe_plan_rows": (_i64, [_i64, _i64, _i64, _i64]),
+    "cutie_moe_sort_workspace": (ctypes.c_size_t, [_i64, _i64, _i64]),
+    "cutie_moe_sort": (
+        _int,
+        [_ptr, _int, _i64, _i64, _i64, _i64, _ptr, _i64, _ptr, _ptr, _ptr, _ptr, ctypes.c_size_t, _ptr],
+    ),
+    "cutie_moe_permute": (
+        _int, [_ptr, _i64, _int, _i64, _i64, _i64, _ptr, _ptr, _i64, _ptr, _i64, _ptr],
+    ),
+    "cutie_moe_combine": (
+        _int, [_ptr, _i64, _int, _ptr, _ptr, _i64, _i64, _i64, _i64, _ptr, _i64, _ptr],
+    ),
+    "cutie_moe_combine_backward": (
+        _int,
+        [_ptr, _i64, _ptr, _i64, _int, _ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _ptr, _i64, _ptr, _ptr],
     ),
     "cutie_device_error": (_int, [_int]),
     "cutie_set_wait_limit": (_i64, [_i64]),

@@ -988,6 +988,164 @@ extern "C" int cutie_moe_fp8(const void* x, int64_t ldx, const void* q, int64_t 
   return CUTIE_OK;
 }
 
+namespace cutie {
+namespace {
+
+constexpr int64_t kMaxChoices = int64_t(1) << 30, kMaxAlign = 65536;
+
+// A plan's sizes; *rows: the rows that any ids may need (-1 and a message where the sizes are refused).
+int check_plan(int64_t T, int64_t k, int64_t E, int64_t align, int64_t* rows) {
+  *rows = -1;
+  if (T < 0 || k <= 0 || E <= 0 || align <= 0)
+    return fail(CUTIE_ERR_INVALID_ARGUMENT, "need T >= 0 and k, E, align > 0 (got %lld, %lld, %lld, %lld)",
+                (long long)T, (long long)k, (long long)E, (long long)align);
+  if (E > kMoeMaxExperts)
+    return fail(CUTIE_ERR_UNSUPPORTED, "at most %d experts (got %lld)", kMoeMaxExperts, (long long)E);
+  if (align > kMaxAlign)
+    return fail(CUTIE_ERR_UNSUPPORTED, "align must be at most %lld (got %lld)", (long long)kMaxAlign,
+                (long long)align);
+  if (T > kMaxChoices / k) return fail(CUTIE_ERR_UNSUPPORTED, "T k must be at most 2^30");
+  const int64_t n = T * k, some = E < n ? E : n;
+  const int64_t need = (n + some * (align - 1)) / align * align;
+  if (need > INT32_MAX - 256) return fail(CUTIE_ERR_UNSUPPORTED, "the sorted rows must be below 2^31 - 256");
+  *rows = need;
+  return CUTIE_OK;
+}
+
+// A plan's arrays as the row kernels take them.
+int check_rows(MoeRows* p, const void* positions, const void* sources, bool need_sources, int64_t T, int64_t k,
+               int64_t H, int64_t R, int element_bytes) {
+  if (T < 0 || k <= 0 || H <= 0 || R < 0)
+    return fail(CUTIE_ERR_INVALID_ARGUMENT, "need T, R >= 0 and k, H > 0 (got %lld, %lld, %lld, %lld)",
+                (long long)T, (long long)R, (long long)k, (long long)H);
+  if (T > kMaxChoices / k || R > INT32_MAX - 256 || H > (1 << 24))
+    return fail(CUTIE_ERR_UNSUPPORTED, "T k must be at most 2^30, R below 2^31 - 256, H at most 2^24");
+  if ((T > 0 && positions == nullptr) || (need_sources && R > 0 && sources == nullptr))
+    return fail(CUTIE_ERR_INVALID_ARGUMENT, "the plan's arrays must not be NULL");
+  if (!aligned(positions, 4) || !aligned(sources, 4))
+    return fail(CUTIE_ERR_ALIGNMENT, "the plan's arrays must be 4-byte aligned");
+  *p = MoeRows{};
+  p->positions = static_cast<const int*>(positions);
+  p->sources = static_cast<const int*>(sources);
+  p->T = (int)T, p->k = (int)k, p->R = (int)R;
+  p->row_bytes = H * element_bytes;
+  return CUTIE_OK;
+}
+
+int row_dtype_bytes(int dtype) {
+  return dtype == CUTIE_DTYPE_F32 ? 4 : dtype == CUTIE_DTYPE_BF16 || dtype == CUTIE_DTYPE_F16 ? 2 : 0;
+}
+
+}  // namespace
+}  // namespace cutie
+
+extern "C" int64_t cutie_moe_plan_rows(int64_t T, int64_t k, int64_t E, int64_t align) {
+  g_err[0] = '\0';
+  int64_t rows;
+  check_plan(T, k, E, align, &rows);
+  return rows;
+}
+
+extern "C" size_t cutie_moe_sort_workspace(int64_t T, int64_t k, int64_t E) {
+  g_err[0] = '\0';
+  int64_t rows;
+  return check_plan(T, k, E, 1, &rows) == CUTIE_OK ? moe_sort_workspace(T * k, E) : 0;
+}
+
+extern "C" int cutie_moe_sort(const void* ids, int wide, int64_t T, int64_t k, int64_t E, int64_t align,
+                              void* sources, int64_t R, void* positions, void* offsets, void* counts,
+                              void* workspace, size_t workspace_bytes, void* stream) {
+  g_err[0] = '\0';
+  int64_t need;
+  const int rc = check_plan(T, k, E, align, &need);
+  if (rc != CUTIE_OK) return rc;
+  if (R < need || R > INT32_MAX - 256)
+    return fail(CUTIE_ERR_INVALID_ARGUMENT, "the plan needs from %lld to 2^31 - 256 rows (got %lld)",
+                (long long)need, (long long)R);
+  if (offsets == nullptr || counts == nullptr || (T > 0 && (ids == nullptr || positions == nullptr)) ||
+      (R > 0 && sources == nullptr))
+    return fail(CUTIE_ERR_INVALID_ARGUMENT, "ids and the plan's arrays must not be NULL");
+  if (!aligned(ids, wide ? 8 : 4) || !aligned(sources, 4) || !aligned(positions, 4) || !aligned(offsets, 4) ||
+      !aligned(counts, 4) || !aligned(workspace, 4))
+    return fail(CUTIE_ERR_ALIGNMENT, "ids and the plan's arrays must be aligned to their elements");
+  const size_t bytes = moe_sort_workspace(T * k, E);
+  if (bytes > 0 && (workspace == nullptr || workspace_bytes < bytes))
+    return fail(CUTIE_ERR_INVALID_ARGUMENT, "the sort needs a workspace of %zu bytes (got %zu at %p)", bytes,
+                workspace_bytes, workspace);
+  const cudaError_t e =
+      moe_sort(ids, wide != 0, (int)(T * k), (int)E, (int)align, static_cast<int*>(sources), (int)R,
+               static_cast<int*>(positions), static_cast<int*>(offsets), static_cast<int*>(counts), workspace,
+               static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? CUTIE_OK : cuda_fail(e, "moe sort launch");
+}
+
+extern "C" int cutie_moe_permute(const void* x, int64_t ldx, int element_bytes, int64_t T, int64_t H, int64_t k,
+                                 const void* positions, const void* sources, int64_t R, void* out, int64_t ldo,
+                                 void* stream) {
+  g_err[0] = '\0';
+  if (element_bytes != 1 && element_bytes != 2 && element_bytes != 4)
+    return fail(CUTIE_ERR_UNSUPPORTED, "elements have 1, 2 or 4 bytes (got %d)", element_bytes);
+  MoeRows p;
+  int rc = check_rows(&p, positions, sources, true, T, k, H, R, element_bytes);
+  if (rc != CUTIE_OK) return rc;
+  if (R == 0) return CUTIE_OK;
+  if (T > 0 && (rc = check_matrix("x", x, ldx, H, element_bytes, 1)) != CUTIE_OK) return rc;
+  if ((rc = check_matrix("out", out, ldo, H, element_bytes, 1)) != CUTIE_OK) return rc;
+  p.x = x, p.ldx = ldx * element_bytes;
+  p.out = out, p.ldo = ldo * element_bytes;
+  const cudaError_t e = moe_permute(p, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? CUTIE_OK : cuda_fail(e, "moe permute launch");
+}
+
+extern "C" int cutie_moe_combine(const void* rows, int64_t ldr, int dtype, const void* weights,
+                                 const void* positions, int64_t T, int64_t k, int64_t H, int64_t R, void* out,
+                                 int64_t ldo, void* stream) {
+  g_err[0] = '\0';
+  const int es = row_dtype_bytes(dtype);
+  if (es == 0) return fail(CUTIE_ERR_INVALID_ARGUMENT, "unknown dtype %d", dtype);
+  MoeRows p;
+  int rc = check_rows(&p, positions, nullptr, false, T, k, H, R, es);
+  if (rc != CUTIE_OK) return rc;
+  if (T == 0) return CUTIE_OK;
+  if (R > 0 && (rc = check_matrix("rows", rows, ldr, H, es, 1)) != CUTIE_OK) return rc;
+  if ((rc = check_matrix("out", out, ldo, H, es, 1)) != CUTIE_OK) return rc;
+  if (!aligned(weights, 4)) return fail(CUTIE_ERR_ALIGNMENT, "weights must be 4-byte aligned");
+  p.x = rows, p.ldx = ldr * es;
+  p.out = out, p.ldo = ldo * es;
+  p.w = static_cast<const float*>(weights);
+  const cudaError_t e = moe_combine(p, dtype, false, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? CUTIE_OK : cuda_fail(e, "moe combine launch");
+}
+
+extern "C" int cutie_moe_combine_backward(const void* d_out, int64_t ldd, const void* rows, int64_t ldr, int dtype,
+                                          const void* weights, const void* positions, const void* sources,
+                                          int64_t T, int64_t k, int64_t H, int64_t R, void* d_rows, int64_t lddr,
+                                          void* d_weights, void* stream) {
+  g_err[0] = '\0';
+  const int es = row_dtype_bytes(dtype);
+  if (es == 0) return fail(CUTIE_ERR_INVALID_ARGUMENT, "unknown dtype %d", dtype);
+  MoeRows p;
+  int rc = check_rows(&p, positions, sources, d_rows != nullptr, T, k, H, R, es);
+  if (rc != CUTIE_OK) return rc;
+  if (d_rows == nullptr && d_weights == nullptr) return CUTIE_OK;
+  if (T > 0) {
+    if ((rc = check_matrix("d_out", d_out, ldd, H, es, 1)) != CUTIE_OK) return rc;
+    if (weights == nullptr) return fail(CUTIE_ERR_INVALID_ARGUMENT, "weights is NULL");
+    if (R > 0 && d_weights != nullptr && (rc = check_matrix("rows", rows, ldr, H, es, 1)) != CUTIE_OK) return rc;
+  }
+  if (!aligned(weights, 4) || !aligned(d_weights, 4))
+    return fail(CUTIE_ERR_ALIGNMENT, "weights and d_weights must be 4-byte aligned");
+  if (R > 0 && d_rows != nullptr && (rc = check_matrix("d_rows", d_rows, lddr, H, es, 1)) != CUTIE_OK) return rc;
+  if (T == 0 && (R == 0 || d_rows == nullptr)) return CUTIE_OK;
+  p.dy = d_out, p.lddy = ldd * es;
+  if (d_weights != nullptr) p.x = rows, p.ldx = ldr * es;
+  if (R > 0 && d_rows != nullptr) p.out = d_rows, p.ldo = lddr * es;
+  p.w = static_cast<const float*>(weights);
+  p.dw = static_cast<float*>(d_weights);
+  const cudaError_t e = moe_combine(p, dtype, true, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? CUTIE_OK : cuda_fail(e, "moe combine backward launch");
+}
+
 extern "C" int cutie_device_error(int clear) {
   g_err[0] = '\0';
   int any = 0;

@@ -394,6 +394,26 @@ int moe_fp8(MoeArgs g, const void* q, int64_t ldq, const void* w13, const void* 
             cudaStream_t stream, const char** why);
 cudaError_t device_error_moe(int* out, bool clear);
 
+// Tokens sorted by expert and back (moe_dispatch.cu). Strides in bytes.
+struct MoeRows {
+  const void* x;  // rows that are read: permute [T], combine [R], backward [R] or null
+  int64_t ldx;
+  const void* dy;  // backward: [T]
+  int64_t lddy;
+  void* out;  // permute [R], combine [T], backward [R] or null
+  int64_t ldo;
+  int64_t row_bytes;
+  const float* w;  // [T, k]; combine: or null
+  float* dw;       // backward: [T, k] or null
+  const int *positions, *sources;
+  int T, k, R;
+};
+size_t moe_sort_workspace(int64_t n, int64_t E);
+cudaError_t moe_sort(const void* ids, bool wide, int n, int E, int align, int* sources, int R, int* positions,
+                     int* offsets, int* counts, void* workspace, cudaStream_t stream);
+cudaError_t moe_permute(const MoeRows& p, cudaStream_t stream);
+cudaError_t moe_combine(const MoeRows& p, int dtype, bool backward, cudaStream_t stream);
+
 struct F32Args {
   const float* x;
   int64_t ldx;

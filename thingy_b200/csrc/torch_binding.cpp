@@ -524,6 +524,170 @@ at::Tensor moe_fp8(const at::Tensor& x, const at::Tensor& q, const at::Tensor& q
   return y;
 }
 
+// ---- Tokens sorted by expert and back (cutie_moe_sort, _permute, _combine).
+
+int row_dtype(const at::Tensor& t, const char* name) {
+  switch (t.scalar_type()) {
+    case at::kBFloat16: return CUTIE_DTYPE_BF16;
+    case at::kFloat: return CUTIE_DTYPE_F32;
+    case at::kHalf: return CUTIE_DTYPE_F16;
+    default: bad(std::string(name) + " must be bfloat16, float16 or float32");
+  }
+}
+
+void plan_array(const at::Tensor& t, const char* name, int64_t dims, const at::Device& dev) {
+  if (t.dim() != dims || t.scalar_type() != at::kInt || !t.is_contiguous())
+    bad(std::string("the plan's ") + name + " must be a contiguous int32 tensor of " + std::to_string(dims) +
+        " dimensions");
+  if (t.device() != dev) bad(std::string("the plan's ") + name + " is on the wrong device");
+}
+
+// A matrix whose rows are dense and do not overlap: the tensor, or a copy.
+at::Tensor dense_rows(const at::Tensor& t) {
+  const bool dense = (t.size(1) <= 1 || t.stride(1) == 1) && (t.size(0) <= 1 || t.stride(0) >= t.size(1));
+  return dense ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+int64_t row_stride(const at::Tensor& t) { return t.size(0) <= 1 ? t.size(1) : t.stride(0); }
+
+int64_t moe_plan_rows(int64_t T, int64_t k, int64_t E, int64_t align) {
+  const int64_t rows = cutie_moe_plan_rows(T, k, E, align);
+  if (rows < 0) bad(cutie_last_error());
+  return rows;
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> moe_sort(const at::Tensor& any, int64_t E,
+                                                                    int64_t align) {
+  if (any.dim() != 2 || !any.is_cuda()) bad("topk_ids must be a 2-D CUDA tensor (this library has no CPU path)");
+  if (any.scalar_type() != at::kInt && any.scalar_type() != at::kLong) bad("topk_ids must be int32 or int64");
+  const int64_t T = any.size(0), k = any.size(1), R = moe_plan_rows(T, k, E, align);
+  const at::Device dev = any.device();
+  const c10::cuda::CUDAGuard guard(dev);
+  const at::Tensor ids = any.contiguous();
+  const auto opt = at::TensorOptions().device(dev).dtype(at::kInt);
+  at::Tensor sources = at::empty({R}, opt), positions = at::empty({T, k}, opt);
+  at::Tensor offsets = at::empty({E + 1}, opt), counts = at::empty({E}, opt);
+  const size_t bytes = cutie_moe_sort_workspace(T, k, E);
+  const at::Tensor workspace = bytes > 0 ? at::empty({(int64_t)bytes}, opt.dtype(at::kByte)) : at::Tensor();
+  check_status(cutie_moe_sort(ids.data_ptr(), ids.scalar_type() == at::kLong ? 1 : 0, T, k, E, align,
+                              sources.data_ptr(), R, positions.data_ptr(), offsets.data_ptr(), counts.data_ptr(),
+                              bytes > 0 ? workspace.data_ptr() : nullptr, bytes,
+                              at::cuda::getCurrentCUDAStream(dev.index()).stream()));
+  return {sources, positions, offsets, counts};
+}
+
+at::Tensor permute_rows(const at::Tensor& any, const at::Tensor& sources, const at::Tensor& positions) {
+  const at::Tensor x = dense_rows(any);
+  const int64_t H = x.size(1), R = sources.size(0);
+  at::Tensor out = at::empty({R, H}, x.options());
+  check_status(cutie_moe_permute(x.data_ptr(), row_stride(x), (int)x.element_size(), x.size(0), H,
+                                 positions.size(1), positions.data_ptr(), sources.data_ptr(), R, out.data_ptr(), H,
+                                 at::cuda::getCurrentCUDAStream(x.device().index()).stream()));
+  return out;
+}
+
+at::Tensor combine_rows(const at::Tensor& any, const at::Tensor& weights, const at::Tensor& positions) {
+  const at::Tensor ys = dense_rows(any);
+  const int64_t H = ys.size(1), T = positions.size(0);
+  at::Tensor out = at::empty({T, H}, ys.options());
+  check_status(cutie_moe_combine(ys.data_ptr(), row_stride(ys), row_dtype(ys, "rows"),
+                                 weights.defined() ? weights.data_ptr() : nullptr, positions.data_ptr(), T,
+                                 positions.size(1), H, ys.size(0), out.data_ptr(), H,
+                                 at::cuda::getCurrentCUDAStream(ys.device().index()).stream()));
+  return out;
+}
+
+void no_second_derivatives(const char* name) {
+  if (at::GradMode::is_enabled())
+    throw std::runtime_error(std::string(name) + " has no second derivatives (create_graph)");
+}
+
+struct MoePermute : public torch::autograd::Function<MoePermute> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& sources,
+                            const at::Tensor& positions) {
+    const c10::cuda::CUDAGuard guard(x.device());
+    ctx->save_for_backward({positions});
+    return permute_rows(x, sources, positions);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    no_second_derivatives("moe_permute");
+    torch::autograd::variable_list out(3);
+    if (!grads[0].defined()) return out;
+    const c10::cuda::CUDAGuard guard(grads[0].device());
+    out[0] = combine_rows(grads[0], at::Tensor(), ctx->get_saved_variables()[0]);
+    return out;
+  }
+};
+
+at::Tensor moe_permute(const at::Tensor& x, const at::Tensor& sources, const at::Tensor& positions) {
+  if (x.dim() != 2 || !x.is_cuda()) bad("x must be a 2-D CUDA tensor (this library has no CPU path)");
+  const int64_t es = x.element_size();
+  if (x.is_complex() || (es != 1 && es != 2 && es != 4)) bad("x must have elements of 1, 2 or 4 bytes");
+  plan_array(sources, "sources", 1, x.device());
+  plan_array(positions, "positions", 2, x.device());
+  if (positions.size(0) != x.size(0))
+    bad("x must have a row for each of the plan's " + std::to_string(positions.size(0)) + " tokens");
+  if (at::GradMode::is_enabled() && x.requires_grad()) {
+    row_dtype(x, "x with a gradient");
+    return MoePermute::apply(x, sources, positions);
+  }
+  const c10::cuda::CUDAGuard guard(x.device());
+  return permute_rows(x, sources, positions);
+}
+
+struct MoeCombine : public torch::autograd::Function<MoeCombine> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& ys, const at::Tensor& weights,
+                            const at::Tensor& sources, const at::Tensor& positions, bool need_rows,
+                            bool need_weights) {
+    const c10::cuda::CUDAGuard guard(ys.device());
+    const at::Tensor w = weights.contiguous();
+    ctx->save_for_backward({need_weights ? ys : at::Tensor(), w, sources, positions});
+    ctx->saved_data["rows"] = need_rows;
+    return combine_rows(ys, w, positions);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    no_second_derivatives("moe_combine");
+    torch::autograd::variable_list out(6);
+    if (!grads[0].defined()) return out;
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &w = saved[1], &sources = saved[2], &positions = saved[3];
+    const at::Device dev = grads[0].device();
+    const c10::cuda::CUDAGuard guard(dev);
+    const at::Tensor dy = dense_rows(grads[0]);
+    const int64_t H = dy.size(1), R = sources.size(0);
+    const at::Tensor ys = saved[0].defined() ? dense_rows(saved[0]) : at::Tensor();
+    if (ctx->saved_data["rows"].toBool()) out[0] = at::empty({R, H}, dy.options());
+    if (ys.defined()) out[1] = at::empty_like(w);
+    check_status(cutie_moe_combine_backward(
+        dy.data_ptr(), row_stride(dy), ys.defined() ? ys.data_ptr() : nullptr, ys.defined() ? row_stride(ys) : 0,
+        row_dtype(dy, "the gradient"), w.data_ptr(), positions.data_ptr(), sources.data_ptr(), dy.size(0),
+        positions.size(1), H, R, out[0].defined() ? out[0].data_ptr() : nullptr, H,
+        out[1].defined() ? out[1].data_ptr() : nullptr, at::cuda::getCurrentCUDAStream(dev.index()).stream()));
+    return out;
+  }
+};
+
+at::Tensor moe_combine(const at::Tensor& ys, const at::Tensor& weights, const at::Tensor& sources,
+                       const at::Tensor& positions) {
+  if (ys.dim() != 2 || !ys.is_cuda()) bad("rows must be a 2-D CUDA tensor (this library has no CPU path)");
+  row_dtype(ys, "rows");
+  if (ys.size(1) == 0) bad("rows must have at least one column");
+  plan_array(sources, "sources", 1, ys.device());
+  plan_array(positions, "positions", 2, ys.device());
+  if (ys.size(0) != sources.size(0))
+    bad("rows must have the plan's " + std::to_string(sources.size(0)) + " rows");
+  if (weights.dim() != 2 || weights.size(0) != positions.size(0) || weights.size(1) != positions.size(1) ||
+      weights.scalar_type() != at::kFloat || weights.device() != ys.device())
+    bad("weights must be a float32 [T, k] tensor on the rows' device");
+  const bool grad = at::GradMode::is_enabled();
+  const bool need_rows = grad && ys.requires_grad(), need_weights = grad && weights.requires_grad();
+  if (need_rows || need_weights)
+    return MoeCombine::apply(ys, weights, sources, positions, need_rows, need_weights);
+  const c10::cuda::CUDAGuard guard(ys.device());
+  return combine_rows(ys, weights.contiguous(), positions);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -546,5 +710,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("bias"), py::arg("w13"), py::arg("w13_scale"), py::arg("w2"), py::arg("w2_scale"),
         py::arg("top_k"), py::arg("scoring"), py::arg("renormalize"), py::arg("routed_scale"),
         py::arg("out"), py::arg("topk_ids"), py::arg("topk_weights"), py::arg("workspace"));
+  m.def("moe_plan_rows", &moe_plan_rows, py::arg("T"), py::arg("k"), py::arg("E"), py::arg("align"));
+  m.def("moe_sort", &moe_sort, py::arg("ids"), py::arg("E"), py::arg("align"));
+  m.def("moe_permute", &moe_permute, py::arg("x"), py::arg("sources"), py::arg("positions"));
+  m.def("moe_combine", &moe_combine, py::arg("rows"), py::arg("weights"), py::arg("sources"),
+        py::arg("positions"));
   m.def("abi_version", []() { return cutie_abi_version(); });
 }
