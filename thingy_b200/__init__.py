@@ -22,6 +22,8 @@ Drop-in host API for the reference's hot path (S1ro1/thingy, package
                                                kernel, forward only (no counterpart)
     moe_sort, moe_permute, moe_combine      tokens sorted by expert and back, with weights
                                                applied, and the gradients (no counterpart)
+    fp8_grouped_gemm, fp8_grouped_linear    the experts' products on sorted rows, and their
+                                               linear layer with its gradients (no counterpart)
 
 Every op runs hand-written CUDA from ``lib/libcutie_b200.so`` through the C
 ABI in ``include/cutie.h``; there is no CPU or PyTorch fallback.
@@ -32,9 +34,9 @@ from .dispatch import MoePlan, moe_combine, moe_permute, moe_plan_rows, moe_sort
 from .fp8_utils import (per_block_cast_to_fp8, per_token_cast_to_fp8, per_token_cast_to_fp8_triton,
                         two_way_cast_to_fp8)
 from .fused import empty_scale, residual_rms_norm_fp8, rms_norm_fp8
-from .gemm import fp8_block_gemm
+from .gemm import fp8_block_gemm, fp8_grouped_gemm
 from .layouts import mx_swizzle, mx_swizzle_offset, mx_swizzled_size, mx_unswizzle
-from .linear import fp8_linear
+from .linear import fp8_grouped_linear, fp8_linear
 from .moe import clear_moe_workspaces, moe_fp8, moe_workspace, quantize_experts
 from .rms_norm import RMSNorm, rms_norm, rms_norm_on_stream
 
@@ -45,6 +47,8 @@ __all__ = [
     "clear_moe_workspaces",
     "empty_scale",
     "fp8_block_gemm",
+    "fp8_grouped_gemm",
+    "fp8_grouped_linear",
     "fp8_linear",
     "moe_combine",
     "moe_fp8",

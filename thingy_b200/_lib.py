@@ -42,6 +42,9 @@ EXPORTED_SYMBOLS = (
     "cutie_rms_norm_mxfp8_gemm",
     "cutie_cast_fp8_tiles",
     "cutie_fp8_block_gemm",
+    "cutie_cast_fp8_sorted",
+    "cutie_fp8_grouped_gemm",
+    "cutie_fp8_grouped_wgrad",
     "cutie_moe_fp8",
     "cutie_moe_fp8_workspace",
     "cutie_moe_plan_rows",
@@ -101,6 +104,20 @@ _SIGNATURES = {
     "cutie_fp8_block_gemm": (
         _int,
         [_ptr, _i64, _ptr, _i64, _i64, _ptr, _i64, _ptr, _i64, _i64, _int, _ptr, _i64, _int, _int,
+         _i64, _i64, _i64, _ptr],
+    ),
+    "cutie_cast_fp8_sorted": (
+        _int,
+        [_ptr, _i64, _i64, _i64, _ptr, _int, _ptr, _i64, _ptr, _i64, _ptr, _i64, _ptr, _i64, _ptr],
+    ),
+    "cutie_fp8_grouped_gemm": (
+        _int,
+        [_ptr, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _i64, _ptr, _i64, _ptr, _i64,
+         _int, _i64, _i64, _i64, _ptr],
+    ),
+    "cutie_fp8_grouped_wgrad": (
+        _int,
+        [_ptr, _i64, _ptr, _i64, _i64, _ptr, _i64, _ptr, _i64, _i64, _ptr, _i64, _ptr, _i64, _i64, _int,
          _i64, _i64, _i64, _ptr],
     ),
     "cutie_moe_fp8_workspace": (ctypes.c_size_t, [_i64, _i64, _i64, _i64, _i64]),

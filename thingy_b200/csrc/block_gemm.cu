@@ -148,12 +148,61 @@ struct TileArgs {
   int parts;  // 2 (columns) or 4 (columns and rows) each
   bool d_f32, accumulate;
   long long wait_limit;  // SM cycles a wait may block before it gives up (< 0: never blocks)
+  // experts (kExpertRows, kExpertColumns)
+  const int* offsets;  // [E + 1]
+  int E, R;            // R: sorted rows, a multiple of 128
+  int64_t sb_expert, d_expert;
 };
 
-// Tile t of the banded walk.
-__device__ __forceinline__ void tile_at(const TileArgs& g, int t, int* tm, int* tn) {
+// What a launch of the tiled kernel multiplies:
+//  * kOne: the matrices as they are.
+//  * kExpertRows: A's rows are sorted by expert, B is [E, N, K]: the rows of
+//    A from offsets[e] on go with B's matrix e. Experts begin at multiples of
+//    128, so a tile has one expert.
+//  * kExpertColumns: both operands' columns are sorted by expert (a weight
+//    gradient): D's matrix e is the product over the columns of e. A tile of D
+//    has as many K blocks as its expert has, or none and is zero.
+// The number of tiles, and of a tile's K blocks, is read from the offsets on the
+// GPU. Whatever they hold is cut to 0..R and to whole blocks before its use.
+enum Experts { kOne, kExpertRows, kExpertColumns };
+
+// Where the experts begin, and their tiles before each (kExpertRows).
+template <int MODE>
+struct ExpertTable {
+  int begin[MODE == kOne ? 1 : kMoeMaxExperts + 1];
+  int tiles[MODE == kExpertRows ? kMoeMaxExperts + 1 : 1];
+};
+
+// By the first warps of a CTA, between two barriers of its own.
+template <int MODE>
+__device__ __forceinline__ void fill_experts(const TileArgs& g, ExpertTable<MODE>& x) {
+  for (int e = threadIdx.x; e <= g.E; e += blockDim.x)
+    x.begin[e] = min(max(g.offsets[e], 0), g.R) & ~(kBM - 1);
+  __syncthreads();
+  if (MODE == kExpertRows && threadIdx.x < 32) {
+    const int per = (g.E + 31) / 32, lane = threadIdx.x, e0 = min(lane * per, g.E), e1 = min(e0 + per, g.E);
+    int mine = 0;
+    for (int e = e0; e < e1; ++e) mine += max(x.begin[e + 1] - x.begin[e], 0) / kBM;
+    int sum = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const int v = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += v;
+    }
+    if (lane == 31) x.tiles[g.E] = sum;
+    sum -= mine;
+    for (int e = e0; e < e1; ++e) {
+      x.tiles[e] = sum;
+      sum += max(x.begin[e + 1] - x.begin[e], 0) / kBM;
+    }
+  }
+  __syncthreads();
+}
+
+// Tile t of the banded walk over tiles_m rows of tiles.
+__device__ __forceinline__ void tile_at(const TileArgs& g, int t, int* tm, int* tn, int tiles_m) {
   const int band = t / (g.band * g.tiles_n), first = band * g.band;
-  const int rows = g.tiles_m - first < g.band ? g.tiles_m - first : g.band;
+  const int rows = tiles_m - first < g.band ? tiles_m - first : g.band;
   const int in = t - band * g.band * g.tiles_n;
   *tm = first + in % rows;
   *tn = in / rows;
@@ -162,12 +211,49 @@ __device__ __forceinline__ void tile_at(const TileArgs& g, int t, int* tm, int* 
 template <int BN>
 __device__ __forceinline__ void tile_of(const TileArgs& g, int t, int* tm, int* tn) {
   if (BN == 128 && g.tail >= 0) {
-    tile_at(g, g.tail + t / g.parts, tm, tn);
+    tile_at(g, g.tail + t / g.parts, tm, tn, g.tiles_m);
     *tn = 2 * *tn + (t & 1);
     if (g.parts == 4) *tm = 2 * *tm + ((t >> 1) & 1);
   } else {
-    tile_at(g, t, tm, tn);
+    tile_at(g, t, tm, tn, g.tiles_m);
   }
+}
+
+// A tile as the warps see it. Rows are A's, columns B's (within its expert).
+struct Item {
+  int e, row, col;  // expert, first row of A and first row of B
+  int k0, nkb;      // first column of the operands' K range, its K blocks
+  int row_end;      // of the rows that are stored
+};
+
+// Tile t for rank `rank` of a pair, `rows` of A a tile.
+template <int BN, int MODE>
+__device__ __forceinline__ Item item_of(const TileArgs& g, const ExpertTable<MODE>& x, int t, int rows, int rank) {
+  Item i;
+  int tm, tn;
+  if (MODE == kExpertRows) {
+    int lo = 0, hi = g.E;  // the last expert whose tiles begin at t or before: it has some
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (x.tiles[mid] * g.tiles_n <= t) lo = mid;
+      else hi = mid;
+    }
+    const int first = x.tiles[lo];
+    tile_at(g, t - first * g.tiles_n, &tm, &tn, x.tiles[lo + 1] - first);
+    i.e = lo;
+    i.row = x.begin[lo] + tm * rows + rank * kBM;
+    i.row_end = x.begin[lo + 1];
+    i.k0 = 0, i.nkb = g.KB;
+  } else {
+    const int each = g.tiles_m * g.tiles_n;
+    i.e = t / each;
+    tile_at(g, t - i.e * each, &tm, &tn, g.tiles_m);
+    i.row = tm * rows + rank * kBM;
+    i.row_end = g.M;
+    i.k0 = x.begin[i.e], i.nkb = max(x.begin[i.e + 1] - i.k0, 0) / kBK;
+  }
+  i.col = tn * BN;
+  return i;
 }
 
 // A warp's 32 rows of NC columns. VEC: the rows of D start on 32-byte
@@ -178,14 +264,14 @@ __device__ __forceinline__ void tile_of(const TileArgs& g, int t, int* tm, int* 
 // A template, not a branch: the mere presence of the second form cost the main
 // loop of the first 6%.
 template <int NC, bool VEC>
-__device__ __forceinline__ void store_rows(const TileArgs& g, const float2 (&acc)[NC / 2], int row0,
-                                           int col, int lane, float* stage) {
+__device__ __forceinline__ void store_rows(const TileArgs& g, void* d, int row_end, const float2 (&acc)[NC / 2],
+                                           int row0, int col, int lane, float* stage) {
   if (VEC) {
     const int row = row0 + lane;
-    if (row >= g.M) return;
+    if (row >= row_end) return;
     const int64_t at = (int64_t)row * g.ldd + col;
     if (!g.d_f32) {
-      uint16_t* p = static_cast<uint16_t*>(g.d) + at;
+      uint16_t* p = static_cast<uint16_t*>(d) + at;
 #pragma unroll
       for (int c = 0; c < NC; c += 16) {
         uint32_t w[8];
@@ -194,7 +280,7 @@ __device__ __forceinline__ void store_rows(const TileArgs& g, const float2 (&acc
         if (col + c < g.N) st_stream8(p + c, w);
       }
     } else {
-      float* p = static_cast<float*>(g.d) + at;
+      float* p = static_cast<float*>(d) + at;
 #pragma unroll
       for (int c = 0; c < NC; c += 8) {
         if (col + c >= g.N) break;
@@ -226,14 +312,14 @@ __device__ __forceinline__ void store_rows(const TileArgs& g, const float2 (&acc
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int r = row0 + 4 * i + r4;
-        if (r >= g.M || cc >= g.N) break;
+        if (r >= row_end || cc >= g.N) break;
         const float v = stage[(4 * i + r4) * kStageRow + c8];
         const int64_t to = (int64_t)r * g.ldd + cc;
         if (g.d_f32) {
-          float* p = static_cast<float*>(g.d) + to;
+          float* p = static_cast<float*>(d) + to;
           *p = g.accumulate ? *p + v : v;
         } else {
-          static_cast<uint16_t*>(g.d)[to] = (uint16_t)(f2_to_bf2(make_float2(v, 0.f)) & 0xffffu);
+          static_cast<uint16_t*>(d)[to] = (uint16_t)(f2_to_bf2(make_float2(v, 0.f)) & 0xffffu);
         }
       }
     }
@@ -271,12 +357,22 @@ __device__ __forceinline__ void store_four(const TileArgs& g, int row, int col, 
   }
 }
 
-template <int BN, bool SB_ROWS, bool VEC, bool SPLIT, bool PAIR>
+// Zeros in `cols` columns from `col` on of a row; 32-byte boundaries as for VEC above.
+__device__ __forceinline__ void zero_row(const TileArgs& g, void* d, int64_t row, int col, int cols) {
+  const uint32_t zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  const int per = g.d_f32 ? 8 : 16;
+  char* p = static_cast<char*>(d) + (row * g.ldd + col) * (g.d_f32 ? 4 : 2);
+  for (int c = 0; c < cols && col + c < g.N; c += per, p += 32) st_stream8(p, zero);
+}
+
+template <int BN, bool SB_ROWS, bool VEC, bool SPLIT, bool PAIR, int MODE = kOne>
 __global__ void __launch_bounds__(kThreads, 1)
     block_gemm_kernel(const __grid_constant__ CUtensorMap map_a,
                       const __grid_constant__ CUtensorMap map_b, const TileArgs g) {
   using P = TilePlan<BN, SB_ROWS, VEC, PAIR>;
   static_assert(!PAIR || (BN == 256 && !SPLIT), "pairs make 256 x 256 tiles");
+  static_assert(MODE == kOne || (VEC && !SPLIT && SB_ROWS == (MODE == kExpertColumns)), "forms of the experts");
+  static_assert(MODE != kExpertRows || !PAIR, "a pair's rows could have two experts");
   constexpr int NC = P::kCols;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full_bar[P::kStages];
@@ -292,15 +388,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ uint32_t abort_flag;
   __shared__ uint32_t issued;     // K blocks whose copies were issued
   __shared__ uint32_t committed;  // K blocks whose MMAs were committed
+  __shared__ ExpertTable<MODE> experts;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
   // tiles begin, begin + step, ... are this CTA's, or its pair's
-  const int tiles = g.tiles, begin = PAIR ? blockIdx.x / 2 : blockIdx.x, step = PAIR ? gridDim.x / 2 : gridDim.x;
+  int tiles = g.tiles;
+  const int begin = PAIR ? blockIdx.x / 2 : blockIdx.x, step = PAIR ? gridDim.x / 2 : gridDim.x;
   // K blocks of this CTA: all, or the rank's of its cluster
   const int S = SPLIT ? (int)gridDim.z : 1, rank = SPLIT || PAIR ? (int)tc::cluster_ctarank() : 0;
   const int kb0 = SPLIT ? (int)((int64_t)g.KB * rank / S) : 0;
-  const int nkb = SPLIT ? (int)((int64_t)g.KB * (rank + 1) / S) - kb0 : g.KB;
+  int nkb = SPLIT ? (int)((int64_t)g.KB * (rank + 1) / S) - kb0 : g.KB;
   // and the tile's rows that it adds up
   const int share = (kBM + S - 1) / S, own_lo = min(rank * share, kBM), own_n = min(share, kBM - own_lo);
   volatile uint32_t* abortp = &abort_flag;
@@ -337,6 +435,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = tmem_base_slot;
   griddep_wait();
   griddep_launch_dependents();
+  if constexpr (MODE != kOne) {
+    fill_experts<MODE>(g, experts);
+    if (MODE == kExpertRows) tiles = experts.tiles[g.E] * g.tiles_n;
+  }
 
   if (warp >= kEpiWarps) {
     tc::regs_down<kIssueRegs>();
@@ -347,7 +449,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     for (int t = begin; t < tiles && ok; t += step) {
       int tm, tn;
-      tile_of<BN>(g, t, &tm, &tn);
+      [[maybe_unused]] Item it;
+      if constexpr (MODE == kOne) {
+        tile_of<BN>(g, t, &tm, &tn);
+      } else {
+        it = item_of<BN, MODE>(g, experts, t, (PAIR ? 2 : 1) * kBM, rank);
+        nkb = it.nkb;
+      }
       for (int kb = 0; kb < nkb; ++kb) {
         ok = tc::wait_or_abort(smem_addr(&empty_bar[s]), parity, abortp, g.wait_limit);
         if (!__all_sync(0xffffffffu, ok)) {
@@ -360,8 +468,23 @@ __global__ void __launch_bounds__(kThreads, 1)
             // both CTAs' loads are counted on rank 0's barrier
             if (rank == 0) mbar_arrive_expect_tx(bar, 2 * P::kStageBytes);
             const uint32_t to = tc::mapa(bar, 0);
-            tc::tma_load_2d_pair(st, &map_a, kb * kBK, (2 * tm + rank) * kBM, to);
-            tc::tma_load_2d_pair(st + kBoxBytes, &map_b, kb * kBK, tn * BN + 128 * rank, to);
+            if constexpr (MODE == kOne) {
+              tc::tma_load_2d_pair(st, &map_a, kb * kBK, (2 * tm + rank) * kBM, to);
+              tc::tma_load_2d_pair(st + kBoxBytes, &map_b, kb * kBK, tn * BN + 128 * rank, to);
+            } else {
+              tc::tma_load_2d_pair(st, &map_a, it.k0 + kb * kBK, it.row, to);
+              tc::tma_load_2d_pair(st + kBoxBytes, &map_b, it.k0 + kb * kBK, it.col + 128 * rank, to);
+            }
+          } else if constexpr (MODE != kOne) {
+            mbar_arrive_expect_tx(bar, P::kStageBytes);
+            const int k = it.k0 + kb * kBK;
+            tc::tma_load_2d(st, &map_a, k, it.row, bar);
+#pragma unroll
+            for (int h = 0; h < P::kNB; ++h) {
+              const uint32_t to = st + (1 + h) * kBoxBytes;
+              if (MODE == kExpertRows) tc::tma_load_3d(to, &map_b, k, it.col + 128 * h, it.e, bar);
+              else tc::tma_load_2d(to, &map_b, k, it.col + 128 * h, bar);
+            }
           } else {
             mbar_arrive_expect_tx(bar, P::kStageBytes);
             tc::tma_load_2d(st, &map_a, (kb0 + kb) * kBK, tm * kBM, bar);
@@ -387,6 +510,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t s = 0, parity = 0, buf = 0, buf_parity = 1;
     bool ok = !PAIR || rank == 0;  // rank 0 issues for both
     for (int t = begin; t < tiles && ok; t += step) {
+      if constexpr (MODE == kExpertColumns) nkb = item_of<BN, MODE>(g, experts, t, kBM, 0).nkb;
       for (int kb = 0; kb < nkb; ++kb) {
         ok = tc::wait_or_abort(smem_addr(&full_bar[s]), parity, abortp, g.wait_limit) &&
              tc::wait_or_abort(smem_addr(&acc_empty[buf]), buf_parity, abortp, g.wait_limit);
@@ -426,19 +550,28 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     constexpr int kNS = SB_ROWS ? BN / 32 : 1;
     for (int t = begin; t < tiles && ok; t += step) {
-      int tm, tn;
-      tile_of<BN>(g, t, &tm, &tn);
       const float *pa[4], *pb[kNS];
+      int row0, col0, kb_first = kb0;
+      [[maybe_unused]] const float* sb = g.sb;
+      if constexpr (MODE == kOne) {
+        int tm, tn;
+        tile_of<BN>(g, t, &tm, &tn);
+        row0 = (PAIR ? 2 * tm + rank : tm) * kBM, col0 = tn * BN;
+      } else {
+        const Item it = item_of<BN, MODE>(g, experts, t, (PAIR ? 2 : 1) * kBM, rank);
+        row0 = it.row, col0 = it.col, kb_first = it.k0 / kBK, nkb = it.nkb;
+        if (MODE == kExpertRows) sb += it.e * g.sb_expert;
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int row = (PAIR ? 2 * tm + rank : tm) * kBM + lane + 32 * i;
-        pa[i] = row < g.M ? g.sa + (int64_t)row * g.sa_row + kb0 * g.sa_kb : nullptr;
+        const int row = row0 + lane + 32 * i;
+        pa[i] = row < g.M ? g.sa + (int64_t)row * g.sa_row + kb_first * g.sa_kb : nullptr;
       }
 #pragma unroll
       for (int i = 0; i < kNS; ++i) {
-        const int col = tn * BN + (SB_ROWS ? lane + 32 * i : 128 * lane);
+        const int col = col0 + (SB_ROWS ? lane + 32 * i : 128 * lane);
         const bool some = col < g.N && (SB_ROWS || lane < BN / 128);
-        pb[i] = some ? g.sb + (int64_t)(SB_ROWS ? col : col / 128) * g.sb_row + kb0 * g.sb_kb : nullptr;
+        pb[i] = some ? sb + (int64_t)(SB_ROWS ? col : col / 128) * g.sb_row + kb_first * g.sb_kb : nullptr;
       }
       for (int kb = 0; kb < nkb; ++kb) {
         const int j = kb % kScaleBlocks;
@@ -497,8 +630,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc::fence_after();
       tc::tmem_ld_async(tm_lane + buf * BN, lo);
     };
-    if (begin < tiles) begin_block(0);
-    for (int t = begin; t < tiles; t += step) {
+    // the first tile from t on that has K blocks; those without are zeroed at the end
+    auto some_from = [&](int t) {
+      if constexpr (MODE == kExpertColumns)
+        while (t < tiles && item_of<BN, MODE>(g, experts, t, kBM, 0).nkb == 0) t += step;
+      return t;
+    };
+    int next = some_from(begin);
+    if (next < tiles) begin_block(0);
+    for (int t = next; t < tiles; t = next) {
+      if constexpr (MODE == kExpertColumns) nkb = item_of<BN, MODE>(g, experts, t, kBM, 0).nkb;
+      next = some_from(t + step);
       float2 acc[NC / 2];
 #pragma unroll
       for (int i = 0; i < NC / 2; ++i) acc[i] = make_float2(0.f, 0.f);
@@ -548,7 +690,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             buf ^= 1;
             buf_parity ^= buf == 0;
             if (slot_done && ++slot == P::kScaleSlots) slot = 0, slot_parity ^= 1;
-            if (!last || t + step < tiles) begin_block(last ? 0 : kb + 1);
+            if (!last || next < tiles) begin_block(last ? 0 : kb + 1);
           }
           add(c + CH, hi);
         }
@@ -558,11 +700,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       int tm_i, tn_i;
-      tile_of<BN>(g, t, &tm_i, &tn_i);
-      if constexpr (!SPLIT) {
+      if constexpr (MODE == kOne) tile_of<BN>(g, t, &tm_i, &tn_i);
+      if constexpr (MODE != kOne) {
+        const Item it = item_of<BN, MODE>(g, experts, t, (PAIR ? 2 : 1) * kBM, rank);
+        void* d = MODE == kExpertRows ? g.d : static_cast<char*>(g.d) + it.e * g.d_expert * (g.d_f32 ? 4 : 2);
         if (*abortp == 0u)
-          store_rows<NC, VEC>(g, acc, (PAIR ? 2 * tm_i + rank : tm_i) * kBM + (warp & 3) * 32, tn_i * BN + wg * NC, lane,
-                              stage[VEC ? 0 : warp]);
+          store_rows<NC, VEC>(g, d, it.row_end, acc, it.row + (warp & 3) * 32, it.col + wg * NC, lane, stage[0]);
+      } else if constexpr (!SPLIT) {
+        if (*abortp == 0u)
+          store_rows<NC, VEC>(g, g.d, g.M, acc, (PAIR ? 2 * tm_i + rank : tm_i) * kBM + (warp & 3) * 32,
+                              tn_i * BN + wg * NC, lane, stage[VEC ? 0 : warp]);
       } else {
         // the last accumulator was complete, so this CTA's ring is idle, and so
         // are the others' once they have arrived too: the partial tile to the
@@ -611,6 +758,18 @@ __global__ void __launch_bounds__(kThreads, 1)
             store_four<VEC>(g, row, col, v);
           }
         }
+      }
+    }
+    if constexpr (MODE == kExpertRows) {  // rows behind the last expert's
+      for (int64_t row = (int64_t)experts.begin[g.E] + blockIdx.x * kEpiWarps + warp; row < g.R;
+           row += (int64_t)gridDim.x * kEpiWarps)
+        for (int c = lane * (g.d_f32 ? 8 : 16); c < g.N; c += 32 * (g.d_f32 ? 8 : 16)) zero_row(g, g.d, row, c, 1);
+    } else if constexpr (MODE == kExpertColumns) {  // experts without rows
+      for (int t = begin; t < tiles; t += step) {
+        const Item it = item_of<BN, MODE>(g, experts, t, (PAIR ? 2 : 1) * kBM, rank);
+        const int row = it.row + (warp & 3) * 32 + lane;
+        if (it.nkb == 0 && row < it.row_end)
+          zero_row(g, static_cast<char*>(g.d) + it.e * g.d_expert * (g.d_f32 ? 4 : 2), row, it.col + wg * NC, NC);
       }
     }
   }
@@ -1137,6 +1296,79 @@ cudaError_t device_error_block_gemm(int* out, bool clear) {
   }
   *out = v;
   return e;
+}
+
+namespace {
+
+// A launch of the tiled kernel over `units` tiles at most; B: [E] matrices of rows x K
+// (kExpertRows) or one.
+template <int BN, int MODE, bool PAIR>
+cudaError_t launch_experts(const GroupedGemmArgs& p, const TileArgs& g, int64_t tiles, cudaStream_t stream) {
+  constexpr bool columns = MODE == kExpertColumns;
+  using P = TilePlan<BN, columns, true, PAIR>;
+  auto kernel = block_gemm_kernel<BN, columns, true, false, PAIR, MODE>;
+  static_assert(P::kSmemBytes + P::kScaleSlots * kScaleBlocks * P::kScales * 4 + sizeof(ExpertTable<MODE>) + 768 <=
+                    227 * 1024,
+                "shared memory");
+  cudaError_t e =
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)P::kSmemBytes);
+  if (e != cudaSuccess) return e;
+  CUtensorMap map_a, map_b;
+  const int64_t K = columns ? p.R : p.K;
+  if (!tc::encode_e4m3_operand(&map_a, p.a, columns ? p.N : p.R, K, p.lda, kBM) ||
+      !(columns ? tc::encode_e4m3_operand(&map_b, p.b, p.K, K, p.ldb, kBM)
+                : tc::encode_e4m3_matrices(&map_b, p.b, p.E, p.N, K, p.ldb, p.b_expert, kBM)))
+    return cudaErrorInvalidValue;
+  const int sms = device_sm_count();
+  if constexpr (PAIR) {
+    static std::atomic<int> cache[64][kMaxRanks + 1];
+    const int pairs =
+        max_clusters(reinterpret_cast<const void*>(kernel), kThreads, P::kSmemBytes, dim3(2, 1, 1), cache);
+    if (pairs <= 0) return cudaErrorInvalidConfiguration;
+    return launch_cluster(kernel, dim3(2u * (unsigned)(tiles < pairs ? tiles : pairs)), 2, kThreads, P::kSmemBytes,
+                          stream, map_a, map_b, g);
+  }
+  return launch_pdl(kernel, (unsigned)(tiles < sms ? tiles : sms), kThreads, P::kSmemBytes, stream, map_a, map_b, g);
+}
+
+}  // namespace
+
+int grouped_gemm(const GroupedGemmArgs& p, cudaStream_t stream, const char** why) {
+  TileArgs g{};
+  g.sa = p.sa, g.sa_row = p.sa_row, g.sa_kb = p.sa_kb;
+  g.sb = p.sb, g.sb_row = p.sb_row, g.sb_kb = p.sb_kb, g.sb_expert = p.sb_expert;
+  g.d = p.d, g.ldd = p.ldd, g.d_expert = p.d_expert;
+  g.d_f32 = p.d_f32, g.wait_limit = p.wait_limit;
+  g.offsets = p.offsets, g.E = (int)p.E, g.R = (int)p.R;
+  g.band = kBand, g.tail = -1;
+  const int sms = device_sm_count();
+  cudaError_t e;
+  if (!p.columns) {
+    // 256-wide tiles while every SM can get one (the offsets are on the GPU: R bounds the rows)
+    g.M = (int)p.R, g.N = (int)p.N, g.KB = (int)((p.K + kBK - 1) / kBK);
+    const int64_t rows = p.R / kBM, wide = rows * ((p.N + 255) / 256);
+    const bool narrow = wide < sms;
+    g.tiles_n = (int)((p.N + (narrow ? 127 : 255)) / (narrow ? 128 : 256));
+    e = narrow ? launch_experts<128, kExpertRows, false>(p, g, rows * g.tiles_n, stream)
+               : launch_experts<256, kExpertRows, false>(p, g, wide, stream);
+  } else {
+    // pairs while every pair gets a tile of 256 x 256, then 128 x 256, then 128 x 128
+    g.M = (int)p.N, g.N = (int)p.K;
+    const int64_t m2 = (p.N + 255) / 256, m1 = (p.N + 127) / 128, n2 = (p.K + 255) / 256, n1 = (p.K + 127) / 128;
+    const bool pair = 2 * p.E * m2 * n2 >= sms, wide = p.E * m1 * n2 >= sms;
+    g.tiles_m = (int)(pair ? m2 : m1), g.tiles_n = (int)(pair || wide ? n2 : n1);
+    if (pair) g.band = kBand / 2;
+    const int64_t tiles = p.E * g.tiles_m * g.tiles_n;
+    g.tiles = (int)tiles;
+    e = pair   ? launch_experts<256, kExpertColumns, true>(p, g, tiles, stream)
+        : wide ? launch_experts<256, kExpertColumns, false>(p, g, tiles, stream)
+               : launch_experts<128, kExpertColumns, false>(p, g, tiles, stream);
+  }
+  if (e != cudaSuccess) {
+    *why = cudaGetErrorString(e);
+    return CUTIE_ERR_CUDA;
+  }
+  return CUTIE_OK;
 }
 
 int block_gemm(const BlockGemmArgs& p, cudaStream_t stream, const char** why) {

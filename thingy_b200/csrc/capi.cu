@@ -796,11 +796,9 @@ extern "C" int cutie_rms_norm_mxfp8_gemm(const void* x, int64_t ldx, const void*
   return CUTIE_OK;
 }
 
-extern "C" int cutie_cast_fp8_tiles(const void* x, int64_t ldx, int64_t M, int64_t H,
-                                    int tile_kind, int scale_fmt, void* q, int64_t ldq, void* s,
-                                    int64_t lds, void* qt, int64_t ldqt, void* st, int64_t ldst,
-                                    void* stream) {
-  g_err[0] = '\0';
+static int cast_tiles(const void* x, int64_t ldx, int64_t M, int64_t H, const int* sources,
+                      int tile_kind, int scale_fmt, void* q, int64_t ldq, void* s, int64_t lds,
+                      void* qt, int64_t ldqt, void* st, int64_t ldst, void* stream) {
   if (M < 0 || H <= 0)
     return fail(CUTIE_ERR_INVALID_ARGUMENT, "need M >= 0 and H > 0 (got M=%lld, H=%lld)",
                 (long long)M, (long long)H);
@@ -844,9 +842,32 @@ extern "C" int cutie_cast_fp8_tiles(const void* x, int64_t ldx, int64_t M, int64
   a.s = static_cast<float*>(s), a.lds = lds;
   a.qt = static_cast<uint8_t*>(qt), a.ldqt = ldqt;
   a.st = static_cast<float*>(st), a.ldst = ldst;
+  a.sources = sources;
   const cudaError_t e = launch_cast_tiles(a, block, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "tile cast launch");
   return CUTIE_OK;
+}
+
+extern "C" int cutie_cast_fp8_tiles(const void* x, int64_t ldx, int64_t M, int64_t H,
+                                    int tile_kind, int scale_fmt, void* q, int64_t ldq, void* s,
+                                    int64_t lds, void* qt, int64_t ldqt, void* st, int64_t ldst,
+                                    void* stream) {
+  g_err[0] = '\0';
+  return cast_tiles(x, ldx, M, H, nullptr, tile_kind, scale_fmt, q, ldq, s, lds, qt, ldqt, st, ldst,
+                    stream);
+}
+
+extern "C" int cutie_cast_fp8_sorted(const void* x, int64_t ldx, int64_t R, int64_t H,
+                                     const void* sources, int scale_fmt, void* q, int64_t ldq,
+                                     void* s, int64_t lds, void* qt, int64_t ldqt, void* st,
+                                     int64_t ldst, void* stream) {
+  g_err[0] = '\0';
+  if (R % 128 != 0)
+    return fail(CUTIE_ERR_UNSUPPORTED, "sorted rows come in multiples of 128 (got %lld)", (long long)R);
+  if (R > 0 && sources == nullptr) return fail(CUTIE_ERR_INVALID_ARGUMENT, "sources is NULL");
+  if (!aligned(sources, 4)) return fail(CUTIE_ERR_ALIGNMENT, "sources must be 4-byte aligned");
+  return cast_tiles(x, ldx, R, H, static_cast<const int*>(sources), CUTIE_TILE_TWO_WAY, scale_fmt, q, ldq, s, lds,
+                    qt, ldqt, st, ldst, stream);
 }
 
 extern "C" int cutie_fp8_block_gemm(const void* a, int64_t lda, const void* a_scale,
@@ -901,6 +922,47 @@ extern "C" int cutie_fp8_block_gemm(const void* a, int64_t lda, const void* a_sc
 namespace cutie {
 namespace {
 
+// Sizes, operands and scales of the experts' products; fills all but d.
+int check_grouped(GroupedGemmArgs* g, const void* a, int64_t lda, const void* a_scale, int64_t sa_row,
+                  int64_t sa_kb, const void* b, int64_t ldb, const void* b_scale, int64_t sb_row, int64_t sb_kb,
+                  const void* offsets, int64_t E, int d_dtype, int64_t R, int64_t N, int64_t K) {
+  if (E <= 0 || R < 0 || N <= 0 || K <= 0)
+    return fail(CUTIE_ERR_INVALID_ARGUMENT, "need R >= 0 and E, N, K > 0 (got %lld, %lld, %lld, %lld)",
+                (long long)R, (long long)E, (long long)N, (long long)K);
+  if (E > kMoeMaxExperts)
+    return fail(CUTIE_ERR_UNSUPPORTED, "at most %d experts (got %lld)", kMoeMaxExperts, (long long)E);
+  if (R % 128 != 0)
+    return fail(CUTIE_ERR_UNSUPPORTED, "sorted rows come in multiples of 128 (got %lld)", (long long)R);
+  if (R > INT32_MAX - 512 || N > (1 << 24) || K > (1 << 24))
+    return fail(CUTIE_ERR_UNSUPPORTED, "R must be below 2^31 - 512, N and K at most 2^24");
+  if (d_dtype != CUTIE_DTYPE_BF16 && d_dtype != CUTIE_DTYPE_F32)
+    return fail(CUTIE_ERR_INVALID_ARGUMENT, "unknown d_dtype %d", d_dtype);
+  if (offsets == nullptr) return fail(CUTIE_ERR_INVALID_ARGUMENT, "offsets is NULL");
+  if (R > 0 && (a_scale == nullptr || b_scale == nullptr))
+    return fail(CUTIE_ERR_INVALID_ARGUMENT, "a_scale and b_scale must not be NULL");
+  if (!aligned(a_scale, 4) || !aligned(b_scale, 4) || !aligned(offsets, 4))
+    return fail(CUTIE_ERR_ALIGNMENT, "fp32 scales and offsets must be 4-byte aligned");
+  if (sa_row < 0 || sa_kb < 0 || sb_row < 0 || sb_kb < 0)
+    return fail(CUTIE_ERR_INVALID_ARGUMENT, "scale strides must not be negative");
+  *g = GroupedGemmArgs{};
+  g->a = a, g->lda = lda, g->sa = static_cast<const float*>(a_scale), g->sa_row = sa_row, g->sa_kb = sa_kb;
+  g->b = b, g->ldb = ldb, g->sb = static_cast<const float*>(b_scale), g->sb_row = sb_row, g->sb_kb = sb_kb;
+  g->offsets = static_cast<const int*>(offsets);
+  g->d_f32 = d_dtype == CUTIE_DTYPE_F32;
+  g->E = E, g->R = R, g->N = N, g->K = K;
+  g->wait_limit = g_wait_limit;
+  return CUTIE_OK;
+}
+
+// D's rows are written as 32-byte sectors.
+int check_sectors(const char* name, const void* d, int64_t ldd, int64_t columns, bool f32) {
+  const int per = f32 ? 8 : 16;
+  if (columns % per != 0)
+    return fail(CUTIE_ERR_UNSUPPORTED, "%s's columns must be a multiple of %d (got %lld)", name, per,
+                (long long)columns);
+  return check_matrix(name, d, ldd, columns, 32, per);
+}
+
 int check_moe_sizes(int64_t T, int64_t E, int64_t k, int64_t H, int64_t I) {
   if (T < 0 || E <= 0 || k <= 0 || H <= 0 || I <= 0)
     return fail(CUTIE_ERR_INVALID_ARGUMENT,
@@ -928,6 +990,65 @@ int check_moe_sizes(int64_t T, int64_t E, int64_t k, int64_t H, int64_t I) {
 
 }  // namespace
 }  // namespace cutie
+
+extern "C" int cutie_fp8_grouped_gemm(const void* a, int64_t lda, const void* a_scale, int64_t sa_row,
+                                      int64_t sa_kb, const void* b, int64_t ldb, int64_t b_expert,
+                                      const void* b_scale, int64_t sb_row, int64_t sb_kb, int64_t sb_expert,
+                                      const void* offsets, int64_t E, void* d, int64_t ldd, int d_dtype,
+                                      int64_t R, int64_t N, int64_t K, void* stream) {
+  g_err[0] = '\0';
+  GroupedGemmArgs g;
+  int rc = check_grouped(&g, a, lda, a_scale, sa_row, sa_kb, b, ldb, b_scale, sb_row, sb_kb, offsets, E, d_dtype, R,
+                         N, K);
+  if (rc != CUTIE_OK) return rc;
+  if (R == 0) return CUTIE_OK;
+  if ((rc = check_matrix("a", a, lda, K, 16, 16)) != CUTIE_OK) return rc;
+  if ((rc = check_matrix("b", b, ldb, K, 16, 16)) != CUTIE_OK) return rc;
+  if (b_expert < 0 || b_expert % 16 != 0 || sb_expert < 0)
+    return fail(CUTIE_ERR_ALIGNMENT, "b_expert must be a multiple of 16 and no stride negative");
+  if ((rc = check_sectors("d", d, ldd, N, g.d_f32)) != CUTIE_OK) return rc;
+  if ((R / 128) * ((N + 127) / 128) > INT32_MAX / 2)
+    return fail(CUTIE_ERR_UNSUPPORTED, "R x N has more than 2^30 tiles");
+  g.b_expert = E > 1 ? b_expert : N * ldb, g.sb_expert = sb_expert;
+  g.d = d, g.ldd = ldd;
+  const char* why = "";
+  rc = grouped_gemm(g, static_cast<cudaStream_t>(stream), &why);
+  return rc == CUTIE_OK ? rc : fail(rc, "fp8 grouped gemm: %s", why);
+}
+
+extern "C" int cutie_fp8_grouped_wgrad(const void* a, int64_t lda, const void* a_scale, int64_t sa_row,
+                                       int64_t sa_kb, const void* b, int64_t ldb, const void* b_scale,
+                                       int64_t sb_row, int64_t sb_kb, const void* offsets, int64_t E, void* d,
+                                       int64_t ldd, int64_t d_expert, int d_dtype, int64_t R, int64_t N, int64_t K,
+                                       void* stream) {
+  g_err[0] = '\0';
+  GroupedGemmArgs g;
+  int rc = check_grouped(&g, a, lda, a_scale, sa_row, sa_kb, b, ldb, b_scale, sb_row, sb_kb, offsets, E, d_dtype, R,
+                         N, K);
+  if (rc != CUTIE_OK) return rc;
+  if ((rc = check_sectors("d", d, ldd, K, g.d_f32)) != CUTIE_OK) return rc;
+  if (d_expert < 0 || d_expert % (g.d_f32 ? 8 : 16) != 0)
+    return fail(CUTIE_ERR_ALIGNMENT, "D's matrices must start on 32-byte boundaries");
+  if (E * ((N + 127) / 128) * ((K + 127) / 128) > INT32_MAX / 2)
+    return fail(CUTIE_ERR_UNSUPPORTED, "E x N x K has more than 2^30 tiles");
+  const size_t es = g.d_f32 ? 4 : 2;
+  if (R == 0) {
+    for (int64_t e = 0; e < E; ++e) {
+      const cudaError_t err =
+          cudaMemset2DAsync(static_cast<char*>(d) + e * d_expert * es, (size_t)ldd * es, 0, (size_t)K * es, (size_t)N,
+                            static_cast<cudaStream_t>(stream));
+      if (err != cudaSuccess) return cuda_fail(err, "fp8 grouped wgrad (R = 0)");
+    }
+    return CUTIE_OK;
+  }
+  if ((rc = check_matrix("a", a, lda, R, 16, 16)) != CUTIE_OK) return rc;
+  if ((rc = check_matrix("b", b, ldb, R, 16, 16)) != CUTIE_OK) return rc;
+  g.columns = true;
+  g.d = d, g.ldd = ldd, g.d_expert = d_expert;
+  const char* why = "";
+  rc = grouped_gemm(g, static_cast<cudaStream_t>(stream), &why);
+  return rc == CUTIE_OK ? rc : fail(rc, "fp8 grouped wgrad: %s", why);
+}
 
 extern "C" size_t cutie_moe_fp8_workspace(int64_t T, int64_t E, int64_t top_k, int64_t H,
                                           int64_t I) {

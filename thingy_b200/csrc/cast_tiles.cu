@@ -64,7 +64,10 @@ __device__ __forceinline__ void transpose4(uint32_t a, uint32_t b, uint32_t c, u
   t[2] = __byte_perm(ab1, cd1, 0x5410), t[3] = __byte_perm(ab1, cd1, 0x7632);
 }
 
-template <bool BLOCK, bool TRANSPOSED>
+// SORTED: rows sorted by expert (two-way kind). Padding rows are zeros whatever
+// x holds there, so that they change no column group; a tile that begins with
+// padding is behind the last expert's rows: nothing reads its codes.
+template <bool BLOCK, bool TRANSPOSED, bool SORTED = false>
 __global__ void __launch_bounds__(kThreads, 4)
     cast_tiles_kernel(CastArgs a) {
   __shared__ __align__(16) uint8_t t_codes[TRANSPOSED ? kTile * kTile : 16];
@@ -81,11 +84,19 @@ __global__ void __launch_bounds__(kThreads, 4)
   griddep_wait();
   griddep_launch_dependents();
 
+  uint32_t held = 0xffu;  // bit i: row i of the eight counts
+  if (SORTED) {
+    if (a.sources[tr * kTile] < 0) return;
+    held = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (r0 + i < a.M && a.sources[r0 + i] >= 0) held |= 1u << i;
+  }
   uint32_t x[8][4];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     uint4 w = make_uint4(0, 0, 0, 0);
-    if (col_ok && r0 + i < a.M) w = ld_stream(a.x + (r0 + i) * a.ldx + c0);
+    if (col_ok && r0 + i < a.M && (!SORTED || (held >> i & 1u))) w = ld_stream(a.x + (r0 + i) * a.ldx + c0);
     x[i][0] = w.x, x[i][1] = w.y, x[i][2] = w.z, x[i][3] = w.w;
   }
   const uint32_t all = 0xffffffffu;
@@ -223,7 +234,8 @@ __global__ void __launch_bounds__(kThreads, 4)
 cudaError_t launch_cast_tiles(const CastArgs& a, bool block, cudaStream_t stream) {
   const int64_t tiles = ((a.M + kTile - 1) / kTile) * ((a.H + kTile - 1) / kTile);
   auto kernel = block ? (a.qt != nullptr ? cast_tiles_kernel<true, true> : cast_tiles_kernel<true, false>)
-                      : cast_tiles_kernel<false, true>;
+                      : a.sources != nullptr ? cast_tiles_kernel<false, true, true>
+                                             : cast_tiles_kernel<false, true>;
   return launch_pdl(kernel, (unsigned)tiles, kThreads, 0, stream, a);
 }
 

@@ -327,6 +327,8 @@ struct CastArgs {
   int64_t ldqt;
   float* st;    // block: [H/128, M/128], else group-major [M/128, H]
   int64_t ldst;
+  const int* sources;  // two-way kind: rows whose source is below zero count as zeros, and tiles
+                       // that begin with one are not written (null: all rows count)
 };
 cudaError_t launch_cast_tiles(const CastArgs& a, bool block, cudaStream_t stream);
 
@@ -354,6 +356,27 @@ inline bool aligned_rows_host(const void* p, int64_t ld_bytes, unsigned n) {
 }
 int block_gemm(const BlockGemmArgs& g, cudaStream_t stream, const char** why);
 cudaError_t device_error_block_gemm(int* out, bool clear);
+
+// The experts' products on sorted rows (block_gemm.cu), see cutie_fp8_grouped_gemm
+// and cutie_fp8_grouped_wgrad.
+struct GroupedGemmArgs {
+  bool columns;   // the weight gradient: columns are sorted, not rows
+  const void* a;  // e4m3 [R, K] (columns: [N, R]), 1 x 128 scales
+  int64_t lda;
+  const float* sa;
+  int64_t sa_row, sa_kb;
+  const void* b;  // e4m3 [E, N, K], 128 x 128 scales (columns: [K, R], 1 x 128)
+  int64_t ldb, b_expert;
+  const float* sb;
+  int64_t sb_row, sb_kb, sb_expert;
+  const int* offsets;
+  void* d;  // [R, N] (columns: [E, N, K])
+  int64_t ldd, d_expert;
+  bool d_f32;
+  int64_t E, R, N, K;
+  long long wait_limit;
+};
+int grouped_gemm(const GroupedGemmArgs& g, cudaStream_t stream, const char** why);
 
 // Mixture-of-experts layer for few tokens (moe.cu).
 constexpr int kMoeMaxTokens = 64, kMoeMaxExperts = 512, kMoeMaxTopK = 16;

@@ -434,5 +434,21 @@ inline bool encode_e4m3_operand(CUtensorMap* map, const void* ptr, int64_t rows,
   });
 }
 
+// The same for n matrices `each` bytes apart (a multiple of 16): boxes of one of them.
+inline bool encode_e4m3_matrices(CUtensorMap* map, const void* ptr, int64_t n, int64_t rows, int64_t K,
+                                 int64_t ld, int64_t each, int box_rows = 128) {
+  auto fn = encode_fn();
+  if (fn == nullptr) return false;
+  const cuuint64_t dims[3] = {(cuuint64_t)K, (cuuint64_t)rows, (cuuint64_t)n};
+  const cuuint64_t strides[2] = {(cuuint64_t)ld, (cuuint64_t)each};
+  const cuuint32_t box[3] = {128, (cuuint32_t)box_rows, 1};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  return encode_with_context([&] {
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(ptr), dims, strides, box,
+              estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  });
+}
+
 }  // namespace tc
 }  // namespace cutie

@@ -309,14 +309,20 @@ struct CastPlace {
   // Without a place for the transpose's the block kind writes none. A matrix
   // whose rows are not dense, overlap or start off the 16-byte boundaries is
   // copied first; that of a single row too: the kernel reads C neighbouring
-  // elements.
-  void cast(const at::Tensor& any, void* stream) const {
+  // elements. With `sources` the rows are sorted by expert.
+  void cast(const at::Tensor& any, void* stream, const void* sources = nullptr) const {
     if (R == 0 || C == 0) return;  // no codes
     const bool dense = (C <= 1 || any.stride(1) == 1) &&
                        (R <= 1 || (any.stride(0) >= C && any.stride(0) % 8 == 0)) &&
                        reinterpret_cast<uintptr_t>(any.data_ptr()) % 16 == 0;
     const at::Tensor x = dense ? any : any.clone(at::MemoryFormat::Contiguous);
     const Operand q = rows(), qt = column_base != nullptr ? columns() : Operand();
+    if (sources != nullptr) {
+      check_status(cutie_cast_fp8_sorted(
+          x.data_ptr(), x.stride(0), R, C, sources, CUTIE_SCALE_FP32 + (gradient ? CUTIE_SCALE_GRADIENT : 0), row_base,
+          q.ld, row_base + off_s, q.s_kb, column_base, qt.ld, column_base + off_st, qt.s_kb, stream));
+      return;
+    }
     check_status(cutie_cast_fp8_tiles(
         x.data_ptr(), R <= 1 ? ceil_to(C, 8) : x.stride(0), R, C,
         block ? CUTIE_TILE_BLOCK : CUTIE_TILE_TWO_WAY,
@@ -447,6 +453,187 @@ at::Tensor fp8_linear(const at::Tensor& x, const at::Tensor& weight,
   auto shape = x.sizes().vec();
   shape.back() = weight.size(0);
   return y.reshape(shape);
+}
+
+void no_second_derivatives(const char* name) {
+  if (at::GradMode::is_enabled())
+    throw std::runtime_error(std::string(name) + " has no second derivatives (create_graph)");
+}
+
+// ---- The experts' products on sorted rows (cutie_fp8_grouped_gemm, _wgrad).
+
+// A plan's offsets as the products take them.
+void product_offsets(const at::Tensor& offsets, int64_t align, int64_t E, const at::Device& dev) {
+  if (align <= 0 || align % 128 != 0) bad("the experts' products need a plan with align a multiple of 128");
+  if (offsets.dim() != 1 || offsets.size(0) != E + 1 || offsets.scalar_type() != at::kInt ||
+      !offsets.is_contiguous() || offsets.device() != dev)
+    bad("the plan's offsets must be a contiguous int32 [E + 1] tensor on the rows' device, E = " + std::to_string(E));
+}
+
+// Matrices [E, N, K] of codes and their scales [E, ceil(N/128), ceil(K/128)].
+struct Matrices {
+  const void* q;
+  int64_t ld, each;
+  const void* s;
+  int64_t s_row, s_kb, s_each;
+};
+Matrices expert_matrices(const at::Tensor& q, const at::Tensor& s, int64_t E, int64_t N, int64_t K,
+                         const at::Device& dev, const char* name) {
+  check_codes(q, name);
+  if (q.dim() != 3 || q.size(0) != E || q.size(1) != N || q.size(2) != K)
+    bad(std::string(name) + " must have shape (" + std::to_string(E) + ", " + std::to_string(N) + ", " +
+        std::to_string(K) + ")");
+  if (q.device() != dev) bad(std::string(name) + " is on the wrong device");
+  if (K > 1 && q.stride(2) != 1) bad(std::string(name) + " must be contiguous along its last dimension");
+  if (N > 1 && q.stride(1) < K) bad(std::string(name) + " must not have overlapping rows");
+  if (s.dim() != 3 || s.size(0) != E || s.size(1) != (N + 127) / 128 || s.size(2) != (K + 127) / 128 ||
+      s.scalar_type() != at::kFloat || s.device() != dev)
+    bad(std::string(name) + "'s scales must be float32, one a 128 x 128 block of each expert");
+  return {q.data_ptr(), N > 1 ? q.stride(1) : ceil_to(K, 16), E > 1 ? q.stride(0) : 0,
+          s.data_ptr(), s.stride(1), s.stride(2), s.stride(0)};
+}
+
+void grouped_product(const Operand& a, const Matrices& b, const at::Tensor& offsets, int64_t E, const at::Tensor& d,
+                     int64_t ldd, int64_t R, int64_t N, int64_t K, void* stream) {
+  check_status(cutie_fp8_grouped_gemm(
+      a.q, a.ld, a.s, a.s_row, a.s_kb, b.q, b.ld, b.each, b.s, b.s_row, b.s_kb, b.s_each, offsets.data_ptr(), E,
+      d.data_ptr(), ldd, d.scalar_type() == at::kFloat ? CUTIE_DTYPE_F32 : CUTIE_DTYPE_BF16, R, N, K, stream));
+}
+
+at::Tensor fp8_grouped_gemm(const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor& b,
+                            const at::Tensor& b_scale, const at::Tensor& offsets, int64_t align,
+                            const c10::optional<at::Tensor>& out, bool out_f32) {
+  if (!a.is_cuda()) bad("a must be a CUDA tensor (this library has no CPU path)");
+  const at::Device dev = a.device();
+  check_codes(a, "a");
+  const int64_t lda = matrix_ld(a, "a", dev);
+  if (b.dim() != 3) bad("b must be 3-D [E, N, K]");
+  const int64_t R = a.size(0), K = a.size(1), E = b.size(0), N = b.size(1);
+  product_offsets(offsets, align, E, dev);
+  if (a_scale.dim() != 2 || a_scale.size(0) != R || a_scale.size(1) != (K + 127) / 128 ||
+      a_scale.scalar_type() != at::kFloat || a_scale.device() != dev)
+    bad("a_scale must be a float32 [R, ceil(K/128)] tensor on a's device");
+  const Matrices m = expert_matrices(b, b_scale, E, N, K, dev, "b");
+  const c10::cuda::CUDAGuard guard(dev);
+  if (out.has_value()) {
+    if (out->dim() != 2 || out->size(0) != R || out->size(1) != N || out->device() != dev)
+      bad("out must have shape (" + std::to_string(R) + ", " + std::to_string(N) + ") and be on a's device");
+    if (out->scalar_type() != at::kBFloat16 && out->scalar_type() != at::kFloat)
+      bad("out must be bfloat16 or float32");
+  }
+  at::Tensor d = out.has_value() ? *out
+                                 : at::empty({R, N}, at::TensorOptions().device(dev).dtype(
+                                                         out_f32 ? at::kFloat : at::kBFloat16));
+  const Operand rows{a.data_ptr(), lda, a_scale.data_ptr(), a_scale.stride(0), a_scale.stride(1)};
+  grouped_product(rows, m, offsets, E, d, matrix_ld(d, "out", dev), R, N, K,
+                  at::cuda::getCurrentCUDAStream(dev.index()).stream());
+  return d;
+}
+
+struct FP8GroupedLinear : public torch::autograd::Function<FP8GroupedLinear> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight,
+                            const c10::optional<at::Tensor>& wq, const c10::optional<at::Tensor>& ws,
+                            const c10::optional<at::Tensor>& wqt, const c10::optional<at::Tensor>& wst,
+                            const at::Tensor& sources, const at::Tensor& offsets, bool need_dx, bool need_dw) {
+    const at::Device dev = x.device();
+    const int64_t R = x.size(0), E = weight.size(0), N = weight.size(1), K = weight.size(2);
+    const c10::cuda::CUDAGuard guard(dev);
+    void* stream = at::cuda::getCurrentCUDAStream(dev.index()).stream();
+    CastPlace w(E * N, K, true), xs(R, K, false);  // blocks of 128 do not cross experts: N is a multiple
+    const bool own = !wq.has_value();
+    // what backward reads: the weight's transposed codes, then x's; the rest goes with this call
+    const int64_t held_w = own && need_dx ? w.column_bytes : 0, held_x = need_dw ? xs.column_bytes : 0;
+    const at::Tensor held = held_w + held_x > 0 ? bytes(held_w + held_x, x) : at::Tensor();
+    const at::Tensor scratch = bytes(xs.row_bytes + (own ? w.row_bytes : 0) + (need_dw ? 0 : xs.column_bytes), x);
+    xs.row_base = address(scratch);
+    if (own) {
+      w.row_base = xs.row_base + xs.row_bytes;
+      if (held_w > 0) w.column_base = address(held);
+      const at::Tensor flat = weight.reshape({E * N, K});
+      w.cast(flat.scalar_type() == at::kBFloat16 ? flat : flat.to(at::kBFloat16), stream);
+    }
+    xs.column_base = held_x > 0 ? address(held) + held_w : xs.row_base + xs.row_bytes + (own ? w.row_bytes : 0);
+    xs.cast(x, stream, sources.data_ptr());
+    at::Tensor y = at::empty({R, N}, x.options());
+    Matrices m;
+    if (own) {
+      const Operand q = w.rows();
+      m = {q.q, q.ld, N * q.ld, q.s, q.s_row, q.s_kb, N / 128 * q.s_row};
+    } else {
+      m = expert_matrices(*wq, *ws, E, N, K, dev, "weight_fp8");
+    }
+    grouped_product(xs.rows(), m, offsets, E, y, N, R, N, K, stream);
+    ctx->save_for_backward({held, !own && need_dx ? *wqt : at::Tensor(), !own && need_dx ? *wst : at::Tensor(),
+                            sources, offsets});
+    ctx->saved_data["sizes"] =
+        std::vector<int64_t>{E, N, K, need_dx, need_dw, !own, weight.scalar_type() == at::kFloat};
+    return y;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    no_second_derivatives("fp8_grouped_linear");
+    torch::autograd::variable_list out(10);
+    if (!grads[0].defined()) return out;
+    const auto saved = ctx->get_saved_variables();
+    const auto sizes = ctx->saved_data["sizes"].toIntVector();
+    const int64_t E = sizes[0], N = sizes[1], K = sizes[2];
+    const bool need_dx = sizes[3], need_dw = sizes[4], given_w = sizes[5], dw_f32 = sizes[6];
+    const at::Tensor &dy = grads[0], &sources = saved[3], &offsets = saved[4];
+    const int64_t R = dy.size(0);
+    const at::Device dev = dy.device();
+    const c10::cuda::CUDAGuard guard(dev);
+    void* stream = at::cuda::getCurrentCUDAStream(dev.index()).stream();
+    CastPlace d(R, N, false, true), w(E * N, K, true), xs(R, K, false);
+    const at::Tensor codes = bytes(d.row_bytes + d.column_bytes, dy);
+    d.row_base = address(codes), d.column_base = address(codes) + d.row_bytes;
+    d.cast(dy, stream, sources.data_ptr());
+    if (need_dx) {
+      Matrices m;
+      if (given_w) {
+        m = expert_matrices(saved[1], saved[2], E, K, N, dev, "weight_fp8");
+      } else {
+        w.column_base = address(saved[0]);
+        const Operand q = w.columns();  // [K, E N]: an expert's transpose is N of its columns
+        m = {q.q, q.ld, N, q.s, q.s_row, q.s_kb, N / 128};
+      }
+      out[0] = at::empty({R, K}, dy.options());
+      grouped_product(d.rows(), m, offsets, E, out[0], K, R, K, N, stream);
+    }
+    if (need_dw) {
+      xs.column_base = address(saved[0]) + (need_dx && !given_w ? w.column_bytes : 0);
+      const Operand a = d.columns(), b = xs.columns();
+      out[1] = at::empty({E, N, K}, dy.options().dtype(dw_f32 ? at::kFloat : at::kBFloat16));
+      check_status(cutie_fp8_grouped_wgrad(a.q, a.ld, a.s, a.s_row, a.s_kb, b.q, b.ld, b.s, b.s_row, b.s_kb,
+                                           offsets.data_ptr(), E, out[1].data_ptr(), K, N * K,
+                                           dw_f32 ? CUTIE_DTYPE_F32 : CUTIE_DTYPE_BF16, R, N, K, stream));
+    }
+    return out;
+  }
+};
+
+at::Tensor fp8_grouped_linear(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& sources,
+                              const at::Tensor& offsets, int64_t align, const c10::optional<at::Tensor>& wq,
+                              const c10::optional<at::Tensor>& ws, const c10::optional<at::Tensor>& wqt,
+                              const c10::optional<at::Tensor>& wst) {
+  if (x.dim() != 2 || weight.dim() != 3 || x.size(1) != weight.size(2)) bad("x and weight must be [R, K] and [E, N, K]");
+  if (!x.is_cuda()) bad("x must be a CUDA tensor (this library has no CPU path)");
+  const at::Device dev = x.device();
+  if (weight.device() != dev) bad("weight is on the wrong device");
+  if (x.scalar_type() != at::kBFloat16) bad("x must be bfloat16");
+  if (weight.scalar_type() != at::kBFloat16 && weight.scalar_type() != at::kFloat)
+    bad("weight must be bfloat16 or float32");
+  const int64_t R = x.size(0), E = weight.size(0), N = weight.size(1), K = weight.size(2);
+  if (E == 0 || N == 0 || K == 0 || N % 128 != 0 || K % 128 != 0) bad("weight's sizes must be multiples of 128");
+  product_offsets(offsets, align, E, dev);
+  if (sources.dim() != 1 || sources.size(0) != R || sources.scalar_type() != at::kInt || !sources.is_contiguous() ||
+      sources.device() != dev)
+    bad("x must have the plan's " + std::to_string(sources.size(0)) + " rows, the plan be int32 on x's device");
+  const bool grad = at::GradMode::is_enabled();
+  const bool need_dx = grad && x.requires_grad(), need_dw = grad && weight.requires_grad();
+  if (wq.has_value() != ws.has_value()) bad("weight_fp8 must be (q, s, qt, st)");
+  if (wq.has_value() && need_dx && (!wqt.has_value() || !wst.has_value()))
+    bad("weight_fp8 has no transposed codes: make it with quantize_experts(weight, transposed=True)");
+  return FP8GroupedLinear::apply(x, weight, wq, ws, wqt, wst, sources, offsets, need_dx, need_dw);
 }
 
 // Bytes of workspace of a mixture-of-experts layer; argument errors raise.
@@ -596,11 +783,6 @@ at::Tensor combine_rows(const at::Tensor& any, const at::Tensor& weights, const 
   return out;
 }
 
-void no_second_derivatives(const char* name) {
-  if (at::GradMode::is_enabled())
-    throw std::runtime_error(std::string(name) + " has no second derivatives (create_graph)");
-}
-
 struct MoePermute : public torch::autograd::Function<MoePermute> {
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& sources,
                             const at::Tensor& positions) {
@@ -710,6 +892,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("bias"), py::arg("w13"), py::arg("w13_scale"), py::arg("w2"), py::arg("w2_scale"),
         py::arg("top_k"), py::arg("scoring"), py::arg("renormalize"), py::arg("routed_scale"),
         py::arg("out"), py::arg("topk_ids"), py::arg("topk_weights"), py::arg("workspace"));
+  m.def("fp8_grouped_gemm", &fp8_grouped_gemm, py::arg("a"), py::arg("a_scale"), py::arg("b"), py::arg("b_scale"),
+        py::arg("offsets"), py::arg("align"), py::arg("out"), py::arg("out_f32"));
+  m.def("fp8_grouped_linear", &fp8_grouped_linear, py::arg("x"), py::arg("weight"), py::arg("sources"),
+        py::arg("offsets"), py::arg("align"), py::arg("wq"), py::arg("ws"), py::arg("wqt"), py::arg("wst"));
   m.def("moe_plan_rows", &moe_plan_rows, py::arg("T"), py::arg("k"), py::arg("E"), py::arg("align"));
   m.def("moe_sort", &moe_sort, py::arg("ids"), py::arg("E"), py::arg("align"));
   m.def("moe_permute", &moe_permute, py::arg("x"), py::arg("sources"), py::arg("positions"));

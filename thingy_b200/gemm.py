@@ -173,3 +173,23 @@ def fp8_block_gemm(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_sc
         raise ValueError(f"out_dtype must be bfloat16 or float32, got {out_dtype}")
     return require_binding().fp8_block_gemm(a, a_scale, b, b_scale, out,
                                             out_dtype == torch.float32, bool(accumulate))
+
+
+def fp8_grouped_gemm(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor, plan,
+                     out: torch.Tensor | None = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """[R, N]: the rows of each expert times its matrix, (a * a_scale) @ (b[e] * b_scale[e]).T, on the current stream.
+
+    ``plan``: a ``MoePlan`` with ``align`` a multiple of 128. a: e4m3 [R, K] in
+    the plan's order, a_scale: fp32 [R, ceil(K/128)] in any layout
+    (``moe_permute`` of codes and of scales); b: e4m3 [E, N, K], b_scale: fp32
+    [E, ceil(N/128), ceil(K/128)] (``quantize_experts``), of any strides with
+    dense rows. N is a multiple of 16 (fp32 out: 8); rows of a and b start on 16-byte
+    boundaries, those of out on 32-byte ones. Sums are held in fp32, rounded once.
+    Rows in padding are what a holds there (zeros from ``moe_permute``) times
+    the matrix; rows behind the last expert's are zero. Forward only:
+    ``fp8_grouped_linear`` is the layer with gradients.
+    """
+    if out_dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"out_dtype must be bfloat16 or float32, got {out_dtype}")
+    return require_binding().fp8_grouped_gemm(a, a_scale, b, b_scale, plan.offsets, plan.align, out,
+                                              out_dtype == torch.float32)

@@ -35,3 +35,20 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_fp8=None) -> torch.
     """
     wq, ws, wqt, wst = (None, None, None, None) if weight_fp8 is None else weight_fp8
     return require_binding().fp8_linear(x, weight, wq, ws, wqt, wst)
+
+
+def fp8_grouped_linear(x: torch.Tensor, weight: torch.Tensor, plan, weight_fp8=None) -> torch.Tensor:
+    """bf16 [R, N]: the experts' ``fp8_linear`` on sorted rows, ``x[r] @ weight[e].T`` for the rows of expert e.
+
+    ``plan``: a ``MoePlan`` with ``align`` a multiple of 128; x: bf16 [R, K] in
+    its order (``moe_permute``), weight: bf16 or fp32 [E, N, K], K and N
+    multiples of 128. Rows in padding count as zeros, whatever x and the
+    gradient hold there, and come back as zeros; an expert without rows has a
+    zero weight gradient. ``weight_fp8``: (q, s, qt, st) of
+    ``quantize_experts(weight, transposed=True)``, cast once for several calls
+    (inference: (q, s, None, None)). Casts, gradients and their scales are
+    ``fp8_linear``'s, expert by expert: groups of 128 along the rows never hold
+    rows of two experts. Nothing is copied to the host.
+    """
+    wq, ws, wqt, wst = (None, None, None, None) if weight_fp8 is None else weight_fp8
+    return require_binding().fp8_grouped_linear(x, weight, plan.sources, plan.offsets, plan.align, wq, ws, wqt, wst)

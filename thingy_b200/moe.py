@@ -110,10 +110,19 @@ def moe_fp8(
                        topk_weights, workspace)
 
 
-def quantize_experts(w: torch.Tensor, use_ue8m0: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
-    """bf16 [E, R, C] -> e4m3 codes [E, R, C] and fp32 scales [E, R/128, C/128] of 128 x 128 blocks."""
+def quantize_experts(w: torch.Tensor, use_ue8m0: bool = False, transposed: bool = False):
+    """bf16 [E, R, C] -> e4m3 codes [E, R, C] and fp32 scales [E, R/128, C/128] of 128 x 128 blocks.
+
+    With ``transposed`` returns (q, s, qt, st): also the codes [E, C, R] of the
+    matrices' transposes and their scales [E, C/128, R/128], for input
+    gradients (``fp8_grouped_linear``); those are views of all experts side by side.
+    """
     if w.dim() != 3 or w.shape[1] % 128 != 0 or w.shape[2] % 128 != 0:
         raise ValueError(f"w must be [E, R, C] with R and C multiples of 128, got {tuple(w.shape)}")
     E, R, C = w.shape
+    if transposed:
+        q, s, qt, st = per_block_cast_to_fp8(w.reshape(E * R, C), use_ue8m0, transposed=True)
+        return (q.view(E, R, C), s.view(E, R // 128, C // 128), qt.view(C, E, R).transpose(0, 1),
+                st.view(C // 128, E, R // 128).transpose(0, 1))
     q, s = per_block_cast_to_fp8(w.reshape(E * R, C), use_ue8m0)
     return q.view(E, R, C), s.view(E, R // 128, C // 128)
