@@ -475,6 +475,34 @@ CUTIE_API int cutie_moe_combine_backward(const void* d_out, int64_t ldd, const v
                                          int64_t lddr, void* d_weights, void* stream);
 
 /*
+ * One step of AdamW over `count` tensors in as few launches as their table
+ * needs (480 tensors each). For every element, in fp32 and rounded operation
+ * by operation:
+ *   g' = g grad_scale;  m' = b1 m + (1 - b1) g';  v' = b2 v + (1 - b2) (g' g')
+ *   p' = p (1 - lr decay) - (lr / (1 - b1^step)) (m' / (sqrt(v') / sqrt(1 - b2^step) + eps))
+ * params, grads, exp_avg, exp_avg_sq: host arrays of device pointers to sizes[i]
+ * contiguous elements; param_dtype and grad_dtype: CUTIE_DTYPE_*, the same, or
+ * fp32 gradients, or bf16 gradients of fp32 parameters. Without scales
+ * (avg_scale, sq_scale NULL) the states are fp32; with them exp_avg holds e4m3
+ * codes of m, exp_avg_sq of sqrt(v), and the scales fp32 values a group of 128
+ * elements of a tensor (the last group may be shorter), max(amax / 448, 2^-92).
+ * Codes are rounded up or down at random, the nearer the likelier, by a hash of
+ * (seed, step, the tensor's index in the list, the element): the same inputs
+ * give the same bits. An infinite gradient makes its group's codes NaN.
+ * step >= 1, or step_ptr: an int64 on the GPU (read when the kernel runs, so a
+ * captured call may count); lr, or lr_ptr: an fp32 on the GPU. grad_scale: an fp32
+ * on the GPU or NULL. Any alignment of elements; 16-byte aligned tensors (codes
+ * 8) are faster. No tensor may overlap another. Asynchronous on `stream`.
+ */
+CUTIE_API int cutie_adamw(int64_t count, void* const* params, int param_dtype,
+                          const void* const* grads, int grad_dtype, void* const* exp_avg,
+                          void* const* avg_scale, void* const* exp_avg_sq, void* const* sq_scale,
+                          const int64_t* sizes, int64_t step, const void* step_ptr, double lr,
+                          const void* lr_ptr, double beta1, double beta2, double eps,
+                          double weight_decay, const void* grad_scale, uint64_t seed,
+                          void* stream);
+
+/*
  * Device-side status of this library's kernels on the current device: 0 when
  * no kernel has hit a failure since the last clear; otherwise the first error
  * code recorded (1 = a bulk-copy wait ran out: a row never arrived in shared

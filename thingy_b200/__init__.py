@@ -24,6 +24,8 @@ Drop-in host API for the reference's hot path (S1ro1/thingy, package
                                                applied, and the gradients (no counterpart)
     fp8_grouped_gemm, fp8_grouped_linear    the experts' products on sorted rows, and their
                                                linear layer with its gradients (no counterpart)
+    adamw_step, adamw_state, AdamW          an optimizer step over many tensors in one launch,
+                                               states in 32 bits or in 8 (no counterpart)
 
 Every op runs hand-written CUDA from ``lib/libcutie_b200.so`` through the C
 ABI in ``include/cutie.h``; there is no CPU or PyTorch fallback.
@@ -38,12 +40,16 @@ from .gemm import fp8_block_gemm, fp8_grouped_gemm
 from .layouts import mx_swizzle, mx_swizzle_offset, mx_swizzled_size, mx_unswizzle
 from .linear import fp8_grouped_linear, fp8_linear
 from .moe import clear_moe_workspaces, moe_fp8, moe_workspace, quantize_experts
+from .optim import AdamW, adamw_state, adamw_step
 from .rms_norm import RMSNorm, rms_norm, rms_norm_on_stream
 
 __all__ = [
+    "AdamW",
     "MoePlan",
     "RMSNorm",
     "ResidualRMSNormFP8",
+    "adamw_state",
+    "adamw_step",
     "clear_moe_workspaces",
     "empty_scale",
     "fp8_block_gemm",

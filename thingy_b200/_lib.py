@@ -53,6 +53,7 @@ EXPORTED_SYMBOLS = (
     "cutie_moe_permute",
     "cutie_moe_combine",
     "cutie_moe_combine_backward",
+    "cutie_adamw",
     "cutie_device_error",
     "cutie_set_wait_limit",
     "cutie_last_error",
@@ -142,6 +143,11 @@ _SIGNATURES = {
     "cutie_moe_combine_backward": (
         _int,
         [_ptr, _i64, _ptr, _i64, _int, _ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _ptr, _i64, _ptr, _ptr],
+    ),
+    "cutie_adamw": (
+        _int,
+        [_i64, _ptr, _int, _ptr, _int, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _ptr, ctypes.c_double, _ptr,
+         ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double, _ptr, ctypes.c_uint64, _ptr],
     ),
     "cutie_device_error": (_int, [_int]),
     "cutie_set_wait_limit": (_i64, [_i64]),

@@ -1267,6 +1267,68 @@ extern "C" int cutie_moe_combine_backward(const void* d_out, int64_t ldd, const 
   return e == cudaSuccess ? CUTIE_OK : cuda_fail(e, "moe combine backward launch");
 }
 
+extern "C" int cutie_adamw(int64_t count, void* const* params, int param_dtype, const void* const* grads,
+                           int grad_dtype, void* const* exp_avg, void* const* avg_scale, void* const* exp_avg_sq,
+                           void* const* sq_scale, const int64_t* sizes, int64_t step, const void* step_ptr, double lr,
+                           const void* lr_ptr, double beta1, double beta2, double eps, double weight_decay,
+                           const void* grad_scale, uint64_t seed, void* stream) {
+  g_err[0] = '\0';
+  if (count < 0) return fail(CUTIE_ERR_INVALID_ARGUMENT, "count must not be negative (got %lld)", (long long)count);
+  const int ps = row_dtype_bytes(param_dtype), gs = row_dtype_bytes(grad_dtype);
+  if (ps == 0 || gs == 0)
+    return fail(CUTIE_ERR_INVALID_ARGUMENT, "unknown dtype %d of parameters or %d of gradients", param_dtype, grad_dtype);
+  if (param_dtype != grad_dtype && grad_dtype != CUTIE_DTYPE_F32 &&
+      !(param_dtype == CUTIE_DTYPE_F32 && grad_dtype == CUTIE_DTYPE_BF16))
+    return fail(CUTIE_ERR_UNSUPPORTED,
+                "gradients have the parameters' dtype, or fp32, or bf16 for fp32 parameters (dtypes %d and %d)",
+                grad_dtype, param_dtype);
+  // written so that a NaN is refused
+  if (!(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1))
+    return fail(CUTIE_ERR_INVALID_ARGUMENT, "betas must be in [0, 1) (got %g, %g)", beta1, beta2);
+  if (!(eps >= 0 && eps <= 3e38) || !(weight_decay >= 0 && weight_decay <= 3e38))
+    return fail(CUTIE_ERR_INVALID_ARGUMENT, "eps and weight_decay must not be negative (got %g, %g)", eps, weight_decay);
+  if (lr_ptr == nullptr && !(lr >= 0 && lr <= 3e38))
+    return fail(CUTIE_ERR_INVALID_ARGUMENT, "lr must not be negative (got %g)", lr);
+  if (step_ptr == nullptr && step < 1)
+    return fail(CUTIE_ERR_INVALID_ARGUMENT, "step counts from 1 (got %lld)", (long long)step);
+  if (!aligned(step_ptr, 8) || !aligned(lr_ptr, 4) || !aligned(grad_scale, 4))
+    return fail(CUTIE_ERR_ALIGNMENT, "step, lr and grad_scale must be aligned to their elements");
+  if ((avg_scale == nullptr) != (sq_scale == nullptr))
+    return fail(CUTIE_ERR_INVALID_ARGUMENT, "avg_scale and sq_scale must be given together");
+  if (count == 0) return CUTIE_OK;
+  if (params == nullptr || grads == nullptr || exp_avg == nullptr || exp_avg_sq == nullptr || sizes == nullptr)
+    return fail(CUTIE_ERR_INVALID_ARGUMENT, "the lists must not be NULL");
+  if (count > INT32_MAX) return fail(CUTIE_ERR_UNSUPPORTED, "at most 2^31 - 1 tensors");
+  const uintptr_t ss = avg_scale != nullptr ? 1 : 4;
+  for (int64_t i = 0; i < count; ++i) {
+    if (sizes[i] < 0 || sizes[i] > (int64_t(1) << 40))
+      return fail(CUTIE_ERR_INVALID_ARGUMENT, "tensor %lld has %lld elements: 0 to 2^40 are taken", (long long)i,
+                  (long long)sizes[i]);
+    if (sizes[i] == 0) continue;
+    if (params[i] == nullptr || grads[i] == nullptr || exp_avg[i] == nullptr || exp_avg_sq[i] == nullptr ||
+        (avg_scale != nullptr && (avg_scale[i] == nullptr || sq_scale[i] == nullptr)))
+      return fail(CUTIE_ERR_INVALID_ARGUMENT, "tensor %lld: a pointer is NULL", (long long)i);
+    if (!aligned(params[i], ps) || !aligned(grads[i], gs) || !aligned(exp_avg[i], ss) || !aligned(exp_avg_sq[i], ss) ||
+        (avg_scale != nullptr && (!aligned(avg_scale[i], 4) || !aligned(sq_scale[i], 4))))
+      return fail(CUTIE_ERR_ALIGNMENT, "tensor %lld must be aligned to its elements", (long long)i);
+  }
+  AdamwTensors l{params, grads, exp_avg, exp_avg_sq, reinterpret_cast<float* const*>(avg_scale),
+                 reinterpret_cast<float* const*>(sq_scale), sizes, count, param_dtype, grad_dtype};
+  AdamwStep a{};
+  a.lr = lr, a.decay = weight_decay, a.beta1 = beta1, a.beta2 = beta2;
+  a.bias1 = 1.0 - std::pow(beta1, (double)step);
+  a.root = (float)(1.0 / std::sqrt(1.0 - std::pow(beta2, (double)step)));
+  a.eps = (float)eps, a.b1 = (float)beta1, a.b2 = (float)beta2;
+  a.c1 = (float)(1.0 - beta1), a.c2 = (float)(1.0 - beta2);
+  a.step = step;
+  a.step_ptr = static_cast<const int64_t*>(step_ptr);
+  a.lr_ptr = static_cast<const float*>(lr_ptr);
+  a.clip = static_cast<const float*>(grad_scale);
+  a.seed_key = adamw_seed_key(seed);
+  const cudaError_t e = adamw(l, a, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? CUTIE_OK : cuda_fail(e, "adamw launch");
+}
+
 extern "C" int cutie_device_error(int clear) {
   g_err[0] = '\0';
   int any = 0;

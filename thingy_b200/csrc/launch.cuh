@@ -437,6 +437,30 @@ cudaError_t moe_sort(const void* ids, bool wide, int n, int E, int align, int* s
 cudaError_t moe_permute(const MoeRows& p, cudaStream_t stream);
 cudaError_t moe_combine(const MoeRows& p, int dtype, bool backward, cudaStream_t stream);
 
+// AdamW over a list of tensors (adamw.cu); host arrays of `count`.
+struct AdamwTensors {
+  void* const* p;
+  const void* const* g;
+  void* const* m;  // fp32, or e4m3 codes with scales ms and vs
+  void* const* v;
+  float* const* ms;  // null: states in 32 bits
+  float* const* vs;
+  const int64_t* n;
+  int64_t count;
+  int p_dtype, g_dtype;
+};
+struct AdamwStep {
+  double lr, decay, beta1, beta2, bias1;  // bias1 = 1 - beta1^step
+  float root, eps, b1, b2, c1, c2;        // root = 1 / sqrt(1 - beta2^step), c = 1 - b
+  int64_t step;
+  const int64_t* step_ptr;  // on the GPU, in the place of the host's value; or null
+  const float* lr_ptr;
+  const float* clip;  // factor of the gradients, or null
+  uint32_t seed_key;
+};
+uint32_t adamw_seed_key(uint64_t seed);
+cudaError_t adamw(const AdamwTensors& l, const AdamwStep& a, cudaStream_t stream);
+
 struct F32Args {
   const float* x;
   int64_t ldx;

@@ -8,10 +8,14 @@
 // RuntimeError (the status codes of cutie.h).
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <stdexcept>
 #include <string>
+#include <utility>
+#include <vector>
 
 #include "cutie.h"
 
@@ -870,6 +874,135 @@ at::Tensor moe_combine(const at::Tensor& ys, const at::Tensor& weights, const at
   return combine_rows(ys, weights.contiguous(), positions);
 }
 
+// ---- AdamW over lists of tensors (cutie_adamw). The lists are read as Python
+// sequences here: hundreds of tensors would cost more in argument conversion
+// than in the kernel.
+struct Sequence {
+  PyObject* fast;
+  explicit Sequence(PyObject* o, const char* name) : fast(PySequence_Fast(o, "")) {
+    if (fast == nullptr) {
+      PyErr_Clear();
+      bad(std::string(name) + " must be a sequence of tensors");
+    }
+  }
+  Sequence(const Sequence&) = delete;
+  ~Sequence() { Py_DECREF(fast); }
+  int64_t size() const { return PySequence_Fast_GET_SIZE(fast); }
+  PyObject* operator[](int64_t i) const { return PySequence_Fast_GET_ITEM(fast, i); }
+};
+
+const at::Tensor& tensor_of(PyObject* o, const char* name) {
+  if (!THPVariable_Check(o)) bad(std::string(name) + " must hold tensors");
+  return THPVariable_Unpack(o);
+}
+
+// Written ranges must not overlap: a tensor listed twice would be a race.
+void check_apart(std::vector<std::pair<uintptr_t, uintptr_t>>& ranges, const char* name) {
+  const auto after = [](const auto& x, const auto& y) { return x.second <= y.first; };
+  bool sorted = true;
+  for (size_t i = 1; i < ranges.size() && sorted; ++i) sorted = after(ranges[i - 1], ranges[i]);
+  if (sorted) return;
+  std::sort(ranges.begin(), ranges.end());
+  for (size_t i = 1; i < ranges.size(); ++i)
+    if (!after(ranges[i - 1], ranges[i])) bad(std::string(name) + " must not overlap one another");
+}
+
+// A step or a rate: a number, or one element on the GPU.
+const at::Tensor* device_scalar(PyObject* o, const char* name, at::ScalarType dtype, const at::Device& dev) {
+  if (!THPVariable_Check(o)) return nullptr;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (t.numel() != 1 || t.scalar_type() != dtype || t.device() != dev)
+    bad(std::string(name) + " must be a number or one " + (dtype == at::kLong ? "int64" : "float32") +
+        " on the parameters' device");
+  return &t;
+}
+
+void adamw_step(const py::object& params, const py::object& grads, const py::object& avgs, const py::object& sqs,
+                const py::object& step, const py::object& lr, double beta1, double beta2, double eps,
+                double weight_decay, const c10::optional<at::Tensor>& grad_scale, int64_t seed) {
+  const Sequence P(params.ptr(), "params"), G(grads.ptr(), "grads"), M(avgs.ptr(), "exp_avgs"), V(sqs.ptr(), "exp_avg_sqs");
+  const int64_t count = P.size();
+  if (G.size() != count || M.size() != count || V.size() != count)
+    bad("params, grads, exp_avgs and exp_avg_sqs must have the same length");
+  if (count == 0) return;
+  const at::Tensor& p0 = tensor_of(P[0], "params");
+  const at::Tensor& g0 = tensor_of(G[0], "grads");
+  if (!p0.is_cuda()) bad("params must be CUDA tensors (this library has no CPU path)");
+  const at::Device dev = p0.device();
+  const int p_dtype = row_dtype(p0, "params"), g_dtype = row_dtype(g0, "grads");
+  const bool codes = PyTuple_Check(M[0]) || PyList_Check(M[0]);
+  const c10::cuda::CUDAGuard guard(dev);
+  std::vector<void*> p(count), m(count), v(count), ms, vs;
+  std::vector<const void*> g(count);
+  std::vector<int64_t> n(count);
+  if (codes) ms.resize(count), vs.resize(count);
+  std::vector<at::Tensor> copies;  // of gradients that are not dense
+  std::vector<std::pair<uintptr_t, uintptr_t>> rp, rm, rv;
+  rp.reserve(count), rm.reserve(count), rv.reserve(count);
+  const auto range = [](std::vector<std::pair<uintptr_t, uintptr_t>>& r, const at::Tensor& t) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(t.data_ptr());
+    if (t.numel() > 0) r.emplace_back(a, a + t.numel() * t.element_size());
+  };
+  const auto state = [&](PyObject* o, int64_t i, const at::Tensor& param, const char* name, void** place, void** scale,
+                         std::vector<std::pair<uintptr_t, uintptr_t>>& r) {
+    if ((PyTuple_Check(o) || PyList_Check(o)) != codes)
+      bad("states are all tensors, or all pairs of codes and scales");
+    if (!codes) {
+      const at::Tensor& t = tensor_of(o, name);
+      if (t.scalar_type() != at::kFloat || t.device() != dev || !t.is_contiguous() || t.sizes() != param.sizes())
+        bad(std::string(name) + " must be contiguous float32 tensors of the parameters' shapes, on their device");
+      *place = t.data_ptr();
+      range(r, t);
+      return;
+    }
+    const Sequence pair(o, name);
+    if (pair.size() != 2) bad(std::string(name) + " must hold pairs of codes and scales");
+    const at::Tensor &q = tensor_of(pair[0], name), &s = tensor_of(pair[1], name);
+    if ((q.scalar_type() != at::kFloat8_e4m3fn && q.scalar_type() != at::kByte) || q.device() != dev ||
+        !q.is_contiguous() || q.numel() != n[i])
+      bad(std::string(name) + "'s codes must be contiguous float8_e4m3fn, one for each element of the parameter");
+    if (s.scalar_type() != at::kFloat || s.device() != dev || !s.is_contiguous() || s.numel() != (n[i] + 127) / 128)
+      bad(std::string(name) + "'s scales must be contiguous float32, one for each 128 elements");
+    *place = q.data_ptr(), *scale = s.data_ptr();
+    range(r, q);
+  };
+  for (int64_t i = 0; i < count; ++i) {
+    const at::Tensor &pt = tensor_of(P[i], "params"), &gt = tensor_of(G[i], "grads");
+    if (pt.scalar_type() != p0.scalar_type() || gt.scalar_type() != g0.scalar_type())
+      bad("all params must have one dtype, and all grads one");
+    if (pt.device() != dev || gt.device() != dev) bad("params and grads must be on one device");
+    if (!pt.is_contiguous()) bad("params must be contiguous");
+    if (gt.sizes() != pt.sizes()) bad("grads must have the parameters' shapes");
+    n[i] = pt.numel();
+    p[i] = pt.data_ptr();
+    range(rp, pt);
+    if (gt.is_contiguous()) {
+      g[i] = gt.data_ptr();
+    } else {
+      copies.push_back(gt.contiguous());
+      g[i] = copies.back().data_ptr();
+    }
+    state(M[i], i, pt, "exp_avgs", &m[i], codes ? &ms[i] : nullptr, rm);
+    state(V[i], i, pt, "exp_avg_sqs", &v[i], codes ? &vs[i] : nullptr, rv);
+  }
+  check_apart(rp, "params");
+  check_apart(rm, "exp_avgs");
+  check_apart(rv, "exp_avg_sqs");
+  const at::Tensor* st = device_scalar(step.ptr(), "step", at::kLong, dev);
+  const at::Tensor* lt = device_scalar(lr.ptr(), "lr", at::kFloat, dev);
+  if (grad_scale.has_value() &&
+      (grad_scale->numel() != 1 || grad_scale->scalar_type() != at::kFloat || grad_scale->device() != dev))
+    bad("grad_scale must be one float32 on the parameters' device");
+  check_status(cutie_adamw(
+      count, p.data(), p_dtype, g.data(), g_dtype, m.data(), codes ? ms.data() : nullptr, v.data(),
+      codes ? vs.data() : nullptr, n.data(), st != nullptr ? 0 : step.cast<int64_t>(),
+      st != nullptr ? st->data_ptr() : nullptr, lt != nullptr ? 0.0 : lr.cast<double>(),
+      lt != nullptr ? lt->data_ptr() : nullptr, beta1, beta2, eps, weight_decay, ptr_or_null(grad_scale),
+      (uint64_t)seed, at::cuda::getCurrentCUDAStream(dev.index()).stream()));
+  // what autograd saved of the parameters is out of date
+  for (int64_t i = 0; i < count; ++i) THPVariable_Unpack(P[i]).unsafeGetTensorImpl()->bump_version();
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -901,5 +1034,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("moe_permute", &moe_permute, py::arg("x"), py::arg("sources"), py::arg("positions"));
   m.def("moe_combine", &moe_combine, py::arg("rows"), py::arg("weights"), py::arg("sources"),
         py::arg("positions"));
+  m.def("adamw_step", &adamw_step, py::arg("params"), py::arg("grads"), py::arg("exp_avgs"),
+        py::arg("exp_avg_sqs"), py::arg("step"), py::arg("lr"), py::arg("beta1"), py::arg("beta2"), py::arg("eps"),
+        py::arg("weight_decay"), py::arg("grad_scale"), py::arg("seed"));
   m.def("abi_version", []() { return cutie_abi_version(); });
 }
