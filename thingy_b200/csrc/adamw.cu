@@ -1,5 +1,4 @@
-// AdamW over many tensors in one launch (sm_100a). For each element, in fp32
-// with every product and sum rounded by itself:
+// AdamW over many tensors in one launch (sm_100a). For each element, in fp32:
 //   g' = g c                           c: what clipping leaves of the gradients, or 1
 //   m' = b1 m + (1 - b1) g'
 //   v' = b2 v + (1 - b2) (g' g')
@@ -13,10 +12,15 @@
 // itself, codes are 2^-3 apart. A positive r' never becomes zero, so no element
 // is divided by eps alone because its code was lost.
 //
-// Bound: memory, each value once. CTAs walk chunks of 4096 elements of one
-// tensor, found by a search in the table that is the kernel's argument (no copy
-// to the GPU, nothing to keep for a graph); a thread takes 8 neighbouring
-// elements at a time, 16 lanes a group of 128.
+// CTAs walk chunks of 4096 elements of one tensor, found by a search in the
+// table that is the kernel's argument (no copy to the GPU, nothing to keep for a
+// graph). Bound: memory, each value once, for states in 32 bits, whose kernel
+// rounds every product and sum by itself. With codes (10 bytes an element of
+// bf16) it is the issue of instructions: so that kernel works on pairs (f32x2),
+// with fused sums, square roots and reciprocals of 2^-23 (the codes are rounded
+// by 2^-4), 16 elements a thread, so that a group's maxima and scales are shared
+// by 8 lanes: 89 thread instructions an element and 412 us for 134M in the form
+// that the other kernel has.
 #include <cuda_fp16.h>
 
 #include "cutie.h"
@@ -164,140 +168,233 @@ __device__ __forceinline__ void store8(F16* p, bool vec, int n, const float (&f)
   store8_half(p, vec, n, w);
 }
 
-// A magnitude at most 448 to one of its neighbours in e4m3 by 16 random bits: added
-// below the three bits of mantissa that stay, the rest cut off. Subnormal codes
-// have the spacing of the first binade, so they are rounded one binade up.
-__device__ __forceinline__ float round8(float y, uint32_t bits) {
-  const float up = y < 0x1p-6f ? 0x1p-6f : 0.f;
-  const float z = __uint_as_float((__float_as_uint(__fadd_rn(y, up)) + (bits << 4)) & 0xfff00000u);
-  return fminf(__fsub_rn(z, up), 448.f);
-}
+// Pairs of neighbouring values.
+__device__ __forceinline__ float2 pair_of(const float (&f)[kEach], int i) { return make_float2(f[2 * i], f[2 * i + 1]); }
 
-// Codes and scale of a group of 128 elements, 16 lanes with 8 each; bits: 16 random ones an element.
-template <bool POSITIVE>
-__device__ __forceinline__ void store_state(E4m3* p, float* scale, bool vec, int n, bool first,
-                                            const float (&x)[kEach], const uint32_t (&bits)[kEach]) {
+// The scale of a group of 128 values, 8 lanes with 16 each; NaN counts as nothing.
+__device__ __forceinline__ float group_scale(const float2 (&x)[2][4]) {
   float amax = 0.f;
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) amax = fmaxf(amax, i < n ? fabsf(x[i]) : 0.f);
+  for (int h = 0; h < 2; ++h)
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  const float s = fmaxf(__fdiv_rn(amax, 448.f), kMinState), rs = __fdiv_rn(1.f, s);
-  uint32_t w[2];
-  float z[kEach];
+    for (int i = 0; i < 4; ++i) amax = fmaxf(fmaxf(amax, fabsf(x[h][i].x)), fabsf(x[h][i].y));
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    const float y = __fmul_rn(fabsf(x[i]), rs);
-    z[i] = round8(y, bits[i]);
-    if (POSITIVE && x[i] > 0.f) z[i] = fmaxf(z[i], 0x1p-9f);
-    if (!(y == y)) z[i] = y;  // NaN stays
-    if (!POSITIVE) z[i] = copysignf(z[i], x[i]);
-  }
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-    w[i] = f4_to_e4m3x4(make_float2(z[4 * i], z[4 * i + 1]), make_float2(z[4 * i + 2], z[4 * i + 3]));
-  if (first && n > 0) *scale = s;
+  for (int o = 4; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  return amax <= 3.4e38f ? make_scale(amax, false, kMinState) : amax;
+}
+
+// The code of x in the upper byte; rs: the scale's reciprocal, bits: 16 random ones
+// from bit 8 on. They are added below the three bits of mantissa that stay and the
+// rest is cut off. All in integers: 2^-120 brings the least normal code, 2^-6, to
+// fp32's least normal value, so that both have their subnormal codes at the same
+// bits. The largest value is 448 (1 + 2^-23) and cannot carry past its code.
+template <bool POSITIVE>
+__device__ __forceinline__ uint32_t code_of(float x, float rs, uint32_t bits) {
+  const float y = __fmul_rn(__fmul_rn(fabsf(x), rs), 0x1p-120f);
+  const uint32_t v = (min(__float_as_uint(y), 0x07f00000u) << 4) + bits;  // NaN: code 0x7f
+  return POSITIVE ? max(v, x > 0.f ? 0x01000000u : 0u) : v | (__float_as_uint(x) & 0x80000000u);
+}
+__device__ __forceinline__ uint32_t upper_bytes(const uint32_t (&v)[kEach], int i) {
+  return __byte_perm(__byte_perm(v[i], v[i + 1], 0x0073), __byte_perm(v[i + 2], v[i + 3], 0x0073), 0x5410);
+}
+__device__ __forceinline__ void store8(E4m3* p, bool vec, int n, const uint32_t (&v)[kEach]) {
+  const uint2 w = make_uint2(upper_bytes(v, 0), upper_bytes(v, 4));
   if (vec) {
-    *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    *reinterpret_cast<uint2*>(p) = w;
   } else {
 #pragma unroll
     for (int i = 0; i < kEach; ++i)
-      if (i < n) p[i].bits = (uint8_t)(w[i / 4] >> (8 * (i & 3)));
+      if (i < n) p[i].bits = (uint8_t)(v[i] >> 24);
   }
 }
 
 __device__ __forceinline__ bool on16(const void* p) { return (reinterpret_cast<uint64_t>(p) & 15u) == 0; }
 
-template <class P, class G, bool CODES, int N>
-__global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ Table<N> t, int tensors,
-                                                         const AdamwStep a) {
-  __shared__ float factor[3];  // of the decay, of the root, of the update
-  __shared__ uint32_t step_key;
-  griddep_wait();
-  griddep_launch_dependents();
-  if (threadIdx.x == 0) {
-    // 1 - b^t in 64 bits: in 32 its first digits are gone while b^t is near one
-    const int64_t step = a.step_ptr != nullptr ? *a.step_ptr : a.step;
-    const double lr = a.lr_ptr != nullptr ? (double)*a.lr_ptr : a.lr;
-    factor[0] = (float)(1.0 - lr * a.decay);
-    if (a.step_ptr != nullptr) {
-      factor[1] = (float)rsqrt(1.0 - pow(a.beta2, (double)step));
-      factor[2] = (float)(lr / (1.0 - pow(a.beta1, (double)step)));
-    } else {
-      factor[1] = a.root;
-      factor[2] = (float)(lr / a.bias1);
-    }
-    step_key = mix(a.seed_key ^ (uint32_t)step);
+// What a step's constants are, made by one thread; 1 - b^t in 64 bits: in 32 its
+// first digits are gone while b^t is near one.
+struct Factors {
+  float keep, root, rate;  // of p, of sqrt(v'), of the update
+  uint32_t key;
+};
+__device__ __forceinline__ void make_factors(const AdamwStep& a, Factors& f) {
+  const double lr = a.lr_ptr != nullptr ? (double)*a.lr_ptr : a.lr;
+  const int64_t step = a.step_ptr != nullptr ? *a.step_ptr : a.step;
+  f.keep = (float)(1.0 - lr * a.decay);
+  if (a.step_ptr != nullptr) {
+    f.root = (float)rsqrt(1.0 - pow(a.beta2, (double)step));
+    f.rate = (float)(lr / (1.0 - pow(a.beta1, (double)step)));
+  } else {
+    f.root = a.root;
+    f.rate = (float)(lr / a.bias1);
   }
-  __syncthreads();
-  const float c = a.clip != nullptr ? *a.clip : 1.f;
-  const float b1 = a.b1, b2 = a.b2, c1 = a.c1, c2 = a.c2;
-  const float eps = a.eps, keep = factor[0], root = factor[1], rate = factor[2];
-  using S = typename std::conditional<CODES, E4m3, float>::type;
-  for (uint32_t chunk = blockIdx.x; chunk < t.first[tensors]; chunk += gridDim.x) {
-  int lo = 0, hi = tensors;  // the last tensor whose chunks begin at this one or before
+  f.key = mix(a.seed_key ^ (uint32_t)step);
+}
+
+// The last tensor whose chunks begin at `chunk` or before.
+template <int N>
+__device__ __forceinline__ int tensor_at(const Table<N>& t, int tensors, uint32_t chunk) {
+  int lo = 0, hi = tensors;
   while (hi - lo > 1) {
     const int mid = (lo + hi) / 2;
     if (t.first[mid] <= chunk) lo = mid;
     else hi = mid;
   }
-  const int64_t begin = (int64_t)(chunk - t.first[lo]) * kChunk, size = t.n[lo];
-  const G* g = static_cast<const G*>(t.g[lo]) + begin;
-  P* p = static_cast<P*>(t.p[lo]) + begin;
-  const int count = (int)min((int64_t)kChunk, size - begin);
-  S *m = static_cast<S*>(t.m[lo]) + begin, *v = static_cast<S*>(t.v[lo]) + begin;
-  const bool vec_all = on16(g) && on16(p) &&
-                       (CODES ? ((reinterpret_cast<uint64_t>(m) | reinterpret_cast<uint64_t>(v)) & 7u) == 0
-                              : on16(m) && on16(v));
-  const uint32_t key = CODES ? mix(step_key ^ t.ordinal[lo]) : 0u;
-  // whole warps go on: the lanes of a group exchange their maxima
-  for (int at = (int)threadIdx.x * kEach; at - (int)(threadIdx.x & 31) * kEach < count; at += kThreads * kEach) {
-    const int n = max(0, min(kEach, count - at));
-    const bool vec = vec_all && n == kEach;
-    float pf[kEach], gf[kEach], mf[kEach], vf[kEach];
-    float ms = 0.f, vs = 0.f;
-    const int64_t group = (begin + at) / kGroup;
-    if (n > 0) {
-      load8(g + at, vec, n, gf);
-      load8(p + at, vec, n, pf);
-      load8(m + at, vec, n, mf);
-      load8(v + at, vec, n, vf);
-      if (CODES) ms = t.ms[lo][group], vs = t.vs[lo][group];
-    } else {
+  return lo;
+}
+
+// A chunk of tensor i from element `begin` on. WHOLE: all of its elements are there
+// and on the vectors' boundaries, so that nothing in it branches.
+struct Chunk {
+  int i, count;
+  int64_t begin;
+};
+template <int N>
+__device__ __forceinline__ Chunk chunk_at(const Table<N>& t, int tensors, uint32_t chunk) {
+  Chunk k;
+  k.i = tensor_at(t, tensors, chunk);
+  k.begin = (int64_t)(chunk - t.first[k.i]) * kChunk;
+  k.count = (int)min((int64_t)kChunk, t.n[k.i] - k.begin);
+  return k;
+}
+
+template <class P, class G, bool WHOLE, int N>
+__device__ __forceinline__ void step_values(const Table<N>& t, const Chunk& k, const AdamwStep& a, const Factors& f,
+                                            float c) {
+  const G* g = static_cast<const G*>(t.g[k.i]) + k.begin;
+  P* p = static_cast<P*>(t.p[k.i]) + k.begin;
+  float *m = static_cast<float*>(t.m[k.i]) + k.begin, *v = static_cast<float*>(t.v[k.i]) + k.begin;
 #pragma unroll
-      for (int i = 0; i < kEach; ++i) pf[i] = gf[i] = mf[i] = vf[i] = 0.f;
-    }
+  for (int at = (int)threadIdx.x * kEach, step = 0; step < kChunk / (kThreads * kEach); ++step, at += kThreads * kEach) {
+    const int n = WHOLE ? kEach : min(kEach, k.count - at);
+    if (!WHOLE && n <= 0) break;
+    float pf[kEach], gf[kEach], mf[kEach], vf[kEach];
+    load8(g + at, WHOLE, n, gf);
+    load8(p + at, WHOLE, n, pf);
+    load8(m + at, WHOLE, n, mf);
+    load8(v + at, WHOLE, n, vf);
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      if (CODES) {
-        mf[i] = __fmul_rn(mf[i], ms);
-        const float r = __fmul_rn(vf[i], vs);
-        vf[i] = __fmul_rn(r, r);
-      }
       const float gc = __fmul_rn(gf[i], c);
-      mf[i] = __fadd_rn(__fmul_rn(b1, mf[i]), __fmul_rn(c1, gc));
-      vf[i] = __fadd_rn(__fmul_rn(b2, vf[i]), __fmul_rn(c2, __fmul_rn(gc, gc)));
-      const float r = __fsqrt_rn(vf[i]);
-      const float d = __fadd_rn(__fmul_rn(r, root), eps);
-      pf[i] = __fsub_rn(__fmul_rn(pf[i], keep), __fmul_rn(rate, __fdiv_rn(mf[i], d)));
-      if (CODES) vf[i] = r;
+      mf[i] = __fadd_rn(__fmul_rn(a.b1, mf[i]), __fmul_rn(a.c1, gc));
+      vf[i] = __fadd_rn(__fmul_rn(a.b2, vf[i]), __fmul_rn(a.c2, __fmul_rn(gc, gc)));
+      const float d = __fadd_rn(__fmul_rn(__fsqrt_rn(vf[i]), f.root), a.eps);
+      pf[i] = __fsub_rn(__fmul_rn(pf[i], f.keep), __fmul_rn(f.rate, __fdiv_rn(mf[i], d)));
     }
-    if (n > 0) store8(p + at, vec, n, pf);
-    if constexpr (CODES) {
-      uint32_t low[kEach], high[kEach];
-#pragma unroll
-      for (int i = 0; i < kEach; ++i) {
-        const uint32_t h = mix((uint32_t)(begin + at + i) * 0x9E3779B9u + key);
-        low[i] = h & 0xffffu, high[i] = h >> 16;
-      }
-      const bool first = (threadIdx.x & 15) == 0;
-      store_state<false>(m + at, t.ms[lo] + group, vec, n, first, mf, low);
-      store_state<true>(v + at, t.vs[lo] + group, vec, n, first, vf, high);
-    } else if (n > 0) {
-      store8(m + at, vec, n, mf);
-      store8(v + at, vec, n, vf);
-    }
+    store8(p + at, WHOLE, n, pf);
+    store8(m + at, WHOLE, n, mf);
+    store8(v + at, WHOLE, n, vf);
   }
+}
+
+template <class P, class G, int N>
+__global__ void __launch_bounds__(kThreads, 5)
+    adamw_kernel(const __grid_constant__ Table<N> t, int tensors, const AdamwStep a) {
+  __shared__ Factors shared;
+  griddep_wait();
+  griddep_launch_dependents();
+  if (threadIdx.x == 0) make_factors(a, shared);
+  __syncthreads();
+  const Factors f = shared;
+  const float c = a.clip != nullptr ? *a.clip : 1.f;
+  for (uint32_t chunk = blockIdx.x; chunk < t.first[tensors]; chunk += gridDim.x) {
+    const Chunk k = chunk_at(t, tensors, chunk);
+    if (k.count == kChunk && on16(t.g[k.i]) && on16(t.p[k.i]) && on16(t.m[k.i]) && on16(t.v[k.i]))
+      step_values<P, G, true>(t, k, a, f, c);
+    else
+      step_values<P, G, false>(t, k, a, f, c);
+  }
+}
+
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float fast_root(float x) {
+  float r;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// Of zero or of at least 2^-75 (the root of fp32's least value) as it is used here.
+__device__ __forceinline__ float fast_reciprocal(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+template <class P, class G, bool WHOLE, int N>
+__device__ __forceinline__ void step_codes(const Table<N>& t, const Chunk& k, const AdamwStep& a, const Factors& f,
+                                           float c) {
+  // m' = b1 m + g (c1 c);  v' = (r sqrt(b2))^2 + (g (c sqrt(c2)))^2
+  const float2 g_m = both(__fmul_rn(a.c1, c)), g_r = both(__fmul_rn(a.root_c2, c));
+  const float2 keep = both(f.keep), root = both(f.root), rate = both(-f.rate), eps = both(a.eps);
+  const int at = ((int)threadIdx.x >> 3) * kGroup + ((int)threadIdx.x & 7) * kEach;
+  const int64_t from = k.begin + at, group = k.begin / kGroup + ((int)threadIdx.x >> 3);
+  const G* g = static_cast<const G*>(t.g[k.i]) + from;
+  P* p = static_cast<P*>(t.p[k.i]) + from;
+  E4m3 *m = static_cast<E4m3*>(t.m[k.i]) + from, *v = static_cast<E4m3*>(t.v[k.i]) + from;
+  // whole warps go on: the lanes of a group exchange their maxima
+  const int n[2] = {WHOLE ? kEach : max(0, min(kEach, k.count - at)), WHOLE ? kEach : max(0, min(kEach, k.count - at - 64))};
+  float ms = 0.f, rs = 0.f;
+  float gf[2][kEach], pf[2][kEach], mf[2][kEach], rf[2][kEach];
+  if (n[0] > 0) ms = t.ms[k.i][group], rs = t.vs[k.i][group];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    load8(g + 64 * h, WHOLE, n[h], gf[h]);
+    load8(p + 64 * h, WHOLE, n[h], pf[h]);
+    load8(m + 64 * h, WHOLE, n[h], mf[h]);
+    load8(v + 64 * h, WHOLE, n[h], rf[h]);
+  }
+  const float2 ms2 = both(__fmul_rn(ms, a.b1)), rs2 = both(__fmul_rn(rs, a.root_b2));
+  float2 m2[2][4], r2[2][4];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float out[kEach];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 gi = pair_of(gf[h], i), b = __fmul2_rn(pair_of(rf[h], i), rs2), e = __fmul2_rn(gi, g_r);
+      m2[h][i] = __ffma2_rn(pair_of(mf[h], i), ms2, __fmul2_rn(gi, g_m));
+      const float2 v2 = __ffma2_rn(b, b, __fmul2_rn(e, e));
+      r2[h][i] = make_float2(fast_root(v2.x), fast_root(v2.y));
+      const float2 d = __ffma2_rn(r2[h][i], root, eps);
+      const float2 u = __fmul2_rn(m2[h][i], make_float2(fast_reciprocal(d.x), fast_reciprocal(d.y)));
+      const float2 q = __ffma2_rn(u, rate, __fmul2_rn(pair_of(pf[h], i), keep));
+      out[2 * i] = q.x, out[2 * i + 1] = q.y;
+    }
+    store8(p + 64 * h, WHOLE, n[h], out);
+  }
+  const float m_scale = group_scale(m2), r_scale = group_scale(r2);
+  if ((threadIdx.x & 7) == 0 && n[0] > 0) t.ms[k.i][group] = m_scale, t.vs[k.i][group] = r_scale;
+  const float m_rcp = __frcp_rn(m_scale), r_rcp = __frcp_rn(r_scale);
+  const uint32_t key = mix(f.key ^ t.ordinal[k.i]);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t mv[kEach], rv[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const uint32_t bits = mix((uint32_t)(from + 64 * h + i) * 0x9E3779B9u + key);
+      mv[i] = code_of<false>(i & 1 ? m2[h][i / 2].y : m2[h][i / 2].x, m_rcp, __byte_perm(bits, 0, 0x4104));
+      rv[i] = code_of<true>(i & 1 ? r2[h][i / 2].y : r2[h][i / 2].x, r_rcp, __byte_perm(bits, 0, 0x4324));
+    }
+    store8(m + 64 * h, WHOLE, n[h], mv);
+    store8(v + 64 * h, WHOLE, n[h], rv);
+  }
+}
+
+__device__ __forceinline__ bool on8(const void* p) { return (reinterpret_cast<uint64_t>(p) & 7u) == 0; }
+
+template <class P, class G, int N>
+__global__ void __launch_bounds__(kThreads, 4)
+    adamw_codes_kernel(const __grid_constant__ Table<N> t, int tensors, const AdamwStep a) {
+  __shared__ Factors shared;
+  griddep_wait();
+  griddep_launch_dependents();
+  if (threadIdx.x == 0) make_factors(a, shared);
+  __syncthreads();
+  const Factors f = shared;
+  const float c = a.clip != nullptr ? *a.clip : 1.f;
+  for (uint32_t chunk = blockIdx.x; chunk < t.first[tensors]; chunk += gridDim.x) {
+    const Chunk k = chunk_at(t, tensors, chunk);
+    if (k.count == kChunk && on16(t.g[k.i]) && on16(t.p[k.i]) && on8(t.m[k.i]) && on8(t.v[k.i]))
+      step_codes<P, G, true>(t, k, a, f, c);
+    else
+      step_codes<P, G, false>(t, k, a, f, c);
   }
 }
 
@@ -324,8 +421,9 @@ cudaError_t launch_table(const AdamwTensors& l, const AdamwStep& step, cudaStrea
     if (k == 0) continue;
     t.first[k] = (uint32_t)chunks;
     const uint64_t most = (uint64_t)kCtas * device_sm_count();
-    const cudaError_t e = launch_pdl(adamw_kernel<P, G, CODES, N>, (unsigned)(chunks < most ? chunks : most), kThreads,
-                                     0, stream, t, k, step);
+    const unsigned grid = (unsigned)(chunks < most ? chunks : most);
+    auto kernel = CODES ? adamw_codes_kernel<P, G, N> : adamw_kernel<P, G, N>;
+    const cudaError_t e = launch_pdl(kernel, grid, kThreads, 0, stream, t, k, step);
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
