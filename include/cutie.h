@@ -346,20 +346,21 @@ CUTIE_API int cutie_cast_fp8_sorted(const void* x, int64_t ldx, int64_t R, int64
  * The experts' products on sorted rows: for each expert e, rows offsets[e] to
  * offsets[e + 1] of
  *   D = dequant(A) dequant(B[e])^T
- * and zeros in the rows behind the last expert's. A: e4m3 [R, K] (lda), fp32
+ * and zeros in padding, the rows of e from offsets[e] + counts[e] on, and in
+ * the rows behind the last expert's. A: e4m3 [R, K] (lda), fp32
  * scales of 1 x 128 groups, element (r, kb) at r * sa_row + kb * sa_kb. B:
  * e4m3 [E, N, K], row n of expert e at e * b_expert + n * ldb, fp32 scales of
  * 128 x 128 blocks at e * sb_expert + nb * sb_row + kb * sb_kb. D: bf16 or fp32
  * [R, N] (ldd). offsets: int32 [E + 1] on the GPU, multiples of 128 that do
- * not decrease, the last at most R (cutie_moe_sort, align 128); E <= 512, R a
- * multiple of 128. Rows of A and B and b_expert on 16-byte, rows of D on
+ * not decrease, the last at most R (cutie_moe_sort, align 128); counts: int32
+ * [E] likewise, or NULL: no padding; E <= 512, R a multiple of 128. Rows of A and B and b_expert on 16-byte, rows of D on
  * 32-byte boundaries, N a multiple of 16 (fp32: 8). With B's strides exchanged
  * the same call is the input gradient. Sums as in cutie_fp8_block_gemm.
  */
 CUTIE_API int cutie_fp8_grouped_gemm(const void* a, int64_t lda, const void* a_scale,
                                      int64_t sa_row, int64_t sa_kb, const void* b, int64_t ldb,
                                      int64_t b_expert, const void* b_scale, int64_t sb_row,
-                                     int64_t sb_kb, int64_t sb_expert, const void* offsets,
+                                     int64_t sb_kb, int64_t sb_expert, const void* offsets, const void* counts,
                                      int64_t E, void* d, int64_t ldd, int d_dtype, int64_t R,
                                      int64_t N, int64_t K, void* stream);
 

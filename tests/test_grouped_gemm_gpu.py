@@ -63,6 +63,7 @@ def test_product(counts, N, K, out_dtype):
     R, KB = plan.sources.shape[0], -(-K // 128)
     g = torch.Generator(device="cuda").manual_seed(N + K)
     a, sa = codes(g, R, K), torch.rand(R, KB, generator=g, device="cuda") + 0.5
+    a[plan.sources < 0] = torch.tensor(float("nan")).to(F8).cuda()
     b, sb = codes(g, E, N, K), torch.rand(E, -(-N // 128), KB, generator=g, device="cuda") + 0.5
     out = torch.full((R, N), float("nan"), dtype=out_dtype, device="cuda")
     got = tb.fp8_grouped_gemm(a, sa, b, sb, plan, out=out)
@@ -70,8 +71,8 @@ def test_product(counts, N, K, out_dtype):
     off = plan.offsets.tolist()
     for e in range(E):
         rows = slice(off[e], off[e + 1])
-        check(got[rows], dequant_rows(a[rows], sa[rows]), dequant_blocks(b[e], sb[e]), out_dtype)
-    assert bool((got[off[E]:] == 0).all())
+        check(got[rows][: counts[e]], dequant_rows(a[rows], sa[rows])[: counts[e]], dequant_blocks(b[e], sb[e]), out_dtype)
+    assert bool((got[plan.sources < 0] == 0).all())  # whatever a holds there
     # scales in the other order, another stride of the experts, the same bits
     wide = torch.zeros(E, N + 3, K, dtype=F8, device="cuda")
     wide[:, :N] = b
@@ -91,7 +92,7 @@ def test_product_equals_the_single_one():
     got = tb.fp8_grouped_gemm(a, sa, b, sb, plan, out_dtype=torch.float32)
     off = plan.offsets.tolist()
     for e in range(E):
-        rows = slice(off[e], off[e + 1])
+        rows = slice(off[e], off[e] + counts[e])
         want = tb.fp8_block_gemm(a[rows], sa[rows], b[e], sb[e], out_dtype=torch.float32)
         size = dequant_rows(a[rows], sa[rows]).abs() @ dequant_blocks(b[e], sb[e]).abs().t()
         assert bool(((got[rows] - want).double().abs() <= 2 * sum_error(K) * size).all())  # other forms there, K may be split
@@ -104,10 +105,11 @@ def test_offsets_are_cut_to_the_rows():
     a, sa = codes(g, R, K), torch.ones(R, 2, device="cuda")
     b, sb = codes(g, 3, N, K), torch.ones(3, 2, 2, device="cuda")
     none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    counts = torch.tensor([1 << 30, -5, 200], dtype=torch.int32, device="cuda")
     for values in ([0, 128, 900, 5000], [-300, 128, 0, 512], [0, 100, 300, 511], [512, 512, 512, 512], [0, 0, 0, 0]):
         offsets = torch.tensor(values, dtype=torch.int32, device="cuda")
         guard = torch.full((R + 256, N), 7.0, device="cuda")
-        tb.fp8_grouped_gemm(a, sa, b, sb, tb.MoePlan(none, none, offsets, none, 128), out=guard[128 : 128 + R])
+        tb.fp8_grouped_gemm(a, sa, b, sb, tb.MoePlan(none, none, offsets, counts, 128), out=guard[128 : 128 + R])
         assert bool((guard[:128] == 7).all()) and bool((guard[128 + R :] == 7).all())
         assert tb._lib.device_error() == 0
 

@@ -113,8 +113,8 @@ _SIGNATURES = {
     ),
     "cutie_fp8_grouped_gemm": (
         _int,
-        [_ptr, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _i64, _ptr, _i64, _ptr, _i64,
-         _int, _i64, _i64, _i64, _ptr],
+        [_ptr, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _i64, _ptr, _ptr, _i64, _ptr,
+         _i64, _int, _i64, _i64, _i64, _ptr],
     ),
     "cutie_fp8_grouped_wgrad": (
         _int,

@@ -78,7 +78,7 @@ cudaError_t launch_cluster(K kernel, dim3 grid, unsigned pair, int threads, size
 //  * warp 8, one thread: TMA of the A box and the BN / 128 B boxes of a K
 //    block into a ring of stages (128-byte swizzled rows; rows and columns
 //    past the matrices are zero-filled, so M, N and K may be any).
-//  * warp 9, one thread: four MMAs of 128 x BN x 32 a K block into one of two
+//  * warp 9, one thread: four MMAs of 128 x BN x 32 a K block into one of 512 / BN
 //    accumulator buffers in tensor memory; a commit hands the buffer to the
 //    epilogue, a second frees the stage.
 //  * warps 0-7: the outer sum. Warp group g = warp / 4 keeps columns
@@ -118,7 +118,8 @@ struct TilePlan {
   static constexpr uint32_t kStageBytes = (1 + kNB) * kBoxBytes;
   static constexpr int kStages = kNB == 2 ? 4 : 6;
   static constexpr size_t kSmemBytes = kStages * kStageBytes + 1024;
-  static constexpr uint32_t kTmemCols = 2 * BN;
+  static constexpr int kBufs = 512 / BN;  // accumulators
+  static constexpr uint32_t kTmemCols = kBufs * BN;
   static constexpr int kCols = BN / 2;  // columns of a warp group
   // scales of a K block: 128 rows', then the columns' (a scale each, or a block's)
   static constexpr int kScales = 128 + (SB_ROWS ? BN : 4);
@@ -150,7 +151,9 @@ struct TileArgs {
   long long wait_limit;  // SM cycles a wait may block before it gives up (< 0: never blocks)
   // experts (kExpertRows, kExpertColumns)
   const int* offsets;  // [E + 1]
+  const int* counts;   // [E] rows before the padding (null: all count)
   int E, R;            // R: sorted rows, a multiple of 128
+  int a_box;           // rows of A's boxes (kExpertRows): 32 or 128
   int64_t sb_expert, d_expert;
 };
 
@@ -158,7 +161,9 @@ struct TileArgs {
 //  * kOne: the matrices as they are.
 //  * kExpertRows: A's rows are sorted by expert, B is [E, N, K]: the rows of
 //    A from offsets[e] on go with B's matrix e. Experts begin at multiples of
-//    128, so a tile has one expert.
+//    128, so a tile has one expert. Of a tile's rows only boxes that hold some
+//    before the padding are loaded; padding is stored as zeros, whatever the
+//    sums over what was in shared memory are.
 //  * kExpertColumns: both operands' columns are sorted by expert (a weight
 //    gradient): D's matrix e is the product over the columns of e. A tile of D
 //    has as many K blocks as its expert has, or none and is zero.
@@ -171,6 +176,7 @@ template <int MODE>
 struct ExpertTable {
   int begin[MODE == kOne ? 1 : kMoeMaxExperts + 1];
   int tiles[MODE == kExpertRows ? kMoeMaxExperts + 1 : 1];
+  int end[MODE == kExpertRows ? kMoeMaxExperts : 1];  // of the rows before the padding
 };
 
 // By the first warps of a CTA, between two barriers of its own.
@@ -179,6 +185,10 @@ __device__ __forceinline__ void fill_experts(const TileArgs& g, ExpertTable<MODE
   for (int e = threadIdx.x; e <= g.E; e += blockDim.x)
     x.begin[e] = min(max(g.offsets[e], 0), g.R) & ~(kBM - 1);
   __syncthreads();
+  if (MODE == kExpertRows)
+    for (int e = threadIdx.x; e < g.E; e += blockDim.x)
+      x.end[e] = g.counts == nullptr ? x.begin[e + 1]
+                                     : x.begin[e] + min(max(g.counts[e], 0), max(x.begin[e + 1] - x.begin[e], 0));
   if (MODE == kExpertRows && threadIdx.x < 32) {
     const int per = (g.E + 31) / 32, lane = threadIdx.x, e0 = min(lane * per, g.E), e1 = min(e0 + per, g.E);
     int mine = 0;
@@ -223,33 +233,31 @@ __device__ __forceinline__ void tile_of(const TileArgs& g, int t, int* tm, int* 
 struct Item {
   int e, row, col;  // expert, first row of A and first row of B
   int k0, nkb;      // first column of the operands' K range, its K blocks
-  int row_end;      // of the rows that are stored
+  int row_end;      // of the rows that are stored, and of those that are not padding
+  int some_end;
 };
 
-// Tile t for rank `rank` of a pair, `rows` of A a tile.
+// Tile t for rank `rank` of a pair, `rows` of A a tile; e: an expert at or before
+// its own (the tile's before it: a warp's tiles only rise).
 template <int BN, int MODE>
-__device__ __forceinline__ Item item_of(const TileArgs& g, const ExpertTable<MODE>& x, int t, int rows, int rank) {
+__device__ __forceinline__ Item item_of(const TileArgs& g, const ExpertTable<MODE>& x, int t, int rows, int rank,
+                                        int& e) {
   Item i;
   int tm, tn;
   if (MODE == kExpertRows) {
-    int lo = 0, hi = g.E;  // the last expert whose tiles begin at t or before: it has some
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) / 2;
-      if (x.tiles[mid] * g.tiles_n <= t) lo = mid;
-      else hi = mid;
-    }
-    const int first = x.tiles[lo];
-    tile_at(g, t - first * g.tiles_n, &tm, &tn, x.tiles[lo + 1] - first);
-    i.e = lo;
-    i.row = x.begin[lo] + tm * rows + rank * kBM;
-    i.row_end = x.begin[lo + 1];
+    while (x.tiles[e + 1] * g.tiles_n <= t) ++e;  // t < tiles[E] tiles_n
+    const int first = x.tiles[e];
+    tile_at(g, t - first * g.tiles_n, &tm, &tn, x.tiles[e + 1] - first);
+    i.e = e;
+    i.row = x.begin[e] + tm * rows + rank * kBM;
+    i.row_end = x.begin[e + 1], i.some_end = x.end[e];
     i.k0 = 0, i.nkb = g.KB;
   } else {
     const int each = g.tiles_m * g.tiles_n;
     i.e = t / each;
     tile_at(g, t - i.e * each, &tm, &tn, g.tiles_m);
     i.row = tm * rows + rank * kBM;
-    i.row_end = g.M;
+    i.row_end = i.some_end = g.M;
     i.k0 = x.begin[i.e], i.nkb = max(x.begin[i.e + 1] - i.k0, 0) / kBK;
   }
   i.col = tn * BN;
@@ -264,11 +272,15 @@ __device__ __forceinline__ Item item_of(const TileArgs& g, const ExpertTable<MOD
 // A template, not a branch: the mere presence of the second form cost the main
 // loop of the first 6%.
 template <int NC, bool VEC>
-__device__ __forceinline__ void store_rows(const TileArgs& g, void* d, int row_end, const float2 (&acc)[NC / 2],
-                                           int row0, int col, int lane, float* stage) {
+__device__ __forceinline__ void store_rows(const TileArgs& g, void* d, int row_end, float2 (&acc)[NC / 2],
+                                           int row0, int col, int lane, float* stage, int some_end = INT32_MAX) {
   if (VEC) {
     const int row = row0 + lane;
     if (row >= row_end) return;
+    if (row >= some_end) {
+#pragma unroll
+      for (int i = 0; i < NC / 2; ++i) acc[i] = make_float2(0.f, 0.f);
+    }
     const int64_t at = (int64_t)row * g.ldd + col;
     if (!g.d_f32) {
       uint16_t* p = static_cast<uint16_t*>(d) + at;
@@ -377,8 +389,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full_bar[P::kStages];
   __shared__ __align__(8) uint64_t empty_bar[P::kStages];
-  __shared__ __align__(8) uint64_t acc_full[2];
-  __shared__ __align__(8) uint64_t acc_empty[2];
+  __shared__ __align__(8) uint64_t acc_full[P::kBufs];
+  __shared__ __align__(8) uint64_t acc_empty[P::kBufs];
   __shared__ __align__(8) uint64_t scale_full[P::kScaleSlots];
   __shared__ __align__(8) uint64_t scale_empty[P::kScaleSlots];
   __shared__ __align__(16) float scales[P::kScaleSlots][kScaleBlocks][P::kScales];
@@ -402,6 +414,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   // and the tile's rows that it adds up
   const int share = (kBM + S - 1) / S, own_lo = min(rank * share, kBM), own_n = min(share, kBM - own_lo);
   volatile uint32_t* abortp = &abort_flag;
+  [[maybe_unused]] int expert = 0;  // of the warp's last tile
 
   if (threadIdx.x == 0) {
     tc::prefetch_map(&map_a);
@@ -410,7 +423,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(smem_addr(&full_bar[s]), 1);
       mbar_init(smem_addr(&empty_bar[s]), 1);
     }
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < P::kBufs; ++b) {
       mbar_init(smem_addr(&acc_full[b]), 1);
       mbar_init(smem_addr(&acc_empty[b]), (PAIR ? 2 : 1) * kEpiWarps);
     }
@@ -453,7 +466,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if constexpr (MODE == kOne) {
         tile_of<BN>(g, t, &tm, &tn);
       } else {
-        it = item_of<BN, MODE>(g, experts, t, (PAIR ? 2 : 1) * kBM, rank);
+        it = item_of<BN, MODE>(g, experts, t, (PAIR ? 2 : 1) * kBM, rank, expert);
         nkb = it.nkb;
       }
       for (int kb = 0; kb < nkb; ++kb) {
@@ -476,9 +489,16 @@ __global__ void __launch_bounds__(kThreads, 1)
               tc::tma_load_2d_pair(st + kBoxBytes, &map_b, it.k0 + kb * kBK, it.col + 128 * rank, to);
             }
           } else if constexpr (MODE != kOne) {
-            mbar_arrive_expect_tx(bar, P::kStageBytes);
             const int k = it.k0 + kb * kBK;
-            tc::tma_load_2d(st, &map_a, k, it.row, bar);
+            if (MODE == kExpertRows) {
+              const int n = max(0, min(kBM, it.some_end - it.row) + g.a_box - 1) / g.a_box;
+              mbar_arrive_expect_tx(bar, P::kNB * kBoxBytes + (uint32_t)(n * g.a_box * kBK));
+              for (int i = 0; i < n; ++i)
+                tc::tma_load_2d(st + (uint32_t)(i * g.a_box * kBK), &map_a, k, it.row + i * g.a_box, bar);
+            } else {
+              mbar_arrive_expect_tx(bar, P::kStageBytes);
+              tc::tma_load_2d(st, &map_a, k, it.row, bar);
+            }
 #pragma unroll
             for (int h = 0; h < P::kNB; ++h) {
               const uint32_t to = st + (1 + h) * kBoxBytes;
@@ -510,7 +530,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t s = 0, parity = 0, buf = 0, buf_parity = 1;
     bool ok = !PAIR || rank == 0;  // rank 0 issues for both
     for (int t = begin; t < tiles && ok; t += step) {
-      if constexpr (MODE == kExpertColumns) nkb = item_of<BN, MODE>(g, experts, t, kBM, 0).nkb;
+      if constexpr (MODE == kExpertColumns) nkb = item_of<BN, MODE>(g, experts, t, kBM, 0, expert).nkb;
       for (int kb = 0; kb < nkb; ++kb) {
         ok = tc::wait_or_abort(smem_addr(&full_bar[s]), parity, abortp, g.wait_limit) &&
              tc::wait_or_abort(smem_addr(&acc_empty[buf]), buf_parity, abortp, g.wait_limit);
@@ -540,8 +560,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
         if (++s == P::kStages) s = 0, parity ^= 1;
-        buf ^= 1;
-        buf_parity ^= buf == 0;
+        if (++buf == P::kBufs) buf = 0, buf_parity ^= 1;
       }
     }
   } else if (warp == kEpiWarps + 2) {
@@ -558,7 +577,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tile_of<BN>(g, t, &tm, &tn);
         row0 = (PAIR ? 2 * tm + rank : tm) * kBM, col0 = tn * BN;
       } else {
-        const Item it = item_of<BN, MODE>(g, experts, t, (PAIR ? 2 : 1) * kBM, rank);
+        const Item it = item_of<BN, MODE>(g, experts, t, (PAIR ? 2 : 1) * kBM, rank, expert);
         row0 = it.row, col0 = it.col, kb_first = it.k0 / kBK, nkb = it.nkb;
         if (MODE == kExpertRows) sb += it.e * g.sb_expert;
       }
@@ -612,7 +631,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // the piece's scales are in registers before its load is waited for. After
     // an abort the waits return at once and the loads go on (tensor memory is
     // still this CTA's).
-    constexpr int CH = SB_ROWS ? 16 : 32;
+    constexpr int CH = 32;
     uint32_t lo[CH], hi[CH];
     uint32_t buf = 0, buf_parity = 0, slot = 0, slot_parity = 0;
     float sc = 0.f;  // the row's scale of the block, times the column block's
@@ -633,13 +652,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     // the first tile from t on that has K blocks; those without are zeroed at the end
     auto some_from = [&](int t) {
       if constexpr (MODE == kExpertColumns)
-        while (t < tiles && item_of<BN, MODE>(g, experts, t, kBM, 0).nkb == 0) t += step;
+        while (t < tiles && item_of<BN, MODE>(g, experts, t, kBM, 0, expert).nkb == 0) t += step;
       return t;
     };
     int next = some_from(begin);
     if (next < tiles) begin_block(0);
     for (int t = next; t < tiles; t = next) {
-      if constexpr (MODE == kExpertColumns) nkb = item_of<BN, MODE>(g, experts, t, kBM, 0).nkb;
+      if constexpr (MODE == kExpertColumns) nkb = item_of<BN, MODE>(g, experts, t, kBM, 0, expert).nkb;
       next = some_from(t + step);
       float2 acc[NC / 2];
 #pragma unroll
@@ -649,13 +668,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float s = sc;
         const float* col = sb;
         const uint32_t tm = tm_lane + buf * BN;
-        float4 f[SB_ROWS ? CH / 4 : 1];
-        auto column_scales = [&](int c) {  // of piece c, before its load is waited for
-          if (SB_ROWS) {
-#pragma unroll
-            for (int i = 0; i < CH / 4; ++i) f[i] = *reinterpret_cast<const float4*>(col + c + 4 * i);
-          }
-        };
         auto add = [&](int c, const uint32_t(&v)[CH]) {
           const float2 s2 = make_float2(s, s);
 #pragma unroll
@@ -663,8 +675,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             float2 d0 = make_float2(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]));
             float2 d1 = make_float2(__uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]));
             if (SB_ROWS) {
-              d0 = __fmul2_rn(d0, make_float2(f[i].x, f[i].y));
-              d1 = __fmul2_rn(d1, make_float2(f[i].z, f[i].w));
+              const float4 f = *reinterpret_cast<const float4*>(col + c + 4 * i);
+              d0 = __fmul2_rn(d0, make_float2(f.x, f.y));
+              d1 = __fmul2_rn(d1, make_float2(f.z, f.w));
             }
             acc[c / 2 + 2 * i] = __ffma2_rn(d0, s2, acc[c / 2 + 2 * i]);
             acc[c / 2 + 2 * i + 1] = __ffma2_rn(d1, s2, acc[c / 2 + 2 * i + 1]);
@@ -674,11 +687,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t done = smem_addr(&scale_empty[slot]);
 #pragma unroll
         for (int c = 0; c < NC; c += 2 * CH) {
-          column_scales(c);
           tc::tmem_ld_wait(lo);
           tc::tmem_ld_async(tm + (uint32_t)(c + CH), hi);
           add(c, lo);
-          column_scales(c + CH);
           tc::tmem_ld_wait(hi);
           if (c + 2 * CH < NC) {
             tc::tmem_ld_async(tm + (uint32_t)(c + 2 * CH), lo);
@@ -687,8 +698,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
             if (PAIR) tc::arrive_cluster_if(first, tc::mapa(smem_addr(&acc_empty[buf]), 0));
             else tc::arrive_if(first, smem_addr(&acc_empty[buf]));
-            buf ^= 1;
-            buf_parity ^= buf == 0;
+            if (++buf == P::kBufs) buf = 0, buf_parity ^= 1;
             if (slot_done && ++slot == P::kScaleSlots) slot = 0, slot_parity ^= 1;
             if (!last || next < tiles) begin_block(last ? 0 : kb + 1);
           }
@@ -702,10 +712,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       int tm_i, tn_i;
       if constexpr (MODE == kOne) tile_of<BN>(g, t, &tm_i, &tn_i);
       if constexpr (MODE != kOne) {
-        const Item it = item_of<BN, MODE>(g, experts, t, (PAIR ? 2 : 1) * kBM, rank);
+        const Item it = item_of<BN, MODE>(g, experts, t, (PAIR ? 2 : 1) * kBM, rank, expert);
         void* d = MODE == kExpertRows ? g.d : static_cast<char*>(g.d) + it.e * g.d_expert * (g.d_f32 ? 4 : 2);
         if (*abortp == 0u)
-          store_rows<NC, VEC>(g, d, it.row_end, acc, it.row + (warp & 3) * 32, it.col + wg * NC, lane, stage[0]);
+          store_rows<NC, VEC>(g, d, it.row_end, acc, it.row + (warp & 3) * 32, it.col + wg * NC, lane, stage[0],
+                              it.some_end);
       } else if constexpr (!SPLIT) {
         if (*abortp == 0u)
           store_rows<NC, VEC>(g, g.d, g.M, acc, (PAIR ? 2 * tm_i + rank : tm_i) * kBM + (warp & 3) * 32,
@@ -766,7 +777,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int c = lane * (g.d_f32 ? 8 : 16); c < g.N; c += 32 * (g.d_f32 ? 8 : 16)) zero_row(g, g.d, row, c, 1);
     } else if constexpr (MODE == kExpertColumns) {  // experts without rows
       for (int t = begin; t < tiles; t += step) {
-        const Item it = item_of<BN, MODE>(g, experts, t, (PAIR ? 2 : 1) * kBM, rank);
+        const Item it = item_of<BN, MODE>(g, experts, t, (PAIR ? 2 : 1) * kBM, rank, expert);
         const int row = it.row + (warp & 3) * 32 + lane;
         if (it.nkb == 0 && row < it.row_end)
           zero_row(g, static_cast<char*>(g.d) + it.e * g.d_expert * (g.d_f32 ? 4 : 2), row, it.col + wg * NC, NC);
@@ -793,7 +804,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_wait_bounded(smem_addr(&full_bar[k % P::kStages]), (k / P::kStages) & 1u,
                           kDrainLimitCycles);
       if (m > 0)
-        mbar_wait_bounded(smem_addr(&acc_full[(m - 1) & 1u]), ((m - 1) >> 1) & 1u,
+        mbar_wait_bounded(smem_addr(&acc_full[(m - 1) % P::kBufs]), ((m - 1) / P::kBufs) & 1u,
                           kDrainLimitCycles);
       // and what nothing counts now: a pair's loads on their way here, or parts of
       // a rank that gave up later than this one
@@ -1315,7 +1326,7 @@ cudaError_t launch_experts(const GroupedGemmArgs& p, const TileArgs& g, int64_t 
   if (e != cudaSuccess) return e;
   CUtensorMap map_a, map_b;
   const int64_t K = columns ? p.R : p.K;
-  if (!tc::encode_e4m3_operand(&map_a, p.a, columns ? p.N : p.R, K, p.lda, kBM) ||
+  if (!tc::encode_e4m3_operand(&map_a, p.a, columns ? p.N : p.R, K, p.lda, columns ? kBM : g.a_box) ||
       !(columns ? tc::encode_e4m3_operand(&map_b, p.b, p.K, K, p.ldb, kBM)
                 : tc::encode_e4m3_matrices(&map_b, p.b, p.E, p.N, K, p.ldb, p.b_expert, kBM)))
     return cudaErrorInvalidValue;
@@ -1339,18 +1350,24 @@ int grouped_gemm(const GroupedGemmArgs& p, cudaStream_t stream, const char** why
   g.sb = p.sb, g.sb_row = p.sb_row, g.sb_kb = p.sb_kb, g.sb_expert = p.sb_expert;
   g.d = p.d, g.ldd = p.ldd, g.d_expert = p.d_expert;
   g.d_f32 = p.d_f32, g.wait_limit = p.wait_limit;
-  g.offsets = p.offsets, g.E = (int)p.E, g.R = (int)p.R;
+  g.offsets = p.offsets, g.counts = p.counts, g.E = (int)p.E, g.R = (int)p.R;
   g.band = kBand, g.tail = -1;
   const int sms = device_sm_count();
   cudaError_t e;
   if (!p.columns) {
-    // 256-wide tiles while every SM can get one (the offsets are on the GPU: R bounds the rows)
+    // 256-wide tiles unless 128-wide ones, which take a little more than half as long,
+    // need less time in whole rounds. (The offsets are on the GPU: R bounds the rows.)
     g.M = (int)p.R, g.N = (int)p.N, g.KB = (int)((p.K + kBK - 1) / kBK);
-    const int64_t rows = p.R / kBM, wide = rows * ((p.N + 255) / 256);
-    const bool narrow = wide < sms;
-    g.tiles_n = (int)((p.N + (narrow ? 127 : 255)) / (narrow ? 128 : 256));
-    e = narrow ? launch_experts<128, kExpertRows, false>(p, g, rows * g.tiles_n, stream)
-               : launch_experts<256, kExpertRows, false>(p, g, wide, stream);
+    const int64_t rows = p.R / kBM, n2 = (p.N + 255) / 256, n1 = (p.N + 127) / 128;
+    // few rows an expert: small boxes of A, and the weights' bytes bound both widths
+    const bool few = p.counts != nullptr && p.R < 192 * p.E;
+    const int64_t likely = few && rows > p.E ? p.E : rows;
+    const int64_t rounds2 = (likely * n2 + sms - 1) / sms, rounds1 = (likely * n1 + sms - 1) / sms;
+    g.a_box = few ? 32 : kBM;
+    const bool narrow = (few ? 10 : 12) * rounds1 < 20 * rounds2;
+    g.tiles_n = (int)(narrow ? n1 : n2);
+    e = narrow ? launch_experts<128, kExpertRows, false>(p, g, rows * n1, stream)
+               : launch_experts<256, kExpertRows, false>(p, g, rows * n2, stream);
   } else {
     // pairs while every pair gets a tile of 256 x 256, then 128 x 256, then 128 x 128
     g.M = (int)p.N, g.N = (int)p.K;

@@ -994,7 +994,7 @@ int check_moe_sizes(int64_t T, int64_t E, int64_t k, int64_t H, int64_t I) {
 extern "C" int cutie_fp8_grouped_gemm(const void* a, int64_t lda, const void* a_scale, int64_t sa_row,
                                       int64_t sa_kb, const void* b, int64_t ldb, int64_t b_expert,
                                       const void* b_scale, int64_t sb_row, int64_t sb_kb, int64_t sb_expert,
-                                      const void* offsets, int64_t E, void* d, int64_t ldd, int d_dtype,
+                                      const void* offsets, const void* counts, int64_t E, void* d, int64_t ldd, int d_dtype,
                                       int64_t R, int64_t N, int64_t K, void* stream) {
   g_err[0] = '\0';
   GroupedGemmArgs g;
@@ -1004,12 +1004,14 @@ extern "C" int cutie_fp8_grouped_gemm(const void* a, int64_t lda, const void* a_
   if (R == 0) return CUTIE_OK;
   if ((rc = check_matrix("a", a, lda, K, 16, 16)) != CUTIE_OK) return rc;
   if ((rc = check_matrix("b", b, ldb, K, 16, 16)) != CUTIE_OK) return rc;
+  if (!aligned(counts, 4)) return fail(CUTIE_ERR_ALIGNMENT, "counts must be 4-byte aligned");
   if (b_expert < 0 || b_expert % 16 != 0 || sb_expert < 0)
     return fail(CUTIE_ERR_ALIGNMENT, "b_expert must be a multiple of 16 and no stride negative");
   if ((rc = check_sectors("d", d, ldd, N, g.d_f32)) != CUTIE_OK) return rc;
   if ((R / 128) * ((N + 127) / 128) > INT32_MAX / 2)
     return fail(CUTIE_ERR_UNSUPPORTED, "R x N has more than 2^30 tiles");
   g.b_expert = E > 1 ? b_expert : N * ldb, g.sb_expert = sb_expert;
+  g.counts = static_cast<const int*>(counts);
   g.d = d, g.ldd = ldd;
   const char* why = "";
   rc = grouped_gemm(g, static_cast<cudaStream_t>(stream), &why);

@@ -370,6 +370,7 @@ struct GroupedGemmArgs {
   const float* sb;
   int64_t sb_row, sb_kb, sb_expert;
   const int* offsets;
+  const int* counts;  // rows before the padding, or null (rows only)
   void* d;  // [R, N] (columns: [E, N, K])
   int64_t ldd, d_expert;
   bool d_f32;

@@ -466,12 +466,16 @@ void no_second_derivatives(const char* name) {
 
 // ---- The experts' products on sorted rows (cutie_fp8_grouped_gemm, _wgrad).
 
-// A plan's offsets as the products take them.
-void product_offsets(const at::Tensor& offsets, int64_t align, int64_t E, const at::Device& dev) {
+// A plan's offsets and counts as the products take them.
+void product_offsets(const at::Tensor& offsets, const at::Tensor& counts, int64_t align, int64_t E,
+                     const at::Device& dev) {
   if (align <= 0 || align % 128 != 0) bad("the experts' products need a plan with align a multiple of 128");
   if (offsets.dim() != 1 || offsets.size(0) != E + 1 || offsets.scalar_type() != at::kInt ||
       !offsets.is_contiguous() || offsets.device() != dev)
     bad("the plan's offsets must be a contiguous int32 [E + 1] tensor on the rows' device, E = " + std::to_string(E));
+  if (counts.dim() != 1 || counts.size(0) != E || counts.scalar_type() != at::kInt || !counts.is_contiguous() ||
+      counts.device() != dev)
+    bad("the plan's counts must be a contiguous int32 [E] tensor on the rows' device");
 }
 
 // Matrices [E, N, K] of codes and their scales [E, ceil(N/128), ceil(K/128)].
@@ -497,15 +501,16 @@ Matrices expert_matrices(const at::Tensor& q, const at::Tensor& s, int64_t E, in
           s.data_ptr(), s.stride(1), s.stride(2), s.stride(0)};
 }
 
-void grouped_product(const Operand& a, const Matrices& b, const at::Tensor& offsets, int64_t E, const at::Tensor& d,
-                     int64_t ldd, int64_t R, int64_t N, int64_t K, void* stream) {
+void grouped_product(const Operand& a, const Matrices& b, const at::Tensor& offsets, const at::Tensor& counts,
+                     int64_t E, const at::Tensor& d, int64_t ldd, int64_t R, int64_t N, int64_t K, void* stream) {
   check_status(cutie_fp8_grouped_gemm(
-      a.q, a.ld, a.s, a.s_row, a.s_kb, b.q, b.ld, b.each, b.s, b.s_row, b.s_kb, b.s_each, offsets.data_ptr(), E,
+      a.q, a.ld, a.s, a.s_row, a.s_kb, b.q, b.ld, b.each, b.s, b.s_row, b.s_kb, b.s_each, offsets.data_ptr(), counts.data_ptr(), E,
       d.data_ptr(), ldd, d.scalar_type() == at::kFloat ? CUTIE_DTYPE_F32 : CUTIE_DTYPE_BF16, R, N, K, stream));
 }
 
 at::Tensor fp8_grouped_gemm(const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor& b,
-                            const at::Tensor& b_scale, const at::Tensor& offsets, int64_t align,
+                            const at::Tensor& b_scale, const at::Tensor& offsets, const at::Tensor& counts,
+                            int64_t align,
                             const c10::optional<at::Tensor>& out, bool out_f32) {
   if (!a.is_cuda()) bad("a must be a CUDA tensor (this library has no CPU path)");
   const at::Device dev = a.device();
@@ -513,7 +518,7 @@ at::Tensor fp8_grouped_gemm(const at::Tensor& a, const at::Tensor& a_scale, cons
   const int64_t lda = matrix_ld(a, "a", dev);
   if (b.dim() != 3) bad("b must be 3-D [E, N, K]");
   const int64_t R = a.size(0), K = a.size(1), E = b.size(0), N = b.size(1);
-  product_offsets(offsets, align, E, dev);
+  product_offsets(offsets, counts, align, E, dev);
   if (a_scale.dim() != 2 || a_scale.size(0) != R || a_scale.size(1) != (K + 127) / 128 ||
       a_scale.scalar_type() != at::kFloat || a_scale.device() != dev)
     bad("a_scale must be a float32 [R, ceil(K/128)] tensor on a's device");
@@ -529,7 +534,7 @@ at::Tensor fp8_grouped_gemm(const at::Tensor& a, const at::Tensor& a_scale, cons
                                  : at::empty({R, N}, at::TensorOptions().device(dev).dtype(
                                                          out_f32 ? at::kFloat : at::kBFloat16));
   const Operand rows{a.data_ptr(), lda, a_scale.data_ptr(), a_scale.stride(0), a_scale.stride(1)};
-  grouped_product(rows, m, offsets, E, d, matrix_ld(d, "out", dev), R, N, K,
+  grouped_product(rows, m, offsets, counts, E, d, matrix_ld(d, "out", dev), R, N, K,
                   at::cuda::getCurrentCUDAStream(dev.index()).stream());
   return d;
 }
@@ -538,7 +543,8 @@ struct FP8GroupedLinear : public torch::autograd::Function<FP8GroupedLinear> {
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight,
                             const c10::optional<at::Tensor>& wq, const c10::optional<at::Tensor>& ws,
                             const c10::optional<at::Tensor>& wqt, const c10::optional<at::Tensor>& wst,
-                            const at::Tensor& sources, const at::Tensor& offsets, bool need_dx, bool need_dw) {
+                            const at::Tensor& sources, const at::Tensor& offsets, const at::Tensor& counts,
+                            bool need_dx, bool need_dw) {
     const at::Device dev = x.device();
     const int64_t R = x.size(0), E = weight.size(0), N = weight.size(1), K = weight.size(2);
     const c10::cuda::CUDAGuard guard(dev);
@@ -566,9 +572,9 @@ struct FP8GroupedLinear : public torch::autograd::Function<FP8GroupedLinear> {
     } else {
       m = expert_matrices(*wq, *ws, E, N, K, dev, "weight_fp8");
     }
-    grouped_product(xs.rows(), m, offsets, E, y, N, R, N, K, stream);
+    grouped_product(xs.rows(), m, offsets, counts, E, y, N, R, N, K, stream);
     ctx->save_for_backward({held, !own && need_dx ? *wqt : at::Tensor(), !own && need_dx ? *wst : at::Tensor(),
-                            sources, offsets});
+                            sources, offsets, counts});
     ctx->saved_data["sizes"] =
         std::vector<int64_t>{E, N, K, need_dx, need_dw, !own, weight.scalar_type() == at::kFloat};
     return y;
@@ -576,13 +582,13 @@ struct FP8GroupedLinear : public torch::autograd::Function<FP8GroupedLinear> {
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grads) {
     no_second_derivatives("fp8_grouped_linear");
-    torch::autograd::variable_list out(10);
+    torch::autograd::variable_list out(11);
     if (!grads[0].defined()) return out;
     const auto saved = ctx->get_saved_variables();
     const auto sizes = ctx->saved_data["sizes"].toIntVector();
     const int64_t E = sizes[0], N = sizes[1], K = sizes[2];
     const bool need_dx = sizes[3], need_dw = sizes[4], given_w = sizes[5], dw_f32 = sizes[6];
-    const at::Tensor &dy = grads[0], &sources = saved[3], &offsets = saved[4];
+    const at::Tensor &dy = grads[0], &sources = saved[3], &offsets = saved[4], &counts = saved[5];
     const int64_t R = dy.size(0);
     const at::Device dev = dy.device();
     const c10::cuda::CUDAGuard guard(dev);
@@ -601,7 +607,7 @@ struct FP8GroupedLinear : public torch::autograd::Function<FP8GroupedLinear> {
         m = {q.q, q.ld, N, q.s, q.s_row, q.s_kb, N / 128};
       }
       out[0] = at::empty({R, K}, dy.options());
-      grouped_product(d.rows(), m, offsets, E, out[0], K, R, K, N, stream);
+      grouped_product(d.rows(), m, offsets, counts, E, out[0], K, R, K, N, stream);
     }
     if (need_dw) {
       xs.column_base = address(saved[0]) + (need_dx && !given_w ? w.column_bytes : 0);
@@ -616,7 +622,8 @@ struct FP8GroupedLinear : public torch::autograd::Function<FP8GroupedLinear> {
 };
 
 at::Tensor fp8_grouped_linear(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& sources,
-                              const at::Tensor& offsets, int64_t align, const c10::optional<at::Tensor>& wq,
+                              const at::Tensor& offsets, const at::Tensor& counts, int64_t align,
+                              const c10::optional<at::Tensor>& wq,
                               const c10::optional<at::Tensor>& ws, const c10::optional<at::Tensor>& wqt,
                               const c10::optional<at::Tensor>& wst) {
   if (x.dim() != 2 || weight.dim() != 3 || x.size(1) != weight.size(2)) bad("x and weight must be [R, K] and [E, N, K]");
@@ -628,7 +635,7 @@ at::Tensor fp8_grouped_linear(const at::Tensor& x, const at::Tensor& weight, con
     bad("weight must be bfloat16 or float32");
   const int64_t R = x.size(0), E = weight.size(0), N = weight.size(1), K = weight.size(2);
   if (E == 0 || N == 0 || K == 0 || N % 128 != 0 || K % 128 != 0) bad("weight's sizes must be multiples of 128");
-  product_offsets(offsets, align, E, dev);
+  product_offsets(offsets, counts, align, E, dev);
   if (sources.dim() != 1 || sources.size(0) != R || sources.scalar_type() != at::kInt || !sources.is_contiguous() ||
       sources.device() != dev)
     bad("x must have the plan's " + std::to_string(sources.size(0)) + " rows, the plan be int32 on x's device");
@@ -637,7 +644,7 @@ at::Tensor fp8_grouped_linear(const at::Tensor& x, const at::Tensor& weight, con
   if (wq.has_value() != ws.has_value()) bad("weight_fp8 must be (q, s, qt, st)");
   if (wq.has_value() && need_dx && (!wqt.has_value() || !wst.has_value()))
     bad("weight_fp8 has no transposed codes: make it with quantize_experts(weight, transposed=True)");
-  return FP8GroupedLinear::apply(x, weight, wq, ws, wqt, wst, sources, offsets, need_dx, need_dw);
+  return FP8GroupedLinear::apply(x, weight, wq, ws, wqt, wst, sources, offsets, counts, need_dx, need_dw);
 }
 
 // Bytes of workspace of a mixture-of-experts layer; argument errors raise.
@@ -1026,9 +1033,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("top_k"), py::arg("scoring"), py::arg("renormalize"), py::arg("routed_scale"),
         py::arg("out"), py::arg("topk_ids"), py::arg("topk_weights"), py::arg("workspace"));
   m.def("fp8_grouped_gemm", &fp8_grouped_gemm, py::arg("a"), py::arg("a_scale"), py::arg("b"), py::arg("b_scale"),
-        py::arg("offsets"), py::arg("align"), py::arg("out"), py::arg("out_f32"));
+        py::arg("offsets"), py::arg("counts"), py::arg("align"), py::arg("out"), py::arg("out_f32"));
   m.def("fp8_grouped_linear", &fp8_grouped_linear, py::arg("x"), py::arg("weight"), py::arg("sources"),
-        py::arg("offsets"), py::arg("align"), py::arg("wq"), py::arg("ws"), py::arg("wqt"), py::arg("wst"));
+        py::arg("offsets"), py::arg("counts"), py::arg("align"), py::arg("wq"), py::arg("ws"), py::arg("wqt"), py::arg("wst"));
   m.def("moe_plan_rows", &moe_plan_rows, py::arg("T"), py::arg("k"), py::arg("E"), py::arg("align"));
   m.def("moe_sort", &moe_sort, py::arg("ids"), py::arg("E"), py::arg("align"));
   m.def("moe_permute", &moe_permute, py::arg("x"), py::arg("sources"), py::arg("positions"));

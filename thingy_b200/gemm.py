@@ -185,11 +185,10 @@ def fp8_grouped_gemm(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_
     [E, ceil(N/128), ceil(K/128)] (``quantize_experts``), of any strides with
     dense rows. N is a multiple of 16 (fp32 out: 8); rows of a and b start on 16-byte
     boundaries, those of out on 32-byte ones. Sums are held in fp32, rounded once.
-    Rows in padding are what a holds there (zeros from ``moe_permute``) times
-    the matrix; rows behind the last expert's are zero. Forward only:
+    Rows in padding are zero, whatever a holds there. Forward only:
     ``fp8_grouped_linear`` is the layer with gradients.
     """
     if out_dtype not in (torch.bfloat16, torch.float32):
         raise ValueError(f"out_dtype must be bfloat16 or float32, got {out_dtype}")
-    return require_binding().fp8_grouped_gemm(a, a_scale, b, b_scale, plan.offsets, plan.align, out,
+    return require_binding().fp8_grouped_gemm(a, a_scale, b, b_scale, plan.offsets, plan.counts, plan.align, out,
                                               out_dtype == torch.float32)

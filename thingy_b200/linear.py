@@ -51,4 +51,4 @@ def fp8_grouped_linear(x: torch.Tensor, weight: torch.Tensor, plan, weight_fp8=N
     rows of two experts. Nothing is copied to the host.
     """
     wq, ws, wqt, wst = (None, None, None, None) if weight_fp8 is None else weight_fp8
-    return require_binding().fp8_grouped_linear(x, weight, plan.sources, plan.offsets, plan.align, wq, ws, wqt, wst)
+    return require_binding().fp8_grouped_linear(x, weight, plan.sources, plan.offsets, plan.counts, plan.align, wq, ws, wqt, wst)
