@@ -179,9 +179,9 @@ struct ExpertTable {
   int end[MODE == kExpertRows ? kMoeMaxExperts : 1];  // of the rows before the padding
 };
 
-// By the first warps of a CTA, between two barriers of its own.
-template <int MODE>
-__device__ __forceinline__ void fill_experts(const TileArgs& g, ExpertTable<MODE>& x) {
+// By all of a CTA's threads. `rows` of a tile; FULL: tiles cover the padding too.
+template <int MODE, bool FULL = true>
+__device__ __forceinline__ void fill_experts(const TileArgs& g, ExpertTable<MODE>& x, int rows = kBM) {
   for (int e = threadIdx.x; e <= g.E; e += blockDim.x)
     x.begin[e] = min(max(g.offsets[e], 0), g.R) & ~(kBM - 1);
   __syncthreads();
@@ -189,10 +189,12 @@ __device__ __forceinline__ void fill_experts(const TileArgs& g, ExpertTable<MODE
     for (int e = threadIdx.x; e < g.E; e += blockDim.x)
       x.end[e] = g.counts == nullptr ? x.begin[e + 1]
                                      : x.begin[e] + min(max(g.counts[e], 0), max(x.begin[e + 1] - x.begin[e], 0));
+  if (MODE == kExpertRows) __syncthreads();
+  auto tiles_of = [&](int e) { return max((FULL ? x.begin[e + 1] : x.end[e]) - x.begin[e] + rows - 1, 0) / rows; };
   if (MODE == kExpertRows && threadIdx.x < 32) {
     const int per = (g.E + 31) / 32, lane = threadIdx.x, e0 = min(lane * per, g.E), e1 = min(e0 + per, g.E);
     int mine = 0;
-    for (int e = e0; e < e1; ++e) mine += max(x.begin[e + 1] - x.begin[e], 0) / kBM;
+    for (int e = e0; e < e1; ++e) mine += tiles_of(e);
     int sum = mine;
 #pragma unroll
     for (int o = 1; o < 32; o *= 2) {
@@ -203,7 +205,7 @@ __device__ __forceinline__ void fill_experts(const TileArgs& g, ExpertTable<MODE
     sum -= mine;
     for (int e = e0; e < e1; ++e) {
       x.tiles[e] = sum;
-      sum += max(x.begin[e + 1] - x.begin[e], 0) / kBM;
+      sum += tiles_of(e);
     }
   }
   __syncthreads();
@@ -1311,6 +1313,292 @@ cudaError_t device_error_block_gemm(int* out, bool clear) {
 
 namespace {
 
+// ------------------------------------------------------------------ experts with few rows
+//
+// Bound by reading the experts' weights once, and built like the product of few rows:
+// the weight is the 128-row side of the MMA, the expert's rows its N side, up to BR
+// of them, as many (in sixteens) as there are. A persistent CTA an SM walks items
+// of one expert, 128 of its columns and BR of its rows; the copies of the next
+// item run on while one is stored. Taken up to kEMeanRows rows an expert in the
+// mean, against tiles of 128 rows, whose sums go over the padding too: 64 experts of
+// 2048 x 7168 with 9 rows 152 against 178 us (940 MB: 96% of the copy bandwidth),
+// 37 rows 164 against 182, 50 rows 190 against 182; of 4096 x 2048 with 25 rows 103
+// against 112, 50 rows 128 against 114.
+constexpr int kERows = 64, kEStages = 4, kEMeanRows = 40;
+
+struct ExpertFewPlan {
+  static constexpr uint32_t kBlockBytes = kBoxBytes + kERows * kBK;
+  static constexpr uint32_t kStageBytes = kFewStep * kBlockBytes;
+  static constexpr size_t kSmemBytes = kEStages * kStageBytes + 1024;
+  static constexpr int kBufs = 2;  // of kFewStep x kERows columns
+  static constexpr uint32_t kTmemCols = kBufs * kFewStep * kERows;
+  static constexpr int kScales = kERows + 4;  // the rows', then the weight block's
+  static_assert(kSmemBytes + kFewScaleSlots * kScaleBlocks * kScales * 4 + sizeof(ExpertTable<kExpertRows>) + 512 <=
+                    227 * 1024,
+                "shared memory");
+};
+
+// Item t: expert, first row, rows, first column.
+struct ExpertItem {
+  int e, row, rows, col;
+};
+__device__ __forceinline__ ExpertItem expert_item(const TileArgs& g, const ExpertTable<kExpertRows>& x, int t, int& e) {
+  while (x.tiles[e + 1] * g.tiles_n <= t) ++e;  // t < tiles[E] tiles_n
+  const int first = x.tiles[e], parts = x.tiles[e + 1] - first, in = t - first * g.tiles_n;
+  ExpertItem i;
+  i.e = e;
+  i.row = x.begin[e] + in % parts * kERows;  // parts of one weight after another
+  i.rows = min(x.end[e] - i.row, kERows);
+  i.col = in / parts * kBM;
+  return i;
+}
+
+__global__ void __launch_bounds__(kFewThreads, 1)
+    expert_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                      const TileArgs g) {
+  using P = ExpertFewPlan;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t full_bar[kEStages];
+  __shared__ __align__(8) uint64_t empty_bar[kEStages];
+  __shared__ __align__(8) uint64_t acc_full[P::kBufs];
+  __shared__ __align__(8) uint64_t acc_empty[P::kBufs];
+  __shared__ __align__(8) uint64_t scale_full[kFewScaleSlots];
+  __shared__ __align__(8) uint64_t scale_empty[kFewScaleSlots];
+  __shared__ __align__(16) float scales[kFewScaleSlots][kScaleBlocks][P::kScales];
+  __shared__ ExpertTable<kExpertRows> experts;
+  __shared__ uint32_t tmem_base_slot;
+  __shared__ uint32_t abort_flag;
+  __shared__ uint32_t issued, committed;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
+  volatile uint32_t* abortp = &abort_flag;
+  if (threadIdx.x == 0) {
+    tc::prefetch_map(&map_a);
+    tc::prefetch_map(&map_b);
+    for (int s = 0; s < kEStages; ++s) {
+      mbar_init(smem_addr(&full_bar[s]), 1);
+      mbar_init(smem_addr(&empty_bar[s]), 1);
+    }
+    for (int b = 0; b < P::kBufs; ++b) {
+      mbar_init(smem_addr(&acc_full[b]), 1);
+      mbar_init(smem_addr(&acc_empty[b]), 4);
+    }
+    for (int s = 0; s < kFewScaleSlots; ++s) {
+      mbar_init(smem_addr(&scale_full[s]), 32);
+      mbar_init(smem_addr(&scale_empty[s]), 4);
+    }
+    abort_flag = 0;
+    issued = committed = 0;
+    mbar_init_fence();
+  }
+  if (warp == 5) tc::tmem_alloc(smem_addr(&tmem_base_slot), P::kTmemCols);
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const uint32_t tmem = tmem_base_slot;
+  griddep_wait();
+  griddep_launch_dependents();
+  fill_experts<kExpertRows, false>(g, experts, kERows);
+  const int items = experts.tiles[g.E] * g.tiles_n, begin = blockIdx.x, step = gridDim.x;
+  int expert = 0;
+
+  if (warp == 4) {
+    // ---- operands
+    const bool leader = tc::elect_one();
+    uint32_t s = 0, parity = 1;
+    bool ok = true;
+    for (int t = begin; t < items && ok; t += step) {
+      const ExpertItem it = expert_item(g, experts, t, expert);
+      const int boxes = (it.rows + 31) / 32;
+      for (int kb = 0; kb < g.KB; kb += kFewStep) {
+        ok = __all_sync(0xffffffffu, tc::wait_or_abort(smem_addr(&empty_bar[s]), parity, abortp, g.wait_limit));
+        if (!ok) break;
+        if (leader) {
+          const int n = min(kFewStep, g.KB - kb);
+          uint32_t st = base + s * P::kStageBytes;
+          const uint32_t bar = smem_addr(&full_bar[s]);
+          mbar_arrive_expect_tx(bar, (uint32_t)n * (kBoxBytes + (uint32_t)boxes * 32 * kBK));
+          for (int j = 0; j < n; ++j, st += P::kBlockBytes) {
+            tc::tma_load_3d(st, &map_b, (kb + j) * kBK, it.col, it.e, bar);
+            for (int i = 0; i < boxes; ++i)
+              tc::tma_load_2d(st + kBoxBytes + (uint32_t)(i * 32 * kBK), &map_a, (kb + j) * kBK, it.row + 32 * i, bar);
+          }
+          ++issued;
+        }
+        if (++s == kEStages) s = 0, parity ^= 1;
+      }
+    }
+  } else if (warp == 5) {
+    // ---- MMAs
+    const bool leader = tc::elect_one();
+    const uint32_t lo0 = tc::sw128_lo(base), hi = tc::sw128_hi();
+    uint32_t s = 0, parity = 0, buf = 0, buf_parity = 1;
+    bool ok = true;
+    for (int t = begin; t < items && ok; t += step) {
+      const ExpertItem it = expert_item(g, experts, t, expert);
+      const uint32_t idesc = tc::f8_idesc(kBM, (it.rows + 15) & ~15);
+      for (int kb = 0; kb < g.KB; kb += kFewStep) {
+        ok = tc::wait_or_abort(smem_addr(&full_bar[s]), parity, abortp, g.wait_limit) &&
+             tc::wait_or_abort(smem_addr(&acc_empty[buf]), buf_parity, abortp, g.wait_limit);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc::fence_after();
+        if (leader) {
+          uint32_t lo = lo0 + s * (P::kStageBytes >> 4), d = tmem + buf * kFewStep * kERows;
+          const int n = min(kFewStep, g.KB - kb);
+          for (int j = 0; j < n; ++j, lo += P::kBlockBytes >> 4, d += kERows) {
+#pragma unroll
+            for (int kk = 0; kk < kBK / 32; ++kk)
+              tc::mma_f8(d, lo + 2 * kk, lo + (kBoxBytes >> 4) + 2 * kk, hi, idesc, kk != 0);
+          }
+          tc::commit(smem_addr(&empty_bar[s]));
+          tc::commit(smem_addr(&acc_full[buf]));
+          ++committed;
+        }
+        __syncwarp();
+        if (++s == kEStages) s = 0, parity ^= 1;
+        if (++buf == P::kBufs) buf = 0, buf_parity ^= 1;
+      }
+    }
+  } else if (warp == 6) {
+    // ---- scales
+    uint32_t s = 0, parity = 1;
+    bool ok = true;
+    for (int t = begin; t < items && ok; t += step) {
+      const ExpertItem it = expert_item(g, experts, t, expert);
+      const float *pa[kERows / 32], *pb = nullptr;
+#pragma unroll
+      for (int i = 0; i < kERows / 32; ++i)
+        pa[i] = lane + 32 * i < it.rows ? g.sa + (int64_t)(it.row + lane + 32 * i) * g.sa_row : nullptr;
+      if (lane == 0) pb = g.sb + it.e * g.sb_expert + (int64_t)(it.col / kBM) * g.sb_row;
+      for (int kb = 0; kb < g.KB; ++kb) {
+        const int j = kb % kScaleBlocks;
+        if (j == 0) {
+          ok = __all_sync(0xffffffffu, tc::wait_or_abort(smem_addr(&scale_empty[s]), parity, abortp, g.wait_limit));
+          if (!ok) break;
+        }
+#pragma unroll
+        for (int i = 0; i < kERows / 32; ++i)
+          if (pa[i] != nullptr) {
+            tc::cp_async_4(smem_addr(&scales[s][j][lane + 32 * i]), pa[i]);
+            pa[i] += g.sa_kb;
+          }
+        if (pb != nullptr) {
+          tc::cp_async_4(smem_addr(&scales[s][j][kERows]), pb);
+          pb += g.sb_kb;
+        }
+        if (j == kScaleBlocks - 1 || kb == g.KB - 1) {
+          tc::cp_async_arrive(smem_addr(&scale_full[s]));
+          if (++s == kFewScaleSlots) s = 0, parity ^= 1;
+        }
+      }
+    }
+    tc::cp_async_wait_all();
+  } else {
+    // ---- sums: a column of D (a weight row) a thread
+    const int r = warp * 32 + lane;
+    const uint32_t tm_lane = tmem + ((uint32_t)(warp * 32) << 16);
+    uint32_t buf = 0, buf_parity = 0, slot = 0, slot_parity = 0;
+    bool ok = true;
+    for (int t = begin; t < items && ok; t += step) {
+      const ExpertItem it = expert_item(g, experts, t, expert);
+      float2 acc[kERows / 2];
+#pragma unroll
+      for (int c = 0; c < kERows / 2; ++c) acc[c] = make_float2(0.f, 0.f);
+      for (int kb = 0; kb < g.KB; kb += kFewStep) {
+        const int j0 = kb % kScaleBlocks;
+        ok = (j0 != 0 || tc::wait_or_abort(smem_addr(&scale_full[slot]), slot_parity, abortp, g.wait_limit)) &&
+             tc::wait_or_abort(smem_addr(&acc_full[buf]), buf_parity, abortp, g.wait_limit);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc::fence_after();
+#pragma unroll
+        for (int j = 0; j < kFewStep; ++j) {
+          if (kb + j >= g.KB) break;
+          const float* sc = scales[slot][j0 + j];
+          const float2 sw = make_float2(sc[kERows], sc[kERows]);
+#pragma unroll
+          for (int c = 0; c < kERows; c += 16) {
+            if (c >= it.rows) break;
+            uint32_t v[16];
+            tc::tmem_ld_async(tm_lane + (buf * kFewStep + j) * kERows + (uint32_t)c, v);
+            float2 f[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float4 q = *reinterpret_cast<const float4*>(sc + c + 4 * i);
+              f[2 * i] = __fmul2_rn(make_float2(q.x, q.y), sw);
+              f[2 * i + 1] = __fmul2_rn(make_float2(q.z, q.w), sw);
+            }
+            tc::tmem_ld_wait(v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              acc[c / 2 + i] = __ffma2_rn(
+                  make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), f[i], acc[c / 2 + i]);
+          }
+        }
+        tc::fence_before();
+        __syncwarp();
+        tc::arrive_if(lane == 0, smem_addr(&acc_empty[buf]));
+        if (++buf == P::kBufs) buf = 0, buf_parity ^= 1;
+        if (j0 + kFewStep == kScaleBlocks || kb + kFewStep >= g.KB) {
+          tc::arrive_if(lane == 0, smem_addr(&scale_empty[slot]));
+          if (++slot == kFewScaleSlots) slot = 0, slot_parity ^= 1;
+        }
+      }
+      if (!ok) break;
+      if (it.col + r < g.N) {
+#pragma unroll
+        for (int c = 0; c < kERows; ++c) {
+          if (c >= it.rows) break;
+          const float v = c & 1 ? acc[c / 2].y : acc[c / 2].x;
+          const int64_t at = (int64_t)(it.row + c) * g.ldd + it.col + r;
+          if (g.d_f32) static_cast<float*>(g.d)[at] = v;
+          else static_cast<uint16_t*>(g.d)[at] = (uint16_t)(f2_to_bf2(make_float2(v, 0.f)) & 0xffffu);
+        }
+      }
+      // padding behind an expert's last rows
+      if (it.row + it.rows == experts.end[it.e]) {
+        const int per = g.d_f32 ? 8 : 16, sectors = kBM / per;
+        for (int i = (int)threadIdx.x; i < (experts.begin[it.e + 1] - experts.end[it.e]) * sectors; i += 128)
+          zero_row(g, g.d, experts.end[it.e] + i / sectors, it.col + i % sectors * per, 1);
+      }
+    }
+    // rows behind the last expert's
+    const int per = g.d_f32 ? 8 : 16;
+    for (int64_t row = (int64_t)experts.begin[g.E] + blockIdx.x * 4 + warp; row < g.R; row += (int64_t)gridDim.x * 4)
+      for (int c = lane * per; c < g.N; c += 32 * per) zero_row(g, g.d, row, c, 1);
+  }
+  __syncwarp();
+  tc::fence_before();
+  __syncthreads();
+  if (*abortp) {
+    if (threadIdx.x == 0) {
+      atomicCAS(&g_block_gemm_device_error, kDevErrNone, kDevErrBulkWaitTimeout);
+      const uint32_t n = issued, m = committed;  // copies and MMAs in flight finish first
+      for (uint32_t k = n > kEStages ? n - kEStages : 0; k < n; ++k)
+        mbar_wait_bounded(smem_addr(&full_bar[k % kEStages]), (k / kEStages) & 1u, kDrainLimitCycles);
+      if (m > 0)
+        mbar_wait_bounded(smem_addr(&acc_full[(m - 1) % P::kBufs]), ((m - 1) / P::kBufs) & 1u, kDrainLimitCycles);
+    }
+    __syncthreads();
+  }
+  if (warp == 5) tc::tmem_dealloc(tmem, P::kTmemCols);
+}
+
+cudaError_t launch_expert_few(const GroupedGemmArgs& p, const TileArgs& g, int64_t items, cudaStream_t stream) {
+  const cudaError_t e = cudaFuncSetAttribute(expert_few_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             (int)ExpertFewPlan::kSmemBytes);
+  if (e != cudaSuccess) return e;
+  CUtensorMap map_a, map_b;
+  if (!tc::encode_e4m3_operand(&map_a, p.a, p.R, p.K, p.lda, 32) ||
+      !tc::encode_e4m3_matrices(&map_b, p.b, p.E, p.N, p.K, p.ldb, p.b_expert, kBM))
+    return cudaErrorInvalidValue;
+  const int sms = device_sm_count();
+  return launch_pdl(expert_few_kernel, (unsigned)(items < sms ? items : sms), kFewThreads, ExpertFewPlan::kSmemBytes,
+                    stream, map_a, map_b, g);
+}
+
 // A launch of the tiled kernel over `units` tiles at most; B: [E] matrices of rows x K
 // (kExpertRows) or one.
 template <int BN, int MODE, bool PAIR>
@@ -1359,15 +1647,17 @@ int grouped_gemm(const GroupedGemmArgs& p, cudaStream_t stream, const char** why
     // need less time in whole rounds. (The offsets are on the GPU: R bounds the rows.)
     g.M = (int)p.R, g.N = (int)p.N, g.KB = (int)((p.K + kBK - 1) / kBK);
     const int64_t rows = p.R / kBM, n2 = (p.N + 255) / 256, n1 = (p.N + 127) / 128;
-    // few rows an expert: small boxes of A, and the weights' bytes bound both widths
-    const bool few = p.counts != nullptr && p.R < 192 * p.E;
-    const int64_t likely = few && rows > p.E ? p.E : rows;
-    const int64_t rounds2 = (likely * n2 + sms - 1) / sms, rounds1 = (likely * n1 + sms - 1) / sms;
-    g.a_box = few ? 32 : kBM;
-    const bool narrow = (few ? 10 : 12) * rounds1 < 20 * rounds2;
-    g.tiles_n = (int)(narrow ? n1 : n2);
-    e = narrow ? launch_experts<128, kExpertRows, false>(p, g, rows * n1, stream)
-               : launch_experts<256, kExpertRows, false>(p, g, rows * n2, stream);
+    if (p.counts != nullptr && p.R < (127 + kEMeanRows) * p.E) {  // R: the rows, and up to 127 an expert more
+      g.tiles_n = (int)n1;
+      e = launch_expert_few(p, g, rows * (kBM / kERows) * n1, stream);
+    } else {
+      const int64_t rounds2 = (rows * n2 + sms - 1) / sms, rounds1 = (rows * n1 + sms - 1) / sms;
+      g.a_box = p.counts != nullptr && p.R < 192 * p.E ? 32 : kBM;
+      const bool narrow = 12 * rounds1 < 20 * rounds2;
+      g.tiles_n = (int)(narrow ? n1 : n2);
+      e = narrow ? launch_experts<128, kExpertRows, false>(p, g, rows * n1, stream)
+                 : launch_experts<256, kExpertRows, false>(p, g, rows * n2, stream);
+    }
   } else {
     // pairs while every pair gets a tile of 256 x 256, then 128 x 256, then 128 x 128
     g.M = (int)p.N, g.N = (int)p.K;
