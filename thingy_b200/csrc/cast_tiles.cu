@@ -84,20 +84,25 @@ __global__ void __launch_bounds__(kThreads, 4)
   griddep_wait();
   griddep_launch_dependents();
 
-  uint32_t held = 0xffu;  // bit i: row i of the eight counts
-  if (SORTED) {
-    if (a.sources[tr * kTile] < 0) return;
-    held = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (r0 + i < a.M && a.sources[r0 + i] >= 0) held |= 1u << i;
-  }
+  // SORTED: the sources of the warp's 16 rows, lane 16: of the tile's first; read
+  // beside the rows, not before them (M is a multiple of 128)
+  const int source = SORTED && lane <= 16 ? a.sources[tr * kTile + (lane < 16 ? 16 * warp + lane : 0)] : 0;
   uint32_t x[8][4];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     uint4 w = make_uint4(0, 0, 0, 0);
-    if (col_ok && r0 + i < a.M && (!SORTED || (held >> i & 1u))) w = ld_stream(a.x + (r0 + i) * a.ldx + c0);
+    if (col_ok && r0 + i < a.M) w = ld_stream(a.x + (r0 + i) * a.ldx + c0);
     x[i][0] = w.x, x[i][1] = w.y, x[i][2] = w.z, x[i][3] = w.w;
+  }
+  if (SORTED) {
+    const uint32_t none = __ballot_sync(0xffffffffu, source < 0);
+    if (none >> 16 & 1u) return;
+    const uint32_t mine = none >> (rg & 1) * 8 & 0xffu;
+    if (mine != 0) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (mine >> i & 1u) x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0u;
+    }
   }
   const uint32_t all = 0xffffffffu;
   uint2 codes[BLOCK ? 8 : 1];  // block kind: the rows' codes, which its transpose shares
