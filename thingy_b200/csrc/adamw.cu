@@ -48,6 +48,7 @@ struct Table {
   int64_t n[N];
   uint32_t first[N + 1];  // chunks before the tensor's
   uint32_t ordinal[N];    // its place in the caller's list
+  int8_t head[N];         // elements before the first that all of its arrays have on 16 bytes; -1: none
 };
 static_assert(sizeof(Table<kManyTensors>) + sizeof(AdamwStep) + 64 <= 32764, "a launch's argument");
 
@@ -208,8 +209,6 @@ __device__ __forceinline__ void store8(E4m3* p, bool vec, int n, const uint32_t 
   }
 }
 
-__device__ __forceinline__ bool on16(const void* p) { return (reinterpret_cast<uint64_t>(p) & 15u) == 0; }
-
 // What a step's constants are, made by one thread; 1 - b^t in 64 bits: in 32 its
 // first digits are gone while b^t is near one.
 struct Factors {
@@ -242,17 +241,21 @@ __device__ __forceinline__ int tensor_at(const Table<N>& t, int tensors, uint32_
   return lo;
 }
 
-// A chunk of tensor i from element `begin` on. WHOLE: all of its elements are there
-// and on the vectors' boundaries, so that nothing in it branches.
+// A chunk of tensor i from element `begin` on, vectors where `vec`. WHOLE: all of its
+// elements are there and on the vectors' boundaries, so that nothing in it branches.
+// States in 32 bits: tensors inside of a buffer that begin between vectors have their
+// first chunk behind `head` elements, which go one by one.
 struct Chunk {
   int i, count;
+  bool vec;
   int64_t begin;
 };
 template <int N>
 __device__ __forceinline__ Chunk chunk_at(const Table<N>& t, int tensors, uint32_t chunk) {
   Chunk k;
   k.i = tensor_at(t, tensors, chunk);
-  k.begin = (int64_t)(chunk - t.first[k.i]) * kChunk;
+  k.vec = t.head[k.i] >= 0;
+  k.begin = (int64_t)(chunk - t.first[k.i]) * kChunk + max((int)t.head[k.i], 0);
   k.count = (int)min((int64_t)kChunk, t.n[k.i] - k.begin);
   return k;
 }
@@ -267,11 +270,12 @@ __device__ __forceinline__ void step_values(const Table<N>& t, const Chunk& k, c
   for (int at = (int)threadIdx.x * kEach, step = 0; step < kChunk / (kThreads * kEach); ++step, at += kThreads * kEach) {
     const int n = WHOLE ? kEach : min(kEach, k.count - at);
     if (!WHOLE && n <= 0) break;
+    const bool vec = WHOLE || (k.vec && n == kEach);
     float pf[kEach], gf[kEach], mf[kEach], vf[kEach];
-    load8(g + at, WHOLE, n, gf);
-    load8(p + at, WHOLE, n, pf);
-    load8(m + at, WHOLE, n, mf);
-    load8(v + at, WHOLE, n, vf);
+    load8(g + at, vec, n, gf);
+    load8(p + at, vec, n, pf);
+    load8(m + at, vec, n, mf);
+    load8(v + at, vec, n, vf);
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       const float gc = __fmul_rn(gf[i], c);
@@ -280,9 +284,9 @@ __device__ __forceinline__ void step_values(const Table<N>& t, const Chunk& k, c
       const float d = __fadd_rn(__fmul_rn(__fsqrt_rn(vf[i]), f.root), a.eps);
       pf[i] = __fsub_rn(__fmul_rn(pf[i], f.keep), __fmul_rn(f.rate, __fdiv_rn(mf[i], d)));
     }
-    store8(p + at, WHOLE, n, pf);
-    store8(m + at, WHOLE, n, mf);
-    store8(v + at, WHOLE, n, vf);
+    store8(p + at, vec, n, pf);
+    store8(m + at, vec, n, mf);
+    store8(v + at, vec, n, vf);
   }
 }
 
@@ -297,11 +301,13 @@ __global__ void __launch_bounds__(kThreads, 5)
   const Factors f = shared;
   const float c = a.clip != nullptr ? *a.clip : 1.f;
   for (uint32_t chunk = blockIdx.x; chunk < t.first[tensors]; chunk += gridDim.x) {
-    const Chunk k = chunk_at(t, tensors, chunk);
-    if (k.count == kChunk && on16(t.g[k.i]) && on16(t.p[k.i]) && on16(t.m[k.i]) && on16(t.v[k.i]))
-      step_values<P, G, true>(t, k, a, f, c);
-    else
+    Chunk k = chunk_at(t, tensors, chunk);
+    if (k.vec && k.count == kChunk) step_values<P, G, true>(t, k, a, f, c);
+    else step_values<P, G, false>(t, k, a, f, c);
+    if (t.head[k.i] > 0 && chunk == t.first[k.i]) {
+      k.begin = 0, k.count = (int)min((int64_t)t.head[k.i], t.n[k.i]), k.vec = false;
       step_values<P, G, false>(t, k, a, f, c);
+    }
   }
 }
 
@@ -331,15 +337,16 @@ __device__ __forceinline__ void step_codes(const Table<N>& t, const Chunk& k, co
   E4m3 *m = static_cast<E4m3*>(t.m[k.i]) + from, *v = static_cast<E4m3*>(t.v[k.i]) + from;
   // whole warps go on: the lanes of a group exchange their maxima
   const int n[2] = {WHOLE ? kEach : max(0, min(kEach, k.count - at)), WHOLE ? kEach : max(0, min(kEach, k.count - at - 64))};
+  const bool vec[2] = {WHOLE || (k.vec && n[0] == kEach), WHOLE || (k.vec && n[1] == kEach)};
   float ms = 0.f, rs = 0.f;
   float gf[2][kEach], pf[2][kEach], mf[2][kEach], rf[2][kEach];
   if (n[0] > 0) ms = t.ms[k.i][group], rs = t.vs[k.i][group];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    load8(g + 64 * h, WHOLE, n[h], gf[h]);
-    load8(p + 64 * h, WHOLE, n[h], pf[h]);
-    load8(m + 64 * h, WHOLE, n[h], mf[h]);
-    load8(v + 64 * h, WHOLE, n[h], rf[h]);
+    load8(g + 64 * h, vec[h], n[h], gf[h]);
+    load8(p + 64 * h, vec[h], n[h], pf[h]);
+    load8(m + 64 * h, vec[h], n[h], mf[h]);
+    load8(v + 64 * h, vec[h], n[h], rf[h]);
   }
   const float2 ms2 = both(__fmul_rn(ms, a.b1)), rs2 = both(__fmul_rn(rs, a.root_b2));
   float2 m2[2][4], r2[2][4];
@@ -357,7 +364,7 @@ __device__ __forceinline__ void step_codes(const Table<N>& t, const Chunk& k, co
       const float2 q = __ffma2_rn(u, rate, __fmul2_rn(pair_of(pf[h], i), keep));
       out[2 * i] = q.x, out[2 * i + 1] = q.y;
     }
-    store8(p + 64 * h, WHOLE, n[h], out);
+    store8(p + 64 * h, vec[h], n[h], out);
   }
   const float m_scale = group_scale(m2), r_scale = group_scale(r2);
   if ((threadIdx.x & 7) == 0 && n[0] > 0) t.ms[k.i][group] = m_scale, t.vs[k.i][group] = r_scale;
@@ -372,12 +379,10 @@ __device__ __forceinline__ void step_codes(const Table<N>& t, const Chunk& k, co
       mv[i] = code_of<false>(i & 1 ? m2[h][i / 2].y : m2[h][i / 2].x, m_rcp, __byte_perm(bits, 0, 0x4104));
       rv[i] = code_of<true>(i & 1 ? r2[h][i / 2].y : r2[h][i / 2].x, r_rcp, __byte_perm(bits, 0, 0x4324));
     }
-    store8(m + 64 * h, WHOLE, n[h], mv);
-    store8(v + 64 * h, WHOLE, n[h], rv);
+    store8(m + 64 * h, vec[h], n[h], mv);
+    store8(v + 64 * h, vec[h], n[h], rv);
   }
 }
-
-__device__ __forceinline__ bool on8(const void* p) { return (reinterpret_cast<uint64_t>(p) & 7u) == 0; }
 
 template <class P, class G, int N>
 __global__ void __launch_bounds__(kThreads, 4)
@@ -391,11 +396,24 @@ __global__ void __launch_bounds__(kThreads, 4)
   const float c = a.clip != nullptr ? *a.clip : 1.f;
   for (uint32_t chunk = blockIdx.x; chunk < t.first[tensors]; chunk += gridDim.x) {
     const Chunk k = chunk_at(t, tensors, chunk);
-    if (k.count == kChunk && on16(t.g[k.i]) && on16(t.p[k.i]) && on8(t.m[k.i]) && on8(t.v[k.i]))
+    if (k.vec && k.count == kChunk)
       step_codes<P, G, true>(t, k, a, f, c);
     else
       step_codes<P, G, false>(t, k, a, f, c);
   }
+}
+
+// The first element that starts a vector of 8 in each of the arrays (codes: element 0
+// or none, a group of 128 is the tensor's own); -1 where there is none.
+template <class P, class G, bool CODES>
+int head_of(const void* p, const void* g, const void* m, const void* v) {
+  auto bits = [](const void* x) { return reinterpret_cast<uint64_t>(x); };
+  for (int h = 0; h < (CODES ? 1 : kEach); ++h) {
+    const uint64_t wide = (bits(p) + h * sizeof(P)) | (bits(g) + h * sizeof(G)) |
+                          (CODES ? 0 : (bits(m) + h * sizeof(float)) | (bits(v) + h * sizeof(float)));
+    if (wide % 16 == 0 && (!CODES || (bits(m) | bits(v)) % 8 == 0)) return h;
+  }
+  return -1;
 }
 
 template <class P, class G, bool CODES, int N>
@@ -408,13 +426,15 @@ cudaError_t launch_table(const AdamwTensors& l, const AdamwStep& step, cudaStrea
     for (; from < l.count && k < N; ++from) {
       const int64_t n = l.n[from];
       if (n == 0) continue;
-      const uint64_t mine = ((uint64_t)n + kChunk - 1) / kChunk;
+      const int head = head_of<P, G, CODES>(l.p[from], l.g[from], l.m[from], l.v[from]);
+      const uint64_t rest = head > 0 && n > head ? n - head : n, mine = (rest + kChunk - 1) / kChunk;
       if (chunks + mine > INT32_MAX) break;  // checked: one tensor's fit
       t.g[k] = l.g[from], t.p[k] = l.p[from], t.m[k] = l.m[from], t.v[k] = l.v[from];
       t.ms[k] = CODES ? l.ms[from] : nullptr, t.vs[k] = CODES ? l.vs[from] : nullptr;
       t.n[k] = n;
       t.first[k] = (uint32_t)chunks;
       t.ordinal[k] = (uint32_t)from;
+      t.head[k] = (int8_t)head;
       chunks += mine;
       ++k;
     }

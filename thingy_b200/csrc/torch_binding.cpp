@@ -899,7 +899,7 @@ struct Sequence {
 };
 
 const at::Tensor& tensor_of(PyObject* o, const char* name) {
-  if (!THPVariable_Check(o)) bad(std::string(name) + " must hold tensors");
+  if (!THPVariable_CheckExact(o) && !THPVariable_Check(o)) bad(std::string(name) + " must hold tensors");
   return THPVariable_Unpack(o);
 }
 
