@@ -12,9 +12,9 @@
 // itself, codes are 2^-3 apart. A positive r' never becomes zero, so no element
 // is divided by eps alone because its code was lost.
 //
-// CTAs walk chunks of 4096 elements of one tensor, found by a search in the
-// table that is the kernel's argument (no copy to the GPU, nothing to keep for a
-// graph). Bound: memory, each value once, for states in 32 bits, whose kernel
+// A CTA takes a run of neighbouring chunks of 4096 elements of one tensor; the
+// tensor of its first is found by a search in the table that is the kernel's
+// argument (no copy to the GPU, nothing to keep for a graph). Bound: memory, each value once, for states in 32 bits, whose kernel
 // rounds every product and sum by itself. With codes (10 bytes an element of
 // bf16) it is the issue of instructions: so that kernel works on pairs (f32x2),
 // with fused sums, square roots and reciprocals of 2^-23 (the codes are rounded
@@ -30,7 +30,7 @@ namespace cutie {
 namespace {
 
 constexpr int kThreads = 256, kEach = 8, kChunk = 4096, kGroup = 128;
-constexpr int kCtas = 8;  // an SM, at most
+constexpr int kCtas = 5, kCodesCtas = 4;  // an SM at once
 constexpr float kMinState = 0x1p-92f;
 
 // Tensors a launch: its argument is the table, 32 KB at most. Short lists take
@@ -184,16 +184,26 @@ __device__ __forceinline__ float group_scale(const float2 (&x)[2][4]) {
   return amax <= 3.4e38f ? make_scale(amax, false, kMinState) : amax;
 }
 
-// The code of x in the upper byte; rs: the scale's reciprocal, bits: 16 random ones
-// from bit 8 on. They are added below the three bits of mantissa that stay and the
-// rest is cut off. All in integers: 2^-120 brings the least normal code, 2^-6, to
-// fp32's least normal value, so that both have their subnormal codes at the same
-// bits. The largest value is 448 (1 + 2^-23) and cannot carry past its code.
-template <bool POSITIVE>
-__device__ __forceinline__ uint32_t code_of(float x, float rs, uint32_t bits) {
-  const float y = __fmul_rn(__fmul_rn(fabsf(x), rs), 0x1p-120f);
-  const uint32_t v = (min(__float_as_uint(y), 0x07f00000u) << 4) + bits;  // NaN: code 0x7f
-  return POSITIVE ? max(v, x > 0.f ? 0x01000000u : 0u) : v | (__float_as_uint(x) & 0x80000000u);
+// The code of y >= 0 in the upper byte; y: the value over its scale times 2^-120,
+// bits: 16 random ones from bit 8 on. They are added below the three bits of
+// mantissa that stay and the rest is cut off. All in integers: 2^-120 brings the
+// least normal code, 2^-6, to fp32's least normal value, so that both have their
+// subnormal codes at the same bits. The largest value is 448 (1 + 2^-23) and
+// cannot carry past its code.
+__device__ __forceinline__ uint32_t code_of(float y, uint32_t bits) {
+  return (min(__float_as_uint(y), 0x07f00000u) << 4) + bits;  // NaN: code 0x7f
+}
+__device__ __forceinline__ uint32_t signed_code(float x, float rs, uint32_t bits) {
+  const uint32_t v = code_of(__fmul_rn(__fmul_rn(fabsf(x), rs), 0x1p-120f), bits);
+  return v | (__float_as_uint(x) & 0x80000000u);
+}
+// Of a root: two at a time, and never zero for one above zero.
+__device__ __forceinline__ void root_codes(float2 x, float rs, uint32_t bits0, uint32_t bits1, uint32_t& v0,
+                                           uint32_t& v1) {
+  const float2 y = __fmul2_rn(__fmul2_rn(x, make_float2(rs, rs)), make_float2(0x1p-120f, 0x1p-120f));
+  v0 = code_of(y.x, bits0), v1 = code_of(y.y, bits1);
+  if (x.x > 0.f) v0 = max(v0, 0x01000000u);
+  if (x.y > 0.f) v1 = max(v1, 0x01000000u);
 }
 __device__ __forceinline__ uint32_t upper_bytes(const uint32_t (&v)[kEach], int i) {
   return __byte_perm(__byte_perm(v[i], v[i + 1], 0x0073), __byte_perm(v[i + 2], v[i + 3], 0x0073), 0x5410);
@@ -251,13 +261,18 @@ struct Chunk {
   int64_t begin;
 };
 template <int N>
-__device__ __forceinline__ Chunk chunk_at(const Table<N>& t, int tensors, uint32_t chunk) {
+__device__ __forceinline__ Chunk chunk_at(const Table<N>& t, int i, uint32_t chunk) {
   Chunk k;
-  k.i = tensor_at(t, tensors, chunk);
+  k.i = i;
   k.vec = t.head[k.i] >= 0;
   k.begin = (int64_t)(chunk - t.first[k.i]) * kChunk + max((int)t.head[k.i], 0);
   k.count = (int)min((int64_t)kChunk, t.n[k.i] - k.begin);
   return k;
+}
+
+// The first chunk of CTA `cta`.
+__device__ __forceinline__ uint32_t run_begin(uint32_t chunks, uint32_t cta) {
+  return (uint32_t)((uint64_t)chunks * cta / gridDim.x);
 }
 
 template <class P, class G, bool WHOLE, int N>
@@ -291,7 +306,7 @@ __device__ __forceinline__ void step_values(const Table<N>& t, const Chunk& k, c
 }
 
 template <class P, class G, int N>
-__global__ void __launch_bounds__(kThreads, 5)
+__global__ void __launch_bounds__(kThreads, kCtas)
     adamw_kernel(const __grid_constant__ Table<N> t, int tensors, const AdamwStep a) {
   __shared__ Factors shared;
   griddep_wait();
@@ -301,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, 5)
   const Factors f = shared;
   const float c = a.clip != nullptr ? *a.clip : 1.f;
   for (uint32_t chunk = blockIdx.x; chunk < t.first[tensors]; chunk += gridDim.x) {
-    Chunk k = chunk_at(t, tensors, chunk);
+    Chunk k = chunk_at(t, tensor_at(t, tensors, chunk), chunk);
     if (k.vec && k.count == kChunk) step_values<P, G, true>(t, k, a, f, c);
     else step_values<P, G, false>(t, k, a, f, c);
     if (t.head[k.i] > 0 && chunk == t.first[k.i]) {
@@ -374,18 +389,34 @@ __device__ __forceinline__ void step_codes(const Table<N>& t, const Chunk& k, co
   for (int h = 0; h < 2; ++h) {
     uint32_t mv[kEach], rv[kEach];
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const uint32_t bits = mix((uint32_t)(from + 64 * h + i) * 0x9E3779B9u + key);
-      mv[i] = code_of<false>(i & 1 ? m2[h][i / 2].y : m2[h][i / 2].x, m_rcp, __byte_perm(bits, 0, 0x4104));
-      rv[i] = code_of<true>(i & 1 ? r2[h][i / 2].y : r2[h][i / 2].x, r_rcp, __byte_perm(bits, 0, 0x4324));
+    for (int i = 0; i < kEach; i += 2) {
+      const uint32_t b0 = mix((uint32_t)(from + 64 * h + i) * 0x9E3779B9u + key);
+      const uint32_t b1 = mix((uint32_t)(from + 64 * h + i + 1) * 0x9E3779B9u + key);
+      mv[i] = signed_code(m2[h][i / 2].x, m_rcp, __byte_perm(b0, 0, 0x4104));
+      mv[i + 1] = signed_code(m2[h][i / 2].y, m_rcp, __byte_perm(b1, 0, 0x4104));
+      root_codes(r2[h][i / 2], r_rcp, __byte_perm(b0, 0, 0x4324), __byte_perm(b1, 0, 0x4324), rv[i], rv[i + 1]);
     }
     store8(m + 64 * h, vec[h], n[h], mv);
     store8(v + 64 * h, vec[h], n[h], rv);
   }
 }
 
+// The chunk from element `at` on into the L2, while the one before it is computed.
 template <class P, class G, int N>
-__global__ void __launch_bounds__(kThreads, 4)
+__device__ __forceinline__ void fetch_next(const Table<N>& t, int i, int64_t at) {
+  const uint32_t n = (uint32_t)min((int64_t)kChunk, t.n[i] - at) & ~15u;
+  auto fetch = [](const void* p, uint32_t bytes) {
+    if (bytes > 0 && reinterpret_cast<uint64_t>(p) % 16 == 0)
+      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
+  };
+  fetch(static_cast<const P*>(t.p[i]) + at, n * (uint32_t)sizeof(P));
+  fetch(static_cast<const G*>(t.g[i]) + at, n * (uint32_t)sizeof(G));
+  fetch(static_cast<const E4m3*>(t.m[i]) + at, n);
+  fetch(static_cast<const E4m3*>(t.v[i]) + at, n);
+}
+
+template <class P, class G, int N>
+__global__ void __launch_bounds__(kThreads, kCodesCtas)
     adamw_codes_kernel(const __grid_constant__ Table<N> t, int tensors, const AdamwStep a) {
   __shared__ Factors shared;
   griddep_wait();
@@ -394,8 +425,13 @@ __global__ void __launch_bounds__(kThreads, 4)
   __syncthreads();
   const Factors f = shared;
   const float c = a.clip != nullptr ? *a.clip : 1.f;
-  for (uint32_t chunk = blockIdx.x; chunk < t.first[tensors]; chunk += gridDim.x) {
-    const Chunk k = chunk_at(t, tensors, chunk);
+  const uint32_t end = run_begin(t.first[tensors], blockIdx.x + 1);
+  uint32_t chunk = run_begin(t.first[tensors], blockIdx.x);
+  for (int i = tensor_at(t, tensors, chunk); chunk < end; ++chunk) {
+    while (t.first[i + 1] <= chunk) ++i;
+    const Chunk k = chunk_at(t, i, chunk);
+    if (threadIdx.x == 0 && chunk + 1 < end && chunk + 1 < t.first[i + 1] && k.vec)
+      fetch_next<P, G>(t, i, k.begin + kChunk);
     if (k.vec && k.count == kChunk)
       step_codes<P, G, true>(t, k, a, f, c);
     else
@@ -440,7 +476,7 @@ cudaError_t launch_table(const AdamwTensors& l, const AdamwStep& step, cudaStrea
     }
     if (k == 0) continue;
     t.first[k] = (uint32_t)chunks;
-    const uint64_t most = (uint64_t)kCtas * device_sm_count();
+    const uint64_t most = (uint64_t)(CODES ? 4 * kCodesCtas : 2 * kCtas) * device_sm_count();
     const unsigned grid = (unsigned)(chunks < most ? chunks : most);
     auto kernel = CODES ? adamw_codes_kernel<P, G, N> : adamw_kernel<P, G, N>;
     const cudaError_t e = launch_pdl(kernel, grid, kThreads, 0, stream, t, k, step);
