@@ -19,8 +19,9 @@
 // bf16) it is the issue of instructions: so that kernel works on pairs (f32x2),
 // with fused sums, square roots and reciprocals of 2^-23 (the codes are rounded
 // by 2^-4), 16 elements a thread, so that a group's maxima and scales are shared
-// by 8 lanes: 89 thread instructions an element and 412 us for 134M in the form
-// that the other kernel has.
+// by 8 lanes: 51 thread instructions an element instead of 89 in the other kernel's
+// form, 278 us instead of 412 for 134M elements, 75% of the copy bandwidth. (Copies
+// through shared memory a chunk ahead: 9% more instructions, no gain.)
 #include <cuda_fp16.h>
 
 #include "cutie.h"
