@@ -301,6 +301,7 @@ CUTIE_API int cutie_rms_norm_mxfp8_gemm(const void* x, int64_t ldx, const void* 
 enum {
   CUTIE_TILE_BLOCK = 0,
   CUTIE_TILE_TWO_WAY = 1,
+  CUTIE_TILE_BLOCK_F32 = 8, /* CUTIE_TILE_BLOCK of an fp32 x, rounded to bf16 first */
 };
 enum {
   CUTIE_SCALE_GRADIENT = 16, /* added to scale_fmt, CUTIE_TILE_TWO_WAY only  */

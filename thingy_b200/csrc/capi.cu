@@ -807,6 +807,8 @@ static int cast_tiles(const void* x, int64_t ldx, int64_t M, int64_t H, const in
                 (long long)H);
   if (H > INT32_MAX - 128)
     return fail(CUTIE_ERR_UNSUPPORTED, "H must be below 2^31 - 128");
+  const bool f32 = tile_kind == CUTIE_TILE_BLOCK_F32;
+  if (f32) tile_kind = CUTIE_TILE_BLOCK;
   if (tile_kind != CUTIE_TILE_BLOCK && tile_kind != CUTIE_TILE_TWO_WAY)
     return fail(CUTIE_ERR_INVALID_ARGUMENT, "unknown tile_kind %d", tile_kind);
   const bool gradient = (scale_fmt & CUTIE_SCALE_GRADIENT) != 0;
@@ -826,7 +828,7 @@ static int cast_tiles(const void* x, int64_t ldx, int64_t M, int64_t H, const in
   if (GM > INT32_MAX / GH)
     return fail(CUTIE_ERR_UNSUPPORTED, "M x H has more than 2^31 tiles");
   int rc;
-  if ((rc = check_matrix("x", x, ldx, H, 16, 8)) != CUTIE_OK) return rc;
+  if ((rc = check_matrix("x", x, ldx, H, 16, f32 ? 4 : 8)) != CUTIE_OK) return rc;
   if ((rc = check_matrix("q", q, ldq, H, 8, 8)) != CUTIE_OK) return rc;
   if ((rc = check_matrix("s", s, lds, block ? GH : M, 4, 1)) != CUTIE_OK) return rc;
   if (qt != nullptr) {
@@ -834,7 +836,7 @@ static int cast_tiles(const void* x, int64_t ldx, int64_t M, int64_t H, const in
     if ((rc = check_matrix("st", st, ldst, block ? GM : H, 4, 1)) != CUTIE_OK) return rc;
   }
   CastArgs a{};
-  a.x = static_cast<const uint16_t*>(x), a.ldx = ldx;
+  a.x = x, a.x_f32 = f32, a.ldx = ldx;
   a.M = M, a.H = (int)H;
   a.pow2 = fmt == CUTIE_SCALE_FP32_POW2;
   a.gradient = gradient;

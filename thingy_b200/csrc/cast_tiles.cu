@@ -64,10 +64,14 @@ __device__ __forceinline__ void transpose4(uint32_t a, uint32_t b, uint32_t c, u
   t[2] = __byte_perm(ab1, cd1, 0x5410), t[3] = __byte_perm(ab1, cd1, 0x7632);
 }
 
+__device__ __forceinline__ uint32_t pair_to_bf2(uint32_t a, uint32_t b) {
+  return f2_to_bf2(make_float2(__uint_as_float(a), __uint_as_float(b)));
+}
+
 // SORTED: rows sorted by expert (two-way kind). Padding rows are zeros whatever
 // x holds there, so that they change no column group; a tile that begins with
 // padding is behind the last expert's rows: nothing reads its codes.
-template <bool BLOCK, bool TRANSPOSED, bool SORTED = false>
+template <bool BLOCK, bool TRANSPOSED, bool SORTED = false, bool F32 = false>
 __global__ void __launch_bounds__(kThreads, 4)
     cast_tiles_kernel(CastArgs a) {
   __shared__ __align__(16) uint8_t t_codes[TRANSPOSED ? kTile * kTile : 16];
@@ -91,7 +95,16 @@ __global__ void __launch_bounds__(kThreads, 4)
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     uint4 w = make_uint4(0, 0, 0, 0);
-    if (col_ok && r0 + i < a.M) w = ld_stream(a.x + (r0 + i) * a.ldx + c0);
+    if (col_ok && r0 + i < a.M) {
+      if (F32) {
+        const float* f = static_cast<const float*>(a.x) + (r0 + i) * a.ldx + c0;
+        const uint4 lo = ld_stream(f), hi = ld_stream(f + 4);
+        w = make_uint4(pair_to_bf2(lo.x, lo.y), pair_to_bf2(lo.z, lo.w), pair_to_bf2(hi.x, hi.y),
+                       pair_to_bf2(hi.z, hi.w));
+      } else {
+        w = ld_stream(static_cast<const uint16_t*>(a.x) + (r0 + i) * a.ldx + c0);
+      }
+    }
     x[i][0] = w.x, x[i][1] = w.y, x[i][2] = w.z, x[i][3] = w.w;
   }
   if (SORTED) {
@@ -238,7 +251,9 @@ __global__ void __launch_bounds__(kThreads, 4)
 
 cudaError_t launch_cast_tiles(const CastArgs& a, bool block, cudaStream_t stream) {
   const int64_t tiles = ((a.M + kTile - 1) / kTile) * ((a.H + kTile - 1) / kTile);
-  auto kernel = block ? (a.qt != nullptr ? cast_tiles_kernel<true, true> : cast_tiles_kernel<true, false>)
+  auto kernel = block && a.x_f32 ? (a.qt != nullptr ? cast_tiles_kernel<true, true, false, true>
+                                                    : cast_tiles_kernel<true, false, false, true>)
+                : block ? (a.qt != nullptr ? cast_tiles_kernel<true, true> : cast_tiles_kernel<true, false>)
                       : a.sources != nullptr ? cast_tiles_kernel<false, true, true>
                                              : cast_tiles_kernel<false, true>;
   return launch_pdl(kernel, (unsigned)tiles, kThreads, 0, stream, a);

@@ -313,7 +313,8 @@ cudaError_t launch_backward(const BwdArgs& a, float eps, bool dw_wanted, uint16_
 
 // Casts to e4m3 in both orientations (cast_tiles.cu).
 struct CastArgs {
-  const uint16_t* x;  // bf16 [M, H]
+  const void* x;  // bf16 [M, H]; block kind: or fp32, rounded to bf16 first
+  bool x_f32;
   int64_t ldx;
   int64_t M;
   int H;

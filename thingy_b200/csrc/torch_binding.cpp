@@ -316,8 +316,9 @@ struct CastPlace {
   // elements. With `sources` the rows are sorted by expert.
   void cast(const at::Tensor& any, void* stream, const void* sources = nullptr) const {
     if (R == 0 || C == 0) return;  // no codes
+    const bool f32 = any.scalar_type() == at::kFloat;  // weights: rounded to bf16 on the way
     const bool dense = (C <= 1 || any.stride(1) == 1) &&
-                       (R <= 1 || (any.stride(0) >= C && any.stride(0) % 8 == 0)) &&
+                       (R <= 1 || (any.stride(0) >= C && any.stride(0) % (f32 ? 4 : 8) == 0)) &&
                        reinterpret_cast<uintptr_t>(any.data_ptr()) % 16 == 0;
     const at::Tensor x = dense ? any : any.clone(at::MemoryFormat::Contiguous);
     const Operand q = rows(), qt = column_base != nullptr ? columns() : Operand();
@@ -329,7 +330,7 @@ struct CastPlace {
     }
     check_status(cutie_cast_fp8_tiles(
         x.data_ptr(), R <= 1 ? ceil_to(C, 8) : x.stride(0), R, C,
-        block ? CUTIE_TILE_BLOCK : CUTIE_TILE_TWO_WAY,
+        f32 ? CUTIE_TILE_BLOCK_F32 : block ? CUTIE_TILE_BLOCK : CUTIE_TILE_TWO_WAY,
         CUTIE_SCALE_FP32 + (gradient ? CUTIE_SCALE_GRADIENT : 0), row_base, q.ld, row_base + off_s,
         block ? q.s_row : q.s_kb, column_base, qt.ld,
         column_base != nullptr ? column_base + off_st : nullptr, block ? qt.s_row : qt.s_kb, stream));
@@ -383,7 +384,7 @@ struct FP8Linear : public torch::autograd::Function<FP8Linear> {
     if (own) {
       w.row_base = xs.row_base + xs.row_bytes;
       if (held_w > 0) w.column_base = address(held);
-      w.cast(weight.scalar_type() == at::kBFloat16 ? weight : weight.to(at::kBFloat16), stream);
+      w.cast(weight, stream);
     }
     // the two-way cast always writes both
     if (held_x > 0) xs.column_base = address(held) + held_w;
@@ -559,8 +560,7 @@ struct FP8GroupedLinear : public torch::autograd::Function<FP8GroupedLinear> {
     if (own) {
       w.row_base = xs.row_base + xs.row_bytes;
       if (held_w > 0) w.column_base = address(held);
-      const at::Tensor flat = weight.reshape({E * N, K});
-      w.cast(flat.scalar_type() == at::kBFloat16 ? flat : flat.to(at::kBFloat16), stream);
+      w.cast(weight.reshape({E * N, K}), stream);
     }
     xs.column_base = held_x > 0 ? address(held) + held_w : xs.row_base + xs.row_bytes + (own ? w.row_bytes : 0);
     xs.cast(x, stream, sources.data_ptr());
