@@ -478,8 +478,8 @@ CUTIE_API int cutie_moe_combine_backward(const void* d_out, int64_t ldd, const v
 
 /*
  * One step of AdamW over `count` tensors in as few launches as their table
- * needs (480 tensors each). For every element, in fp32 (with 32-bit states every
- * operation is rounded by itself, with codes to a few 2^-24):
+ * needs (480 tensors each). For every element, in fp32, rounded operation by
+ * operation (with codes only the states are, the update to a few 2^-24):
  *   g' = g grad_scale;  m' = b1 m + (1 - b1) g';  v' = b2 v + (1 - b2) (g' g')
  *   p' = p (1 - lr decay) - (lr / (1 - b1^step)) (m' / (sqrt(v') / sqrt(1 - b2^step) + eps))
  * params, grads, exp_avg, exp_avg_sq: host arrays of device pointers to sizes[i]

@@ -2,6 +2,7 @@
 
 import ctypes
 
+import numpy as np
 import pytest
 import torch
 
@@ -63,3 +64,24 @@ def test_hash_bits_are_even():
             # the two halves of a hash, and neighbours', are not alike: a mean product of n uniform pairs
             for a, b in (pair, (pair[0][1:], pair[0][:-1])):
                 assert abs(float((a * b).mean())) <= 6 / 12 / n**0.5
+
+
+def test_square_root_iteration_is_correctly_rounded():
+    """Markstein's iteration as the kernel makes it, from every start within two ulps, for every mantissa of two
+    binades (a power of four changes exponents alone). Products of fp32 values are exact in 64 bits, and so are the
+    residuals; the last sum is rounded by its exact correction in ulps."""
+    f32, f64 = np.float32, np.float64
+    for base in (0x3F800000, 0x40000000):
+        for at in range(0, 1 << 23, 1 << 21):
+            a = np.arange(base + at, base + at + (1 << 21), dtype=np.uint32).view(f32).astype(f64)
+            s = np.sqrt(a)  # 53 bits: a root is never so near to the middle of two fp32 values
+            want = s.astype(f32)
+            for k in (-2, -1, 0, 1, 2):
+                y = ((1.0 / s).astype(f32).view(np.int32) + np.int32(k)).view(f32).astype(f64)
+                g, h = (a * y).astype(f32).astype(f64), 0.5 * y
+                r = (0.5 - g * h).astype(f32).astype(f64)
+                g1, h1 = (g + g * r).astype(f32), (h + h * r).astype(f32).astype(f64)
+                d = (a - g1.astype(f64) ** 2).astype(f32).astype(f64)
+                ulp = np.spacing(g1).astype(f64)
+                got = (g1.astype(f64) + np.rint(d * h1 / ulp) * ulp).astype(f32)
+                assert np.array_equal(got, want)

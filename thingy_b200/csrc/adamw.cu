@@ -14,14 +14,17 @@
 //
 // A CTA takes a run of neighbouring chunks of 4096 elements of one tensor; the
 // tensor of its first is found by a search in the table that is the kernel's
-// argument (no copy to the GPU, nothing to keep for a graph). Bound: memory, each value once, for states in 32 bits, whose kernel
-// rounds every product and sum by itself. With codes (10 bytes an element of
-// bf16) it is the issue of instructions: so that kernel works on pairs (f32x2),
-// with fused sums, square roots and reciprocals of 2^-23 (the codes are rounded
-// by 2^-4), 16 elements a thread, so that a group's maxima and scales are shared
-// by 8 lanes: 51 thread instructions an element instead of 89 in the other kernel's
-// form, 278 us instead of 412 for 134M elements, 75% of the copy bandwidth. (Copies
-// through shared memory a chunk ahead: 9% more instructions, no gain.)
+// argument (no copy to the GPU, nothing to keep for a graph). Bound: memory, each
+// value once, for states in 32 bits, whose kernel rounds every product and sum by
+// itself. With codes (10 bytes an element of bf16) it is the issue of
+// instructions: so that kernel multiplies in pairs (f32x2) and takes 16 elements a
+// thread, whose group shares its maxima and scales over 8 lanes. What becomes codes
+// has the same bits as in the other kernel (one code more or less would move the
+// scale of its group in the next step); the update has a fused sum and an
+// approximate reciprocal (2^-23). 134M elements in 316 us, 66% of the copy
+// bandwidth, 64 thread instructions an element, against 412 and 89 in the other
+// kernel's form. Tried: copies through shared memory a chunk ahead (9% more
+// instructions, no gain), approximate roots and fused sums for the codes too (278).
 #include <cuda_fp16.h>
 
 #include "cutie.h"
@@ -328,11 +331,6 @@ __global__ void __launch_bounds__(kThreads, kCtas)
 }
 
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
-__device__ __forceinline__ float fast_root(float x) {
-  float r;
-  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
 // Of zero or of at least 2^-75 (the root of fp32's least value) as it is used here.
 __device__ __forceinline__ float fast_reciprocal(float x) {
   float r;
@@ -340,11 +338,35 @@ __device__ __forceinline__ float fast_reciprocal(float x) {
   return r;
 }
 
+// RN(sqrt(a)) of zeros and of 2^-96 to 2^96 in pairs, by Markstein's iteration (P.
+// Markstein, IBM J. Res. Dev. 34(1), 1990): from y = 1 / sqrt(a) within two ulps,
+// g = a y and h = y / 2, r = 1/2 - g h, g1 = g + g r, h1 = h + h r, and g1 + (a - g1^2) h1
+// is correctly rounded: tests/test_adamw_capi.py goes through every mantissa and
+// start. Half the instructions of the general root. (Signs as they save negations.)
+__device__ __forceinline__ float2 exact_roots(float2 a) {
+  float2 y;
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y.x) : "f"(a.x));
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y.y) : "f"(a.y));
+  y = make_float2(fminf(y.x, 0x1p60f), fminf(y.y, 0x1p60f));  // of a zero: g = 0, and the rest of the steps too
+  const float2 g = __fmul2_rn(a, y), nh = __fmul2_rn(y, both(-0.5f)), r = __ffma2_rn(g, nh, both(0.5f));
+  const float2 g1 = __ffma2_rn(g, r, g), nh1 = __ffma2_rn(nh, r, nh);
+  return __ffma2_rn(__ffma2_rn(g1, g1, __fmul2_rn(a, both(-1.f))), nh1, g1);
+}
+// Whether all of 8 values are zero or in that range.
+__device__ __forceinline__ bool plain_range(const float2 (&a)[4]) {
+  uint32_t lo = 0xffffffffu, hi = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t x = __float_as_uint(a[i].x), y = __float_as_uint(a[i].y);
+    lo = min(lo, min(x - 1u, y - 1u)), hi = max(hi, max(x, y));
+  }
+  return lo >= 0x0f800000u - 1u && hi <= 0x6f800000u;
+}
+
 template <class P, class G, bool WHOLE, int N>
 __device__ __forceinline__ void step_codes(const Table<N>& t, const Chunk& k, const AdamwStep& a, const Factors& f,
                                            float c) {
-  // m' = b1 m + g (c1 c);  v' = (r sqrt(b2))^2 + (g (c sqrt(c2)))^2
-  const float2 g_m = both(__fmul_rn(a.c1, c)), g_r = both(__fmul_rn(a.root_c2, c));
+  const float2 c2 = both(c), b1 = both(a.b1), b2 = both(a.b2), g_m = both(a.c1), g_v = both(a.c2);
   const float2 keep = both(f.keep), root = both(f.root), rate = both(-f.rate), eps = both(a.eps);
   const int at = ((int)threadIdx.x >> 3) * kGroup + ((int)threadIdx.x & 7) * kEach;
   const int64_t from = k.begin + at, group = k.begin / kGroup + ((int)threadIdx.x >> 3);
@@ -364,17 +386,30 @@ __device__ __forceinline__ void step_codes(const Table<N>& t, const Chunk& k, co
     load8(m + 64 * h, vec[h], n[h], mf[h]);
     load8(v + 64 * h, vec[h], n[h], rf[h]);
   }
-  const float2 ms2 = both(__fmul_rn(ms, a.b1)), rs2 = both(__fmul_rn(rs, a.root_b2));
   float2 m2[2][4], r2[2][4];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     float out[kEach];
+    float2 v2[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float2 gi = pair_of(gf[h], i), b = __fmul2_rn(pair_of(rf[h], i), rs2), e = __fmul2_rn(gi, g_r);
-      m2[h][i] = __ffma2_rn(pair_of(mf[h], i), ms2, __fmul2_rn(gi, g_m));
-      const float2 v2 = __ffma2_rn(b, b, __fmul2_rn(e, e));
-      r2[h][i] = make_float2(fast_root(v2.x), fast_root(v2.y));
+      // what becomes codes is rounded as written: products in pairs, sums one by one
+      // (a sum in pairs would be fused with the product before it)
+      const float2 gi = __fmul2_rn(pair_of(gf[h], i), c2), r = __fmul2_rn(pair_of(rf[h], i), both(rs));
+      const float2 m = __fmul2_rn(b1, __fmul2_rn(pair_of(mf[h], i), both(ms))), mg = __fmul2_rn(g_m, gi);
+      const float2 v = __fmul2_rn(b2, __fmul2_rn(r, r)), vg = __fmul2_rn(g_v, __fmul2_rn(gi, gi));
+      m2[h][i] = make_float2(__fadd_rn(m.x, mg.x), __fadd_rn(m.y, mg.y));
+      v2[i] = make_float2(__fadd_rn(v.x, vg.x), __fadd_rn(v.y, vg.y));
+    }
+    if (plain_range(v2)) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r2[h][i] = exact_roots(v2[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r2[h][i] = make_float2(__fsqrt_rn(v2[i].x), __fsqrt_rn(v2[i].y));
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
       const float2 d = __ffma2_rn(r2[h][i], root, eps);
       const float2 u = __fmul2_rn(m2[h][i], make_float2(fast_reciprocal(d.x), fast_reciprocal(d.y)));
       const float2 q = __ffma2_rn(u, rate, __fmul2_rn(pair_of(pf[h], i), keep));

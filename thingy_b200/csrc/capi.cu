@@ -1324,7 +1324,6 @@ extern "C" int cutie_adamw(int64_t count, void* const* params, int param_dtype, 
   a.root = (float)(1.0 / std::sqrt(1.0 - std::pow(beta2, (double)step)));
   a.eps = (float)eps, a.b1 = (float)beta1, a.b2 = (float)beta2;
   a.c1 = (float)(1.0 - beta1), a.c2 = (float)(1.0 - beta2);
-  a.root_b2 = (float)std::sqrt(beta2), a.root_c2 = (float)std::sqrt(1.0 - beta2);
   a.step = step;
   a.step_ptr = static_cast<const int64_t*>(step_ptr);
   a.lr_ptr = static_cast<const float*>(lr_ptr);

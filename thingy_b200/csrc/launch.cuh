@@ -454,7 +454,6 @@ struct AdamwTensors {
 struct AdamwStep {
   double lr, decay, beta1, beta2, bias1;  // bias1 = 1 - beta1^step
   float root, eps, b1, b2, c1, c2;        // root = 1 / sqrt(1 - beta2^step), c = 1 - b
-  float root_b2, root_c2;                 // square roots
   int64_t step;
   const int64_t* step_ptr;  // on the GPU, in the place of the host's value; or null
   const float* lr_ptr;
