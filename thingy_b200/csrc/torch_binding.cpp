@@ -1007,7 +1007,10 @@ void adamw_step(const py::object& params, const py::object& grads, const py::obj
       lt != nullptr ? lt->data_ptr() : nullptr, beta1, beta2, eps, weight_decay, ptr_or_null(grad_scale),
       (uint64_t)seed, at::cuda::getCurrentCUDAStream(dev.index()).stream()));
   // what autograd saved of the parameters is out of date
-  for (int64_t i = 0; i < count; ++i) THPVariable_Unpack(P[i]).unsafeGetTensorImpl()->bump_version();
+  for (int64_t i = 0; i < count; ++i) {
+    const at::Tensor& t = THPVariable_Unpack(P[i]);
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  }
 }
 
 }  // namespace

@@ -8,7 +8,9 @@ whole fused contract (bench.py:10-11): (q, scale, residual_out, normalized).
 
 What follows the quantizer has ops too: ``thingy_b200::per_block_cast_to_fp8``,
 ``thingy_b200::two_way_cast_to_fp8``, ``thingy_b200::fp8_block_gemm`` and
-``thingy_b200::moe_fp8``.
+``thingy_b200::moe_fp8``; for many tokens ``thingy_b200::moe_sort``,
+``thingy_b200::moe_permute``, ``thingy_b200::fp8_grouped_gemm`` (a plan with align 128)
+and ``thingy_b200::moe_combine``. They are forward only.
 
 Importing this module also registers ``cutie::per_token_fp8_quant`` itself,
 the name the reference's callers use (``torch.ops.cutie.per_token_fp8_quant``),
@@ -23,10 +25,11 @@ from __future__ import annotations
 
 import torch
 
+from .dispatch import MoePlan, moe_combine, moe_permute, moe_sort
 from .fp8_utils import per_token_cast_to_fp8
 from .fp8_utils import per_block_cast_to_fp8, two_way_cast_to_fp8
 from .fused import residual_rms_norm_fp8
-from .gemm import fp8_block_gemm
+from .gemm import fp8_block_gemm, fp8_grouped_gemm
 from .moe import moe_fp8
 
 GROUP_SIZE = 128
@@ -117,6 +120,51 @@ def moe_fp8_op(x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor, router: to
 def _moe_fp8_fake(x, q, scale, router, w13, w13_scale, w2, w2_scale, top_k, scoring, renormalize,
                   routed_scale, bias):
     return torch.empty_like(x, memory_format=torch.contiguous_format)
+
+
+@torch.library.custom_op("thingy_b200::moe_sort", mutates_args=())
+def moe_sort_op(topk_ids: torch.Tensor, num_experts: int, align: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    return moe_sort(topk_ids, num_experts, align=align)[:4]
+
+
+@moe_sort_op.register_fake
+def _moe_sort_fake(topk_ids, num_experts, align):
+    T, k = topk_ids.shape
+    rows = (T * k + min(num_experts, T * k) * (align - 1)) // align * align
+    return (topk_ids.new_empty((rows,), dtype=torch.int32), topk_ids.new_empty((T, k), dtype=torch.int32),
+            topk_ids.new_empty((num_experts + 1,), dtype=torch.int32), topk_ids.new_empty((num_experts,), dtype=torch.int32))
+
+
+@torch.library.custom_op("thingy_b200::moe_permute", mutates_args=())
+def moe_permute_op(x: torch.Tensor, sources: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
+    return moe_permute(x, MoePlan(sources, positions, None, None, 1))
+
+
+@moe_permute_op.register_fake
+def _moe_permute_fake(x, sources, positions):
+    return x.new_empty((sources.shape[0], x.shape[1]))
+
+
+@torch.library.custom_op("thingy_b200::moe_combine", mutates_args=())
+def moe_combine_op(rows: torch.Tensor, weights: torch.Tensor, sources: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
+    return moe_combine(rows, weights, MoePlan(sources, positions, None, None, 1))
+
+
+@moe_combine_op.register_fake
+def _moe_combine_fake(rows, weights, sources, positions):
+    return rows.new_empty((positions.shape[0], rows.shape[1]))
+
+
+@torch.library.custom_op("thingy_b200::fp8_grouped_gemm", mutates_args=())
+def fp8_grouped_gemm_op(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor,
+                        offsets: torch.Tensor, counts: torch.Tensor, fp32_out: bool) -> torch.Tensor:
+    return fp8_grouped_gemm(a, a_scale, b, b_scale, MoePlan(None, None, offsets, counts, 128),
+                            out_dtype=torch.float32 if fp32_out else torch.bfloat16)
+
+
+@fp8_grouped_gemm_op.register_fake
+def _fp8_grouped_gemm_fake(a, a_scale, b, b_scale, offsets, counts, fp32_out):
+    return a.new_empty((a.shape[0], b.shape[1]), dtype=torch.float32 if fp32_out else torch.bfloat16)
 
 
 def _reference_op_defined() -> bool:
