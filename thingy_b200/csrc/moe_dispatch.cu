@@ -27,6 +27,7 @@ namespace {
 // above, a first launch counts each chunk and in the second every CTA adds up
 // the chunks before its own. Latency bounds both: the ids and the plan are a few
 // MB at most.
+constexpr size_t kSortStatic = (4 * kMoeMaxExperts + 32) * sizeof(int);  // shared memory of its own, at most
 constexpr int kSortThreads = 1024, kSortOne = 4096, kSortChunk = 2048, kSortMaxChunks = 512;
 
 struct SortArgs {
@@ -441,9 +442,11 @@ cudaError_t moe_sort(const void* ids, bool wide, int n, int E, int align, int* s
     a.chunk_counts = nullptr;
   }
   const size_t smem = (size_t)(kSortThreads / 32) * (E + 1) * sizeof(int);
-  const cudaError_t e = cudaFuncSetAttribute(sort_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             (kSortThreads / 32) * (kMoeMaxExperts + 1) * (int)sizeof(int));
-  if (e != cudaSuccess) return e;
+  if (smem + kSortStatic > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(sort_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               (kSortThreads / 32) * (kMoeMaxExperts + 1) * (int)sizeof(int));
+    if (e != cudaSuccess) return e;
+  }
   return launch_pdl(sort_place_kernel, grid, kSortThreads, smem, stream, a);
 }
 

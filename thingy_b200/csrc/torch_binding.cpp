@@ -761,9 +761,14 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> moe_sort(const at::Te
   const at::Device dev = any.device();
   const c10::cuda::CUDAGuard guard(dev);
   const at::Tensor ids = any.contiguous();
+  // one allocation: four of them are half of a small sort's time on the host
+  const at::AutoDispatchBelowADInplaceOrView below;
   const auto opt = at::TensorOptions().device(dev).dtype(at::kInt);
-  at::Tensor sources = at::empty({R}, opt), positions = at::empty({T, k}, opt);
-  at::Tensor offsets = at::empty({E + 1}, opt), counts = at::empty({E}, opt);
+  const int64_t at_positions = ceil_to(R, 64), at_offsets = at_positions + ceil_to(T * k, 64);
+  const int64_t at_counts = at_offsets + ceil_to(E + 1, 64);
+  const at::Tensor buffer = at::empty({at_counts + E}, opt);
+  at::Tensor sources = buffer.as_strided({R}, {1}, 0), positions = buffer.as_strided({T, k}, {k, 1}, at_positions);
+  at::Tensor offsets = buffer.as_strided({E + 1}, {1}, at_offsets), counts = buffer.as_strided({E}, {1}, at_counts);
   const size_t bytes = cutie_moe_sort_workspace(T, k, E);
   const at::Tensor workspace = bytes > 0 ? at::empty({(int64_t)bytes}, opt.dtype(at::kByte)) : at::Tensor();
   check_status(cutie_moe_sort(ids.data_ptr(), ids.scalar_type() == at::kLong ? 1 : 0, T, k, E, align,
