@@ -754,21 +754,24 @@ int64_t moe_plan_rows(int64_t T, int64_t k, int64_t E, int64_t align) {
 }
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> moe_sort(const at::Tensor& any, int64_t E,
-                                                                    int64_t align) {
+                                                                    int64_t align, bool apart) {
   if (any.dim() != 2 || !any.is_cuda()) bad("topk_ids must be a 2-D CUDA tensor (this library has no CPU path)");
   if (any.scalar_type() != at::kInt && any.scalar_type() != at::kLong) bad("topk_ids must be int32 or int64");
   const int64_t T = any.size(0), k = any.size(1), R = moe_plan_rows(T, k, E, align);
   const at::Device dev = any.device();
   const c10::cuda::CUDAGuard guard(dev);
   const at::Tensor ids = any.contiguous();
-  // one allocation: four of them are half of a small sort's time on the host
+  // one allocation, unless the results have to be apart (torch.library's): four are
+  // half of a small sort's time on the host
   const at::AutoDispatchBelowADInplaceOrView below;
   const auto opt = at::TensorOptions().device(dev).dtype(at::kInt);
   const int64_t at_positions = ceil_to(R, 64), at_offsets = at_positions + ceil_to(T * k, 64);
   const int64_t at_counts = at_offsets + ceil_to(E + 1, 64);
-  const at::Tensor buffer = at::empty({at_counts + E}, opt);
-  at::Tensor sources = buffer.as_strided({R}, {1}, 0), positions = buffer.as_strided({T, k}, {k, 1}, at_positions);
-  at::Tensor offsets = buffer.as_strided({E + 1}, {1}, at_offsets), counts = buffer.as_strided({E}, {1}, at_counts);
+  const at::Tensor buffer = apart ? at::Tensor() : at::empty({at_counts + E}, opt);
+  at::Tensor sources = apart ? at::empty({R}, opt) : buffer.as_strided({R}, {1}, 0);
+  at::Tensor positions = apart ? at::empty({T, k}, opt) : buffer.as_strided({T, k}, {k, 1}, at_positions);
+  at::Tensor offsets = apart ? at::empty({E + 1}, opt) : buffer.as_strided({E + 1}, {1}, at_offsets);
+  at::Tensor counts = apart ? at::empty({E}, opt) : buffer.as_strided({E}, {1}, at_counts);
   const size_t bytes = cutie_moe_sort_workspace(T, k, E);
   const at::Tensor workspace = bytes > 0 ? at::empty({(int64_t)bytes}, opt.dtype(at::kByte)) : at::Tensor();
   check_status(cutie_moe_sort(ids.data_ptr(), ids.scalar_type() == at::kLong ? 1 : 0, T, k, E, align,
@@ -1045,7 +1048,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("fp8_grouped_linear", &fp8_grouped_linear, py::arg("x"), py::arg("weight"), py::arg("sources"),
         py::arg("offsets"), py::arg("counts"), py::arg("align"), py::arg("wq"), py::arg("ws"), py::arg("wqt"), py::arg("wst"));
   m.def("moe_plan_rows", &moe_plan_rows, py::arg("T"), py::arg("k"), py::arg("E"), py::arg("align"));
-  m.def("moe_sort", &moe_sort, py::arg("ids"), py::arg("E"), py::arg("align"));
+  m.def("moe_sort", &moe_sort, py::arg("ids"), py::arg("E"), py::arg("align"), py::arg("apart"));
   m.def("moe_permute", &moe_permute, py::arg("x"), py::arg("sources"), py::arg("positions"));
   m.def("moe_combine", &moe_combine, py::arg("rows"), py::arg("weights"), py::arg("sources"),
         py::arg("positions"));

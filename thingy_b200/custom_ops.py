@@ -25,12 +25,13 @@ from __future__ import annotations
 
 import torch
 
-from .dispatch import MoePlan, moe_combine, moe_permute, moe_sort
+from .dispatch import MoePlan, moe_combine, moe_permute
 from .fp8_utils import per_token_cast_to_fp8
 from .fp8_utils import per_block_cast_to_fp8, two_way_cast_to_fp8
 from .fused import residual_rms_norm_fp8
 from .gemm import fp8_block_gemm, fp8_grouped_gemm
 from .moe import moe_fp8
+from .ops import require_binding
 
 GROUP_SIZE = 128
 
@@ -124,7 +125,7 @@ def _moe_fp8_fake(x, q, scale, router, w13, w13_scale, w2, w2_scale, top_k, scor
 
 @torch.library.custom_op("thingy_b200::moe_sort", mutates_args=())
 def moe_sort_op(topk_ids: torch.Tensor, num_experts: int, align: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
-    return moe_sort(topk_ids, num_experts, align=align)[:4]
+    return require_binding().moe_sort(topk_ids, num_experts, align, True)
 
 
 @moe_sort_op.register_fake

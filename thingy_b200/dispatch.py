@@ -50,7 +50,7 @@ def moe_sort(topk_ids: torch.Tensor, num_experts: int, *, align: int = 1) -> Moe
     align)`` rows, whatever the ids; rows that hold no choice are padding.
     num_experts <= 512.
     """
-    return MoePlan(*require_binding().moe_sort(topk_ids, int(num_experts), int(align)), int(align))
+    return MoePlan(*require_binding().moe_sort(topk_ids, int(num_experts), int(align), False), int(align))
 
 
 def moe_permute(x: torch.Tensor, plan: MoePlan) -> torch.Tensor:
