@@ -26,7 +26,7 @@ def test_plan_rows_refused(lib, sizes):
 def test_workspace_only_above_one_cta(lib):
     assert lib.cutie_moe_sort_workspace(512, 8, 64) == 0
     assert lib.cutie_moe_sort_workspace(513, 8, 64) == 3 * 64 * 4
-    assert lib.cutie_moe_sort_workspace(2**27, 8, 512) == 512 * 512 * 4
+    assert lib.cutie_moe_sort_workspace(2**27, 8, 512) == 128 * 512 * 4
 
 
 def test_sort_refused(lib):
