@@ -83,6 +83,28 @@ def test_product(counts, N, K, out_dtype):
     assert torch.equal(again, got)
 
 
+@pytest.mark.parametrize("counts", [[300, 0, 1, 127], [7] * 40])  # either kernel
+def test_operands_of_other_strides(counts):
+    """Rows of A and D inside wider ones, one matrix for all experts: the same bits; off the boundaries: refused."""
+    E, plan, N, K = len(counts), plan_of(counts), 256, 384
+    R = plan.sources.shape[0]
+    g = torch.Generator(device="cuda").manual_seed(8)
+    a, sa = codes(g, R, K), torch.rand(R, 3, generator=g, device="cuda")
+    b, sb = codes(g, 1, N, K), torch.rand(1, 2, 3, generator=g, device="cuda")
+    want = tb.fp8_grouped_gemm(a, sa, b.expand(E, N, K).contiguous(), sb.expand(E, 2, 3).contiguous(), plan)
+    wide = torch.zeros(R, K + 48, dtype=F8, device="cuda")
+    wide[:, 16 : 16 + K] = a
+    out = torch.full((R, N + 32), 7.0, dtype=torch.bfloat16, device="cuda")
+    got = tb.fp8_grouped_gemm(wide[:, 16 : 16 + K], sa, b.expand(E, N, K), sb.expand(E, 2, 3), plan, out=out[:, 16 : 16 + N])
+    assert torch.equal(got, want)
+    assert bool((out[:, :16] == 7).all()) and bool((out[:, 16 + N :] == 7).all())
+    for bad in (wide[:, 8 : 8 + K], wide.view(torch.uint8)[:, 1 : 1 + K]):
+        with pytest.raises(ValueError, match="aligned"):
+            tb.fp8_grouped_gemm(bad, sa, b.expand(E, N, K), sb.expand(E, 2, 3), plan)
+    with pytest.raises(ValueError, match="aligned"):
+        tb.fp8_grouped_gemm(a, sa, b.expand(E, N, K), sb.expand(E, 2, 3), plan, out=out[:, 8 : 8 + N])
+
+
 def test_product_equals_the_single_one():
     """An expert alone: the same tiles, the same sums as fp8_block_gemm over its rows."""
     counts = [384, 1, 200]

@@ -158,6 +158,26 @@ def test_rows_of_other_strides():
         assert torch.allclose(ga[1], gb[1], rtol=0, atol=float(H * 2.0**-24 * (dy.float().abs().sum(1).max() * r.abs().max())))
 
 
+def test_rows_past_32_bits_of_offsets():
+    """More than 2^31 elements of sorted rows: permute, combine and its backward at the far end."""
+    T, k, H = 40000, 8, 7168
+    ids = torch.arange(T * k, device="cuda", dtype=torch.int32).reshape(T, k) % 64
+    plan = tb.moe_sort(ids, 64)
+    assert plan.sources.numel() * H > 2**31
+    x = torch.randint(-8, 8, (T, H), device="cuda", dtype=torch.int8, generator=torch.Generator(device="cuda").manual_seed(1)).bfloat16()
+    xs = tb.moe_permute(x, plan)
+    src = plan.sources.long()
+    for r in (0, 1, 299999, T * k // 2, T * k - 2, T * k - 1):
+        assert torch.equal(xs[r], x[src[r] // k])
+    w = torch.full((T, k), 0.25, device="cuda")
+    assert torch.equal(tb.moe_combine(xs, w, plan), 2 * x)  # small integers: exact in bf16
+    wg, rg = w.requires_grad_(), xs.requires_grad_()
+    drows, dw = torch.autograd.grad(tb.moe_combine(rg, wg, plan), (rg, wg), x)
+    for r in (0, 299999, T * k - 1):
+        assert torch.equal(drows[r], 0.25 * x[src[r] // k])
+    assert torch.equal(dw, x.float().square().sum(1, keepdim=True).expand(T, k))  # integers below 2^24
+
+
 def test_gradients_of_a_sum_and_of_broadcasts():
     """Gradients that come expanded (a sum's) and inputs used twice."""
     T, k, H = 20, 4, 48
