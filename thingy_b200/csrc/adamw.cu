@@ -512,7 +512,9 @@ cudaError_t launch_table(const AdamwTensors& l, const AdamwStep& step, cudaStrea
     }
     if (k == 0) continue;
     t.first[k] = (uint32_t)chunks;
-    const uint64_t most = (uint64_t)(CODES ? 4 * kCodesCtas : 2 * kCtas) * device_sm_count();
+    // CTAs in turn, not one round: chunks deal out evenly (20M fp32 in 200 tensors: 2
+    // rounds 107 us, 16 98); with codes runs of some length
+    const uint64_t most = (uint64_t)(CODES ? 4 * kCodesCtas : 16 * kCtas) * device_sm_count();
     const unsigned grid = (unsigned)(chunks < most ? chunks : most);
     auto kernel = CODES ? adamw_codes_kernel<P, G, N> : adamw_kernel<P, G, N>;
     const cudaError_t e = launch_pdl(kernel, grid, kThreads, 0, stream, t, k, step);
