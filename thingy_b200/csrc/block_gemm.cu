@@ -633,7 +633,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // the piece's scales are in registers before its load is waited for. After
     // an abort the waits return at once and the loads go on (tensor memory is
     // still this CTA's).
-    constexpr int CH = 32;
+    constexpr int CH = SB_ROWS ? 16 : 32;
     uint32_t lo[CH], hi[CH];
     uint32_t buf = 0, buf_parity = 0, slot = 0, slot_parity = 0;
     float sc = 0.f;  // the row's scale of the block, times the column block's
@@ -670,6 +670,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float s = sc;
         const float* col = sb;
         const uint32_t tm = tm_lane + buf * BN;
+        float4 f[SB_ROWS ? CH / 4 : 1];
+        auto column_scales = [&](int c) {  // of piece c, before its load is waited for
+          if (SB_ROWS) {
+#pragma unroll
+            for (int i = 0; i < CH / 4; ++i) f[i] = *reinterpret_cast<const float4*>(col + c + 4 * i);
+          }
+        };
         auto add = [&](int c, const uint32_t(&v)[CH]) {
           const float2 s2 = make_float2(s, s);
 #pragma unroll
@@ -677,9 +684,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             float2 d0 = make_float2(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]));
             float2 d1 = make_float2(__uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]));
             if (SB_ROWS) {
-              const float4 f = *reinterpret_cast<const float4*>(col + c + 4 * i);
-              d0 = __fmul2_rn(d0, make_float2(f.x, f.y));
-              d1 = __fmul2_rn(d1, make_float2(f.z, f.w));
+              d0 = __fmul2_rn(d0, make_float2(f[i].x, f[i].y));
+              d1 = __fmul2_rn(d1, make_float2(f[i].z, f[i].w));
             }
             acc[c / 2 + 2 * i] = __ffma2_rn(d0, s2, acc[c / 2 + 2 * i]);
             acc[c / 2 + 2 * i + 1] = __ffma2_rn(d1, s2, acc[c / 2 + 2 * i + 1]);
@@ -689,9 +695,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t done = smem_addr(&scale_empty[slot]);
 #pragma unroll
         for (int c = 0; c < NC; c += 2 * CH) {
+          column_scales(c);
           tc::tmem_ld_wait(lo);
           tc::tmem_ld_async(tm + (uint32_t)(c + CH), hi);
           add(c, lo);
+          column_scales(c + CH);
           tc::tmem_ld_wait(hi);
           if (c + 2 * CH < NC) {
             tc::tmem_ld_async(tm + (uint32_t)(c + 2 * CH), lo);
