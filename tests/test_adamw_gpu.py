@@ -395,6 +395,29 @@ def test_optimizer_captured():
         assert torch.equal(eager, captured)
 
 
+def test_optimizer_captured_without_a_gradient():
+    """Parameters that would part company within a graph: refused, and nothing has changed."""
+    ps = [torch.randn(10, device="cuda", requires_grad=True) for _ in range(2)]
+    opt = tb.AdamW(ps, lr=0.1, capturable=True)
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    opt.step()
+    ps[1].grad = None
+    before = [p.detach().clone() for p in ps]
+    with pytest.raises(RuntimeError, match="same steps"):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            opt.step()
+    assert all(torch.equal(p, q) for p, q in zip(ps, before))
+    assert [int(opt.state[p]["step"]) for p in ps] == [1, 1]
+    opt.step()  # eager: they part
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    graph.replay()
+    assert [int(opt.state[p]["step"]) for p in ps] == [3, 1]
+
+
 def test_version_counters_see_the_step():
     p = torch.randn(8, device="cuda", requires_grad=True)
     y = (p * p).sum()
@@ -418,6 +441,11 @@ def test_refusals():
         (lambda: step([p], [g], [m], [v], step=1, lr=0.1, weight_decay=-1.0), "weight_decay"),
         (lambda: step([p, p], [g, g], [m, tb.adamw_state(p)], [v, tb.adamw_state(p)], step=1, lr=0.1), "params must not overlap"),
         (lambda: step([p, torch.zeros_like(p)], [g, g], [m, m], [v, tb.adamw_state(p)], step=1, lr=0.1), "exp_avgs must not overlap"),
+        (lambda: step([p], [g], [m], [m], step=1, lr=0.1), "share memory"),
+        (lambda: step([p], [g], [p], [v], step=1, lr=0.1), "share memory"),
+        (lambda: step([p], [g], [m8], [(v8[0], m8[1])], step=1, lr=0.1), "share memory"),
+        (lambda: step([p, torch.zeros_like(p)], [g, g], [m8, (tb.adamw_state(p, 8)[0], m8[1])], [v8, tb.adamw_state(p, 8)], step=1,
+                      lr=0.1), "scales must not overlap"),
         (lambda: step([p], [g], [m], [v, v], step=1, lr=0.1), "same length"),
         (lambda: step([p], [g[:100]], [m], [v], step=1, lr=0.1), "shapes"),
         (lambda: step([p], [None], [m], [v], step=1, lr=0.1), "hold tensors"),

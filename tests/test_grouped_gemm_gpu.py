@@ -227,6 +227,22 @@ def test_linear_against_differences():
         assert abs((loss(up) - loss(down)) / 2 - float(dw[e, n, k])) <= tol
 
 
+def test_one_weight_for_all_experts():
+    """A weight that is expanded over the experts: its gradient is the sum of theirs."""
+    plan = plan_of([100, 60, 0, 200])
+    R = plan.sources.shape[0]
+    g = torch.Generator(device="cuda").manual_seed(12)
+    x = torch.randn(R, 256, generator=g, device="cuda").bfloat16()
+    dy = torch.randn(R, 128, generator=g, device="cuda").bfloat16()
+    one = (0.05 * torch.randn(1, 128, 256, generator=g, device="cuda")).requires_grad_()
+    each = one.detach().expand(4, 128, 256).contiguous().requires_grad_()
+    y = tb.fp8_grouped_linear(x, one.expand(4, 128, 256), plan)
+    assert torch.equal(y, tb.fp8_grouped_linear(x, each, plan))
+    (d1,) = torch.autograd.grad(y, one, dy)
+    (d4,) = torch.autograd.grad(tb.fp8_grouped_linear(x, each, plan), each, dy)
+    assert torch.equal(d1, d4.sum(0, keepdim=True))
+
+
 def test_no_rows():
     plan = tb.moe_sort(torch.zeros(0, 2, dtype=torch.int32, device="cuda"), 4, align=128)
     x = torch.zeros(0, 128, dtype=torch.bfloat16, device="cuda").requires_grad_()
@@ -316,6 +332,8 @@ def test_refusals():
         (lambda: tb.fp8_grouped_linear(x, w.cpu(), plan), "wrong device"),
         (lambda: tb.fp8_grouped_linear(x, w[0], plan), "E, N, K"),
         (lambda: tb.fp8_grouped_linear(x.requires_grad_(), w, plan, (b, sb, None, None)), "transposed"),
+        (lambda: tb.fp8_grouped_linear(x, w, plan, (b, sb, b, sb)), "transposes"),
+        (lambda: tb.fp8_grouped_linear(x.detach(), w, plan, (b[:1], sb, None, None)), "weight_fp8"),
         (lambda: tb.fp8_grouped_gemm(a, sa, b, sb, loose), "multiple of 128"),
         (lambda: tb.fp8_grouped_gemm(a[:-1], sa[:-1], b, sb, plan), "multiples of 128"),
         (lambda: tb.fp8_grouped_gemm(a, sa[:, :0], b, sb, plan), "a_scale"),

@@ -644,6 +644,8 @@ at::Tensor fp8_grouped_linear(const at::Tensor& x, const at::Tensor& weight, con
   if (wq.has_value() != ws.has_value()) bad("weight_fp8 must be (q, s, qt, st)");
   if (wq.has_value() && need_dx && (!wqt.has_value() || !wst.has_value()))
     bad("weight_fp8 has no transposed codes: make it with quantize_experts(weight, transposed=True)");
+  if (wq.has_value()) expert_matrices(*wq, *ws, E, N, K, dev, "weight_fp8");
+  if (wq.has_value() && need_dx) expert_matrices(*wqt, *wst, E, K, N, dev, "weight_fp8's transposes");
   return FP8GroupedLinear::apply(x, weight, wq, ws, wqt, wst, sources, offsets, counts, need_dx, need_dw);
 }
 
@@ -952,14 +954,15 @@ void adamw_step(const py::object& params, const py::object& grads, const py::obj
   std::vector<int64_t> n(count);
   if (codes) ms.resize(count), vs.resize(count);
   std::vector<at::Tensor> copies;  // of gradients that are not dense
-  std::vector<std::pair<uintptr_t, uintptr_t>> rp, rm, rv;
-  rp.reserve(count), rm.reserve(count), rv.reserve(count);
+  std::vector<std::pair<uintptr_t, uintptr_t>> rp, rm, rv, rms, rvs;
+  for (auto* r : {&rp, &rm, &rv, &rms, &rvs}) r->reserve(count);
   const auto range = [](std::vector<std::pair<uintptr_t, uintptr_t>>& r, const at::Tensor& t) {
     const uintptr_t a = reinterpret_cast<uintptr_t>(t.data_ptr());
     if (t.numel() > 0) r.emplace_back(a, a + t.numel() * t.element_size());
   };
   const auto state = [&](PyObject* o, int64_t i, const at::Tensor& param, const char* name, void** place, void** scale,
-                         std::vector<std::pair<uintptr_t, uintptr_t>>& r) {
+                         std::vector<std::pair<uintptr_t, uintptr_t>>& r,
+                         std::vector<std::pair<uintptr_t, uintptr_t>>& rs) {
     if ((PyTuple_Check(o) || PyList_Check(o)) != codes)
       bad("states are all tensors, or all pairs of codes and scales");
     if (!codes) {
@@ -980,6 +983,7 @@ void adamw_step(const py::object& params, const py::object& grads, const py::obj
       bad(std::string(name) + "'s scales must be contiguous float32, one for each 128 elements");
     *place = q.data_ptr(), *scale = s.data_ptr();
     range(r, q);
+    range(rs, s);
   };
   for (int64_t i = 0; i < count; ++i) {
     const at::Tensor &pt = tensor_of(P[i], "params"), &gt = tensor_of(G[i], "grads");
@@ -997,12 +1001,16 @@ void adamw_step(const py::object& params, const py::object& grads, const py::obj
       copies.push_back(gt.contiguous());
       g[i] = copies.back().data_ptr();
     }
-    state(M[i], i, pt, "exp_avgs", &m[i], codes ? &ms[i] : nullptr, rm);
-    state(V[i], i, pt, "exp_avg_sqs", &v[i], codes ? &vs[i] : nullptr, rv);
+    state(M[i], i, pt, "exp_avgs", &m[i], codes ? &ms[i] : nullptr, rm, rms);
+    state(V[i], i, pt, "exp_avg_sqs", &v[i], codes ? &vs[i] : nullptr, rv, rvs);
+    if (n[i] > 0 && (m[i] == v[i] || p[i] == m[i] || p[i] == v[i] || (codes && ms[i] == vs[i])))
+      bad("a parameter and its states must not share memory");
   }
   check_apart(rp, "params");
   check_apart(rm, "exp_avgs");
   check_apart(rv, "exp_avg_sqs");
+  check_apart(rms, "exp_avgs' scales");
+  check_apart(rvs, "exp_avg_sqs' scales");
   const at::Tensor* st = device_scalar(step.ptr(), "step", at::kLong, dev);
   const at::Tensor* lt = device_scalar(lr.ptr(), "lr", at::kFloat, dev);
   if (grad_scale.has_value() &&

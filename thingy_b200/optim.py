@@ -160,6 +160,9 @@ class AdamW(torch.optim.Optimizer):
                 sharers.setdefault(id(self.state[p]["step"]), []).append(p)
         for p in own:
             now.setdefault(id(self.state[p]["step"]), []).append(p)
+        split = any(len(ps) < len(sharers[key]) for key, ps in now.items())
+        if split and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a captured step needs a gradient for every parameter that has had the same steps")
         for key, ps in now.items():
             step = self.state[ps[0]]["step"]
             if len(ps) < len(sharers[key]):  # some stay behind: the others count on their own from here
