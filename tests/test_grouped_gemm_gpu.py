@@ -288,6 +288,43 @@ def test_wait_limit(counts):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("N,K", [(2048, 2048), (256, 128)])  # pairs, and 128-wide tiles
+def test_wait_limit_of_the_weight_gradient(N, K):
+    """The same for the gradient, an expert without rows among them."""
+    counts = [700, 0, 300, 64]
+    plan = plan_of(counts)
+    R, E = plan.sources.shape[0], len(counts)
+    g = torch.Generator(device="cuda").manual_seed(10)
+    a, b = codes(g, N, R), codes(g, K, R)
+    sa, sb = torch.rand(N, R // 128, generator=g, device="cuda"), torch.rand(K, R // 128, generator=g, device="cuda")
+    d = torch.zeros(E, N, K, device="cuda")
+    lib = tb._lib.load()
+
+    def launch():
+        tb._lib.check(lib.cutie_fp8_grouped_wgrad(
+            a.data_ptr(), R, sa.data_ptr(), R // 128, 1, b.data_ptr(), R, sb.data_ptr(), R // 128, 1, plan.offsets.data_ptr(), E,
+            d.data_ptr(), K, N * K, tb._lib.DTYPE_F32, R, N, K, torch.cuda.current_stream().cuda_stream))
+        return d.clone()
+
+    want = launch()
+    off = plan.offsets.tolist()
+    for e in range(E):
+        cols = slice(off[e], off[e + 1])
+        left, right = (q[:, cols].double() * spread(s[:, off[e] // 128 : off[e + 1] // 128], off[e + 1] - off[e])
+                       for q, s in ((a, sa), (b, sb)))
+        check(want[e], left, right, torch.float32)
+    torch.cuda.synchronize()
+    tb._lib.device_error()
+    old = tb._lib.set_wait_limit(-1)
+    try:
+        launch()
+        torch.cuda.synchronize()
+    finally:
+        tb._lib.set_wait_limit(old)
+    assert tb._lib.device_error() == 1
+    assert torch.equal(launch(), want) and tb._lib.device_error() == 0
+
+
 def test_repeats_and_graphs():
     E, N, K, T, k = 8, 256, 384, 300, 2
     g = torch.Generator(device="cuda").manual_seed(3)
