@@ -335,8 +335,8 @@ CUTIE_API int cutie_fp8_block_gemm(const void* a, int64_t lda, const void* a_sca
 /*
  * The two-way cast (CUTIE_TILE_TWO_WAY) of rows sorted by expert
  * (cutie_moe_sort with align a multiple of 128): rows whose source is -1 count as
- * zeros, whatever x holds there, and tiles of 128 rows behind the last
- * expert's are left unwritten. R is a multiple of 128.
+ * zeros, whatever x holds there; all codes and scales are written. R is a multiple
+ * of 128.
  */
 CUTIE_API int cutie_cast_fp8_sorted(const void* x, int64_t ldx, int64_t R, int64_t H,
                                     const void* sources, int scale_fmt, void* q, int64_t ldq,

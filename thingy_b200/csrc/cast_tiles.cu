@@ -69,8 +69,9 @@ __device__ __forceinline__ uint32_t pair_to_bf2(uint32_t a, uint32_t b) {
 }
 
 // SORTED: rows sorted by expert (two-way kind). Padding rows are zeros whatever
-// x holds there, so that they change no column group; a tile that begins with
-// padding is behind the last expert's rows: nothing reads its codes.
+// x holds there, so that they change no column group. Tiles that are all padding
+// are written too: where experts begin at multiples of 256 or more they lie within
+// one, and the weight gradient goes over all of its columns.
 template <bool BLOCK, bool TRANSPOSED, bool SORTED = false, bool F32 = false>
 __global__ void __launch_bounds__(kThreads, 4)
     cast_tiles_kernel(CastArgs a) {
@@ -88,9 +89,9 @@ __global__ void __launch_bounds__(kThreads, 4)
   griddep_wait();
   griddep_launch_dependents();
 
-  // SORTED: the sources of the warp's 16 rows, lane 16: of the tile's first; read
-  // beside the rows, not before them (M is a multiple of 128)
-  const int source = SORTED && lane <= 16 ? a.sources[tr * kTile + (lane < 16 ? 16 * warp + lane : 0)] : 0;
+  // SORTED: the sources of the warp's 16 rows; read beside the rows, not before them
+  // (M is a multiple of 128)
+  const int source = SORTED && lane < 16 ? a.sources[tr * kTile + 16 * warp + lane] : 0;
   uint32_t x[8][4];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -109,7 +110,6 @@ __global__ void __launch_bounds__(kThreads, 4)
   }
   if (SORTED) {
     const uint32_t none = __ballot_sync(0xffffffffu, source < 0);
-    if (none >> 16 & 1u) return;
     const uint32_t mine = none >> (rg & 1) * 8 & 0xffu;
     if (mine != 0) {
 #pragma unroll

@@ -328,8 +328,8 @@ struct CastArgs {
   int64_t ldqt;
   float* st;    // block: [H/128, M/128], else group-major [M/128, H]
   int64_t ldst;
-  const int* sources;  // two-way kind: rows whose source is below zero count as zeros, and tiles
-                       // that begin with one are not written (null: all rows count)
+  const int* sources;  // two-way kind: rows whose source is below zero count as zeros (null: all
+                       // rows count)
 };
 cudaError_t launch_cast_tiles(const CastArgs& a, bool block, cudaStream_t stream);
 
