@@ -348,7 +348,7 @@ CUTIE_API int cutie_cast_fp8_sorted(const void* x, int64_t ldx, int64_t R, int64
  * offsets[e + 1] of
  *   D = dequant(A) dequant(B[e])^T
  * and zeros in padding, the rows of e from offsets[e] + counts[e] on, and in
- * the rows behind the last expert's. A: e4m3 [R, K] (lda), fp32
+ * the rows before the first expert's and behind the last's. A: e4m3 [R, K] (lda), fp32
  * scales of 1 x 128 groups, element (r, kb) at r * sa_row + kb * sa_kb. B:
  * e4m3 [E, N, K], row n of expert e at e * b_expert + n * ldb, fp32 scales of
  * 128 x 128 blocks at e * sb_expert + nb * sb_row + kb * sb_kb. D: bf16 or fp32

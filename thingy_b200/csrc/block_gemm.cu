@@ -378,6 +378,12 @@ __device__ __forceinline__ void zero_row(const TileArgs& g, void* d, int64_t row
   char* p = static_cast<char*>(d) + (row * g.ldd + col) * (g.d_f32 ? 4 : 2);
   for (int c = 0; c < cols && col + c < g.N; c += per, p += 32) st_stream8(p, zero);
 }
+// Zeros in rows lo to hi of D, a row a warp: warp `at` of `of` takes rows at, at + of, ...
+__device__ __forceinline__ void zero_rows(const TileArgs& g, int lo, int hi, int at, int of, int lane) {
+  const int per = g.d_f32 ? 8 : 16;
+  for (int64_t row = lo + (at + of - lo % of) % of; row < hi; row += of)
+    for (int c = lane * per; c < g.N; c += 32 * per) zero_row(g, g.d, row, c, 1);
+}
 
 template <int BN, bool SB_ROWS, bool VEC, bool SPLIT, bool PAIR, int MODE = kOne>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -781,10 +787,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     }
-    if constexpr (MODE == kExpertRows) {  // rows behind the last expert's
-      for (int64_t row = (int64_t)experts.begin[g.E] + blockIdx.x * kEpiWarps + warp; row < g.R;
-           row += (int64_t)gridDim.x * kEpiWarps)
-        for (int c = lane * (g.d_f32 ? 8 : 16); c < g.N; c += 32 * (g.d_f32 ? 8 : 16)) zero_row(g, g.d, row, c, 1);
+    if constexpr (MODE == kExpertRows) {  // rows before the first expert's and behind the last's
+      const int at = blockIdx.x * kEpiWarps + warp, of = gridDim.x * kEpiWarps;
+      zero_rows(g, 0, experts.begin[0], at, of, lane);
+      zero_rows(g, experts.begin[g.E], g.R, at, of, lane);
     } else if constexpr (MODE == kExpertColumns) {  // experts without rows
       for (int t = begin; t < tiles; t += step) {
         const Item it = item_of<BN, MODE>(g, experts, t, (PAIR ? 2 : 1) * kBM, rank, expert);
@@ -1572,10 +1578,18 @@ __global__ void __launch_bounds__(kFewThreads, 1)
           zero_row(g, g.d, experts.end[it.e] + i / sectors, it.col + i % sectors * per, 1);
       }
     }
-    // rows behind the last expert's
-    const int per = g.d_f32 ? 8 : 16;
-    for (int64_t row = (int64_t)experts.begin[g.E] + blockIdx.x * 4 + warp; row < g.R; row += (int64_t)gridDim.x * 4)
-      for (int c = lane * per; c < g.N; c += 32 * per) zero_row(g, g.d, row, c, 1);
+    // rows before the first expert's and behind the last's, and of experts that are all padding
+    const int at = blockIdx.x * 4 + warp, of = gridDim.x * 4;
+    zero_rows(g, 0, experts.begin[0], at, of, lane);
+    zero_rows(g, experts.begin[g.E], g.R, at, of, lane);
+    for (int e0 = 0; e0 < g.E; e0 += 32) {
+      const int e = e0 + lane;
+      const bool empty = e < g.E && experts.end[e] == experts.begin[e] && experts.begin[e + 1] > experts.begin[e];
+      for (unsigned todo = __ballot_sync(0xffffffffu, empty); todo != 0; todo &= todo - 1) {
+        const int x = e0 + __ffs(todo) - 1;
+        zero_rows(g, experts.begin[x], experts.begin[x + 1], at, of, lane);
+      }
+    }
   }
   __syncwarp();
   tc::fence_before();
