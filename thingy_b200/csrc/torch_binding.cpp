@@ -913,15 +913,42 @@ const at::Tensor& tensor_of(PyObject* o, const char* name) {
   return THPVariable_Unpack(o);
 }
 
-// Written ranges must not overlap: a tensor listed twice would be a race.
-void check_apart(std::vector<std::pair<uintptr_t, uintptr_t>>& ranges, const char* name) {
-  const auto after = [](const auto& x, const auto& y) { return x.second <= y.first; };
-  bool sorted = true;
-  for (size_t i = 1; i < ranges.size() && sorted; ++i) sorted = after(ranges[i - 1], ranges[i]);
-  if (sorted) return;
-  std::sort(ranges.begin(), ranges.end());
+// Addresses [first, second) of tensors. What a step writes must not overlap: it would be a
+// race. A list in the order of its addresses (views of one buffer) is not sorted.
+using Ranges = std::vector<std::pair<uintptr_t, uintptr_t>>;
+
+bool in_order(const Ranges& ranges) {
   for (size_t i = 1; i < ranges.size(); ++i)
-    if (!after(ranges[i - 1], ranges[i])) bad(std::string(name) + " must not overlap one another");
+    if (ranges[i - 1].second > ranges[i].first) return false;
+  return true;
+}
+
+void check_apart(Ranges& ranges, const char* name) {
+  if (in_order(ranges)) return;
+  std::sort(ranges.begin(), ranges.end());
+  if (!in_order(ranges)) bad(std::string(name) + " must not overlap one another");
+}
+
+// The same between two lists in the order of their addresses, of which x may overlap itself.
+bool apart(const Ranges& x, const Ranges& y) {
+  for (size_t i = 0, j = 0; i < x.size() && j < y.size();) {
+    if (y.back().second <= x[i].first) return true;
+    if (x[i].second <= y[j].first) ++i;
+    else if (y[j].second <= x[i].first) ++j;
+    else return false;
+  }
+  return true;
+}
+
+// What a step writes, lists that are apart each, and what it reads.
+void check_memory(Ranges& read, const std::vector<const Ranges*>& written) {
+  for (size_t i = 0; i < written.size(); ++i)
+    for (size_t j = 0; j < i; ++j)
+      if (!apart(*written[i], *written[j]))
+        bad("a parameter and its states must not share memory, nor with another's");
+  if (!std::is_sorted(read.begin(), read.end())) std::sort(read.begin(), read.end());
+  for (const Ranges* w : written)
+    if (!apart(read, *w)) bad("grads must not share memory with parameters or states");
 }
 
 // A step or a rate: a number, or one element on the GPU.
@@ -954,15 +981,14 @@ void adamw_step(const py::object& params, const py::object& grads, const py::obj
   std::vector<int64_t> n(count);
   if (codes) ms.resize(count), vs.resize(count);
   std::vector<at::Tensor> copies;  // of gradients that are not dense
-  std::vector<std::pair<uintptr_t, uintptr_t>> rp, rm, rv, rms, rvs;
-  for (auto* r : {&rp, &rm, &rv, &rms, &rvs}) r->reserve(count);
-  const auto range = [](std::vector<std::pair<uintptr_t, uintptr_t>>& r, const at::Tensor& t) {
+  Ranges rp, rg, rm, rv, rms, rvs;
+  for (auto* r : {&rp, &rg, &rm, &rv, &rms, &rvs}) r->reserve(count);
+  const auto range = [](Ranges& r, const at::Tensor& t) {
     const uintptr_t a = reinterpret_cast<uintptr_t>(t.data_ptr());
     if (t.numel() > 0) r.emplace_back(a, a + t.numel() * t.element_size());
   };
   const auto state = [&](PyObject* o, int64_t i, const at::Tensor& param, const char* name, void** place, void** scale,
-                         std::vector<std::pair<uintptr_t, uintptr_t>>& r,
-                         std::vector<std::pair<uintptr_t, uintptr_t>>& rs) {
+                         Ranges& r, Ranges& rs) {
     if ((PyTuple_Check(o) || PyList_Check(o)) != codes)
       bad("states are all tensors, or all pairs of codes and scales");
     if (!codes) {
@@ -997,20 +1023,20 @@ void adamw_step(const py::object& params, const py::object& grads, const py::obj
     range(rp, pt);
     if (gt.is_contiguous()) {
       g[i] = gt.data_ptr();
+      range(rg, gt);
     } else {
       copies.push_back(gt.contiguous());
       g[i] = copies.back().data_ptr();
     }
     state(M[i], i, pt, "exp_avgs", &m[i], codes ? &ms[i] : nullptr, rm, rms);
     state(V[i], i, pt, "exp_avg_sqs", &v[i], codes ? &vs[i] : nullptr, rv, rvs);
-    if (n[i] > 0 && (m[i] == v[i] || p[i] == m[i] || p[i] == v[i] || (codes && ms[i] == vs[i])))
-      bad("a parameter and its states must not share memory");
   }
   check_apart(rp, "params");
   check_apart(rm, "exp_avgs");
   check_apart(rv, "exp_avg_sqs");
   check_apart(rms, "exp_avgs' scales");
   check_apart(rvs, "exp_avg_sqs' scales");
+  check_memory(rg, {&rp, &rm, &rv, &rms, &rvs});
   const at::Tensor* st = device_scalar(step.ptr(), "step", at::kLong, dev);
   const at::Tensor* lt = device_scalar(lr.ptr(), "lr", at::kFloat, dev);
   if (grad_scale.has_value() &&

@@ -42,8 +42,9 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, betas=(0.9, 0.
 
     step counts from 1: an int, or an int64 tensor on the GPU that is read when the
     kernel runs (for captured steps); lr: a number or a float32 tensor likewise;
-    grad_scale: a float32 tensor, what clipping leaves of the gradients. No
-    tensor may be listed twice or overlap another.
+    grad_scale: a float32 tensor, what clipping leaves of the gradients.
+    Parameters and states that share memory with one another, or with a
+    gradient, are refused.
     """
     beta1, beta2 = betas
     require_binding().adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr, float(beta1), float(beta2),
