@@ -59,7 +59,9 @@ class AdamW(torch.optim.Optimizer):
     replayed; lr may then be a float32 tensor on the GPU that the program
     changes; the step before the capture makes the states.
     ``step(grad_scale=...)`` takes the factor of a clipped norm. Parameters
-    without a gradient are left as they are; sparse gradients are refused.
+    without a gradient are left as they are. Refused are sparse gradients and
+    parameters that are not contiguous; a refused step does not count for the
+    parameters that it leaves as they were.
     """
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, *,
@@ -113,6 +115,7 @@ class AdamW(torch.optim.Optimizer):
         fresh = [p for p in own if not self.state[p]]
         if torch.cuda.is_current_stream_capturing() and (fresh or not group["capturable"]):
             raise RuntimeError("a captured step needs capturable=True and one step before it, which makes the states")
+        lr = group["lr"] if group["capturable"] else float(group["lr"])
         self._make_states(group, fresh)
         self._count(group, own)
         # a launch for the parameters of one age and of the same dtypes
@@ -122,15 +125,20 @@ class AdamW(torch.optim.Optimizer):
             key = (id(age) if group["capturable"] else age, p.dtype, p.grad.dtype, p.device)
             lists.setdefault(key, []).append(p)
         names = ("exp_avg", "exp_avg_sq")
-        lr = group["lr"] if group["capturable"] else float(group["lr"])
-        for number, ps in enumerate(lists.values()):
-            states = [self.state[p] for p in ps]
-            if group["state_bits"] == 8:
-                m, v = ([(s[name], s[name + "_scale"]) for s in states] for name in names)
-            else:
-                m, v = ([s[name] for s in states] for name in names)
-            adamw_step(ps, [p.grad for p in ps], m, v, step=states[0]["step"], lr=lr, betas=group["betas"],
-                       eps=group["eps"], weight_decay=group["weight_decay"], grad_scale=grad_scale, seed=seed + number)
+        lists, done = list(lists.values()), 0
+        try:
+            for ps in lists:
+                states = [self.state[p] for p in ps]
+                if group["state_bits"] == 8:
+                    m, v = ([(s[name], s[name + "_scale"]) for s in states] for name in names)
+                else:
+                    m, v = ([s[name] for s in states] for name in names)
+                adamw_step(ps, [p.grad for p in ps], m, v, step=states[0]["step"], lr=lr, betas=group["betas"],
+                           eps=group["eps"], weight_decay=group["weight_decay"], grad_scale=grad_scale, seed=seed + done)
+                done += 1
+        except BaseException:
+            self._take_back(group, [p for ps in lists[done:] for p in ps])
+            raise
 
     def _make_states(self, group, fresh):
         """Zeros. On the GPU, parameters that begin together share their count."""
@@ -150,24 +158,40 @@ class AdamW(torch.optim.Optimizer):
                     counts[p.device] = torch.zeros((), dtype=torch.int64, device=p.device)
                 state["step"] = counts[p.device]
 
-    def _count(self, group, own):
-        if not group["capturable"]:
-            for p in own:
-                self.state[p]["step"] += 1
-            return
+    def _sharers(self, group, own):
+        """For each count on the GPU that parameters of `own` have: those of them, and all of the group's that have it."""
         sharers, now = {}, {}
         for p in group["params"]:
             if self.state[p]:
                 sharers.setdefault(id(self.state[p]["step"]), []).append(p)
         for p in own:
             now.setdefault(id(self.state[p]["step"]), []).append(p)
-        split = any(len(ps) < len(sharers[key]) for key, ps in now.items())
-        if split and torch.cuda.is_current_stream_capturing():
+        return [(ps, sharers[key]) for key, ps in now.items()]
+
+    def _add(self, ps, sharers, n):
+        step = self.state[ps[0]]["step"]
+        if len(ps) < len(sharers):  # some stay behind: the others count on their own from here
+            step = step.clone()
+            for p in ps:
+                self.state[p]["step"] = step
+        step.add_(n)
+
+    def _count(self, group, own):
+        if not group["capturable"]:
+            for p in own:
+                self.state[p]["step"] += 1
+            return
+        shared = self._sharers(group, own)
+        if any(len(ps) < len(all_) for ps, all_ in shared) and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("a captured step needs a gradient for every parameter that has had the same steps")
-        for key, ps in now.items():
-            step = self.state[ps[0]]["step"]
-            if len(ps) < len(sharers[key]):  # some stay behind: the others count on their own from here
-                step = step.clone()
-                for p in ps:
-                    self.state[p]["step"] = step
-            step.add_(1)
+        for ps, all_ in shared:
+            self._add(ps, all_, 1)
+
+    def _take_back(self, group, own):
+        """Parameters whose step was refused have not made it."""
+        if not group["capturable"]:
+            for p in own:
+                self.state[p]["step"] -= 1
+        elif not torch.cuda.is_current_stream_capturing():  # a capture that fails has counted nothing
+            for ps, all_ in self._sharers(group, own):
+                self._add(ps, all_, -1)
