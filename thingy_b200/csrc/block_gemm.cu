@@ -1333,11 +1333,11 @@ namespace {
 // the weight is the 128-row side of the MMA, the expert's rows its N side, up to BR
 // of them, as many (in sixteens) as there are. A persistent CTA an SM walks items
 // of one expert, 128 of its columns and BR of its rows; the copies of the next
-// item run on while one is stored. Taken up to kEMeanRows rows an expert in the
-// mean, against tiles of 128 rows, whose sums go over the padding too: 64 experts of
-// 2048 x 7168 with 9 rows 152 against 178 us (940 MB: 96% of the copy bandwidth),
-// 37 rows 164 against 182, 50 rows 190 against 182; of 4096 x 2048 with 25 rows 103
-// against 112, 50 rows 128 against 114.
+// item run on while one is stored. Taken up to kEMeanRows rows an expert in the mean
+// (of experts that begin at multiples of 128), against tiles of 128 rows, whose sums go
+// over the padding too: 64 experts of 2048 x 7168 with 9 rows 144 to 153 against 178 us
+// (940 MB: 94 to 100% of the copy bandwidth), 37 rows 164 against 182, 50 rows 190 against
+// 182; of 4096 x 2048 with 25 rows 103 against 112, 50 rows 128 against 114.
 constexpr int kERows = 64, kEStages = 4, kEMeanRows = 40;
 
 struct ExpertFewPlan {
@@ -1669,7 +1669,10 @@ int grouped_gemm(const GroupedGemmArgs& p, cudaStream_t stream, const char** why
     // need less time in whole rounds. (The offsets are on the GPU: R bounds the rows.)
     g.M = (int)p.R, g.N = (int)p.N, g.KB = (int)((p.K + kBK - 1) / kBK);
     const int64_t rows = p.R / kBM, n2 = (p.N + 255) / 256, n1 = (p.N + 127) / 128;
-    if (p.counts != nullptr && p.R < (127 + kEMeanRows) * p.E) {  // R: the rows, and up to 127 an expert more
+    // R, which is all that the host knows, holds the rows and up to 127 an expert more
+    // where experts begin at multiples of 128. Plans of a larger align or capacity hold
+    // more padding, and go to the tiles with fewer rows an expert in the mean.
+    if (p.counts != nullptr && p.R < (127 + kEMeanRows) * p.E) {
       g.tiles_n = (int)n1;
       e = launch_expert_few(p, g, rows * (kBM / kERows) * n1, stream);
     } else {
