@@ -21,7 +21,7 @@
 // thread, whose group shares its maxima and scales over 8 lanes. What becomes codes
 // has the same bits as in the other kernel (one code more or less would move the
 // scale of its group in the next step); the update has a fused sum and an
-// approximate reciprocal (2^-23). 134M elements in 303 to 316 us, 66% of the copy
+// approximate reciprocal (2^-23). 134M elements in 311 to 319 us, 66% of the copy
 // bandwidth, 64 thread instructions an element, against 412 and 89 in the other
 // kernel's form. Tried: copies through shared memory a chunk ahead (9% more
 // instructions, no gain), approximate roots and fused sums for the codes too (278).
@@ -34,7 +34,7 @@ namespace cutie {
 namespace {
 
 constexpr int kThreads = 256, kEach = 8, kChunk = 4096, kGroup = 128;
-constexpr int kCtas = 5, kCodesCtas = 3;  // an SM at once (codes: four spill, 308 against 303 us)
+constexpr int kCtas = 5, kCodesCtas = 3;  // an SM at once (codes: four spill, 318 against 312 us)
 constexpr float kMinState = 0x1p-92f;
 
 // Tensors a launch: its argument is the table, 32 KB at most. Short lists take

@@ -25,6 +25,10 @@ class MoePlan(NamedTuple):
     positions [T, k]: the sorted row of each choice, -1 where it is absent.
     offsets [E + 1]: where each expert's rows begin, multiples of ``align``.
     counts [E]: how many rows each expert has, without its padding.
+
+    ``moe_sort`` makes one. A program may make its own, for a fixed capacity an
+    expert, say: offsets that do not decrease, sources and positions that name each
+    other, rows of an expert from its offset on and padding behind them.
     """
 
     sources: torch.Tensor
